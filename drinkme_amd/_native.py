@@ -1,4 +1,4 @@
-"""ctypes binding of libdmx_radix.so (include/dmx_radix.h).
+"""ctypes binding of libdmx_radix.so (include/dmx_radix.h, include/dmx_kv.h).
 
 The library is built in-tree by `python -m drinkme_amd.build` (or
 __graft_entry__.build()). There is no fallback: a missing library raises
@@ -81,6 +81,41 @@ SIGNATURES = {
     "dmx_synth_bf16": (_I, [_U64, _U64, _U64, ct.c_double, _U32, _P, _P, _SZ]),
 }
 
+ROTARY_HALF = 0
+ROTARY_INTERLEAVED = 1
+
+
+class KvCache(ct.Structure):
+    """dmx_kv_cache."""
+    _fields_ = [("k_codes", _P), ("v_codes", _P), ("k_scales", _P), ("v_scales", _P), ("pages", _U32),
+                ("heads", _U32), ("page", _U32), ("dim", _U32)]
+
+
+class KvSeqs(ct.Structure):
+    """dmx_kv_seqs."""
+    _fields_ = [("table", _P), ("lengths", _P), ("cu", _P), ("batch", _U32), ("table_cols", _U32), ("total", _U32),
+                ("max_tokens", _U32)]
+
+
+class KvRows(ct.Structure):
+    """dmx_rows."""
+    _fields_ = [("at", _P), ("token_stride", ct.c_int64), ("head_stride", ct.c_int64), ("heads", _U32)]
+
+
+class KvRotaryTable(ct.Structure):
+    """dmx_rotary_table."""
+    _fields_ = [("at", _P), ("positions", _U32), ("dim", _U32), ("layout", _I)]
+
+
+# every symbol include/dmx_kv.h declares
+KV_SIGNATURES = {
+    "dmx_rotary": (_I, [_P, _P, _U32, _U32, _U32, _I, _P, _I, _P, _P, _P, _SZ]),
+    "dmx_kv_append": (_I, [_P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _SZ]),
+    "dmx_kv_read": (_I, [_P, _P, _P, _P, _P, _P, _SZ]),
+    "dmx_kv_attention_workspace": (_U64, [_P, _P, _U32, _I, _U32, _U32]),
+    "dmx_kv_attention": (_I, [_P, _P, _P, _I, ct.c_float, _I, _U32, _U32, _P, _P, _P, _U64, _P, _P, _SZ]),
+}
+
 _lib = None
 
 
@@ -91,7 +126,7 @@ def lib():
         if not os.path.exists(LIB):
             raise ImportError(f"libdmx_radix.so is not built ({LIB}); run `python -m drinkme_amd.build`")
         L = ct.CDLL(LIB)
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in {**SIGNATURES, **KV_SIGNATURES}.items():
             fn = getattr(L, name)
             fn.restype = res
             fn.argtypes = args

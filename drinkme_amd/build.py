@@ -3,9 +3,9 @@
     python -m drinkme_amd.build
 
 The host codec (csrc/codec.cpp) and the pack-file reader and writer
-(csrc/pack_io.cpp) are compiled with g++, the kernels (csrc/kernels.hip)
-with hipcc for gfx950 only, and all linked into one shared library that
-ctypes loads (drinkme_amd/_native.py). Packed-fp32 instructions are
+(csrc/pack_io.cpp) are compiled with g++, the kernels (csrc/kernels.hip, and
+those of the key/value cache, csrc/kv_kernels.hip) with hipcc for gfx950 only,
+and all linked into one shared library that ctypes loads (drinkme_amd/_native.py). Packed-fp32 instructions are
 disabled for the device code (-packed-fp32-ops): hipcc otherwise forms
 v_pk_*_f32 from scalar float code. The host-only command line tool
 lib/dmx_pack (csrc/dmx_pack.cpp) is linked from the same host sources. The
@@ -65,10 +65,13 @@ def build(verbose: bool = False) -> str:
         obj = os.path.join(OBJ, f"{src}.o")
         _run([*host, "-c", os.path.join(CSRC, f"{src}.cpp"), "-o", obj], verbose)
         objs.append(obj)
-    kern_o = os.path.join(OBJ, "kernels.o")
-    _run([hipcc, *device_flags(), "-c", os.path.join(CSRC, "kernels.hip"), "-o", kern_o], verbose)
+    kernels = []
+    for src in ("kernels", "kv_kernels"):
+        obj = os.path.join(OBJ, f"{src}.o")
+        _run([hipcc, *device_flags(), "-c", os.path.join(CSRC, f"{src}.hip"), "-o", obj], verbose)
+        kernels.append(obj)
     tmp = LIB + ".tmp"
-    _run([hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-pthread", objs[0], objs[1], kern_o, "-o", tmp],
+    _run([hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-pthread", objs[0], objs[1], *kernels, "-o", tmp],
          verbose)
     os.replace(tmp, LIB)
     _run(["g++", "-pthread", *objs, "-o", CLI + ".tmp"], verbose)
