@@ -38,31 +38,60 @@ struct AttnArgs {
     float2* part_ml; // [splits][total * q_heads]: maximum (log2 domain), sum
 };
 
+// Segments of V: 128 channels (lane i reads word i, 8 channels), then 64
+// (word i / 2, 4 channels) and 32 (word i / 4, 2 channels) for the rest of W.
+template <int W>
+struct Segments {
+    static constexpr int wide = W / 4, rest = W & 3;
+    static constexpr int count = wide + (rest ? rest == 3 ? 2 : 1 : 0);
+    static constexpr int size(int s) { return s < wide ? 8 : s == wide && rest >= 2 ? 4 : 2; }  // channels a lane
+    static constexpr int word(int s) { return s <= wide ? 16 * s : 16 * wide + 8; }             // first word
+    static constexpr int tile(int s) { return s <= wide ? 8 * s : 8 * wide + 4; }               // first result tile
+};
+
 // One lane's share of a 32-token block, as loaded.
 template <int W>
 struct Block {
-    uint32_t k[2][W];  // tokens 8 (i >> 2) + 4 s + (i & 3): words W j .. W j + W - 1
-    uint32_t ks[2][2]; // the exponent bytes of the first and the last of those words
-    uint32_t v[W / 4 + (W & 3 ? (W & 3) == 3 ? 2 : 1 : 0)][8];  // per segment: tokens 8 j .. 8 j + 7
-    uint32_t vs[W / 4 + (W & 3 ? (W & 3) == 3 ? 2 : 1 : 0)][2];
+    uint32_t k[2][W];   // tokens 8 (i >> 2) + 4 s + (i & 3): words W j .. W j + W - 1
+    uint32_t ks[2][2];  // the exponent bytes of the first and the last of those words
+    uint32_t v[Segments<W>::count][8];   // per segment: tokens 8 j .. 8 j + 7
+    uint32_t vs[Segments<W>::count][2];  // their exponent bytes
+    bool ok;                             // false: no page for this lane's K tokens
 };
 
-__device__ __forceinline__ float scale_of(uint32_t e) { return __uint_as_float(e << 23); }
+// The page numbers of a lane's K and V tokens in a block.
+struct Entry {
+    uint32_t k, v;
+};
+
+// The scale operand of the conversions takes the exponent bits alone; sign and
+// mantissa may hold anything (measured over all exponents and codes).
+template <int N>
+__device__ __forceinline__ float scale_of(uint32_t bytes) {  // of byte N
+    return __uint_as_float(N == 3 ? bytes >> 1 : bytes << (23 - 8 * N));
+}
 
 template <int B>
 __device__ __forceinline__ uint32_t pair_of(uint32_t word, float scale) {
     const bf16x2 r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, B);
     return __builtin_bit_cast(uint32_t, r);
 }
+__device__ __forceinline__ uint32_t pair_at(int b, uint32_t word, float scale) {  // b: a constant once unrolled
+    return b == 0 ? pair_of<0>(word, scale) : b == 1 ? pair_of<1>(word, scale) : b == 2 ? pair_of<2>(word, scale) : pair_of<3>(word, scale);
+}
 
-// The maximum over the four lanes that share i.
+// The maximum and the sum over the four lanes that share i.
 __device__ __forceinline__ float max_over_j(float x) {
-    x = fmaxf(x, __shfl_xor(x, 16));
-    return fmaxf(x, __shfl_xor(x, 32));
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ float sum_over_j(float x) {
-    x += __shfl_xor(x, 16);
-    return x + __shfl_xor(x, 32);
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 // x as P bf16 pieces whose sum it is (to 8 P bits).
@@ -80,22 +109,199 @@ __device__ __forceinline__ void pieces(const float (&x)[8], bf16x8 (&out)[P]) {
         }
 }
 
-// Segments of V: 128 channels (lane i reads word i, 8 channels), then 64
-// (word i / 2, 4 channels) and 32 (word i / 4, 2 channels) for the rest of W.
-template <int W>
-struct Segments {
-    static constexpr int wide = W / 4, rest = W & 3;
-    static constexpr int count = wide + (rest ? rest == 3 ? 2 : 1 : 0);
-    static constexpr int size(int s) { return s < wide ? 8 : s == wide && rest >= 2 ? 4 : 2; }  // channels a lane
-    static constexpr int word(int s) { return s <= wide ? 16 * s : 16 * wide + 8; }             // first word
-    static constexpr int tile(int s) { return s <= wide ? 8 * s : 8 * wide + 4; }               // first result tile
+// What a wave keeps of its query rows: 16 a tile, lane (i, j) of row i.
+template <int W, int P, int NR>
+struct State {
+    static constexpr int NT = 2 * W;
+    int hi[NR], lo[NR];  // the positions that the lane's row sees
+    bf16x8 q[NR][P][W];
+    float mx[NR], sum[NR];  // the weights' reference (log2 domain) and the lane's share of their sum
+    f32x4 o[NR][NT];        // channels 4 j + r of tile n, in Segments' order
 };
+
+template <int W>
+__device__ __forceinline__ Entry entries(const AttnArgs& a, uint32_t b, int blk, int i, int j) {
+    const uint32_t shift = a.cache.page_shift, last = (uint32_t)a.seqs.cols - 1;
+    const int32_t* row = a.seqs.table + (int64_t)b * a.seqs.cols;
+    const uint32_t kc = ((uint32_t)blk * 32 + 8 * (i >> 2)) >> shift, vc = ((uint32_t)blk * 32 + 8 * j) >> shift;
+    Entry e;
+    e.k = (uint32_t)row[min(kc, last)];
+    e.v = (uint32_t)row[min(vc, last)];
+    if (kc > last) e.k = ~0u;
+    return e;
+}
+
+template <int W>
+__device__ __forceinline__ void fetch(const AttnArgs& a, uint32_t h, int blk, Entry e, int i, int j, Block<W>& x) {
+    using S = Segments<W>;
+    const uint32_t shift = a.cache.page_shift, mask = (1u << shift) - 1u;
+    x.ok = e.k < a.cache.pages;
+    const uint32_t kp = x.ok ? e.k : 0u, vp = e.v < a.cache.pages ? e.v : 0u;
+    const uint64_t kt = (((uint64_t)kp * a.cache.heads + h) << shift) + (((uint32_t)blk * 32 + 8 * (i >> 2)) & mask) + (i & 3);
+    const uint64_t vt = (((uint64_t)vp * a.cache.heads + h) << shift) + (((uint32_t)blk * 32 + 8 * j) & mask);
+    const int g0 = (W * j) >> 2, g1 = (W * j + W - 1) >> 2;
+    const uint32_t* kc = a.cache.k_codes + kt * (4 * W) + W * j;
+    const uint8_t* ks = a.cache.k_scales + kt * W;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        __builtin_memcpy(x.k[s], kc + 4 * s * (4 * W), 4 * W);
+        x.ks[s][0] = ks[4 * s * W + g0];
+        if (W != 2 && W != 4) x.ks[s][1] = ks[4 * s * W + g1];
+    }
+    const uint32_t* vc = a.cache.v_codes + vt * (4 * W);
+    const uint8_t* vs = static_cast<const uint8_t*>(__builtin_assume_aligned(a.cache.v_scales + vt * W, 8));
+#pragma unroll
+    for (int s = 0; s < S::count; ++s) {
+        const int w = S::word(s) + (i * 2 * S::size(s) >> 4);
+        __builtin_memcpy(x.v[s], vc + 8 * w, 32);
+        __builtin_memcpy(x.vs[s], __builtin_assume_aligned(vs + 8 * (w >> 2), 8), 8);
+    }
+}
+
+// Where some row does not see some token of the block. A weight of 0 does not
+// hide a NaN in the product: values of no sequence and NaN blocks go as zeros,
+// and the NaN blocks' channels become NaN in the rows that see one (an
+// indicator's product says which).
+template <int W, int P, int NR>
+__device__ __forceinline__ void hide_values(State<W, P, NR>& st, Block<W>& x, int t0, int hi_all) {
+    using S = Segments<W>;
+    bool nan = false;
+#pragma unroll
+    for (int s = 0; s < S::count; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t byte = (x.vs[s][e >> 2] >> (8 * (e & 3))) & 255u;
+            const bool out = t0 + e >= hi_all;
+            nan |= !out && byte == 255u;
+            if (out || byte == 255u) x.v[s][e] = 0;
+            if (out) x.vs[s][e >> 2] &= ~(255u << (8 * (e & 3)));
+        }
+    if (!__any(nan)) return;
+#pragma unroll
+    for (int s = 0; s < S::count; ++s) {
+        bf16x8 is;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool n = ((x.vs[s][e >> 2] >> (8 * (e & 3))) & 255u) == 255u;
+            is[e] = n ? (__bf16)1.f : (__bf16)0.f;
+            if (n) x.vs[s][e >> 2] &= ~(255u << (8 * (e & 3)));
+        }
+#pragma unroll
+        for (int t = 0; t < NR; ++t) {
+            bf16x8 seen;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) seen[e] = t0 + e >= st.lo[t] && t0 + e < st.hi[t] ? (__bf16)1.f : (__bf16)0.f;
+            const f32x4 n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(is, seen, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+            for (int c = 0; c < S::size(s); ++c)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (n[r] > 0.f) st.o[t][S::tile(s) + c][r] = NAN;
+        }
+    }
+}
+
+// A block's part of the rows' results.
+template <int W, int P, int NR>
+__device__ __forceinline__ void attend_block(State<W, P, NR>& st, Block<W>& x, float scale, int blk, int i, int j, bool part,
+                                             int hi_all) {
+    using S = Segments<W>;
+    const int t0 = blk * 32 + 8 * j;  // this lane's scores are of tokens t0 .. t0 + 7
+
+    // scores: S^T = K Q^T
+    f32x4 sc[NR][2];
+#pragma unroll
+    for (int t = 0; t < NR; ++t) sc[t][0] = sc[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        const float e0 = scale_of<0>(x.ok ? x.ks[s][0] : 255u);
+        const float e1 = W == 2 || W == 4 ? e0 : scale_of<0>(x.ok ? x.ks[s][1] : 255u);
+#pragma unroll
+        for (int c = 0; c < W; ++c) {
+            const float e = W == 8 ? (c < 4 ? e0 : e1) : W == 2 || W == 4 ? e0 : ((W * j + c) >> 2) == ((W * j) >> 2) ? e0 : e1;
+            const u32x4 f = {pair_of<0>(x.k[s][c], e), pair_of<1>(x.k[s][c], e), pair_of<2>(x.k[s][c], e),
+                             pair_of<3>(x.k[s][c], e)};
+            const bf16x8 kf = __builtin_bit_cast(bf16x8, f);
+#pragma unroll
+            for (int t = 0; t < NR; ++t)
+#pragma unroll
+                for (int p = 0; p < P; ++p)
+                    sc[t][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, st.q[t][p][c], sc[t][s], 0, 0, 0);
+        }
+    }
+
+    // softmax: the reference mx follows the maximum only when a score passes it
+    // by 2^8, so that most blocks need no product over the lanes and no
+    // rescaling; weights up to 2^8 cost no precision
+    bf16x8 pf[NR][P];
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = sc[t][e >> 2][e & 3];
+        if (part) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (t0 + e < st.lo[t] || t0 + e >= st.hi[t]) p[e] = -INFINITY;
+        }
+        float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7]))) * scale;
+        if (__any(top > st.mx[t] + 8.f)) {
+            top = fmaxf(st.mx[t], max_over_j(top));
+            const float alpha = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.mx[t] - top);
+            st.sum[t] *= alpha;
+#pragma unroll
+            for (int c = 0; c < 2 * W; ++c) st.o[t][c] *= alpha;
+            st.mx[t] = top;
+        }
+        const float base = st.mx[t] == -INFINITY ? 0.f : -st.mx[t];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], scale, base));
+            st.sum[t] += p[e];
+        }
+        pieces<P>(p, pf[t]);
+    }
+
+    if (part) hide_values(st, x, t0, hi_all);
+
+    // O^T += V^T P^T
+#pragma unroll
+    for (int s = 0; s < S::count; ++s) {
+        const uint32_t a = x.vs[s][0], b = x.vs[s][1];
+        const float e[8] = {scale_of<0>(a), scale_of<1>(a), scale_of<2>(a), scale_of<3>(a),
+                            scale_of<0>(b), scale_of<1>(b), scale_of<2>(b), scale_of<3>(b)};
+        uint32_t w[8];
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+            w[n] = S::size(s) == 8 ? x.v[s][n] : S::size(s) == 4 ? x.v[s][n] >> (16 * (i & 1)) : x.v[s][n] >> (8 * (i & 3));
+#pragma unroll
+        for (int c = 0; c < S::size(s); c += 2) {
+            u32x4 even, odd;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const uint32_t u = pair_at(c / 2, w[2 * n], e[2 * n]), v = pair_at(c / 2, w[2 * n + 1], e[2 * n + 1]);
+                even[n] = __builtin_amdgcn_perm(v, u, 0x05040100u);
+                odd[n] = __builtin_amdgcn_perm(v, u, 0x07060302u);
+            }
+            const bf16x8 ve = __builtin_bit_cast(bf16x8, even), vo = __builtin_bit_cast(bf16x8, odd);
+            const int n = S::tile(s) + c;
+#pragma unroll
+            for (int t = 0; t < NR; ++t)
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    st.o[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ve, pf[t][p], st.o[t][n], 0, 0, 0);
+                    st.o[t][n + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vo, pf[t][p], st.o[t][n + 1], 0, 0, 0);
+                }
+        }
+    }
+}
 
 // W: dim / 32. P: bf16 pieces of the queries and weights (1: bf16, 3: fp32).
 // NR: tiles of 16 query rows a wave. ROWS: the workgroup's waves take rows of
 // their own and every token; else they share the rows and deal the tokens.
+// Registers: two waves a SIMD where 256 of them do.
 template <int W, int P, int NR, bool ROWS>
-__global__ __launch_bounds__(64 * kAttnWaves) void k_attend(const AttnArgs a) {
+__global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) void k_attend(const AttnArgs a) {
     using S = Segments<W>;
     constexpr int D = 32 * W, NT = D / 16;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -117,214 +323,77 @@ __global__ __launch_bounds__(64 * kAttnWaves) void k_attend(const AttnArgs a) {
     const int blk_lo = lo_all >> 5, blk_hi = hi_all > lo_all ? (hi_all + 31) >> 5 : blk_lo;
     const int per = (blk_hi - blk_lo + (int)a.splits - 1) / (int)a.splits;
     const int blk_first = blk_lo + (int)split * per, blk_end = min(blk_first + per, blk_hi);
+    constexpr int step = ROWS ? 1 : kAttnWaves;
+    int blk = blk_first + (ROWS ? 0 : (int)wave);
 
-    // this lane's row of each tile
-    int hi[NR], lo[NR];
+    // Loads run ahead of their use: page numbers two blocks, a block's codes one.
+    Block<W> x[2];
+    Entry e[2] = {};
+    if (blk < blk_end) {
+        e[0] = entries<W>(a, b, blk, i, j);
+        e[1] = entries<W>(a, b, blk + step, i, j);
+    }
+
+    State<W, P, NR> st;
     int64_t row_out[NR];  // (token, head) in the output, -1: no row
-    bf16x8 qf[NR][P][W];
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
         const int r = r0 + 16 * t + i;
         const bool ok = r < rows;
         const int m = ok ? r / (int)a.group : 0, g = ok ? r - m * (int)a.group : 0;
-        hi[t] = ok ? hi_of(m) : 0;
-        lo[t] = lo_of(m);
+        st.hi[t] = ok ? hi_of(m) : 0;
+        st.lo[t] = lo_of(m);
         const int64_t token = q.token + m, head = (int64_t)h * a.group + g;
         row_out[t] = ok ? token * a.q_heads + head : -1;
         const int64_t at = token * a.q_token + head * a.q_head + 8 * W * j;
 #pragma unroll
         for (int c = 0; c < W; ++c) {
             if constexpr (P == 1) {
-                u32x4 x = {0, 0, 0, 0};
-                if (ok) __builtin_memcpy(&x, static_cast<const uint16_t*>(a.q) + at + 8 * c, 16);
-                qf[t][0][c] = __builtin_bit_cast(bf16x8, x);
+                u32x4 f = {0, 0, 0, 0};
+                if (ok) __builtin_memcpy(&f, static_cast<const uint16_t*>(a.q) + at + 8 * c, 16);
+                st.q[t][0][c] = __builtin_bit_cast(bf16x8, f);
             } else {
-                float x[8];
-                for (int e = 0; e < 8; ++e) x[e] = ok ? static_cast<const float*>(a.q)[at + 8 * c + e] : 0.f;
-                bf16x8 f[P];
-                pieces<P>(x, f);
+                float f[8];
+                for (int n = 0; n < 8; ++n) f[n] = ok ? static_cast<const float*>(a.q)[at + 8 * c + n] : 0.f;
+                bf16x8 split_f[P];
+                pieces<P>(f, split_f);
 #pragma unroll
-                for (int p = 0; p < P; ++p) qf[t][p][c] = f[p];
+                for (int p = 0; p < P; ++p) st.q[t][p][c] = split_f[p];
             }
         }
+        st.mx[t] = -INFINITY;
+        st.sum[t] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NT; ++c) st.o[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    float mx[NR], sum[NR];
-    f32x4 o[NR][NT];
-#pragma unroll
-    for (int t = 0; t < NR; ++t) {
-        mx[t] = -INFINITY;
-        sum[t] = 0.f;
-#pragma unroll
-        for (int c = 0; c < NT; ++c) o[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-
-    const int g0 = (W * j) >> 2, g1 = (W * j + W - 1) >> 2;  // the blocks of this lane's first and last word of K
-    const int step = ROWS ? 1 : kAttnWaves;
-    for (int blk = blk_first + (ROWS ? 0 : (int)wave); blk < blk_end; blk += step) {
-        Block<W> x;
-        bool bad;
-        {
-            const Slot ko = slot_of(a.cache, a.seqs, b, h, (uint32_t)blk * 32 + 8 * (i >> 2));
-            const Slot vo = slot_of(a.cache, a.seqs, b, h, (uint32_t)blk * 32 + 8 * j);
-            bad = !ko.ok;
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const uint64_t token = ko.token + 4 * s + (i & 3);
-                __builtin_memcpy(x.k[s], a.cache.k_codes + token * (D / 8) + W * j, 4 * W);
-                x.ks[s][0] = a.cache.k_scales[token * W + g0];
-                x.ks[s][1] = g1 != g0 ? a.cache.k_scales[token * W + g1] : x.ks[s][0];
-            }
-#pragma unroll
-            for (int s = 0; s < S::count; ++s) {
-                const int lanes = 16 * S::size(s) / 8;  // words of the segment
-                const int w = S::word(s) + i * lanes / 16;
-                __builtin_memcpy(x.v[s], a.cache.v_codes + vo.token * (D / 8) + 8 * w, 32);
-                __builtin_memcpy(x.vs[s], a.cache.v_scales + vo.token * W + 8 * (w >> 2), 8);
-            }
-        }
-        const int t0 = blk * 32 + 8 * j;  // this lane's scores are of tokens t0 .. t0 + 7
+    const auto work = [&](Block<W>& y) {
         const bool part = blk * 32 < full_lo || blk * 32 + 32 > full_hi;
-        const bool any_bad = __any(bad);
-
-        // ------------------------------------------------ scores: S^T = K Q^T
-        f32x4 sc[NR][2];
-#pragma unroll
-        for (int t = 0; t < NR; ++t) sc[t][0] = sc[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            if (any_bad && bad) x.ks[s][0] = x.ks[s][1] = 255;
-            const float e0 = scale_of(x.ks[s][0]), e1 = scale_of(x.ks[s][1]);
-#pragma unroll
-            for (int c = 0; c < W; ++c) {
-                const float e = ((W * j + c) >> 2) == g0 ? e0 : e1;
-                const u32x4 f = {pair_of<0>(x.k[s][c], e), pair_of<1>(x.k[s][c], e), pair_of<2>(x.k[s][c], e),
-                                 pair_of<3>(x.k[s][c], e)};
-                const bf16x8 kf = __builtin_bit_cast(bf16x8, f);
-#pragma unroll
-                for (int t = 0; t < NR; ++t)
-#pragma unroll
-                    for (int p = 0; p < P; ++p)
-                        sc[t][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[t][p][c], sc[t][s], 0, 0, 0);
+        attend_block(st, y, a.scale, blk, i, j, part, hi_all);
+        blk += step;
+    };
+    if (blk < blk_end) {
+        fetch(a, h, blk, e[0], i, j, x[0]);
+        for (;;) {
+            const bool more = blk + step < blk_end;
+            if (more) {
+                fetch(a, h, blk + step, e[1], i, j, x[1]);
+                e[0] = entries<W>(a, b, blk + 2 * step, i, j);
             }
-        }
-
-        // ------------------------------------------------------------ softmax
-        bf16x8 pf[NR][P];
-#pragma unroll
-        for (int t = 0; t < NR; ++t) {
-            float p[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = sc[t][e >> 2][e & 3] * a.scale;
-            if (part) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (t0 + e < lo[t] || t0 + e >= hi[t]) p[e] = -INFINITY;
+            work(x[0]);
+            if (!more) break;
+            const bool again = blk + step < blk_end;
+            if (again) {
+                fetch(a, h, blk + step, e[0], i, j, x[0]);
+                e[1] = entries<W>(a, b, blk + 2 * step, i, j);
             }
-            float top = p[0];
-#pragma unroll
-            for (int e = 1; e < 8; ++e) top = fmaxf(top, p[e]);
-            top = fmaxf(mx[t], max_over_j(top));
-            if (__any(top > mx[t])) {
-                const float alpha = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx[t] - top);
-                sum[t] *= alpha;
-#pragma unroll
-                for (int c = 0; c < NT; ++c) o[t][c] *= alpha;
-                mx[t] = top;
-            }
-            const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                p[e] = __builtin_amdgcn_exp2f(p[e] - base);
-                sum[t] += p[e];
-            }
-            pieces<P>(p, pf[t]);
-        }
-
-        // A weight of 0 does not hide a NaN in the product. Where some row does
-        // not see some token of the block, values of no sequence and NaN blocks
-        // go as zeros, and the NaN blocks' channels become NaN in the rows that
-        // see one (an indicator's product says which).
-        if (part) {
-            bool nan = false;
-#pragma unroll
-            for (int s = 0; s < S::count; ++s)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint32_t byte = (x.vs[s][e >> 2] >> (8 * (e & 3))) & 255u;
-                    const bool out = t0 + e >= hi_all;
-                    nan |= !out && byte == 255u;
-                    if (out || byte == 255u) x.v[s][e] = 0;
-                    if (out) x.vs[s][e >> 2] &= ~(255u << (8 * (e & 3)));
-                }
-            if (__any(nan)) {
-#pragma unroll
-                for (int t = 0; t < NR; ++t) {
-                    bf16x8 seen;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) seen[e] = t0 + e >= lo[t] && t0 + e < hi[t] ? (__bf16)1.f : (__bf16)0.f;
-#pragma unroll
-                    for (int s = 0; s < S::count; ++s) {
-                        bf16x8 is;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            is[e] = ((x.vs[s][e >> 2] >> (8 * (e & 3))) & 255u) == 255u ? (__bf16)1.f : (__bf16)0.f;
-                        const f32x4 n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(is, seen, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-#pragma unroll
-                        for (int c = 0; c < S::size(s); ++c)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                if (n[r] > 0.f) o[t][S::tile(s) + c][r] = NAN;
-                    }
-                }
-#pragma unroll
-                for (int s = 0; s < S::count; ++s)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (((x.vs[s][e >> 2] >> (8 * (e & 3))) & 255u) == 255u) x.vs[s][e >> 2] &= ~(255u << (8 * (e & 3)));
-            }
-        }
-
-        // ------------------------------------------------------ O^T += V^T P^T
-#pragma unroll
-        for (int s = 0; s < S::count; ++s) {
-            float e[8];
-#pragma unroll
-            for (int n = 0; n < 8; ++n) e[n] = scale_of((x.vs[s][n >> 2] >> (8 * (n & 3))) & 255u);
-            uint32_t w[8];
-#pragma unroll
-            for (int n = 0; n < 8; ++n)
-                w[n] = S::size(s) == 8 ? x.v[s][n] : S::size(s) == 4 ? x.v[s][n] >> (16 * (i & 1)) : x.v[s][n] >> (8 * (i & 3));
-#pragma unroll
-            for (int c = 0; c < S::size(s); c += 2) {
-                u32x4 even, odd;
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    uint32_t u, v;
-                    switch (c) {
-                        case 0: u = pair_of<0>(w[2 * n], e[2 * n]), v = pair_of<0>(w[2 * n + 1], e[2 * n + 1]); break;
-                        case 2: u = pair_of<1>(w[2 * n], e[2 * n]), v = pair_of<1>(w[2 * n + 1], e[2 * n + 1]); break;
-                        case 4: u = pair_of<2>(w[2 * n], e[2 * n]), v = pair_of<2>(w[2 * n + 1], e[2 * n + 1]); break;
-                        default: u = pair_of<3>(w[2 * n], e[2 * n]), v = pair_of<3>(w[2 * n + 1], e[2 * n + 1]); break;
-                    }
-                    even[n] = __builtin_amdgcn_perm(v, u, 0x05040100u);
-                    odd[n] = __builtin_amdgcn_perm(v, u, 0x07060302u);
-                }
-                const bf16x8 ve = __builtin_bit_cast(bf16x8, even), vo = __builtin_bit_cast(bf16x8, odd);
-                const int n = S::tile(s) + c;
-#pragma unroll
-                for (int t = 0; t < NR; ++t)
-#pragma unroll
-                    for (int p = 0; p < P; ++p) {
-                        o[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ve, pf[t][p], o[t][n], 0, 0, 0);
-                        o[t][n + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vo, pf[t][p], o[t][n + 1], 0, 0, 0);
-                    }
-            }
+            work(x[1]);
+            if (!again) break;
         }
     }
 
 #pragma unroll
-    for (int t = 0; t < NR; ++t) sum[t] = sum_over_j(sum[t]);
+    for (int t = 0; t < NR; ++t) st.sum[t] = sum_over_j(st.sum[t]);
 
     // the waves' results into wave 0's: 3 to 1 and 2 to 0, then 1 to 0
     if constexpr (!ROWS) {
@@ -333,8 +402,8 @@ __global__ __launch_bounds__(64 * kAttnWaves) void k_attend(const AttnArgs a) {
         if (j == 0) {
 #pragma unroll
             for (int t = 0; t < NR; ++t) {
-                stat[wave][t][i][0] = mx[t];
-                stat[wave][t][i][1] = sum[t];
+                stat[wave][t][i][0] = st.mx[t];
+                stat[wave][t][i][1] = st.sum[t];
             }
         }
         __syncthreads();
@@ -347,109 +416,126 @@ __global__ __launch_bounds__(64 * kAttnWaves) void k_attend(const AttnArgs a) {
 #pragma unroll
             for (int w = 0; w < kAttnWaves; ++w)
                 total += stat[w][t][i][1] * __builtin_amdgcn_exp2f(stat[w][t][i][0] - base);
-            const float own = __builtin_amdgcn_exp2f(mx[t] - base);
+            const float own = __builtin_amdgcn_exp2f(st.mx[t] - base);
 #pragma unroll
-            for (int c = 0; c < NT; ++c) o[t][c] *= own;
-            mx[t] = top;
-            sum[t] = total;
+            for (int c = 0; c < NT; ++c) st.o[t][c] *= own;
+            st.mx[t] = top;
+            st.sum[t] = total;
         }
 #pragma unroll
         for (int t = 0; t < NR; ++t) {
             if (wave >= 2)
 #pragma unroll
-                for (int c = 0; c < NT; ++c) buf[wave - 2][c][lane] = o[t][c];
+                for (int c = 0; c < NT; ++c) buf[wave - 2][c][lane] = st.o[t][c];
             __syncthreads();
             if (wave < 2)
 #pragma unroll
-                for (int c = 0; c < NT; ++c) o[t][c] += buf[wave][c][lane];
+                for (int c = 0; c < NT; ++c) st.o[t][c] += buf[wave][c][lane];
             if (wave == 1)
 #pragma unroll
-                for (int c = 0; c < NT; ++c) buf[1][c][lane] = o[t][c];
+                for (int c = 0; c < NT; ++c) buf[1][c][lane] = st.o[t][c];
             __syncthreads();
             if (wave == 0)
 #pragma unroll
-                for (int c = 0; c < NT; ++c) o[t][c] += buf[1][c][lane];
+                for (int c = 0; c < NT; ++c) st.o[t][c] += buf[1][c][lane];
             __syncthreads();
         }
         if (wave != 0) return;
     }
 
     const int64_t all = (int64_t)a.seqs.total * a.q_heads;
+    const bool done = a.splits == 1;
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
         if (row_out[t] < 0) continue;
-        if (hi[t] > cap) sum[t] = NAN;  // it sees positions that the table has no page for
-        const bool done = a.splits == 1;
-        const float inv = !done || sum[t] == 0.f ? 1.f : 1.f / sum[t];
+        float sum = st.sum[t];
+        if (st.hi[t] > cap) sum = NAN;  // it sees positions that the table has no page for
+        const float inv = !done || sum == 0.f ? 1.f : 1.f / sum;
         if (j == 0) {
             if (!done)
-                a.part_ml[split * all + row_out[t]] = make_float2(mx[t], sum[t]);
+                a.part_ml[split * all + row_out[t]] = make_float2(st.mx[t], sum);
             else if (a.lse)
-                a.lse[row_out[t]] = sum[t] == 0.f ? -INFINITY : (mx[t] + __builtin_amdgcn_logf(sum[t])) * 0.693147180559945309f;
+                a.lse[row_out[t]] = sum == 0.f ? -INFINITY : (st.mx[t] + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f;
         }
 #pragma unroll
-        for (int s = 0; s < S::count; ++s) {
-            constexpr int most = 8;
+        for (int s = 0; s < S::count; ++s)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int size = S::size(s), at = 8 * S::word(s) + size * (4 * j + r);
-                float y[most];
+                float y[8];
 #pragma unroll
-                for (int c = 0; c < size; ++c) y[c] = o[t][S::tile(s) + c][r] * inv;
+                for (int c = 0; c < size; ++c) y[c] = done && sum != sum ? NAN : st.o[t][S::tile(s) + c][r] * inv;
                 if (!done) {
                     float* to = a.part_o + (split * all + row_out[t]) * D + at;
 #pragma unroll
                     for (int c = 0; c < size; ++c) to[c] = y[c];
+                } else if constexpr (P == 1) {
+                    uint16_t* to = static_cast<uint16_t*>(a.out) + row_out[t] * D + at;
+#pragma unroll
+                    for (int c = 0; c < size; ++c) to[c] = __builtin_bit_cast(uint16_t, (__bf16)y[c]);
                 } else {
-                    if (sum[t] != sum[t])
+                    float* to = static_cast<float*>(a.out) + row_out[t] * D + at;
 #pragma unroll
-                        for (int c = 0; c < size; ++c) y[c] = NAN;
-                    if constexpr (P == 1) {
-                        uint16_t* to = static_cast<uint16_t*>(a.out) + row_out[t] * D + at;
-#pragma unroll
-                        for (int c = 0; c < size; ++c) to[c] = __builtin_bit_cast(uint16_t, (__bf16)y[c]);
-                    } else {
-                        float* to = static_cast<float*>(a.out) + row_out[t] * D + at;
-#pragma unroll
-                        for (int c = 0; c < size; ++c) to[c] = y[c];
-                    }
+                    for (int c = 0; c < size; ++c) to[c] = y[c];
                 }
             }
-        }
     }
 }
 
-// The splits' results joined: a wave a row, in the order of the splits.
+// The splits' results joined, in the order of the splits. A row is a wave's, or
+// with `ways` 4 a workgroup's: lane n of a wave weighs split n (64 at most),
+// then dim / 4 lanes add a split's row, 16 bytes a lane, as many splits at a
+// time as lanes allow, and the partial sums meet at the end.
 template <bool F32>
-__global__ __launch_bounds__(256) void k_attend_join(const AttnArgs a, uint32_t dim) {
+__global__ __launch_bounds__(256) void k_attend_join(const AttnArgs a, int dim, int ways) {
+    __shared__ f32x4 part[3][64];
     const int64_t all = (int64_t)a.seqs.total * a.q_heads;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const uint32_t lane = threadIdx.x & 63u;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = ways == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
     if (row >= all) return;
-    float top = -INFINITY;
-    for (uint32_t s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[s * all + row].x);
-    const float base = top == -INFINITY ? 0.f : top;
-    float total = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t s = 0; s < a.splits; ++s) {
-        const float2 ml = a.part_ml[s * all + row];
-        if (ml.y == 0.f) continue;  // nothing seen there
-        const float w = __builtin_amdgcn_exp2f(ml.x - base);
-        total += ml.y * w;
-        const float* from = a.part_o + (s * all + row) * dim;
+    const int splits = (int)a.splits, per = dim / 4, groups = 64 / per;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < splits) ml = a.part_ml[lane * all + row];
+    float top = ml.x;
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
-            if (lane + 64 * n < dim) y[n] += from[lane + 64 * n] * w;
+    for (int n = 32; n; n >>= 1) top = fmaxf(top, __shfl_xor(top, n));
+    const float weight = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
+    float total = ml.y * weight;
+    if (ml.y != ml.y) total = NAN;
+#pragma unroll
+    for (int n = 32; n; n >>= 1) total += __shfl_xor(total, n);
+
+    const int group = lane / per, col = lane - group * per;
+    const int stride = groups * (ways == 4 ? 4 : 1);
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    const f32x4* from = reinterpret_cast<const f32x4*>(a.part_o + row * dim) + col;
+#pragma unroll 4
+    for (int s = (ways == 4 ? wave * groups : 0) + group; s < splits + group; s += stride) {  // (the same count in every lane)
+        const float w = __shfl(weight, s);
+        if (group < groups && s < splits && w != 0.f) y += from[s * (all * per)] * w;
+    }
+    f32x4 sum = y;
+    for (int g = 1; g < groups; ++g)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) sum[n] += __shfl(y[n], (lane + g * per) & 63);
+    if (ways == 4) {
+        if (wave) part[wave - 1][lane] = sum;
+        __syncthreads();
+        if (wave) return;
+        sum += part[0][lane] + part[1][lane] + part[2][lane];
     }
     const float inv = total == 0.f ? 1.f : 1.f / total;
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-        if (lane + 64 * n < dim) {
-            const float v = total != total ? NAN : y[n] * inv;
-            if constexpr (F32)
-                static_cast<float*>(a.out)[row * dim + lane + 64 * n] = v;
-            else
-                static_cast<uint16_t*>(a.out)[row * dim + lane + 64 * n] = __builtin_bit_cast(uint16_t, (__bf16)v);
+    if (lane < per) {
+        f32x4 v = sum * inv;
+        if (total != total) v = f32x4{NAN, NAN, NAN, NAN};
+        if constexpr (F32) {
+            reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + row * dim)[lane] = v;
+        } else {
+            typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+            const bf16x4 r = __builtin_convertvector(v, bf16x4);
+            reinterpret_cast<bf16x4*>(static_cast<uint16_t*>(a.out) + row * dim)[lane] = r;
         }
+    }
     if (a.lse && lane == 0)
         a.lse[row] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * 0.693147180559945309f;
 }

@@ -607,7 +607,7 @@ Plan plan_of(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t q_heads, int 
     if (max_length) length = std::min<uint64_t>(length, max_length);
     if (window) length = std::min<uint64_t>(length, (uint64_t)window + tokens + 31);
     const uint64_t groups = (uint64_t)c->heads * s->batch * std::max(1u, p.row_blocks);
-    const uint64_t wanted = (1024 + groups - 1) / groups, possible = std::max<uint64_t>(1, length / 128);
+    const uint64_t wanted = p.rows ? 256 / groups : (1024 + groups - 1) / groups, possible = length / 128;
     p.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({wanted, possible, 64, 65535 / s->batch}));
     return p;
 }
@@ -683,7 +683,8 @@ extern "C" int dmx_kv_attention(const dmx_kv_cache* cache, const dmx_kv_seqs* se
     }
     if (launch_check(err, errn, "kv attention launch")) return 1;
     if (p.splits == 1) return 0;
-    hipLaunchKernelGGL((dtype == DMX_F32 ? k_attend_join<true> : k_attend_join<false>), dim3((uint32_t)((all + 3) / 4)),
-                       dim3(256), 0, st, a, cache->dim);
+    const int ways = p.splits > 8 ? 4 : 1;
+    hipLaunchKernelGGL((dtype == DMX_F32 ? k_attend_join<true> : k_attend_join<false>),
+                       dim3((uint32_t)(ways == 4 ? all : (all + 3) / 4)), dim3(256), 0, st, a, (int)cache->dim, ways);
     return launch_check(err, errn, "kv attention join launch");
 }

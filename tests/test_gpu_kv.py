@@ -366,8 +366,8 @@ def test_positions_without_a_page():
     got = kv_ops.attention(q, b.cache, t, b.lengths, window=20)  # none of the rows sees it
     check_attention(b, held, q, "bf16", got, None, True, 20)
     got = f64(kv_ops.attention(q, b.cache, b.block_table, i32([60, 2 ** 31 - 1, 65])))  # longer than the table
-    # (the third's first row, at position 63, sees the table's 64 positions and no more)
-    assert np.isfinite(got[[0, 1, 4]]).all() and np.isnan(got[[2, 3, 5]]).all()
+    # (the third's first row, at position 63, sees the table's 64 positions and no more: the last of them noise here)
+    assert np.isfinite(got[:2]).all() and np.isnan(got[[2, 3, 5]]).all()
 
 
 def test_attention_reads_views():
