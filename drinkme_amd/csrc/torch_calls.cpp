@@ -1,5 +1,6 @@
-// The per-call path of the torch launchers (drinkme_amd/radix_ops.py) as a
-// CPython extension: one call checks the activation, allocates the output
+// The per-call path of the torch launchers (drinkme_amd/radix_ops.py) and of
+// the key/value cache's operators (drinkme_amd/kv_ops.py) as a CPython
+// extension: one call checks the activation, allocates the output
 // with torch and launches through the C ABI. What bounds a decode step's
 // small calls is the host: through ctypes and Python's own checks a call of
 // one Linear took 10.1 us on the host for a 5.5 us kernel (k_proj of 1024 x
@@ -15,12 +16,15 @@
 
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
+#include <ATen/core/grad_mode.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <string>
 
+#include "dmx_kv.h"
 #include "dmx_radix.h"
 
 namespace {
@@ -200,6 +204,258 @@ PyObject* narrow(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------- the key/value cache's operators --
+//
+// As above: the plain case or None. Plain here: tensors of the types, shapes
+// and device that kv_ops documents, activations with adjacent channels, nothing
+// that asks for a gradient.
+
+constexpr int64_t kMost = 1ll << 30;
+
+// A dense tensor of `dtype` and `dims` dimensions on device `index`.
+const at::Tensor* dense(PyObject* o, at::ScalarType dtype, int64_t dims, int64_t index) {
+    const at::Tensor* t = exact(o);
+    return t && plain(*t) && t->scalar_type() == dtype && t->dim() == dims && t->get_device() == index ? t : nullptr;
+}
+
+// x [tokens, heads, dim], any strides but for adjacent channels.
+bool rows_at(PyObject* o, const at::Tensor*& x, dmx_rows& r) {
+    using K = c10::DispatchKey;
+    x = exact(o);
+    if (!x || !x->defined() || !x->is_cuda() || x->layout() != at::kStrided || !x->has_storage() || x->dim() != 3 ||
+        x->key_set().has_any(c10::DispatchKeySet({K::FuncTorchBatched, K::FuncTorchGradWrapper, K::Functionalize,
+                                                  K::Python, K::Negative, K::Conjugate, K::ZeroTensor})))
+        return false;
+    if (code(x->scalar_type()) < 0 || x->stride(2) != 1 || x->size(0) >= kMost || x->size(1) >= kMost ||
+        (x->requires_grad() && at::GradMode::is_enabled()))
+        return false;
+    r = {const_cast<void*>(x->const_data_ptr()), x->stride(0), x->stride(1), (uint32_t)x->size(1)};
+    return true;
+}
+
+bool like(const at::Tensor& a, const at::Tensor& b) {
+    return a.scalar_type() == b.scalar_type() && a.get_device() == b.get_device() && a.size(0) == b.size(0) &&
+           a.size(2) == b.size(2);
+}
+
+dmx_rows dense_rows(const at::Tensor& t) {
+    return {t.mutable_data_ptr(), t.size(1) * t.size(2), t.size(2), (uint32_t)t.size(1)};
+}
+
+bool table_of(PyObject* o, long layout, int64_t dim, int64_t index, dmx_rotary_table& r) {
+    const at::Tensor* t = dense(o, at::kFloat, 3, index);
+    if (!t || t->size(2) != 2 || 2 * t->size(1) > dim || t->size(0) >= kMost) return false;
+    r = {static_cast<const float*>(t->const_data_ptr()), (uint32_t)t->size(0), (uint32_t)(2 * t->size(1)), (int)layout};
+    return true;
+}
+
+PyObject* g_cache[4];  // "k_codes", "k_scales", "v_codes", "v_scales"
+bool cache_of(PyObject* o, dmx_kv_cache& c, int64_t& index) {
+    if (!PyDict_Check(o)) return false;
+    const at::Tensor* t[4];
+    for (int n = 0; n < 4; ++n) {
+        PyObject* v = PyDict_GetItem(o, g_cache[n]);  // borrowed
+        t[n] = v ? exact(v) : nullptr;
+        if (!t[n] || !plain(*t[n]) || t[n]->scalar_type() != (n % 2 ? at::kByte : at::kInt) || t[n]->dim() != (n < 2 ? 4 : 5) ||
+            t[n]->get_device() != t[0]->get_device())
+            return false;
+    }
+    const int64_t pages = t[0]->size(0), heads = t[0]->size(1), page = t[0]->size(2), words = t[0]->size(3);
+    if (pages >= kMost || heads >= kMost || page >= kMost || words >= kMost ||
+        t[1]->sizes() != at::IntArrayRef({pages, heads, page, words / 4}) ||
+        t[2]->sizes() != at::IntArrayRef({pages, heads, page / 8, words, 8}) ||
+        t[3]->sizes() != at::IntArrayRef({pages, heads, page / 8, words / 4, 8}))
+        return false;
+    index = t[0]->get_device();
+    c.k_codes = static_cast<uint32_t*>(t[0]->mutable_data_ptr());
+    c.k_scales = static_cast<uint8_t*>(t[1]->mutable_data_ptr());
+    c.v_codes = static_cast<uint32_t*>(t[2]->mutable_data_ptr());
+    c.v_scales = static_cast<uint8_t*>(t[3]->mutable_data_ptr());
+    c.pages = (uint32_t)pages, c.heads = (uint32_t)heads, c.page = (uint32_t)page, c.dim = (uint32_t)(8 * words);
+    return true;
+}
+
+bool seqs_of(PyObject* table, PyObject* lengths, PyObject* cu, int64_t total, int64_t max_tokens, int64_t index,
+             dmx_kv_seqs& s) {
+    const at::Tensor *t = dense(table, at::kInt, 2, index), *l = dense(lengths, at::kInt, 1, index);
+    const at::Tensor* c = cu == Py_None ? nullptr : dense(cu, at::kInt, 1, index);
+    if (!t || !l || (cu != Py_None && !c) || total < 0 || total >= kMost) return false;
+    const int64_t batch = l->size(0), cols = t->size(1);
+    if (batch < 1 || batch >= kMost || cols < 1 || cols >= kMost || t->size(0) != batch || (c && c->size(0) != batch + 1) ||
+        (!c && total % batch))
+        return false;
+    s.table = static_cast<const int32_t*>(t->const_data_ptr());
+    s.lengths = static_cast<const int32_t*>(l->const_data_ptr());
+    s.cu = c ? static_cast<const int32_t*>(c->const_data_ptr()) : nullptr;
+    s.batch = (uint32_t)batch, s.table_cols = (uint32_t)cols, s.total = (uint32_t)total;
+    s.max_tokens = (uint32_t)(c ? max_tokens : total / batch);
+    return true;
+}
+
+at::Tensor dense_like(const at::Tensor& x) {
+    return at::empty({x.size(0), x.size(1), x.size(2)}, at::TensorOptions().device(x.device()).dtype(x.scalar_type()));
+}
+
+PyObject* pair_of(at::Tensor&& a, at::Tensor&& b) {  // (b undefined: None)
+    PyObject* p = PyTuple_New(2);
+    if (!p) return nullptr;
+    PyObject* x = THPVariable_Wrap(std::move(a));
+    if (x) PyTuple_SET_ITEM(p, 0, x);
+    PyObject* y = !x ? nullptr : b.defined() ? THPVariable_Wrap(std::move(b)) : (Py_INCREF(Py_None), Py_None);
+    if (y) PyTuple_SET_ITEM(p, 1, y);
+    if (!x || !y) {
+        Py_DECREF(p);
+        return nullptr;
+    }
+    return p;
+}
+
+// rotary(q, k or None, positions, table, layout code, stream) -> (q', k')
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 6) return launch_failed("rotary", "six arguments");
+    const long layout = PyLong_AsLong(a[4]);
+    void* stream = PyLong_AsVoidPtr(a[5]);
+    if (PyErr_Occurred()) return nullptr;
+    const at::Tensor *q, *k = nullptr, *p = exact(a[2]);
+    dmx_rows in[2], out[2];
+    dmx_rotary_table t;
+    if (layout < 0 || !modes_off() || !rows_at(a[0], q, in[0])) Py_RETURN_NONE;
+    const int count = a[1] == Py_None ? 1 : 2;
+    if (count == 2 && (!rows_at(a[1], k, in[1]) || !like(*q, *k))) Py_RETURN_NONE;
+    if (!p || !plain(*p) || p->dim() != 1 || p->size(0) != q->size(0) || p->get_device() != q->get_device() ||
+        (p->scalar_type() != at::kInt && p->scalar_type() != at::kLong) || q->size(2) >= kMost ||
+        !table_of(a[3], layout, q->size(2), q->get_device(), t))
+        Py_RETURN_NONE;
+    at::Tensor y, z;
+    char err[512];
+    int st;
+    {
+        pybind11::gil_scoped_release no_gil;
+        y = dense_like(*q);
+        out[0] = dense_rows(y);
+        if (k) {
+            z = dense_like(*k);
+            out[1] = dense_rows(z);
+        }
+        st = dmx_rotary(in, out, count, (uint32_t)q->size(0), (uint32_t)q->size(2), code(q->scalar_type()), p->const_data_ptr(),
+                        p->scalar_type() == at::kLong, &t, stream, err, sizeof err);
+    }
+    return st ? launch_failed("dmx_rotary", err) : pair_of(std::move(y), std::move(z));
+    END_HANDLE_TH_ERRORS
+}
+
+// append(cache, k, v, block_table, lengths, cu, table or None, layout code, q
+// or None, stream) -> True, or q'
+PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 10) return launch_failed("append", "ten arguments");
+    const long layout = PyLong_AsLong(a[7]);
+    void* stream = PyLong_AsVoidPtr(a[9]);
+    if (PyErr_Occurred()) return nullptr;
+    dmx_kv_cache c;
+    dmx_kv_seqs s;
+    dmx_rotary_table t;
+    dmx_rows rk, rv, rq, out;
+    const at::Tensor *k, *v, *q = nullptr;
+    int64_t index;
+    const bool turn = a[6] != Py_None, queries = a[8] != Py_None;
+    if (layout < 0 || !modes_off() || !cache_of(a[0], c, index) || !rows_at(a[1], k, rk) || !rows_at(a[2], v, rv) ||
+        !like(*k, *v) || k->get_device() != index || rk.heads != c.heads || rv.heads != c.heads || k->size(2) != c.dim ||
+        !seqs_of(a[3], a[4], a[5], k->size(0), 0, index, s) || (turn && !table_of(a[6], layout, c.dim, index, t)) ||
+        (queries && (!turn || !rows_at(a[8], q, rq) || !like(*q, *k))))
+        Py_RETURN_NONE;
+    at::Tensor y;
+    char err[512];
+    int st;
+    {
+        pybind11::gil_scoped_release no_gil;
+        if (q) {
+            y = dense_like(*q);
+            out = dense_rows(y);
+        }
+        st = dmx_kv_append(&c, &s, &rk, &rv, q ? &rq : nullptr, q ? &out : nullptr, code(k->scalar_type()), turn ? &t : nullptr,
+                           stream, err, sizeof err);
+    }
+    if (st) return launch_failed("dmx_kv_append", err);
+    if (!q) Py_RETURN_TRUE;
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// read(cache, block_table, lengths, total, cu, stream) -> (k, v)
+PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 6) return launch_failed("read", "six arguments");
+    const int64_t total = PyLong_AsLongLong(a[3]);
+    void* stream = PyLong_AsVoidPtr(a[5]);
+    if (PyErr_Occurred()) return nullptr;
+    dmx_kv_cache c;
+    dmx_kv_seqs s;
+    int64_t index;
+    if (!modes_off() || !cache_of(a[0], c, index) || !seqs_of(a[1], a[2], a[4], total, 0, index, s)) Py_RETURN_NONE;
+    at::Tensor k, v;
+    char err[512];
+    int st;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const auto options = at::TensorOptions().device(at::Device(at::kCUDA, (c10::DeviceIndex)index)).dtype(at::kBFloat16);
+        k = at::empty({total, (int64_t)c.heads, (int64_t)c.dim}, options);
+        v = at::empty({total, (int64_t)c.heads, (int64_t)c.dim}, options);
+        st = dmx_kv_read(&c, &s, static_cast<uint16_t*>(k.mutable_data_ptr()), static_cast<uint16_t*>(v.mutable_data_ptr()),
+                         stream, err, sizeof err);
+    }
+    return st ? launch_failed("dmx_kv_read", err) : pair_of(std::move(k), std::move(v));
+    END_HANDLE_TH_ERRORS
+}
+
+// A whole number at least 1, or `otherwise` for None; -1 for anything less.
+int64_t count_of(PyObject* o, int64_t otherwise) {
+    if (o == Py_None) return otherwise;
+    const int64_t n = PyLong_AsLongLong(o);
+    return n < 1 ? -1 : n;
+}
+
+// attention(q, cache, block_table, lengths, cu, max_tokens or None, max_length
+// or 0, scale or None, causal, window or None, lse, stream) -> out, or (out, lse)
+PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 12) return launch_failed("attention", "twelve arguments");
+    const int64_t max_tokens = count_of(a[5], 0), max_length = PyLong_AsLongLong(a[6]), window = count_of(a[9], 0);
+    const double given = a[7] == Py_None ? 0 : PyFloat_AsDouble(a[7]);
+    const int causal = PyObject_IsTrue(a[8]), want = PyObject_IsTrue(a[10]);
+    void* stream = PyLong_AsVoidPtr(a[11]);
+    if (PyErr_Occurred()) return nullptr;
+    dmx_kv_cache c;
+    dmx_kv_seqs s;
+    dmx_rows r;
+    const at::Tensor* q;
+    int64_t index;
+    if (!modes_off() || !cache_of(a[1], c, index) || !rows_at(a[0], q, r) || q->get_device() != index || q->size(2) != c.dim ||
+        r.heads == 0 || c.heads == 0 || r.heads % c.heads || window < 0 || window >= kMost || max_length < 0 ||
+        max_length >= (1ll << 32) || max_tokens < 0 || max_tokens >= kMost || (max_tokens && a[4] == Py_None) ||
+        !seqs_of(a[2], a[3], a[4], q->size(0), max_tokens ? max_tokens : q->size(0), index, s))
+        Py_RETURN_NONE;
+    const double scale = a[7] == Py_None ? 1 / std::sqrt((double)c.dim) : given;
+    at::Tensor out, lse, ws;
+    char err[512];
+    int st;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const int dt = code(q->scalar_type());
+        out = dense_like(*q);
+        if (want) lse = at::empty({q->size(0), q->size(1)}, at::TensorOptions().device(q->device()).dtype(at::kFloat));
+        const uint64_t bytes = s.total ? dmx_kv_attention_workspace(&c, &s, r.heads, dt, (uint32_t)max_length, (uint32_t)window) : 0;
+        if (bytes) ws = at::empty({(int64_t)bytes}, at::TensorOptions().device(q->device()).dtype(at::kByte));
+        st = dmx_kv_attention(&c, &s, &r, dt, (float)scale, causal, (uint32_t)window, (uint32_t)max_length,
+                              out.mutable_data_ptr(), want ? static_cast<float*>(lse.mutable_data_ptr()) : nullptr,
+                              bytes ? ws.mutable_data_ptr() : nullptr, bytes, stream, err, sizeof err);
+    }
+    if (st) return launch_failed("dmx_kv_attention", err);
+    return want ? pair_of(std::move(out), std::move(lse)) : THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyCFunction fast() {
     return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F));
@@ -207,6 +463,10 @@ PyCFunction fast() {
 PyMethodDef g_methods[] = {{"rows", fast<rows>(), METH_FASTCALL, nullptr},
                            {"group", fast<group>(), METH_FASTCALL, nullptr},
                            {"narrow", fast<narrow>(), METH_FASTCALL, nullptr},
+                           {"rotary", fast<rotary>(), METH_FASTCALL, nullptr},
+                           {"append", fast<append>(), METH_FASTCALL, nullptr},
+                           {"read", fast<read>(), METH_FASTCALL, nullptr},
+                           {"attention", fast<attention>(), METH_FASTCALL, nullptr},
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "dmx_calls", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
@@ -216,6 +476,9 @@ PyMODINIT_FUNC PyInit_dmx_calls(void) {
     const char* names[4] = {"rx_data", "rx_offsets", "rx_palette", "rx_schedule"};
     for (int i = 0; i < 4; ++i)
         if (!(g_keys[i] = PyUnicode_InternFromString(names[i]))) return nullptr;
+    const char* buffers[4] = {"k_codes", "k_scales", "v_codes", "v_scales"};
+    for (int i = 0; i < 4; ++i)
+        if (!(g_cache[i] = PyUnicode_InternFromString(buffers[i]))) return nullptr;
     PyObject* m = PyModule_Create(&g_module);
     // (the torch whose headers this was compiled with: the loader compares)
     if (m && PyModule_AddStringConstant(m, "torch_version", DMX_TORCH_VERSION) < 0) {

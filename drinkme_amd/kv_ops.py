@@ -120,6 +120,12 @@ def rotary_table(positions: int, dim: int, base: float = 10000.0, scaling: dict 
 # ------------------------------------------------------------------ checks --
 
 
+def _current(x):
+    """The handle of the current stream on x's device; 0 off the GPU, where
+    the native call takes nothing."""
+    return _stream(x.device) if x.is_cuda else 0
+
+
 def _no_gradient(what, *tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or detach its inputs")
@@ -220,6 +226,11 @@ def rotary(q: torch.Tensor, k, positions: torch.Tensor, table: torch.Tensor, lay
     ("interleaved"); channels past the table's dim are copied. Views of a fused
     product are read in place. -> (q', k'), dense. A position outside the table
     gives NaN."""
+    native = _native.calls()
+    if native is not None:  # the plain case in one native call; None: anything else
+        outs = native.rotary(q, k, positions, table, LAYOUTS.get(layout, -1), _current(q))
+        if outs is not None:
+            return outs
     _no_gradient("rotary", q, k)
     q = _activation(q, "rotary: q")
     ins = [q] if k is None else [q, _activation(k, "rotary: k", dim=q.shape[2], tokens=q.shape[0], like=q)]
@@ -265,6 +276,11 @@ def append(cache: dict, k: torch.Tensor, v: torch.Tensor, block_table: torch.Ten
     `table` (rotary_table's) keys are rotated by their positions, in fp32,
     before they are coded, and q [T, Hq, D], if given, is rotated in the same
     launch -> q' (else None). A token whose position has no page is dropped."""
+    native = _native.calls()
+    if native is not None:
+        out = native.append(cache, k, v, block_table, lengths, cu, table, LAYOUTS.get(layout, -1), q, _current(k))
+        if out is not None:
+            return out if q is not None else None
     _no_gradient("append", k, v, q)
     c = _cache_of(cache, "append")
     k = _activation(k, "append: k", heads=c.heads, dim=c.dim)
@@ -294,6 +310,11 @@ def read(cache: dict, block_table: torch.Tensor, lengths: torch.Tensor, total: i
     holds them, bf16 [total, H, D] each: `total` / B tokens of each sequence,
     or cu's (the tokens that append writes for the same arguments). A token
     whose position has no page reads NaN."""
+    native = _native.calls()
+    if native is not None:
+        outs = native.read(cache, block_table, lengths, total, cu, _current(lengths))
+        if outs is not None:
+            return outs
     c = _cache_of(cache, "read")
     device = cache["k_codes"].device
     s, held = _seqs_of(block_table, lengths, cu, int(total), None, device, "read")
@@ -317,6 +338,12 @@ def attention(q: torch.Tensor, cache: dict, block_table: torch.Tensor, lengths: 
     `cu`, max_tokens bounds the new tokens of a sequence (T where not given:
     more launches than needed). `max_length`, a bound on `lengths` where the
     block table is wider than needed, shapes the launch only."""
+    native = _native.calls()
+    if native is not None:
+        outs = native.attention(q, cache, block_table, lengths, cu, max_tokens, max_length or 0, scale, causal, window,
+                                return_lse, _current(q))
+        if outs is not None:
+            return outs
     _no_gradient("attention", q)
     c = _cache_of(cache, "attention")
     q = _activation(q, "attention: q", dim=c.dim)

@@ -470,6 +470,33 @@ def test_calls_of_no_tokens():
     assert kv_ops.read(b.cache, b.block_table, b.lengths, 0)[0].shape == x.shape
 
 
+def test_the_general_path_gives_the_native_call_s_results(monkeypatch):
+    """Every operator without the extension of its per-call path: the same
+    kernels through ctypes, the same bits."""
+    from drinkme_amd import _native
+
+    rng = np.random.default_rng(19)
+    b = Batch(rng, [(5, 70), (1, 33), (0, 4)], 2, 96, 16)
+    b.fill(rng)
+    table = kv_ops.rotary_table(128, 48)
+    q, k, v = (heads(rng, (6, n, 96), "bf16") for n in (4, 2, 2))
+
+    def results():
+        out = list(kv_ops.rotary(q, k, b.lengths.repeat(2), table, "interleaved")) + [kv_ops.rotary(q, None, b.lengths.repeat(2), table)[0]]
+        out.append(kv_ops.append(b.cache, k, v, b.block_table, b.lengths, table=table, q=q, **b.args))
+        out += kv_ops.read(b.cache, b.block_table, b.lengths, 6, **b.args)
+        for kw in ({}, {"max_tokens": 5, "scale": 0.5, "window": 9}, {"causal": False, "max_length": 70}):
+            out += kv_ops.attention(q, b.cache, b.block_table, b.lengths, return_lse=True, **b.args, **kw)
+        out.append(kv_ops.attention(q, b.cache, b.block_table, b.lengths, **b.args))
+        assert kv_ops.append(b.cache, k, v, b.block_table, b.lengths, **b.args) is None
+        return out
+
+    native = results()
+    monkeypatch.setattr(_native, "_calls", None)
+    general = results()
+    assert len(native) == len(general) and all(torch.equal(x, y) for x, y in zip(native, general))
+
+
 # ---------------------------------------------------------------- refusals --
 
 
