@@ -13,6 +13,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "dmx_kv.h"
 #include "dmx_radix.h"
@@ -598,10 +599,10 @@ Plan plan_of(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t q_heads, int 
     Plan p;
     const uint32_t tokens = s->cu ? s->max_tokens : s->total / s->batch;
     const uint64_t rows = (uint64_t)tokens * (q_heads / c->heads);
-    const int most = dtype == DMX_F32 ? 1 : c->dim > 128 ? 2 : 4;
+    const int most = dtype == DMX_F32 ? 1 : 2;
     p.rows = rows > 64;
     p.tiles = p.rows ? most : (int)std::min<uint64_t>(most, rows <= 16 ? 1 : rows <= 32 ? 2 : 4);
-    const uint32_t a_block = 16u * p.tiles * (p.rows ? kAttnWaves : 1);
+    const uint32_t a_block = p.rows ? kAttnWaves * (dtype == DMX_F32 ? 16u : 32u) : 16u * p.tiles;
     p.row_blocks = (uint32_t)((rows + a_block - 1) / a_block);
     uint64_t length = (uint64_t)s->table_cols * c->page;
     if (max_length) length = std::min<uint64_t>(length, max_length);
@@ -616,8 +617,20 @@ uint64_t workspace_of(const Plan& p, const dmx_kv_cache* c, const dmx_kv_seqs* s
     return p.splits == 1 ? 0 : (uint64_t)p.splits * s->total * q_heads * (c->dim + 2) * 4;
 }
 
+// Lets a kernel have `bytes` of dynamic LDS on the current device (over 64 KB
+// takes an opt-in), once for each device.
+int allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& devices, char* err, size_t errn) {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev > 63) return fail(err, errn, "no current device");
+    if (devices.load() >> dev & 1) return 0;
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) return fail(err, errn, "kv attention LDS opt-in refused");
+    devices.fetch_or(1ull << dev);
+    return 0;
+}
+
 template <int W>
-void launch_attend(const Plan& p, int dtype, dim3 grid, hipStream_t stream, const AttnArgs& a) {
+int launch_attend(const Plan& p, int dtype, dim3 grid, hipStream_t stream, const AttnArgs& a, char* err, size_t errn) {
     const dim3 block(64 * kAttnWaves);
     if (dtype == DMX_F32) {
         if (p.rows)
@@ -625,7 +638,9 @@ void launch_attend(const Plan& p, int dtype, dim3 grid, hipStream_t stream, cons
         else
             hipLaunchKernelGGL((k_attend<W, 3, 1, false>), grid, block, 0, stream, a);
     } else if (p.rows) {
-        hipLaunchKernelGGL((k_attend<W, 1, W <= 4 ? 4 : 2, true>), grid, block, 0, stream, a);
+        static std::atomic<uint64_t> allowed{0};
+        if (allow_lds(reinterpret_cast<const void*>(k_attend_prompt<W>), Stage<W>::lds, allowed, err, errn)) return 1;
+        hipLaunchKernelGGL((k_attend_prompt<W>), grid, block, Stage<W>::lds, stream, a);
     } else if (p.tiles == 1) {
         hipLaunchKernelGGL((k_attend<W, 1, 1, false>), grid, block, 0, stream, a);
     } else if (p.tiles == 2) {
@@ -633,6 +648,7 @@ void launch_attend(const Plan& p, int dtype, dim3 grid, hipStream_t stream, cons
     } else if constexpr (W <= 4) {
         hipLaunchKernelGGL((k_attend<W, 1, 4, false>), grid, block, 0, stream, a);
     }
+    return launch_check(err, errn, "kv attention launch");
 }
 
 }  // namespace
@@ -674,14 +690,12 @@ extern "C" int dmx_kv_attention(const dmx_kv_cache* cache, const dmx_kv_seqs* se
     a.part_ml = reinterpret_cast<float2*>(a.part_o + (p.splits > 1 ? p.splits * all * cache->dim : 0));
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const dim3 grid(cache->heads, p.row_blocks, seqs->batch * p.splits);
-    switch (cache->dim) {
-        case 64: launch_attend<2>(p, dtype, grid, st, a); break;
-        case 96: launch_attend<3>(p, dtype, grid, st, a); break;
-        case 128: launch_attend<4>(p, dtype, grid, st, a); break;
-        case 192: launch_attend<6>(p, dtype, grid, st, a); break;
-        default: launch_attend<8>(p, dtype, grid, st, a); break;
-    }
-    if (launch_check(err, errn, "kv attention launch")) return 1;
+    const int rc = cache->dim == 64    ? launch_attend<2>(p, dtype, grid, st, a, err, errn)
+                    : cache->dim == 96  ? launch_attend<3>(p, dtype, grid, st, a, err, errn)
+                    : cache->dim == 128 ? launch_attend<4>(p, dtype, grid, st, a, err, errn)
+                    : cache->dim == 192 ? launch_attend<6>(p, dtype, grid, st, a, err, errn)
+                                        : launch_attend<8>(p, dtype, grid, st, a, err, errn);
+    if (rc) return 1;
     if (p.splits == 1) return 0;
     const int ways = p.splits > 8 ? 4 : 1;
     hipLaunchKernelGGL((dtype == DMX_F32 ? k_attend_join<true> : k_attend_join<false>),
