@@ -484,200 +484,244 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
 
 // ------------------------------------------------------------------ prompts --
 //
-// Many rows to a cache head: a workgroup of four waves, 32 rows each, decodes
-// every token once, for all of them, and is bound by the matrix cores and the
-// softmax's instructions. 64 tokens a stage: one wave turns the codes of their
-// keys into operands in LDS, two those of their values (the parts rotate), a
-// stage ahead of their use, from codes loaded a stage before that. The
-// products are v_mfma_f32_32x32x16_bf16's, transposed as above: lane (i, f),
-// i = lane & 31, f = lane >> 5, owns row i and gets of a 32-token block the
-// scores of tokens 16 m + 8 f .. + 7, m = 0, 1, which the second product wants
-// there; operand row n of K is token 16 (n >> 4) + 8 (n >> 2 & 1) + 4 (n >> 3 & 1)
-// + (n & 3).
+// Many rows to a cache head: a workgroup's waves, 32 rows each, decode every
+// token once for all of them, a part each: codes to operands in LDS, 64 tokens
+// a step. The products are v_mfma_f32_32x32x16_bf16's, transposed as above: lane
+// (i, f), i = lane & 31, f = lane >> 5, owns row i and gets of a 32-token block
+// the scores of tokens 16 m + 8 f .. + 7, m = 0, 1, which the second product
+// wants there; operand row n of K is token
+// 16 (n >> 4) + 8 (n >> 2 & 1) + 4 (n >> 3 & 1) + (n & 3).
+//
+// While a block's weights are taken (vector instructions) the next block's
+// scores and the last one's products run on the matrix core, in one straight
+// piece of code. So a step reads keys of blocks 2 s + 1 and 2 s + 2 and values of
+// 2 s - 1 and 2 s: set s. Meanwhile set s + 1 is written, from codes loaded a
+// step before.
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
+// Waves of a workgroup: eight, two a SIMD; four where 256 registers a lane are too few.
+constexpr int prompt_waves(int W) { return W <= 6 ? 8 : 4; }
+
 template <int W>
-struct Stage {
-    static constexpr int frag = 1024;                    // bytes of an operand: 16 a lane
-    static constexpr int keys = 2 * W * frag;            // of a 32-token block: one per 16 channels
-    static constexpr int block = 2 * keys;               // and values: one per 32 channels and 16 tokens
-    static constexpr int bytes = 2 * block;              // two blocks
-    static constexpr int lds = 2 * bytes + 4 * (int)sizeof(int);  // two stages, and whether their values hold a NaN
-    static constexpr int raw = 4 * W + 4 > 10 * Segments<W>::count ? 4 * W + 4 : 10 * Segments<W>::count;
+struct Set {
+    static constexpr int frag = 1024;           // bytes of an operand: 16 a lane
+    static constexpr int block = 2 * W * frag;  // of 32 tokens' keys (one per 16 channels) or values (one per 32 channels
+                                                // and 16 tokens)
+    static constexpr int bytes = 4 * block;     // two blocks of keys, two of values
+    static constexpr int nan = 2 * bytes;       // two sets; then whether values of a set hold a NaN, by part
+    static constexpr int lds = nan + 8 * (int)sizeof(int);
+    static constexpr int raw = 10 * Segments<W>::count > W + 2 ? 10 * Segments<W>::count : W + 2;
 };
 
-// The page numbers that part `part` of a stage needs: of the lane's token in
-// each block's keys (0), or of its eight tokens in a block's values (1, 2).
-__device__ __forceinline__ void stage_pages(const AttnArgs& a, uint32_t b, int stage, int part, int lane, uint32_t (&page)[2]) {
+// Part 0..7 of set s: 0..3 values, 4..7 keys; of the set's block part >> 1 & 1
+// the half part & 1 of the channels (keys: of each lane's words).
+__device__ __forceinline__ int part_block(int s, int part) { return 2 * s + (part >> 1 & 1) + (part < 4 ? -1 : 1); }
+
+// The page number that a lane needs for a part: of its eight tokens' values or
+// its token's key. (Blocks before the first one count as that.)
+__device__ __forceinline__ uint32_t part_page(const AttnArgs& a, uint32_t b, int s, int part, int lane) {
     const uint32_t shift = a.cache.page_shift, last = (uint32_t)a.seqs.cols - 1;
-    const int32_t* row = a.seqs.table + (int64_t)b * a.seqs.cols;
-    const int octet = part == 0 ? 2 * (lane >> 4 & 1) + (lane >> 2 & 1) : lane >> 4;
-    const uint32_t t = (uint32_t)stage * 64 + 8 * octet + (part == 2 ? 32 : 0);
-    const uint32_t c0 = t >> shift, c1 = (t + 32) >> shift;
-    page[0] = c0 > last ? ~0u : (uint32_t)row[c0];
-    page[1] = part || c1 > last ? ~0u : (uint32_t)row[c1];
+    const int octet = part < 4 ? lane >> 4 : 2 * (lane >> 4 & 1) + (lane >> 2 & 1);
+    const uint32_t col = ((uint32_t)max(part_block(s, part), 0) * 32 + 8 * octet) >> shift;
+    return col > last ? ~0u : (uint32_t)a.seqs.table[(int64_t)b * a.seqs.cols + col];
 }
 
 template <int W>
-__device__ __forceinline__ void stage_load(const AttnArgs& a, uint32_t h, int stage, int part, int lane, const uint32_t (&page)[2],
-                                           uint32_t (&raw)[Stage<W>::raw]) {
+__device__ __forceinline__ void part_load(const AttnArgs& a, uint32_t h, int s, int part, int lane, uint32_t page,
+                                          uint32_t (&raw)[Set<W>::raw]) {
     using S = Segments<W>;
-    const uint32_t shift = a.cache.page_shift, mask = (1u << shift) - 1u;
-    const auto at = [&](uint32_t p, uint32_t t) {
-        return (((uint64_t)(p < a.cache.pages ? p : 0u) * a.cache.heads + h) << shift) + (t & mask);
-    };
-    if (part == 0) {
-        const uint32_t t = (uint32_t)stage * 64 + 16 * (lane >> 4 & 1) + 8 * (lane >> 2 & 1) + 4 * (lane >> 3 & 1) + (lane & 3);
-        const int f = lane >> 5, g = 2 * W * f >> 2;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const uint64_t token = at(page[n], t + 32 * n);
-            __builtin_memcpy(&raw[2 * W * n], a.cache.k_codes + token * (4 * W) + 2 * W * f, 8 * W);
-            const uint8_t* e = a.cache.k_scales + token * W + g;  // of the lane's words
-            uint32_t& bytes = raw[4 * W + n];
-            if constexpr (W == 2)
-                bytes = e[0];
-            else if constexpr (W == 8)
-                __builtin_memcpy(&bytes, __builtin_assume_aligned(e, 4), 4);
-            else
-                bytes = e[0] | e[1] << 8 | (W == 6 ? e[2] << 16 : 0);
-            if (page[n] >= a.cache.pages) bytes = ~0u;  // no page: NaN
-        }
-    } else if (part < 3) {
+    const uint32_t shift = a.cache.page_shift, mask = (1u << shift) - 1u, t0 = (uint32_t)max(part_block(s, part), 0) * 32;
+    const bool ok = page < a.cache.pages;
+    const uint64_t base = ((uint64_t)(ok ? page : 0u) * a.cache.heads + h) << shift;
+    if (part < 4) {
         const int i = lane & 15, j = lane >> 4;
-        const uint64_t token = at(page[0], (uint32_t)stage * 64 + 32 * (part - 1) + 8 * j);
+        const uint64_t token = base + ((t0 + 8 * j) & mask);
         const uint32_t* codes = a.cache.v_codes + token * (4 * W);
         const uint8_t* scales = static_cast<const uint8_t*>(__builtin_assume_aligned(a.cache.v_scales + token * W, 8));
 #pragma unroll
-        for (int s = 0; s < S::count; ++s) {
-            const int w = S::word(s) + (i * 2 * S::size(s) >> 4);
-            __builtin_memcpy(&raw[10 * s], codes + 8 * w, 32);
-            __builtin_memcpy(&raw[10 * s + 8], __builtin_assume_aligned(scales + 8 * (w >> 2), 8), 8);
+        for (int n = 0; n < S::count; ++n) {
+            const int w = S::word(n) + (i * 2 * S::size(n) >> 4);
+            __builtin_memcpy(&raw[10 * n], codes + 8 * w, 32);
+            __builtin_memcpy(&raw[10 * n + 8], __builtin_assume_aligned(scales + 8 * (w >> 2), 8), 8);
         }
+    } else {
+        const int j = 2 * (lane >> 5) + (part & 1);
+        const uint32_t t = t0 + 16 * (lane >> 4 & 1) + 8 * (lane >> 2 & 1) + 4 * (lane >> 3 & 1) + (lane & 3);
+        const uint64_t token = base + (t & mask);
+        __builtin_memcpy(&raw[0], a.cache.k_codes + token * (4 * W) + W * j, 4 * W);
+        const int g0 = (W * j) >> 2, g1 = (W * j + W - 1) >> 2;
+        raw[W] = a.cache.k_scales[token * W + g0];
+        if (W != 2 && W != 4) raw[W + 1] = a.cache.k_scales[token * W + g1];
+        if (!ok) raw[W] = raw[W + 1] = 255;  // no page: NaN
     }
 }
 
-// The loaded codes as operands in LDS. Values past `hi`, and NaN blocks, go as
-// zeros; `nan` says that there were some of the latter.
-template <int W>
-__device__ __forceinline__ void stage_write(char* to, int* nan, int stage, int part, int lane, int hi, uint32_t (&raw)[Stage<W>::raw]) {
+// Pairs [first, first + count) of a segment's values (even and odd channels) to
+// their operands. Octet j = 2 m + f: lane slot 32 f of operand m; channels of
+// both parities 16 lanes apart.
+template <int W, int SEG, int FIRST, int COUNT>
+__device__ __forceinline__ void write_values(char* to, int lane, const uint32_t (&raw)[Set<W>::raw]) {
     using S = Segments<W>;
-    using G = Stage<W>;
-    if (part == 0) {
+    const int i = lane & 15, j = lane >> 4;
+    const uint32_t a = raw[10 * SEG + 8], b = raw[10 * SEG + 9];
+    const float e[8] = {scale_of<0>(a), scale_of<1>(a), scale_of<2>(a), scale_of<3>(a),
+                        scale_of<0>(b), scale_of<1>(b), scale_of<2>(b), scale_of<3>(b)};
+    to += (j >> 1) * Set<W>::frag + ((j & 1) * 32 + i) * 16;
+    uint32_t w[8];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const uint32_t bytes = raw[4 * W + n];
-            const float e[4] = {scale_of<0>(bytes), scale_of<1>(bytes), scale_of<2>(bytes), scale_of<3>(bytes)};
+    for (int n = 0; n < 8; ++n)
+        w[n] = S::size(SEG) == 8   ? raw[10 * SEG + n]
+               : S::size(SEG) == 4 ? raw[10 * SEG + n] >> (16 * (i & 1))
+                                   : raw[10 * SEG + n] >> (8 * (i & 3));
 #pragma unroll
-            for (int c = 0; c < 2 * W; ++c) {
-                // word 2 W f + c, block of 32 channels (2 W f + c) / 4
-                const float x = W == 3 ? (lane < 32 ? e[c >> 2] : e[(c + 2) >> 2]) : e[c >> 2];
-                const uint32_t w = raw[2 * W * n + c];
-                const u32x4 f = {pair_of<0>(w, x), pair_of<1>(w, x), pair_of<2>(w, x), pair_of<3>(w, x)};
-                *reinterpret_cast<u32x4*>(to + n * G::block + c * G::frag + lane * 16) = f;
-            }
+    for (int c = FIRST; c < FIRST + COUNT; ++c) {
+        u32x4 even, odd;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const uint32_t u = pair_at(c, w[2 * n], e[2 * n]), v = pair_at(c, w[2 * n + 1], e[2 * n + 1]);
+            even[n] = __builtin_amdgcn_perm(v, u, 0x05040100u);
+            odd[n] = __builtin_amdgcn_perm(v, u, 0x07060302u);
         }
-    } else if (part < 3) {
-        const int i = lane & 15, j = lane >> 4, t0 = stage * 64 + 32 * (part - 1);
-        if (t0 + 32 > hi) {
+        char* tile = to + (S::tile(SEG) + 2 * c) * Set<W>::frag;
+        *reinterpret_cast<u32x4*>(tile) = even;
+        *reinterpret_cast<u32x4*>(tile + 256) = odd;
+    }
+}
+
+template <int W, int HALF, int SEG = 0>
+__device__ __forceinline__ void write_half(char* to, int lane, const uint32_t (&raw)[Set<W>::raw]) {
+    if constexpr (SEG < Segments<W>::count) {
+        constexpr int units = Segments<W>::size(SEG) / 2, some = units > 1 ? units / 2 : HALF;
+        if constexpr (some > 0) write_values<W, SEG, (units > 1 ? HALF * some : 0), some>(to, lane, raw);
+        write_half<W, HALF, SEG + 1>(to, lane, raw);
+    }
+}
+
+// The loaded codes as operands in LDS. Values of no token (before the first or
+// from `hi` on), and NaN blocks, go as zeros; the set's flags say that there
+// were some of the latter.
+template <int W>
+__device__ __forceinline__ void part_write(char* lds, int s, int part, int lane, int hi, uint32_t (&raw)[Set<W>::raw]) {
+    using S = Segments<W>;
+    using G = Set<W>;
+    char* to = lds + (s & 1) * G::bytes + (part >> 1 & 1) * G::block;
+    if (part >= 4) {
+        const int j = 2 * (lane >> 5) + (part & 1);
+        const float e0 = scale_of<0>(raw[W]), e1 = W == 2 || W == 4 ? e0 : scale_of<0>(raw[W + 1]);
+        to += (part & 1) * W * G::frag + lane * 16;
 #pragma unroll
-            for (int s = 0; s < S::count; ++s)
-#pragma unroll
-                for (int n = 0; n < 8; ++n)
-                    if (t0 + 8 * j + n >= hi) {
-                        raw[10 * s + n] = 0;
-                        raw[10 * s + 8 + (n >> 2)] &= ~(255u << (8 * (n & 3)));
-                    }
+        for (int c = 0; c < W; ++c) {
+            const float e = W == 8 ? (c < 4 ? e0 : e1) : W == 2 || W == 4 ? e0 : ((W * j + c) >> 2) == ((W * j) >> 2) ? e0 : e1;
+            const uint32_t w = raw[c];
+            *reinterpret_cast<u32x4*>(to + c * G::frag) = u32x4{pair_of<0>(w, e), pair_of<1>(w, e), pair_of<2>(w, e), pair_of<3>(w, e)};
         }
-        uint32_t all = 0;  // the top bit of each byte that is 255
+        return;
+    }
+    const int block = part_block(s, part);
+    const int t0 = block * 32 + 8 * (lane >> 4);
+    if (block < 0 || block * 32 + 32 > hi) {
 #pragma unroll
-        for (int s = 0; s < S::count; ++s)
-#pragma unroll
-            for (int n = 8; n < 10; ++n) {
-                const uint32_t x = raw[10 * s + n];
-                all |= x & ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-            }
-        const bool any = __any(all != 0);
-        if (any) {
-#pragma unroll
-            for (int s = 0; s < S::count; ++s)
-#pragma unroll
-                for (int n = 0; n < 8; ++n)
-                    if ((raw[10 * s + 8 + (n >> 2)] >> (8 * (n & 3)) & 255u) == 255u) {
-                        raw[10 * s + n] = 0;
-                        raw[10 * s + 8 + (n >> 2)] &= ~(255u << (8 * (n & 3)));
-                    }
-        }
-        if (lane == 0) nan[part - 1] = any;
-        // octet j = 2 m + f: lane slot 32 f of operand m; channels of both parities 16 lanes apart
-        char* at = to + (part - 1) * G::block + G::keys + (j >> 1) * G::frag + ((j & 1) * 32 + i) * 16;
-#pragma unroll
-        for (int s = 0; s < S::count; ++s) {
-            const uint32_t a = raw[10 * s + 8], b = raw[10 * s + 9];
-            const float e[8] = {scale_of<0>(a), scale_of<1>(a), scale_of<2>(a), scale_of<3>(a),
-                                scale_of<0>(b), scale_of<1>(b), scale_of<2>(b), scale_of<3>(b)};
-            uint32_t w[8];
+        for (int x = 0; x < S::count; ++x)
 #pragma unroll
             for (int n = 0; n < 8; ++n)
-                w[n] = S::size(s) == 8   ? raw[10 * s + n]
-                       : S::size(s) == 4 ? raw[10 * s + n] >> (16 * (i & 1))
-                                         : raw[10 * s + n] >> (8 * (i & 3));
-#pragma unroll
-            for (int c = 0; c < S::size(s); c += 2) {
-                u32x4 even, odd;
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    const uint32_t u = pair_at(c / 2, w[2 * n], e[2 * n]), v = pair_at(c / 2, w[2 * n + 1], e[2 * n + 1]);
-                    even[n] = __builtin_amdgcn_perm(v, u, 0x05040100u);
-                    odd[n] = __builtin_amdgcn_perm(v, u, 0x07060302u);
+                if (block < 0 || t0 + n >= hi) {
+                    raw[10 * x + n] = 0;
+                    raw[10 * x + 8 + (n >> 2)] &= ~(255u << (8 * (n & 3)));
                 }
-                char* tile = at + (S::tile(s) + c) * G::frag;  // (S::tile counts 16-channel tiles: half of them, two operands each)
-                *reinterpret_cast<u32x4*>(tile) = even;
-                *reinterpret_cast<u32x4*>(tile + 256) = odd;
-            }
-        }
     }
+    uint32_t all = 0;  // the top bit of each byte that is 255
+#pragma unroll
+    for (int x = 0; x < S::count; ++x)
+#pragma unroll
+        for (int n = 8; n < 10; ++n) {
+            const uint32_t y = raw[10 * x + n];
+            all |= y & ((y & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+        }
+    const bool any = __any(all != 0);
+    if (any) {
+#pragma unroll
+        for (int x = 0; x < S::count; ++x)
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                if ((raw[10 * x + 8 + (n >> 2)] >> (8 * (n & 3)) & 255u) == 255u) {
+                    raw[10 * x + n] = 0;
+                    raw[10 * x + 8 + (n >> 2)] &= ~(255u << (8 * (n & 3)));
+                }
+    }
+    if (lane == 0) reinterpret_cast<int*>(lds + G::nan)[4 * (s & 1) + part] = any;
+    to += 2 * G::block;
+    if (part & 1)
+        write_half<W, 1>(to, lane, raw);
+    else
+        write_half<W, 0>(to, lane, raw);
 }
 
 template <int W>
-__global__ __launch_bounds__(64 * kAttnWaves, W <= 4 ? 2 : 1) void k_attend_prompt(const AttnArgs a) {
+__global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_attend_prompt(const AttnArgs a) {
     using S = Segments<W>;
-    using G = Stage<W>;
-    constexpr int D = 32 * W;
+    using G = Set<W>;
+    constexpr int D = 32 * W, waves = prompt_waves(W), parts = 8 / waves, half = waves / 2;
     extern __shared__ __align__(16) char lds[];
-    int* nan = reinterpret_cast<int*>(lds + 2 * G::bytes);  // [stage & 1][block]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 31, f = lane >> 5;
     const uint32_t h = blockIdx.x, b = blockIdx.z / a.splits, split = blockIdx.z % a.splits;
 
     const Seq q = seq_of(a.seqs, b);
-    const int rows = q.count * (int)a.group;
-    const int first = ((int)gridDim.y - 1 - (int)blockIdx.y) * 32 * kAttnWaves;  // (the longest of a causal prompt go first)
-    if (first >= rows) return;
+    constexpr int unit = 32 * half;  // the rows of half of the waves
+    const int rows = q.count * (int)a.group, units = (rows + unit - 1) / unit, y = blockIdx.y;
+    if (2 * y >= units) return;
+    // Half of the waves take a unit of rows, half another: of a causal prompt the
+    // one as far from its end as the first is from its start, so that workgroups
+    // get alike, else the neighbour.
+    const bool far = a.causal && !a.window;
+    const int low = far ? y : 2 * y, high = far ? units - 1 - y : 2 * y + 1;
+    const int first = (wave < half ? high : low) * unit + 32 * (wave % half);
     const int cap = a.seqs.cols << a.cache.page_shift;
     const auto hi_of = [&](int m) { return a.causal ? q.first + m + 1 : q.length; };
     const auto lo_of = [&](int m) { return a.window ? max(0, q.first + m + 1 - (int)a.window) : 0; };
     const auto new_of = [&](int r) { return r / (int)a.group; };
-    // the stages of the workgroup, and what this wave's rows see of them
-    const int hi_all = min(hi_of(new_of(min(first + 32 * kAttnWaves, rows) - 1)), cap), lo_all = lo_of(new_of(first));
-    const int st_lo = lo_all >> 6, st_hi = hi_all > lo_all ? (hi_all + 63) >> 6 : st_lo;
-    const int per = (st_hi - st_lo + (int)a.splits - 1) / (int)a.splits;
-    const int st_first = st_lo + (int)split * per, st_end = min(st_first + per, st_hi);
-    const int r0 = first + 32 * wave;
-    const bool some = r0 < rows;
-    const int m0 = some ? new_of(r0) : 0, m1 = some ? new_of(min(r0 + 32, rows) - 1) : 0;
-    const int see_hi = some ? min(hi_of(m1), cap) : 0, see_lo = lo_of(m0), full_hi = hi_of(m0), full_lo = lo_of(m1);
+    // the steps of the workgroup, and what this wave's rows see of their tokens
+    const int hi_all = min(hi_of(new_of(min(high * unit + unit, rows) - 1)), cap), lo_all = lo_of(new_of(low * unit));
+    const int s_lo = lo_all >> 6, s_hi = hi_all > lo_all ? (hi_all + 63) >> 6 : s_lo;
+    const int per = (s_hi - s_lo + (int)a.splits - 1) / (int)a.splits;
+    const int s_first = s_lo + (int)split * per, s_end = min(s_first + per, s_hi);
+    const bool some = first < rows && (wave < half || low != high);  // (an odd unit in the middle is the first waves')
+    const int m0 = some ? new_of(first) : 0, m1 = some ? new_of(min(first + 32, rows) - 1) : 0;
+    const int full_hi = some ? hi_of(m0) : 0, full_lo = lo_of(m1);  // every row sees what lies in between,
+    const int see_hi = some ? min(hi_of(m1), cap) : 0, see_lo = lo_of(m0);  // and none what lies outside of these
 
-    uint32_t page[2], raw[G::raw];
-    if (st_first < st_end) {
-        stage_pages(a, b, st_first, wave, lane, page);
-        stage_load<W>(a, h, st_first, wave, lane, page, raw);
-        stage_pages(a, b, st_first + 1, (wave + 1) & 3, lane, page);
+    // Parts of the work on a set: values by four waves, keys by the other four (or
+    // by the same). Values are written when a step begins and keys in its middle,
+    // so that of a SIMD's two waves one has products to run meanwhile.
+    const int vpart = wave & 3, kpart = 4 + (wave & 3);
+    const bool does_v = wave < 4, does_k = waves == 4 || wave >= 4;
+    uint32_t page[2], raw[parts][G::raw];
+    uint32_t(&vraw)[G::raw] = raw[0];
+    uint32_t(&kraw)[G::raw] = raw[parts - 1];
+    const auto next_v = [&](int s) {  // loads set s, then the page numbers of the next
+        part_load<W>(a, h, s, vpart, lane, page[0], vraw);
+        page[0] = part_page(a, b, s + 1, vpart, lane);
+    };
+    const auto next_k = [&](int s) {
+        part_load<W>(a, h, s, kpart, lane, page[1], kraw);
+        page[1] = part_page(a, b, s + 1, kpart, lane);
+    };
+    const auto write_v = [&](int s) { part_write<W>(lds, s, vpart, lane, hi_all, vraw); };
+    const auto write_k = [&](int s) { part_write<W>(lds, s, kpart, lane, hi_all, kraw); };
+    if (s_first < s_end) {
+        if (does_v) {
+            page[0] = part_page(a, b, s_first - 1, vpart, lane);
+            next_v(s_first - 1);
+        }
+        if (does_k) {
+            page[1] = part_page(a, b, s_first - 1, kpart, lane);
+            next_k(s_first - 1);
+        }
     }
 
-    const int r = r0 + i;
-    const bool mine = r < rows;
+    const int r = first + i;
+    const bool mine = some && r < rows;
     const int m = mine ? new_of(r) : 0, g = mine ? r - m * (int)a.group : 0;
     const int hi = mine ? hi_of(m) : 0, lo = lo_of(m);
     const int64_t token = q.token + m, head = (int64_t)h * a.group + g, row_out = token * a.q_heads + head;
@@ -692,50 +736,50 @@ __global__ __launch_bounds__(64 * kAttnWaves, W <= 4 ? 2 : 1) void k_attend_prom
         }
     }
     float mx = -INFINITY, sum = 0.f;
-    f32x16 o[W];
+    f32x16 o[W], sc[2];
+    bf16x8 pf[2];  // the last block's weights
 #pragma unroll
     for (int c = 0; c < W; ++c) o[c] = f32x16{};
+    pf[0] = pf[1] = __builtin_bit_cast(bf16x8, u32x4{0, 0, 0, 0});
 
-    if (st_first < st_end) {
-        stage_write<W>(lds + (st_first & 1) * G::bytes, nan + 2 * (st_first & 1), st_first, wave, lane, hi_all, raw);
-        if (st_first + 1 < st_end) stage_load<W>(a, h, st_first + 1, (wave + 1) & 3, lane, page, raw);
-        stage_pages(a, b, st_first + 2, (wave + 2) & 3, lane, page);
-    }
-    for (int st = st_first; st < st_end; ++st) {
-        // (writes of this stage are done, and reads of the one before)
-        __syncthreads();
-        const int part = (wave + st - st_first + 1) & 3;
-        if (st + 1 < st_end) stage_write<W>(lds + ((st + 1) & 1) * G::bytes, nan + 2 * ((st + 1) & 1), st + 1, part, lane, hi_all, raw);
-        if (st + 2 < st_end) {
-            stage_load<W>(a, h, st + 2, (part + 1) & 3, lane, page, raw);
-            stage_pages(a, b, st + 3, (part + 2) & 3, lane, page);
+    // a block's scores (keys k of a set), and the last block's products (values v)
+    const auto score = [&](const char* from, f32x16& to) {
+        to = f32x16{};
+#pragma unroll
+        for (int c = 0; c < 2 * W; ++c)
+            to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(from + c * G::frag), qf[c], to, 0, 0, 0);
+    };
+    const auto add_up = [&](const char* from) {
+#pragma unroll
+        for (int z = 0; z < 2; ++z)
+#pragma unroll
+            for (int c = 0; c < W; ++c)
+                o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(from + (2 * c + z) * G::frag), pf[z],
+                                                               o[c], 0, 0, 0);
+    };
+    const auto keys = [&](int s, int n) { return lds + (s & 1) * G::bytes + n * G::block + lane * 16; };
+    const auto values = [&](int s, int n) { return lds + (s & 1) * G::bytes + (2 + n) * G::block + lane * 16; };
+    // Of block n's scores: what a row does not see, and the rows' references. Where
+    // one rises, weights taken before (of the block whose values are at `from`) go
+    // into the products first.
+    const auto turn_to = [&](int n, f32x16& x, const char* from) {
+        if (n * 32 < full_lo || n * 32 + 32 > full_hi) {
+            int t = n * 32 + 8 * f;
+            asm volatile("" : "+v"(t));  // (a branch: else the comparisons are made for every block)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int at = t + 16 * (e >> 3) + (e & 7);
+                if (at < lo || at >= hi) x[e] = -INFINITY;
+            }
         }
-        const int t0 = st * 64;
-        if (t0 >= see_hi || t0 + 64 <= see_lo) continue;
-
-        const char* from = lds + (st & 1) * G::bytes + lane * 16;
-        f32x16 sc[2];
+        float top = x[0];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            sc[n] = f32x16{};
-#pragma unroll
-            for (int c = 0; c < 2 * W; ++c)
-                sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(from + n * G::block + c * G::frag),
-                                                                qf[c], sc[n], 0, 0, 0);
-        }
-        const auto at = [&](int n, int x) { return t0 + 32 * n + 16 * (x >> 3) + 8 * f + (x & 7); };  // the token of score x
-        if (t0 < full_lo || t0 + 64 > full_hi) {
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int x = 0; x < 16; ++x)
-                    if (at(n, x) < lo || at(n, x) >= hi) sc[n][x] = -INFINITY;
-        }
-        float top = sc[0][0];
-#pragma unroll
-        for (int x = 1; x < 32; ++x) top = fmaxf(top, sc[x >> 4][x & 15]);
+        for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
         top *= a.scale;
         if (__any(top > mx + 8.f)) {
+            asm volatile("" : "+v"(from));  // (else the operands are read ahead of the branch, for both sides)
+            add_up(from);
+            pf[0] = pf[1] = __builtin_bit_cast(bf16x8, u32x4{0, 0, 0, 0});
             const auto swap = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
             top = fmaxf(mx, fmaxf(__uint_as_float(swap[0]), __uint_as_float(swap[1])));
             const float alpha = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - top);
@@ -744,54 +788,88 @@ __global__ __launch_bounds__(64 * kAttnWaves, W <= 4 ? 2 : 1) void k_attend_prom
             for (int c = 0; c < W; ++c) o[c] *= alpha;
             mx = top;
         }
+    };
+    // block x's weights; the scores of the block after it, and the products of the one before
+    const auto block = [&](f32x16& x, f32x16& next, const char* k, const char* v) {
         const float base = mx == -INFINITY ? 0.f : -mx;
-        bf16x8 pf[2][2];
+        score(k, next);
+        add_up(v);
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(sc[n][x], a.scale, base));
-                sum += p;
-                pf[n][x >> 3][x & 7] = (__bf16)p;
-            }
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int y = 0; y < 2; ++y)
-#pragma unroll
-                for (int c = 0; c < W; ++c)
-                    o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                        *reinterpret_cast<const bf16x8*>(from + n * G::block + G::keys + (2 * c + y) * G::frag), pf[n][y], o[c], 0, 0, 0);
-
-        // NaN blocks among the values: NaN in the rows that see one
-#pragma unroll 1
-        for (int n = 0; n < 2; ++n) {
-            if (!__builtin_amdgcn_readfirstlane(nan[2 * (st & 1) + n])) continue;
-            f32x16 hit[S::count] = {};
-            for (int y = 0; y < 2; ++y) {
-                const int t = t0 + 32 * n + 16 * y + 8 * f;
-                const Slot slot = slot_of(a.cache, a.seqs, b, h, (uint32_t)t);
-                bf16x8 seen;
-#pragma unroll
-                for (int x = 0; x < 8; ++x) seen[x] = t + x >= lo && t + x < hi ? (__bf16)1.f : (__bf16)0.f;
-#pragma unroll
-                for (int s = 0; s < S::count; ++s) {
-                    const int w = S::word(s) + ((i & 15) * 2 * S::size(s) >> 4);
-                    const uint8_t* e = a.cache.v_scales + slot.token * W + 8 * (w >> 2);
-                    bf16x8 is;
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) is[x] = e[x] == 255 && t + x < hi_all ? (__bf16)1.f : (__bf16)0.f;
-                    hit[s] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(is, seen, hit[s], 0, 0, 0);
-                }
-            }
-#pragma unroll
-            for (int s = 0; s < S::count; ++s)
-#pragma unroll
-                for (int c = 0; c < S::size(s) / 2; ++c)
-#pragma unroll
-                    for (int x = 0; x < 16; ++x)
-                        if (hit[s][x] > 0.f) o[S::tile(s) / 2 + c][x] = NAN;
+        for (int e = 0; e < 16; ++e) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(x[e], a.scale, base));
+            sum += p;
+            pf[e >> 3][e & 7] = (__bf16)p;
         }
+        asm volatile("" : "+v"(pf[0]), "+v"(pf[1]), "+v"(sum));  // (here, beside the products, not where they are used)
+    };
+    // NaN blocks among a set's values: NaN in the rows that see one
+    const auto mark_nan = [&](int s) {
+        const int* nan = reinterpret_cast<const int*>(lds + G::nan) + 4 * (s & 1);
+        if (!__builtin_amdgcn_readfirstlane(nan[0] | nan[1] | nan[2] | nan[3])) return;
+#pragma unroll 1
+        for (int n = 0; n < 4; ++n) {
+            const int t = (2 * s - 1) * 32 + 16 * n + 8 * f;
+            const Slot slot = slot_of(a.cache, a.seqs, b, h, (uint32_t)max(t, 0));
+            bf16x8 seen;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) seen[x] = t + x >= lo && t + x < hi ? (__bf16)1.f : (__bf16)0.f;
+#pragma unroll
+            for (int x = 0; x < S::count; ++x) {
+                const int w = S::word(x) + ((i & 15) * 2 * S::size(x) >> 4);
+                const uint8_t* e = a.cache.v_scales + slot.token * W + 8 * (w >> 2);
+                bf16x8 is;
+#pragma unroll
+                for (int z = 0; z < 8; ++z) is[z] = e[z] == 255 && t + z < hi_all ? (__bf16)1.f : (__bf16)0.f;
+                const f32x16 hit = __builtin_amdgcn_mfma_f32_32x32x16_bf16(is, seen, f32x16{}, 0, 0, 0);
+#pragma unroll
+                for (int c = 0; c < S::size(x) / 2; ++c)
+#pragma unroll
+                    for (int z = 0; z < 16; ++z)
+                        if (hit[z] > 0.f) o[S::tile(x) / 2 + c][z] = NAN;
+            }
+        }
+    };
+
+    if (s_first < s_end) {
+        const auto both = [&](int s) {
+            if (does_v) {
+                write_v(s);
+                next_v(s + 1);
+            }
+            if (does_k) {
+                write_k(s);
+                next_k(s + 1);
+            }
+        };
+        both(s_first - 1);
+        __syncthreads();
+        both(s_first);
+        score(keys(s_first - 1, 1), sc[0]);
+        for (int s = s_first; s < s_end; ++s) {
+            __syncthreads();  // (set s is written, and set s - 1 read)
+            if (does_v) {
+                write_v(s + 1);
+                next_v(s + 2);
+            }
+            // (blocks 2 s - 1 .. 2 s + 2)
+            const bool seen = 64 * s - 32 < see_hi && 64 * s + 96 > see_lo;
+            if (seen) {
+                mark_nan(s);
+                turn_to(2 * s, sc[0], values(s, 0));
+                block(sc[0], sc[1], keys(s, 0), values(s, 0));
+            }
+            if (does_k) {
+                write_k(s + 1);
+                next_k(s + 2);
+            }
+            if (seen) {
+                turn_to(2 * s + 1, sc[1], values(s, 1));
+                block(sc[1], sc[0], keys(s, 1), values(s, 1));
+            }
+        }
+        __syncthreads();
+        mark_nan(s_end);
+        add_up(values(s_end, 0));
     }
     {
         const auto swap = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
@@ -813,19 +891,19 @@ __global__ __launch_bounds__(64 * kAttnWaves, W <= 4 ? 2 : 1) void k_attend_prom
 #pragma unroll
         for (int x = 0; x < 8; ++x) {  // operand row 8 (x >> 2) + 4 f + (x & 3), and 16 more for odd channels
             const int size = S::size(s), ch = 8 * S::word(s) + size * (8 * (x >> 2) + 4 * f + (x & 3));
-            float y[8];
+            float v[8];
 #pragma unroll
             for (int c = 0; c < size; ++c) {
-                const float v = o[S::tile(s) / 2 + c / 2][8 * (c & 1) + x] * inv;
-                y[c] = done && sum != sum ? NAN : v;
+                v[c] = o[S::tile(s) / 2 + c / 2][8 * (c & 1) + x] * inv;
+                if (done && sum != sum) v[c] = NAN;
             }
             if (!done) {
 #pragma unroll
-                for (int c = 0; c < size; ++c) a.part_o[at * D + ch + c] = y[c];
+                for (int c = 0; c < size; ++c) a.part_o[at * D + ch + c] = v[c];
             } else {
                 uint16_t* to = static_cast<uint16_t*>(a.out) + at * D + ch;
 #pragma unroll
-                for (int c = 0; c < size; ++c) to[c] = __builtin_bit_cast(uint16_t, (__bf16)y[c]);
+                for (int c = 0; c < size; ++c) to[c] = __builtin_bit_cast(uint16_t, (__bf16)v[c]);
             }
         }
 }

@@ -602,7 +602,7 @@ Plan plan_of(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t q_heads, int 
     const int most = dtype == DMX_F32 ? 1 : 2;
     p.rows = rows > 64;
     p.tiles = p.rows ? most : (int)std::min<uint64_t>(most, rows <= 16 ? 1 : rows <= 32 ? 2 : 4);
-    const uint32_t a_block = p.rows ? kAttnWaves * (dtype == DMX_F32 ? 16u : 32u) : 16u * p.tiles;
+    const uint32_t a_block = !p.rows ? 16u * p.tiles : dtype == DMX_F32 ? 16u * kAttnWaves : 32u * prompt_waves(c->dim / 32);
     p.row_blocks = (uint32_t)((rows + a_block - 1) / a_block);
     uint64_t length = (uint64_t)s->table_cols * c->page;
     if (max_length) length = std::min<uint64_t>(length, max_length);
@@ -639,8 +639,8 @@ int launch_attend(const Plan& p, int dtype, dim3 grid, hipStream_t stream, const
             hipLaunchKernelGGL((k_attend<W, 3, 1, false>), grid, block, 0, stream, a);
     } else if (p.rows) {
         static std::atomic<uint64_t> allowed{0};
-        if (allow_lds(reinterpret_cast<const void*>(k_attend_prompt<W>), Stage<W>::lds, allowed, err, errn)) return 1;
-        hipLaunchKernelGGL((k_attend_prompt<W>), grid, block, Stage<W>::lds, stream, a);
+        if (allow_lds(reinterpret_cast<const void*>(k_attend_prompt<W>), Set<W>::lds, allowed, err, errn)) return 1;
+        hipLaunchKernelGGL((k_attend_prompt<W>), grid, dim3(64 * prompt_waves(W)), Set<W>::lds, stream, a);
     } else if (p.tiles == 1) {
         hipLaunchKernelGGL((k_attend<W, 1, 1, false>), grid, block, 0, stream, a);
     } else if (p.tiles == 2) {
