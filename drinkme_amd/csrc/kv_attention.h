@@ -59,6 +59,30 @@ struct Block {
     bool ok;                             // false: no page for this lane's K tokens
 };
 
+// Where tokens lie. WIDE: a page holds whole 32-token blocks, so that a block's
+// place is the wave's and a lane's part in it an offset that stays; else each
+// lane looks up the page of its own octet of the block.
+template <bool WIDE>
+__device__ __forceinline__ uint32_t page_of(const AttnArgs& a, uint32_t b, uint32_t block, int octet) {
+    const uint32_t col = (block * 32 + (WIDE ? 0 : 8 * octet)) >> a.cache.page_shift;
+    return col >= (uint32_t)a.seqs.cols ? ~0u : (uint32_t)a.seqs.table[(int64_t)b * a.seqs.cols + col];
+}
+
+struct Place {
+    uint64_t base;  // index of (page, head, slot): a block's (WIDE), or an octet's
+    uint32_t in;    // the lane's octet after it, tokens
+    bool ok;        // false: no page there, and the place is in page 0
+};
+
+template <bool WIDE>
+__device__ __forceinline__ Place place_of(const AttnArgs& a, uint32_t h, uint32_t page, uint32_t block, int octet) {
+    if (WIDE) page = __builtin_amdgcn_readfirstlane(page);
+    const uint32_t shift = a.cache.page_shift, mask = (1u << shift) - 1u;
+    const bool ok = page < a.cache.pages;
+    const uint64_t base = (((uint64_t)(ok ? page : 0u) * a.cache.heads + h) << shift) + ((block * 32 + (WIDE ? 0 : 8 * octet)) & mask);
+    return {base, WIDE ? 8u * octet : 0u, ok};
+}
+
 // The page numbers of a lane's K and V tokens in a block.
 struct Entry {
     uint32_t k, v;
@@ -119,42 +143,36 @@ struct State {
     f32x4 o[NR][NT];        // channels 4 j + r of tile n, in Segments' order
 };
 
-template <int W>
+template <bool WIDE>
 __device__ __forceinline__ Entry entries(const AttnArgs& a, uint32_t b, int blk, int i, int j) {
-    const uint32_t shift = a.cache.page_shift, last = (uint32_t)a.seqs.cols - 1;
-    const int32_t* row = a.seqs.table + (int64_t)b * a.seqs.cols;
-    const uint32_t kc = ((uint32_t)blk * 32 + 8 * (i >> 2)) >> shift, vc = ((uint32_t)blk * 32 + 8 * j) >> shift;
     Entry e;
-    e.k = (uint32_t)row[min(kc, last)];
-    e.v = (uint32_t)row[min(vc, last)];
-    if (kc > last) e.k = ~0u;
+    e.k = page_of<WIDE>(a, b, blk, i >> 2);
+    e.v = WIDE ? e.k : page_of<WIDE>(a, b, blk, j);
     return e;
 }
 
-template <int W>
+template <bool WIDE, int W>
 __device__ __forceinline__ void fetch(const AttnArgs& a, uint32_t h, int blk, Entry e, int i, int j, Block<W>& x) {
     using S = Segments<W>;
-    const uint32_t shift = a.cache.page_shift, mask = (1u << shift) - 1u;
-    x.ok = e.k < a.cache.pages;
-    const uint32_t kp = x.ok ? e.k : 0u, vp = e.v < a.cache.pages ? e.v : 0u;
-    const uint64_t kt = (((uint64_t)kp * a.cache.heads + h) << shift) + (((uint32_t)blk * 32 + 8 * (i >> 2)) & mask) + (i & 3);
-    const uint64_t vt = (((uint64_t)vp * a.cache.heads + h) << shift) + (((uint32_t)blk * 32 + 8 * j) & mask);
+    const Place k = place_of<WIDE>(a, h, e.k, blk, i >> 2), v = place_of<WIDE>(a, h, e.v, blk, j);
     const int g0 = (W * j) >> 2, g1 = (W * j + W - 1) >> 2;
-    const uint32_t* kc = a.cache.k_codes + kt * (4 * W) + W * j;
-    const uint8_t* ks = a.cache.k_scales + kt * W;
+    const uint32_t in = k.in + (i & 3);
+    const uint32_t* kc = a.cache.k_codes + k.base * (4 * W);
+    const uint8_t* ks = a.cache.k_scales + k.base * W;
+    x.ok = k.ok;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-        __builtin_memcpy(x.k[s], kc + 4 * s * (4 * W), 4 * W);
-        x.ks[s][0] = ks[4 * s * W + g0];
-        if (W != 2 && W != 4) x.ks[s][1] = ks[4 * s * W + g1];
+        __builtin_memcpy(x.k[s], kc + ((in + 4 * s) * (4 * W) + W * j), 4 * W);
+        x.ks[s][0] = ks[(in + 4 * s) * W + g0];
+        if (W != 2 && W != 4) x.ks[s][1] = ks[(in + 4 * s) * W + g1];
     }
-    const uint32_t* vc = a.cache.v_codes + vt * (4 * W);
-    const uint8_t* vs = static_cast<const uint8_t*>(__builtin_assume_aligned(a.cache.v_scales + vt * W, 8));
+    const uint32_t* vc = a.cache.v_codes + v.base * (4 * W);
+    const uint8_t* vs = a.cache.v_scales + v.base * W;
 #pragma unroll
     for (int s = 0; s < S::count; ++s) {
-        const int w = S::word(s) + (i * 2 * S::size(s) >> 4);
-        __builtin_memcpy(x.v[s], vc + 8 * w, 32);
-        __builtin_memcpy(x.vs[s], __builtin_assume_aligned(vs + 8 * (w >> 2), 8), 8);
+        const uint32_t w = S::word(s) + (i * 2 * S::size(s) >> 4);
+        __builtin_memcpy(x.v[s], vc + (v.in * (4 * W) + 8 * w), 32);
+        __builtin_memcpy(x.vs[s], __builtin_assume_aligned(vs + (v.in * W + 8 * (w >> 2)), 8), 8);
     }
 }
 
@@ -300,7 +318,7 @@ __device__ __forceinline__ void attend_block(State<W, P, NR>& st, Block<W>& x, f
 // NR: tiles of 16 query rows a wave. ROWS: the workgroup's waves take rows of
 // their own and every token; else they share the rows and deal the tokens.
 // Registers: two waves a SIMD where 256 of them do.
-template <int W, int P, int NR, bool ROWS>
+template <int W, int P, int NR, bool ROWS, bool WIDE>
 __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) void k_attend(const AttnArgs a) {
     using S = Segments<W>;
     constexpr int D = 32 * W, NT = D / 16;
@@ -330,8 +348,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
     Block<W> x[2];
     Entry e[2] = {};
     if (blk < blk_end) {
-        e[0] = entries<W>(a, b, blk, i, j);
-        e[1] = entries<W>(a, b, blk + step, i, j);
+        e[0] = entries<WIDE>(a, b, blk, i, j);
+        e[1] = entries<WIDE>(a, b, blk + step, i, j);
     }
 
     State<W, P, NR> st;
@@ -373,19 +391,19 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
         blk += step;
     };
     if (blk < blk_end) {
-        fetch(a, h, blk, e[0], i, j, x[0]);
+        fetch<WIDE>(a, h, blk, e[0], i, j, x[0]);
         for (;;) {
             const bool more = blk + step < blk_end;
             if (more) {
-                fetch(a, h, blk + step, e[1], i, j, x[1]);
-                e[0] = entries<W>(a, b, blk + 2 * step, i, j);
+                fetch<WIDE>(a, h, blk + step, e[1], i, j, x[1]);
+                e[0] = entries<WIDE>(a, b, blk + 2 * step, i, j);
             }
             work(x[0]);
             if (!more) break;
             const bool again = blk + step < blk_end;
             if (again) {
-                fetch(a, h, blk + step, e[0], i, j, x[0]);
-                e[1] = entries<W>(a, b, blk + 2 * step, i, j);
+                fetch<WIDE>(a, h, blk + step, e[0], i, j, x[0]);
+                e[1] = entries<WIDE>(a, b, blk + 2 * step, i, j);
             }
             work(x[1]);
             if (!again) break;
@@ -518,42 +536,40 @@ struct Set {
 // the half part & 1 of the channels (keys: of each lane's words).
 __device__ __forceinline__ int part_block(int s, int part) { return 2 * s + (part >> 1 & 1) + (part < 4 ? -1 : 1); }
 
-// The page number that a lane needs for a part: of its eight tokens' values or
-// its token's key. (Blocks before the first one count as that.)
+// The octet of its block that a lane's part concerns: its eight tokens' values or
+// its token's key.
+__device__ __forceinline__ int part_octet(int part, int lane) { return part < 4 ? lane >> 4 : 2 * (lane >> 4 & 1) + (lane >> 2 & 1); }
+
+// (blocks before the first one count as that)
+template <bool WIDE>
 __device__ __forceinline__ uint32_t part_page(const AttnArgs& a, uint32_t b, int s, int part, int lane) {
-    const uint32_t shift = a.cache.page_shift, last = (uint32_t)a.seqs.cols - 1;
-    const int octet = part < 4 ? lane >> 4 : 2 * (lane >> 4 & 1) + (lane >> 2 & 1);
-    const uint32_t col = ((uint32_t)max(part_block(s, part), 0) * 32 + 8 * octet) >> shift;
-    return col > last ? ~0u : (uint32_t)a.seqs.table[(int64_t)b * a.seqs.cols + col];
+    return page_of<WIDE>(a, b, max(part_block(s, part), 0), part_octet(part, lane));
 }
 
-template <int W>
+template <bool WIDE, int W>
 __device__ __forceinline__ void part_load(const AttnArgs& a, uint32_t h, int s, int part, int lane, uint32_t page,
                                           uint32_t (&raw)[Set<W>::raw]) {
     using S = Segments<W>;
-    const uint32_t shift = a.cache.page_shift, mask = (1u << shift) - 1u, t0 = (uint32_t)max(part_block(s, part), 0) * 32;
-    const bool ok = page < a.cache.pages;
-    const uint64_t base = ((uint64_t)(ok ? page : 0u) * a.cache.heads + h) << shift;
+    const Place p = place_of<WIDE>(a, h, page, max(part_block(s, part), 0), part_octet(part, lane));
     if (part < 4) {
-        const int i = lane & 15, j = lane >> 4;
-        const uint64_t token = base + ((t0 + 8 * j) & mask);
-        const uint32_t* codes = a.cache.v_codes + token * (4 * W);
-        const uint8_t* scales = static_cast<const uint8_t*>(__builtin_assume_aligned(a.cache.v_scales + token * W, 8));
+        const int i = lane & 15;
+        const uint32_t* codes = a.cache.v_codes + p.base * (4 * W);
+        const uint8_t* scales = a.cache.v_scales + p.base * W;
 #pragma unroll
         for (int n = 0; n < S::count; ++n) {
-            const int w = S::word(n) + (i * 2 * S::size(n) >> 4);
-            __builtin_memcpy(&raw[10 * n], codes + 8 * w, 32);
-            __builtin_memcpy(&raw[10 * n + 8], __builtin_assume_aligned(scales + 8 * (w >> 2), 8), 8);
+            const uint32_t w = S::word(n) + (i * 2 * S::size(n) >> 4);
+            __builtin_memcpy(&raw[10 * n], codes + (p.in * (4 * W) + 8 * w), 32);
+            __builtin_memcpy(&raw[10 * n + 8], __builtin_assume_aligned(scales + (p.in * W + 8 * (w >> 2)), 8), 8);
         }
     } else {
         const int j = 2 * (lane >> 5) + (part & 1);
-        const uint32_t t = t0 + 16 * (lane >> 4 & 1) + 8 * (lane >> 2 & 1) + 4 * (lane >> 3 & 1) + (lane & 3);
-        const uint64_t token = base + (t & mask);
-        __builtin_memcpy(&raw[0], a.cache.k_codes + token * (4 * W) + W * j, 4 * W);
+        const uint32_t in = p.in + 4 * (lane >> 3 & 1) + (lane & 3);
         const int g0 = (W * j) >> 2, g1 = (W * j + W - 1) >> 2;
-        raw[W] = a.cache.k_scales[token * W + g0];
-        if (W != 2 && W != 4) raw[W + 1] = a.cache.k_scales[token * W + g1];
-        if (!ok) raw[W] = raw[W + 1] = 255;  // no page: NaN
+        const uint8_t* scales = a.cache.k_scales + p.base * W;
+        __builtin_memcpy(&raw[0], a.cache.k_codes + p.base * (4 * W) + (in * (4 * W) + W * j), 4 * W);
+        raw[W] = scales[in * W + g0];
+        if (W != 2 && W != 4) raw[W + 1] = scales[in * W + g1];
+        if (!p.ok) raw[W] = raw[W + 1] = 255;  // no page: NaN
     }
 }
 
@@ -657,7 +673,7 @@ __device__ __forceinline__ void part_write(char* lds, int s, int part, int lane,
         write_half<W, 0>(to, lane, raw);
 }
 
-template <int W>
+template <int W, bool WIDE>
 __global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_attend_prompt(const AttnArgs a) {
     using S = Segments<W>;
     using G = Set<W>;
@@ -700,22 +716,22 @@ __global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_a
     uint32_t(&vraw)[G::raw] = raw[0];
     uint32_t(&kraw)[G::raw] = raw[parts - 1];
     const auto next_v = [&](int s) {  // loads set s, then the page numbers of the next
-        part_load<W>(a, h, s, vpart, lane, page[0], vraw);
-        page[0] = part_page(a, b, s + 1, vpart, lane);
+        part_load<WIDE, W>(a, h, s, vpart, lane, page[0], vraw);
+        page[0] = part_page<WIDE>(a, b, s + 1, vpart, lane);
     };
     const auto next_k = [&](int s) {
-        part_load<W>(a, h, s, kpart, lane, page[1], kraw);
-        page[1] = part_page(a, b, s + 1, kpart, lane);
+        part_load<WIDE, W>(a, h, s, kpart, lane, page[1], kraw);
+        page[1] = part_page<WIDE>(a, b, s + 1, kpart, lane);
     };
     const auto write_v = [&](int s) { part_write<W>(lds, s, vpart, lane, hi_all, vraw); };
     const auto write_k = [&](int s) { part_write<W>(lds, s, kpart, lane, hi_all, kraw); };
     if (s_first < s_end) {
         if (does_v) {
-            page[0] = part_page(a, b, s_first - 1, vpart, lane);
+            page[0] = part_page<WIDE>(a, b, s_first - 1, vpart, lane);
             next_v(s_first - 1);
         }
         if (does_k) {
-            page[1] = part_page(a, b, s_first - 1, kpart, lane);
+            page[1] = part_page<WIDE>(a, b, s_first - 1, kpart, lane);
             next_k(s_first - 1);
         }
     }

@@ -14,6 +14,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "dmx_kv.h"
 #include "dmx_radix.h"
@@ -629,24 +630,24 @@ int allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& devices, cha
     return 0;
 }
 
-template <int W>
+template <int W, bool WIDE>
 int launch_attend(const Plan& p, int dtype, dim3 grid, hipStream_t stream, const AttnArgs& a, char* err, size_t errn) {
     const dim3 block(64 * kAttnWaves);
     if (dtype == DMX_F32) {
         if (p.rows)
-            hipLaunchKernelGGL((k_attend<W, 3, 1, true>), grid, block, 0, stream, a);
+            hipLaunchKernelGGL((k_attend<W, 3, 1, true, WIDE>), grid, block, 0, stream, a);
         else
-            hipLaunchKernelGGL((k_attend<W, 3, 1, false>), grid, block, 0, stream, a);
+            hipLaunchKernelGGL((k_attend<W, 3, 1, false, WIDE>), grid, block, 0, stream, a);
     } else if (p.rows) {
         static std::atomic<uint64_t> allowed{0};
-        if (allow_lds(reinterpret_cast<const void*>(k_attend_prompt<W>), Set<W>::lds, allowed, err, errn)) return 1;
-        hipLaunchKernelGGL((k_attend_prompt<W>), grid, dim3(64 * prompt_waves(W)), Set<W>::lds, stream, a);
+        if (allow_lds(reinterpret_cast<const void*>(k_attend_prompt<W, WIDE>), Set<W>::lds, allowed, err, errn)) return 1;
+        hipLaunchKernelGGL((k_attend_prompt<W, WIDE>), grid, dim3(64 * prompt_waves(W)), Set<W>::lds, stream, a);
     } else if (p.tiles == 1) {
-        hipLaunchKernelGGL((k_attend<W, 1, 1, false>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((k_attend<W, 1, 1, false, WIDE>), grid, block, 0, stream, a);
     } else if (p.tiles == 2) {
-        hipLaunchKernelGGL((k_attend<W, 1, 2, false>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((k_attend<W, 1, 2, false, WIDE>), grid, block, 0, stream, a);
     } else if constexpr (W <= 4) {
-        hipLaunchKernelGGL((k_attend<W, 1, 4, false>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((k_attend<W, 1, 4, false, WIDE>), grid, block, 0, stream, a);
     }
     return launch_check(err, errn, "kv attention launch");
 }
@@ -690,11 +691,16 @@ extern "C" int dmx_kv_attention(const dmx_kv_cache* cache, const dmx_kv_seqs* se
     a.part_ml = reinterpret_cast<float2*>(a.part_o + (p.splits > 1 ? p.splits * all * cache->dim : 0));
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const dim3 grid(cache->heads, p.row_blocks, seqs->batch * p.splits);
-    const int rc = cache->dim == 64    ? launch_attend<2>(p, dtype, grid, st, a, err, errn)
-                    : cache->dim == 96  ? launch_attend<3>(p, dtype, grid, st, a, err, errn)
-                    : cache->dim == 128 ? launch_attend<4>(p, dtype, grid, st, a, err, errn)
-                    : cache->dim == 192 ? launch_attend<6>(p, dtype, grid, st, a, err, errn)
-                                        : launch_attend<8>(p, dtype, grid, st, a, err, errn);
+    const bool wide = cache->page >= 32;
+    const auto launch = [&](auto w) {
+        constexpr int W = decltype(w)::value;
+        return wide ? launch_attend<W, true>(p, dtype, grid, st, a, err, errn) : launch_attend<W, false>(p, dtype, grid, st, a, err, errn);
+    };
+    const int rc = cache->dim == 64    ? launch(std::integral_constant<int, 2>{})
+                   : cache->dim == 96  ? launch(std::integral_constant<int, 3>{})
+                   : cache->dim == 128 ? launch(std::integral_constant<int, 4>{})
+                   : cache->dim == 192 ? launch(std::integral_constant<int, 6>{})
+                                       : launch(std::integral_constant<int, 8>{});
     if (rc) return 1;
     if (p.splits == 1) return 0;
     const int ways = p.splits > 8 ? 4 : 1;
