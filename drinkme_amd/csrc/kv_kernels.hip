@@ -608,9 +608,18 @@ Plan plan_of(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t q_heads, int 
     uint64_t length = (uint64_t)s->table_cols * c->page;
     if (max_length) length = std::min<uint64_t>(length, max_length);
     if (window) length = std::min<uint64_t>(length, (uint64_t)window + tokens + 31);
+    // Splits: a workgroup a CU, two where a split is still longer than 2048
+    // tokens (an even deal of uneven sequences, and more loads in flight), each of
+    // 128 tokens at least; contexts up to 512 tokens go unsplit, without the join.
+    // Measured, 32 query and 8 key heads of 128, us by splits: 1021 tokens 10.3 (1)
+    // 9.0 (8); 16384 90 (1) 14.9 (16) 13.1 (32) 15.0 (64); 32 sequences of 1024
+    // 12.3 (1) 17.0 (4), of 8192 64.7 (1) 53.4 (2) 56.1 (4); 8 of 4096 27.4 (1)
+    // 15.7 (4) 20.5 (32). Prompts are split only where they fill half of the CUs.
     const uint64_t groups = (uint64_t)c->heads * s->batch * std::max(1u, p.row_blocks);
-    const uint64_t wanted = p.rows ? 256 / groups : (1024 + groups - 1) / groups, possible = length / 128;
-    p.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({wanted, possible, 64, 65535 / s->batch}));
+    uint64_t wanted = std::max<uint64_t>(1, 256 / groups);
+    if (!p.rows && length / wanted > 2048) wanted = std::max<uint64_t>(1, 512 / groups);
+    const uint64_t possible = length <= 512 ? 1 : length / 128;
+    p.splits = (uint32_t)std::min<uint64_t>({wanted, possible, 64, 65535 / s->batch});
     return p;
 }
 
