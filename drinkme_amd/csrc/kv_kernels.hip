@@ -29,12 +29,28 @@ struct Cache {
     uint32_t pages, heads, page_shift;
 };
 
+// A divisor known to the host: n / d, n < 2^31, by a multiplication. With s the
+// least for which 2^s >= d, 2^(32 + s) / d lies between 2^32 and 2^33; mul is
+// its excess over 2^32, rounded up, and the error stays below 1 / d.
+struct Divisor {
+    uint32_t mul, shift, value;
+};
+__device__ __forceinline__ uint32_t operator/(uint32_t n, const Divisor& d) { return (__umulhi(n, d.mul) + n) >> d.shift; }
+
+// n = a * d + b: a into n, b returned.
+__device__ __forceinline__ uint32_t take(uint32_t& n, const Divisor& d) {
+    const uint32_t a = n / d, b = n - a * d.value;
+    n = a;
+    return b;
+}
+
 struct Seqs {
     const int32_t* table;
     const int32_t* lengths;
     const int32_t* cu;
     uint32_t batch, total;
     int cols;
+    Divisor each;  // new tokens of each sequence, where cu is null
 };
 
 struct Rows {
@@ -64,7 +80,7 @@ __device__ __forceinline__ Seq seq_of(const Seqs& s, uint32_t b) {
         q.token = min(max(s.cu[b], 0), (int)s.total);
         q.count = min(max(s.cu[b + 1], q.token), (int)s.total) - q.token;
     } else {
-        q.count = s.total / s.batch;
+        q.count = s.each.value;
         q.token = b * q.count;
     }
     q.length = max(s.lengths[b], 0);
@@ -74,7 +90,7 @@ __device__ __forceinline__ Seq seq_of(const Seqs& s, uint32_t b) {
 
 // The sequence of new token t: the last one that begins at or before it.
 __device__ __forceinline__ uint32_t seq_at(const Seqs& s, uint32_t t) {
-    if (!s.cu) return t / (s.total / s.batch);
+    if (!s.cu) return t / s.each;
     uint32_t lo = 0, hi = s.batch - 1;
     while (lo < hi) {
         const uint32_t mid = (lo + hi + 1) >> 1;
@@ -164,18 +180,21 @@ __device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
     b = y;
 }
 
-// Eight (cos, sin) pairs from angle `first` of a position's row; NaN outside the table.
+// N (cos, sin) pairs from angle `first` of a position's row; NaN outside the table.
+template <int N>
 __device__ __forceinline__ void angles(const Table& t, int64_t position, uint32_t first, float (&c)[8], float (&s)[8]) {
     const bool ok = position >= 0 && position < (int64_t)t.positions;
     const float4* p = reinterpret_cast<const float4*>(t.at + 2 * ((ok ? position : 0) * t.half + first));
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
+    for (int n = 0; n < N / 2; ++n) {
         const float4 v = p[n];
         c[2 * n] = ok ? v.x : NAN, s[2 * n] = ok ? v.y : NAN;
         c[2 * n + 1] = ok ? v.z : NAN, s[2 * n + 1] = ok ? v.w : NAN;
     }
 }
 
+// Items of a rotation: (token, run of heads, c). A lane keeps its token's
+// position and angles for a run of heads.
 struct Rotation {
     Rows in[2], out[2];
     uint32_t n, tokens, dim;
@@ -183,6 +202,8 @@ struct Rotation {
     int wide;
     Table table;
     Seqs seqs;
+    Divisor per, runs;  // items of a head, runs of a token
+    uint32_t run;       // heads of a run
 };
 
 __device__ __forceinline__ int64_t position_of(const Rotation& r, uint32_t t) {
@@ -192,102 +213,132 @@ __device__ __forceinline__ int64_t position_of(const Rotation& r, uint32_t t) {
     return (int64_t)q.first + ((int)t - q.token);
 }
 
-// Item (token, head, c) of 16 channels: two runs of 8. In the turned part the
-// eight pairs of angles 8 c .. 8 c + 7, else 16 channels to copy. Takes 16-byte
-// aligned rows, dim and the turned channels multiples of 16.
+struct RotaryItem {
+    uint32_t c, t, first, end;  // heads of both tensors, in's first
+};
+__device__ __forceinline__ RotaryItem rotary_item_of(const Rotation& r, uint32_t n) {
+    const uint32_t c = take(n, r.per), k = take(n, r.runs), all = r.in[0].heads + (r.n > 1 ? r.in[1].heads : 0);
+    return {c, n, k * r.run, min(k * r.run + r.run, all)};
+}
+
+struct RowAt {
+    void *in, *out;
+    int64_t from, to;
+};
+__device__ __forceinline__ RowAt row_at(const Rotation& r, uint32_t t, uint32_t h) {
+    const bool other = h >= r.in[0].heads;
+    const int64_t k = other ? h - r.in[0].heads : h;
+    return {other ? r.in[1].at : r.in[0].at, other ? r.out[1].at : r.out[0].at,
+            t * (other ? r.in[1].token : r.in[0].token) + k * (other ? r.in[1].head : r.in[0].head),
+            t * (other ? r.out[1].token : r.out[0].token) + k * (other ? r.out[1].head : r.out[0].head)};
+}
+
+// c: 16 channels, two runs of 8. In the turned part the eight pairs of angles
+// 8 c .. 8 c + 7, else 16 channels to copy. Takes 16-byte aligned rows, dim and
+// the turned channels multiples of 16.
 template <bool F32>
-__device__ __forceinline__ void rotary_item(const Rotation& r, uint64_t item) {
-    const uint32_t per = r.dim / 16, heads = r.in[0].heads + (r.n > 1 ? r.in[1].heads : 0);
-    const uint32_t c = item % per;
-    const uint64_t th = item / per;
-    uint32_t h = th % heads;
-    const uint32_t t = th / heads;
+__device__ __forceinline__ void rotate(const Rotation& r, uint32_t item) {
+    const auto [c, t, first, end] = rotary_item_of(r, item);
     if (t >= r.tokens) return;
-    const int which = h >= r.in[0].heads;
-    if (which) h -= r.in[0].heads;
-    const Rows &in = r.in[which], &out = r.out[which];
-    const int64_t from = t * in.token + h * in.head, to = t * out.token + h * out.head;
     const bool turned = 8 * c < r.table.half, split = turned && r.table.layout == DMX_ROTARY_HALF;
     const uint32_t x = split ? 8 * c : 16 * c, y = split ? 8 * c + r.table.half : 16 * c + 8;
-    float a[8], b[8];
-    load8<F32>(in.at, from + x, a);
-    load8<F32>(in.at, from + y, b);
-    if (turned) {
-        float cs[8], sn[8];
-        angles(r.table, position_of(r, t), 8 * c, cs, sn);
+    float cs[8], sn[8];
+    if (turned) angles<8>(r.table, position_of(r, t), 8 * c, cs, sn);
+    for (uint32_t h = first; h < end; ++h) {
+        const RowAt row = row_at(r, t, h);
+        float a[8], b[8];
+        load8<F32>(row.in, row.from + x, a);
+        load8<F32>(row.in, row.from + y, b);
         if (split) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) turn(a[e], b[e], cs[e], sn[e]);
-        } else {
+        } else if (turned) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 turn(a[2 * e], a[2 * e + 1], cs[e], sn[e]);
                 turn(b[2 * e], b[2 * e + 1], cs[4 + e], sn[4 + e]);
             }
         }
+        store8<F32>(row.out, row.to + x, a);
+        store8<F32>(row.out, row.to + y, b);
     }
-    store8<F32>(out.at, to + x, a);
-    store8<F32>(out.at, to + y, b);
+}
+
+// Any sizes, strides and alignment. c: a pair of channels.
+template <bool F32>
+__device__ __forceinline__ void rotate_any(const Rotation& r, uint32_t item) {
+    const auto [c, t, first, end] = rotary_item_of(r, item);
+    if (t >= r.tokens) return;
+    const bool turned = c < r.table.half, split = turned && r.table.layout == DMX_ROTARY_HALF;
+    const uint32_t x = split ? c : 2 * c, y = split ? c + r.table.half : 2 * c + 1;
+    float cs = 0.f, sn = 0.f;
+    if (turned) {
+        const int64_t p = position_of(r, t);
+        const bool ok = p >= 0 && p < (int64_t)r.table.positions;
+        const float* at = r.table.at + 2 * ((ok ? p : 0) * r.table.half + c);
+        cs = ok ? at[0] : NAN, sn = ok ? at[1] : NAN;
+    }
+    for (uint32_t h = first; h < end; ++h) {
+        const RowAt row = row_at(r, t, h);
+        float a = load1<F32>(row.in, row.from + x), b = load1<F32>(row.in, row.from + y);
+        if (turned) turn(a, b, cs, sn);
+        store1<F32>(row.out, row.to + x, a);
+        store1<F32>(row.out, row.to + y, b);
+    }
 }
 
 template <bool F32>
 __global__ __launch_bounds__(256) void k_rotary(const Rotation r) {
-    rotary_item<F32>(r, (uint64_t)blockIdx.x * 256 + threadIdx.x);
+    rotate<F32>(r, blockIdx.x * 256 + threadIdx.x);
 }
-
-// Any sizes, strides and alignment: item (token, head, pair), a pair of
-// channels an item.
-template <bool F32>
-__device__ __forceinline__ void rotary_item_any(const Rotation& r, uint64_t item) {
-    const uint32_t per = r.dim / 2, heads = r.in[0].heads + (r.n > 1 ? r.in[1].heads : 0);
-    const uint32_t c = item % per;
-    const uint64_t th = item / per;
-    uint32_t h = th % heads;
-    const uint32_t t = th / heads;
-    if (t >= r.tokens) return;
-    const int which = h >= r.in[0].heads;
-    if (which) h -= r.in[0].heads;
-    const Rows &in = r.in[which], &out = r.out[which];
-    const int64_t from = t * in.token + h * in.head, to = t * out.token + h * out.head;
-    const bool turned = c < r.table.half, split = turned && r.table.layout == DMX_ROTARY_HALF;
-    const uint32_t x = split ? c : 2 * c, y = split ? c + r.table.half : 2 * c + 1;
-    float a = load1<F32>(in.at, from + x), b = load1<F32>(in.at, from + y);
-    if (turned) {
-        const int64_t p = position_of(r, t);
-        const bool ok = p >= 0 && p < (int64_t)r.table.positions;
-        const float* cs = r.table.at + 2 * ((ok ? p : 0) * r.table.half + c);
-        turn(a, b, ok ? cs[0] : NAN, ok ? cs[1] : NAN);
-    }
-    store1<F32>(out.at, to + x, a);
-    store1<F32>(out.at, to + y, b);
-}
-
 template <bool F32>
 __global__ __launch_bounds__(256) void k_rotary_any(const Rotation r) {
-    rotary_item_any<F32>(r, (uint64_t)blockIdx.x * 256 + threadIdx.x);
+    rotate_any<F32>(r, blockIdx.x * 256 + threadIdx.x);
 }
 
 // ----------------------------------------------------------------- append --
+
+// Items of a call's keys: (token, run of heads, word), words fastest, which lie
+// side by side in the cache and in the activations; of its values: (eight tokens,
+// run of heads, word, token), as the cache has them. A lane keeps its token's
+// place for a run of heads.
+struct Items {
+    Divisor words, runs;
+    uint32_t run;
+};
 
 struct Append {
     Cache cache;
     Seqs seqs;
     Rows k, v;
-    uint32_t dim;
+    Items items;
     Table table;  // at null: keys as they are
     Rotation q;   // the queries' (n 0: none)
-    uint64_t cached;  // words of keys (and as many of values) that the first blocks code
-    uint32_t cached_blocks;
+    uint32_t key_blocks, cached_blocks;  // blocks of keys; of keys and values
 };
 
-// The codes of a lane's eight channels; four adjacent lanes hold a block of 32,
-// whose exponent byte each of them returns.
+// The maximum over the four lanes of a block of 32: adjacent (STRIDE 1), or
+// eight lanes apart.
+template <int STRIDE>
+__device__ __forceinline__ uint32_t max_of_block(uint32_t x) {
+    if constexpr (STRIDE == 1) {
+        x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xB1, 0xF, 0xF, true));  // lane ^ 1
+        return max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4E, 0xF, 0xF, true));  // lane ^ 2
+    } else {
+        x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x128, 0xF, 0xF, true));  // lane ^ 8
+        const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);            // lane ^ 16
+        return max(r[0], r[1]);
+    }
+}
+
+// The codes of a lane's eight channels, and the exponent byte of the block that
+// it holds with three more lanes.
+template <int STRIDE>
 __device__ __forceinline__ uint32_t coded(const float (&x)[8], uint32_t& e) {
     uint32_t top = 0;  // as integers, NaN above infinity above every number
 #pragma unroll
     for (int n = 0; n < 8; ++n) top = max(top, __float_as_uint(x[n]) & 0x7fffffffu);
-    top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0xB1, 0xF, 0xF, true));  // lane ^ 1
-    top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0x4E, 0xF, 0xF, true));  // lane ^ 2
+    top = max_of_block<STRIDE>(top);
     const int exponent = (int)((top + 0x200000u) >> 23) - 2;  // 1.75 and above: the next power's
     const uint32_t unit = (uint32_t)min(max(exponent, 2), 252);
     e = top >= 0x7f800000u ? 255u : unit;
@@ -299,88 +350,127 @@ __device__ __forceinline__ uint32_t coded(const float (&x)[8], uint32_t& e) {
     return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], scale, 3);
 }
 
-// Word (token, head, w) of the keys and of the values. VEC: 16-byte aligned
-// rows, and the turned channels a multiple of 16.
+struct Item {
+    uint32_t w, t, first;
+};
+__device__ __forceinline__ Item key_item(const Items& d, uint32_t n) {
+    const uint32_t w = take(n, d.words), k = take(n, d.runs);
+    return {w, n, k * d.run};
+}
+__device__ __forceinline__ Item value_item(const Items& d, uint32_t n) {
+    const uint32_t t = n & 7;
+    n >>= 3;
+    const uint32_t w = take(n, d.words), k = take(n, d.runs);
+    return {w, n * 8 + t, k * d.run};
+}
+
+// The place of new token t in head 0, and its position; a further head is a
+// page's tokens on.
+__device__ __forceinline__ Slot slot_of_new(const Cache& c, const Seqs& s, uint32_t t, int& p) {
+    const uint32_t b = seq_at(s, t);
+    const Seq q = seq_of(s, b);
+    p = q.first + ((int)t - q.token);
+    Slot at = slot_of(c, s, b, 0, (uint32_t)max(p, 0));
+    at.ok = at.ok && p >= 0;
+    return at;
+}
+
+// Words of the keys. VEC: 16-byte aligned rows, and the turned channels a
+// multiple of 16.
 template <bool F32, bool VEC>
-__device__ __forceinline__ void append_word(const Append& a, uint64_t item) {
-    if (item >= a.cached) return;
-    const uint32_t words = a.dim / 8, w = item % words;
-    const uint64_t th = item / words;
-    const uint32_t h = th % a.cache.heads, t = th / a.cache.heads;
-    const uint32_t b = seq_at(a.seqs, t);
-    const Seq q = seq_of(a.seqs, b);
-    const int p = q.first + ((int)t - q.token);
-    const Slot at = slot_of(a.cache, a.seqs, b, h, (uint32_t)max(p, 0));
-    const bool ok = at.ok && p >= 0;
-    const int64_t kat = t * a.k.token + h * a.k.head, vat = t * a.v.token + h * a.v.head;
-    float k[8], v[8];
-    if constexpr (VEC) {
-        load8<F32>(a.k.at, kat + 8 * w, k);
-        load8<F32>(a.v.at, vat + 8 * w, v);
-        if (a.table.at && 4 * w < a.table.half) {
-            const uint32_t half = a.table.half;
-            float c[8], s[8];
-            if (a.table.layout == DMX_ROTARY_HALF) {
-                const bool second = 8 * w >= half;
-                const uint32_t other = second ? 8 * w - half : 8 * w + half;
+__device__ __forceinline__ void append_keys(const Append& a, uint32_t item) {
+    const auto [w, t, first] = key_item(a.items, item);
+    if (t >= a.seqs.total) return;
+    int p;
+    const Slot at = slot_of_new(a.cache, a.seqs, t, p);
+    const uint32_t words = a.items.words.value, half = a.table.at ? a.table.half : 0;
+    const bool inter = a.table.layout != DMX_ROTARY_HALF, turned = VEC && 4 * w < half, second = !inter && 8 * w >= half;
+    const uint32_t other = second ? 8 * w - half : 8 * w + half;  // (half layout: the word's partner)
+    float c[8], s[8];
+    if (turned && inter)
+        angles<4>(a.table, p, 4 * w, c, s);
+    else if (turned)
+        angles<8>(a.table, p, second ? other : 8 * w, c, s);
+    for (uint32_t h = first; h < min(first + a.items.run, a.cache.heads); ++h) {
+        const int64_t row = t * a.k.token + h * a.k.head;
+        float k[8];
+        if constexpr (VEC) {
+            load8<F32>(a.k.at, row + 8 * w, k);
+            if (turned && !inter) {
                 float y[8];
-                load8<F32>(a.k.at, kat + other, y);
-                angles(a.table, p, second ? other : 8 * w, c, s);
+                load8<F32>(a.k.at, row + other, y);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     float lo = second ? y[e] : k[e], hi = second ? k[e] : y[e];
                     turn(lo, hi, c[e], s[e]);
                     k[e] = second ? hi : lo;
                 }
-            } else {
-                angles(a.table, p, (4 * w) & ~7u, c, s);
+            } else if (turned) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    turn(k[2 * e], k[2 * e + 1], (w & 1) ? c[4 + e] : c[e], (w & 1) ? s[4 + e] : s[e]);
+                    turn(k[2 * e], k[2 * e + 1], c[e], s[e]);
             }
-        }
-    } else {
-        const bool in = a.table.at && p >= 0 && p < (int)a.table.positions;
+        } else {
+            const bool in = p >= 0 && p < (int)a.table.positions;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t ch = 8 * w + e, half = a.table.half;
-            k[e] = load1<F32>(a.k.at, kat + ch);
-            v[e] = load1<F32>(a.v.at, vat + ch);
-            if (a.table.at && ch < 2 * half) {
-                const bool inter = a.table.layout != DMX_ROTARY_HALF, second = inter ? ch & 1 : ch >= half;
-                const uint32_t other = inter ? ch ^ 1 : second ? ch - half : ch + half;
-                const uint32_t angle = inter ? ch / 2 : second ? other : ch;
-                const float* cs = a.table.at + 2 * ((int64_t)(in ? p : 0) * half + angle);
-                const float y = load1<F32>(a.k.at, kat + other);
-                float lo = second ? y : k[e], hi = second ? k[e] : y;
-                turn(lo, hi, in ? cs[0] : NAN, in ? cs[1] : NAN);
-                k[e] = second ? hi : lo;
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t ch = 8 * w + e;
+                k[e] = load1<F32>(a.k.at, row + ch);
+                if (ch < 2 * half) {
+                    const bool high = inter ? ch & 1 : ch >= half;
+                    const uint32_t partner = inter ? ch ^ 1 : high ? ch - half : ch + half;
+                    const uint32_t angle = inter ? ch / 2 : high ? partner : ch;
+                    const float* cs = a.table.at + 2 * ((int64_t)(in ? p : 0) * half + angle);
+                    const float y = load1<F32>(a.k.at, row + partner);
+                    float lo = high ? y : k[e], hi = high ? k[e] : y;
+                    turn(lo, hi, in ? cs[0] : NAN, in ? cs[1] : NAN);
+                    k[e] = high ? hi : lo;
+                }
             }
         }
+        uint32_t e;
+        const uint32_t word = coded<1>(k, e);
+        if (!at.ok) continue;
+        const uint64_t token = at.token + ((uint64_t)h << a.cache.page_shift);
+        a.cache.k_codes[token * words + w] = word;
+        if ((w & 3) == 0) a.cache.k_scales[token * (words / 4) + w / 4] = (uint8_t)e;
     }
-    uint32_t ke, ve;
-    const uint32_t kw = coded(k, ke), vw = coded(v, ve);
-    if (!ok) return;
-    a.cache.k_codes[at.token * words + w] = kw;
-    const uint64_t octet = at.token >> 3, in_octet = at.token & 7;
-    a.cache.v_codes[(octet * words + w) * 8 + in_octet] = vw;
-    if ((w & 3) == 0) {
-        a.cache.k_scales[at.token * (words / 4) + w / 4] = (uint8_t)ke;
-        a.cache.v_scales[(octet * (words / 4) + w / 4) * 8 + in_octet] = (uint8_t)ve;
+}
+
+template <bool F32, bool VEC>
+__device__ __forceinline__ void append_values(const Append& a, uint32_t item) {
+    const auto [w, t, first] = value_item(a.items, item);
+    if (t >= a.seqs.total) return;
+    int p;
+    const Slot at = slot_of_new(a.cache, a.seqs, t, p);
+    const uint32_t words = a.items.words.value;
+    for (uint32_t h = first; h < min(first + a.items.run, a.cache.heads); ++h) {
+        const int64_t from = t * a.v.token + h * a.v.head + 8 * w;
+        float v[8];
+        if constexpr (VEC)
+            load8<F32>(a.v.at, from, v);
+        else
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = load1<F32>(a.v.at, from + e);
+        uint32_t e;
+        const uint32_t word = coded<8>(v, e);
+        if (!at.ok) continue;
+        const uint64_t token = at.token + ((uint64_t)h << a.cache.page_shift), octet = token >> 3, in = token & 7;
+        a.cache.v_codes[(octet * words + w) * 8 + in] = word;
+        if ((w & 3) == 0) a.cache.v_scales[(octet * (words / 4) + w / 4) * 8 + in] = (uint8_t)e;
     }
 }
 
 template <bool F32, bool VEC>
 __global__ __launch_bounds__(256) void k_append(const Append a) {
-    if (blockIdx.x < a.cached_blocks) {
-        append_word<F32, VEC>(a, (uint64_t)blockIdx.x * 256 + threadIdx.x);
-        return;
-    }
-    const uint64_t item = (uint64_t)(blockIdx.x - a.cached_blocks) * 256 + threadIdx.x;
+    const uint32_t x = threadIdx.x;
+    if (blockIdx.x < a.key_blocks) return append_keys<F32, VEC>(a, blockIdx.x * 256 + x);
+    if (blockIdx.x < a.cached_blocks) return append_values<F32, VEC>(a, (blockIdx.x - a.key_blocks) * 256 + x);
+    const uint32_t item = (blockIdx.x - a.cached_blocks) * 256 + x;
     if constexpr (VEC)
-        rotary_item<F32>(a.q, item);
+        rotate<F32>(a.q, item);
     else
-        rotary_item_any<F32>(a.q, item);
+        rotate_any<F32>(a.q, item);
 }
 
 // ------------------------------------------------------------------- read --
@@ -396,22 +486,22 @@ __device__ __forceinline__ uint4 decoded(uint32_t word, uint32_t e) {
                       __builtin_bit_cast(uint32_t, d));
 }
 
-__global__ __launch_bounds__(256) void k_read(const Cache c, const Seqs s, uint32_t dim, uint16_t* k, uint16_t* v) {
-    const uint64_t item = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    const uint32_t words = dim / 8, w = item % words;
-    const uint64_t th = item / words;
-    const uint32_t h = th % c.heads;
-    if (th / c.heads >= s.total) return;
-    const uint32_t t = th / c.heads, b = seq_at(s, t);
-    const Seq q = seq_of(s, b);
-    const int p = q.first + ((int)t - q.token);
-    const Slot at = slot_of(c, s, b, h, (uint32_t)max(p, 0));
-    const bool ok = at.ok && p >= 0;
-    const uint64_t octet = at.token >> 3, in_octet = at.token & 7;
-    const uint32_t ke = c.k_scales[at.token * (words / 4) + w / 4];
-    const uint32_t ve = c.v_scales[(octet * (words / 4) + w / 4) * 8 + in_octet];
-    reinterpret_cast<uint4*>(k)[item] = decoded(c.k_codes[at.token * words + w], ok ? ke : 255u);
-    reinterpret_cast<uint4*>(v)[item] = decoded(c.v_codes[(octet * words + w) * 8 + in_octet], ok ? ve : 255u);
+// Blocks of keys, then (from the key_blocks-th) of values.
+__global__ __launch_bounds__(256) void k_read(const Cache c, const Seqs s, const Items items, uint32_t key_blocks, uint16_t* k,
+                                              uint16_t* v) {
+    const uint32_t words = items.words.value;
+    const bool keys = blockIdx.x < key_blocks;
+    const uint32_t n = (keys ? blockIdx.x : blockIdx.x - key_blocks) * 256 + threadIdx.x;
+    const auto [w, t, first] = keys ? key_item(items, n) : value_item(items, n);
+    if (t >= s.total) return;
+    int p;
+    const Slot at = slot_of_new(c, s, t, p);
+    for (uint32_t h = first; h < min(first + items.run, c.heads); ++h) {
+        const uint64_t token = at.token + ((uint64_t)h << c.page_shift), octet = token >> 3, in = token & 7;
+        const uint32_t e = keys ? c.k_scales[token * (words / 4) + w / 4] : c.v_scales[(octet * (words / 4) + w / 4) * 8 + in];
+        const uint32_t word = keys ? c.k_codes[token * words + w] : c.v_codes[(octet * words + w) * 8 + in];
+        reinterpret_cast<uint4*>(keys ? k : v)[((uint64_t)t * c.heads + h) * words + w] = decoded(word, at.ok ? e : 255u);
+    }
 }
 
 // -------------------------------------------------------------- attention --
@@ -477,7 +567,14 @@ int check_table(const dmx_rotary_table* t, uint32_t dim, char* err, size_t errn)
 Cache cache_of(const dmx_kv_cache* c) {
     return {c->k_codes, c->v_codes, c->k_scales, c->v_scales, c->pages, c->heads, (uint32_t)__builtin_ctz(c->page)};
 }
-Seqs seqs_of(const dmx_kv_seqs* s) { return {s->table, s->lengths, s->cu, s->batch, s->total, (int)s->table_cols}; }
+Divisor divisor_of(uint32_t d) {
+    uint32_t shift = 0;
+    while ((1ull << shift) < d) ++shift;
+    return {(uint32_t)((((1ull << shift) - d) << 32) / d + 1), shift, d};
+}
+Seqs seqs_of(const dmx_kv_seqs* s) {
+    return {s->table, s->lengths, s->cu, s->batch, s->total, (int)s->table_cols, divisor_of(s->cu ? 1 : std::max(1u, s->total / s->batch))};
+}
 Rows rows_of(const dmx_rows* r) { return {r->at, r->token_stride, r->head_stride, r->heads}; }
 Table table_of(const dmx_rotary_table* t) { return {t->at, t->positions, t->dim / 2, t->layout}; }
 
@@ -487,16 +584,36 @@ bool wide_rows(const dmx_rows* r, int dtype) {
     return aligned(r->at, 16) && r->token_stride % n == 0 && r->head_stride % n == 0;
 }
 
+// Blocks of 256 for `items`, whose numbers the kernels hold in 31 bits.
 int launch_blocks(uint64_t items, uint32_t& blocks, char* err, size_t errn) {
-    const uint64_t n = (items + 255) / 256;
-    if (n >= (1ull << 31)) return fail(err, errn, "too many values for one launch");
-    blocks = (uint32_t)n;
+    if (items >= (1ull << 31) - 256) return fail(err, errn, "too many values for one launch");
+    blocks = (uint32_t)((items + 255) / 256);
     return 0;
 }
 
-uint64_t rotary_items(const Rotation& r, bool wide) {
-    const uint64_t heads = r.in[0].heads + (r.n > 1 ? r.in[1].heads : 0);
-    return (uint64_t)r.tokens * heads * (wide ? r.dim / 16 : r.dim / 2);
+// Heads that a lane takes one after the other: more than one where there are
+// lanes enough to fill the device without (256 CUs of 2048, half of them).
+uint32_t run_of(uint64_t items, uint32_t heads) { return (uint32_t)std::min<uint64_t>({heads, 8, std::max<uint64_t>(1, items >> 18)}); }
+
+// Completes a rotation; its items.
+uint64_t rotary_items(Rotation& r, bool wide) {
+    const uint32_t heads = r.in[0].heads + (r.n > 1 ? r.in[1].heads : 0), per = wide ? r.dim / 16 : r.dim / 2;
+    r.run = run_of((uint64_t)r.tokens * heads * per, heads);
+    const uint32_t runs = (heads + r.run - 1) / r.run;
+    r.per = divisor_of(per);
+    r.runs = divisor_of(runs);
+    return (uint64_t)r.tokens * runs * per;
+}
+
+// The items of a call's keys and values, and their blocks.
+int cached_items(const dmx_kv_cache* c, uint32_t total, Items& d, uint32_t& keys, uint32_t& values, char* err, size_t errn) {
+    const uint32_t words = c->dim / 8;
+    d.run = run_of((uint64_t)total * c->heads * words, c->heads);
+    const uint32_t runs = (c->heads + d.run - 1) / d.run;
+    d.words = divisor_of(words);
+    d.runs = divisor_of(runs);
+    const uint64_t each = (uint64_t)runs * words;
+    return launch_blocks(total * each, keys, err, errn) || launch_blocks((total + 7ull) / 8 * 8 * each, values, err, errn);
 }
 
 }  // namespace
@@ -548,7 +665,6 @@ extern "C" int dmx_kv_append(const dmx_kv_cache* cache, const dmx_kv_seqs* seqs,
     a.cache = cache_of(cache);
     a.seqs = seqs_of(seqs);
     a.k = rows_of(k), a.v = rows_of(v);
-    a.dim = cache->dim;
     bool vec = wide_rows(k, dtype) && wide_rows(v, dtype);
     if (table) {
         a.table = table_of(table);
@@ -561,11 +677,11 @@ extern "C" int dmx_kv_append(const dmx_kv_cache* cache, const dmx_kv_seqs* seqs,
         a.q.table = a.table;
         a.q.seqs = a.seqs;
     }
-    a.cached = (uint64_t)seqs->total * cache->heads * (cache->dim / 8);
-    uint32_t more = 0;
-    if (launch_blocks(a.cached, a.cached_blocks, err, errn) || (q && launch_blocks(rotary_items(a.q, vec), more, err, errn)))
+    uint32_t values, more = 0;
+    if (cached_items(cache, seqs->total, a.items, a.key_blocks, values, err, errn) ||
+        (q && launch_blocks(rotary_items(a.q, vec), more, err, errn)))
         return 1;
-    if ((uint64_t)a.cached_blocks + more >= (1ull << 31)) return fail(err, errn, "too many values for one launch");
+    a.cached_blocks = a.key_blocks + values;
     const auto kern = vec ? (dtype == DMX_F32 ? k_append<true, true> : k_append<false, true>)
                           : (dtype == DMX_F32 ? k_append<true, false> : k_append<false, false>);
     hipLaunchKernelGGL(kern, dim3(a.cached_blocks + more), dim3(256), 0, static_cast<hipStream_t>(stream), a);
@@ -578,10 +694,11 @@ extern "C" int dmx_kv_read(const dmx_kv_cache* cache, const dmx_kv_seqs* seqs, u
     if (seqs->total == 0) return 0;
     if (!k || !v) return fail(err, errn, "null output");
     if (!aligned(k, 16) || !aligned(v, 16)) return fail(err, errn, "outputs not 16-byte aligned");
-    uint32_t blocks;
-    if (launch_blocks((uint64_t)seqs->total * cache->heads * (cache->dim / 8), blocks, err, errn)) return 1;
-    hipLaunchKernelGGL(k_read, dim3(blocks), dim3(256), 0, static_cast<hipStream_t>(stream), cache_of(cache),
-                       seqs_of(seqs), cache->dim, k, v);
+    Items items;
+    uint32_t keys, values;
+    if (cached_items(cache, seqs->total, items, keys, values, err, errn)) return 1;
+    hipLaunchKernelGGL(k_read, dim3(keys + values), dim3(256), 0, static_cast<hipStream_t>(stream), cache_of(cache),
+                       seqs_of(seqs), items, keys, k, v);
     return launch_check(err, errn, "kv read launch");
 }
 
