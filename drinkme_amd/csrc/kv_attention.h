@@ -950,11 +950,15 @@ __global__ __launch_bounds__(256) void k_attend_join(const AttnArgs a, int dim, 
     const int group = lane / per, col = lane - group * per;
     const int stride = groups * (ways == 4 ? 4 : 1);
     f32x4 y = {0.f, 0.f, 0.f, 0.f};
-    const f32x4* from = reinterpret_cast<const f32x4*>(a.part_o + row * dim) + col;
+    const f32x4* from = reinterpret_cast<const f32x4*>(a.part_o + row * dim) + (group < groups ? col : 0);
+    // (no branch, so that loads go ahead of the weights: past the last split, and in
+    // lanes past the last group, a row is read again with weight 0)
 #pragma unroll 4
-    for (int s = (ways == 4 ? wave * groups : 0) + group; s < splits + group; s += stride) {  // (the same count in every lane)
-        const float w = __shfl(weight, s);
-        if (group < groups && s < splits && w != 0.f) y += from[s * (all * per)] * w;
+    for (int s0 = ways == 4 ? wave * groups : 0; s0 < splits; s0 += stride) {
+        const int s = s0 + group;
+        const bool in = group < groups && s < splits;
+        const float w = __shfl(weight, s & 63);
+        y += from[min(s, splits - 1) * (all * per)] * (in ? w : 0.f);
     }
     f32x4 sum = y;
     for (int g = 1; g < groups; ++g)
