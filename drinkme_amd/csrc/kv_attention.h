@@ -221,8 +221,8 @@ __device__ __forceinline__ void hide_values(State<W, P, NR>& st, Block<W>& x, in
 
 // A block's part of the rows' results.
 template <int W, int P, int NR>
-__device__ __forceinline__ void attend_block(State<W, P, NR>& st, Block<W>& x, float scale, int blk, int i, int j, bool part,
-                                             int hi_all) {
+__device__ __forceinline__ void attend_block(State<W, P, NR>& st, Block<W>& x, float scale, int blk, int i, int j, bool first,
+                                             bool part, int hi_all) {
     using S = Segments<W>;
     const int t0 = blk * 32 + 8 * j;  // this lane's scores are of tokens t0 .. t0 + 7
 
@@ -248,9 +248,11 @@ __device__ __forceinline__ void attend_block(State<W, P, NR>& st, Block<W>& x, f
         }
     }
 
-    // softmax: the reference mx follows the maximum only when a score passes it
-    // by 2^8, so that most blocks need no product over the lanes and no
-    // rescaling; weights up to 2^8 cost no precision
+    // Softmax. A row's reference is the maximum of the first scores that it sees;
+    // later scores are weighed by it as they come, without a look at their maximum
+    // (weights above 1 cost no precision), until a lane's sum passes 2^20: then the
+    // block is weighed again by a higher one. A row sees its first scores in a wave's
+    // first block or where part is set.
     bf16x8 pf[NR][P];
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
@@ -258,26 +260,43 @@ __device__ __forceinline__ void attend_block(State<W, P, NR>& st, Block<W>& x, f
 #pragma unroll
         for (int e = 0; e < 8; ++e) p[e] = sc[t][e >> 2][e & 3];
         if (part) {
+            int at = t0;
+            asm volatile("" : "+v"(at));  // (a branch: else the comparisons are made for every block)
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (t0 + e < st.lo[t] || t0 + e >= st.hi[t]) p[e] = -INFINITY;
+                if (at + e < st.lo[t] || at + e >= st.hi[t]) p[e] = -INFINITY;
         }
-        float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7]))) * scale;
-        if (__any(top > st.mx[t] + 8.f)) {
-            top = fmaxf(st.mx[t], max_over_j(top));
-            const float alpha = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.mx[t] - top);
+        const auto top_of = [&] {
+            const float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+            return max_over_j(top * scale);
+        };
+        const auto refer_to = [&](float to) {
+            const float alpha = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.mx[t] - to);
             st.sum[t] *= alpha;
 #pragma unroll
             for (int c = 0; c < 2 * W; ++c) st.o[t][c] *= alpha;
-            st.mx[t] = top;
-        }
-        const float base = st.mx[t] == -INFINITY ? 0.f : -st.mx[t];
+            st.mx[t] = to;
+        };
+        if (part || first) refer_to(fmaxf(st.mx[t], top_of()));
+        float w[8], before = st.sum[t];
+        const auto weigh = [&] {
+            const float base = st.mx[t] == -INFINITY ? 0.f : -st.mx[t];
+            st.sum[t] = before;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], scale, base));
-            st.sum[t] += p[e];
+            for (int e = 0; e < 8; ++e) {
+                w[e] = __builtin_amdgcn_exp2f(fmaf(p[e], scale, base));
+                st.sum[t] += w[e];
+            }
+        };
+        weigh();
+        if (__any(st.sum[t] > 0x1p20f)) {
+            const float top = top_of();
+            st.sum[t] = before;
+            refer_to(max_over_j(before + w[0] + w[1] + w[2] + w[3] + w[4] + w[5] + w[6] + w[7]) > 0x1p20f ? fmaxf(st.mx[t] + 16.f, top) : st.mx[t]);
+            before = st.sum[t];
+            weigh();
         }
-        pieces<P>(p, pf[t]);
+        pieces<P>(w, pf[t]);
     }
 
     if (part) hide_values(st, x, t0, hi_all);
@@ -362,17 +381,17 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
         st.hi[t] = ok ? hi_of(m) : 0;
         st.lo[t] = lo_of(m);
         const int64_t token = q.token + m, head = (int64_t)h * a.group + g;
-        row_out[t] = ok ? token * a.q_heads + head : -1;
+        row_out[t] = ok ? token * a.q_heads + head : -1;  // (past the last row: the first one's queries, unused)
         const int64_t at = token * a.q_token + head * a.q_head + 8 * W * j;
 #pragma unroll
         for (int c = 0; c < W; ++c) {
             if constexpr (P == 1) {
-                u32x4 f = {0, 0, 0, 0};
-                if (ok) __builtin_memcpy(&f, static_cast<const uint16_t*>(a.q) + at + 8 * c, 16);
+                u32x4 f;
+                __builtin_memcpy(&f, static_cast<const uint16_t*>(a.q) + at + 8 * c, 16);
                 st.q[t][0][c] = __builtin_bit_cast(bf16x8, f);
             } else {
                 float f[8];
-                for (int n = 0; n < 8; ++n) f[n] = ok ? static_cast<const float*>(a.q)[at + 8 * c + n] : 0.f;
+                __builtin_memcpy(f, static_cast<const float*>(a.q) + at + 8 * c, 32);
                 bf16x8 split_f[P];
                 pieces<P>(f, split_f);
 #pragma unroll
@@ -387,7 +406,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
 
     const auto work = [&](Block<W>& y) {
         const bool part = blk * 32 < full_lo || blk * 32 + 32 > full_hi;
-        attend_block(st, y, a.scale, blk, i, j, part, hi_all);
+        attend_block(st, y, a.scale, blk, i, j, blk < blk_first + step, part, hi_all);
         blk += step;
     };
     if (blk < blk_end) {
@@ -725,14 +744,17 @@ __global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_a
     };
     const auto write_v = [&](int s) { part_write<W>(lds, s, vpart, lane, hi_all, vraw); };
     const auto write_k = [&](int s) { part_write<W>(lds, s, kpart, lane, hi_all, kraw); };
+    uint32_t early[G::raw];  // keys of the set before the first: of its second block are the first scores
     if (s_first < s_end) {
-        if (does_v) {
-            page[0] = part_page<WIDE>(a, b, s_first - 1, vpart, lane);
-            next_v(s_first - 1);
-        }
         if (does_k) {
-            page[1] = part_page<WIDE>(a, b, s_first - 1, kpart, lane);
-            next_k(s_first - 1);
+            const uint32_t p = part_page<WIDE>(a, b, s_first - 1, kpart, lane);
+            page[1] = part_page<WIDE>(a, b, s_first, kpart, lane);
+            part_load<WIDE, W>(a, h, s_first - 1, kpart, lane, p, early);
+            next_k(s_first);
+        }
+        if (does_v) {
+            page[0] = part_page<WIDE>(a, b, s_first, vpart, lane);
+            next_v(s_first);
         }
     }
 
@@ -740,14 +762,15 @@ __global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_a
     const bool mine = some && r < rows;
     const int m = mine ? new_of(r) : 0, g = mine ? r - m * (int)a.group : 0;
     const int hi = mine ? hi_of(m) : 0, lo = lo_of(m);
+    // (past the last row: the first one's queries, unused)
     const int64_t token = q.token + m, head = (int64_t)h * a.group + g, row_out = token * a.q_heads + head;
     bf16x8 qf[2 * W];
     {
         const uint16_t* at = static_cast<const uint16_t*>(a.q) + token * a.q_token + head * a.q_head + 16 * W * f;
 #pragma unroll
         for (int c = 0; c < 2 * W; ++c) {
-            u32x4 x = {0, 0, 0, 0};
-            if (mine) __builtin_memcpy(&x, at + 8 * c, 16);
+            u32x4 x;
+            __builtin_memcpy(&x, at + 8 * c, 16);
             qf[c] = __builtin_bit_cast(bf16x8, x);
         }
     }
@@ -775,11 +798,29 @@ __global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_a
     };
     const auto keys = [&](int s, int n) { return lds + (s & 1) * G::bytes + n * G::block + lane * 16; };
     const auto values = [&](int s, int n) { return lds + (s & 1) * G::bytes + (2 + n) * G::block + lane * 16; };
-    // Of block n's scores: what a row does not see, and the rows' references. Where
-    // one rises, weights taken before (of the block whose values are at `from`) go
-    // into the products first.
-    const auto turn_to = [&](int n, f32x16& x, const char* from) {
-        if (n * 32 < full_lo || n * 32 + 32 > full_hi) {
+    const auto top_of = [&](const f32x16& x) {
+        float top = x[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
+        top *= a.scale;
+        const auto swap = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+        return fmaxf(__uint_as_float(swap[0]), __uint_as_float(swap[1]));
+    };
+    const auto refer_to = [&](float to) {
+        const float alpha = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - to);
+        sum *= alpha;
+#pragma unroll
+        for (int c = 0; c < W; ++c) o[c] *= alpha;
+        mx = to;
+    };
+    // Where rows may see their first scores (in the first block and in those that
+    // not every row sees all of): what a row does not see of block n's, and its
+    // reference. Weights taken before (of the block whose values are at `from`)
+    // go into the products first.
+    const auto turn_to = [&](int n, f32x16& x, const char* from, bool start) {
+        const bool part = n * 32 < full_lo || n * 32 + 32 > full_hi;
+        if (!part && !start) return;
+        if (part) {
             int t = n * 32 + 8 * f;
             asm volatile("" : "+v"(t));  // (a branch: else the comparisons are made for every block)
 #pragma unroll
@@ -788,28 +829,15 @@ __global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_a
                 if (at < lo || at >= hi) x[e] = -INFINITY;
             }
         }
-        float top = x[0];
-#pragma unroll
-        for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
-        top *= a.scale;
-        if (__any(top > mx + 8.f)) {
-            asm volatile("" : "+v"(from));  // (else the operands are read ahead of the branch, for both sides)
-            add_up(from);
-            pf[0] = pf[1] = __builtin_bit_cast(bf16x8, u32x4{0, 0, 0, 0});
-            const auto swap = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-            top = fmaxf(mx, fmaxf(__uint_as_float(swap[0]), __uint_as_float(swap[1])));
-            const float alpha = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - top);
-            sum *= alpha;
-#pragma unroll
-            for (int c = 0; c < W; ++c) o[c] *= alpha;
-            mx = top;
-        }
+        const float top = top_of(x);
+        if (!__any(top > mx + 8.f)) return;
+        asm volatile("" : "+v"(from));  // (else the operands are read ahead of the branch, for both sides)
+        add_up(from);
+        pf[0] = pf[1] = __builtin_bit_cast(bf16x8, u32x4{0, 0, 0, 0});
+        refer_to(fmaxf(mx, top));
     };
-    // block x's weights; the scores of the block after it, and the products of the one before
-    const auto block = [&](f32x16& x, f32x16& next, const char* k, const char* v) {
+    const auto weigh = [&](const f32x16& x) {
         const float base = mx == -INFINITY ? 0.f : -mx;
-        score(k, next);
-        add_up(v);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             const float p = __builtin_amdgcn_exp2f(fmaf(x[e], a.scale, base));
@@ -817,6 +845,21 @@ __global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_a
             pf[e >> 3][e & 7] = (__bf16)p;
         }
         asm volatile("" : "+v"(pf[0]), "+v"(pf[1]), "+v"(sum));  // (here, beside the products, not where they are used)
+    };
+    // block x's weights; the scores of the block after it, and the products of the one before
+    // (later scores are weighed by a row's reference as they come: k_attend)
+    const auto block = [&](f32x16& x, f32x16& next, const char* k, const char* v) {
+        const float before = sum;
+        score(k, next);
+        add_up(v);
+        weigh(x);
+        if (__any(sum > 0x1p20f)) {
+            const auto swap = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+            const bool over = fmaxf(__uint_as_float(swap[0]), __uint_as_float(swap[1])) > 0x1p20f;
+            sum = before;
+            refer_to(over ? fmaxf(mx + 16.f, top_of(x)) : mx);
+            weigh(x);
+        }
     };
     // NaN blocks among a set's values: NaN in the rows that see one
     const auto mark_nan = [&](int s) {
@@ -847,19 +890,16 @@ __global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_a
     };
 
     if (s_first < s_end) {
-        const auto both = [&](int s) {
-            if (does_v) {
-                write_v(s);
-                next_v(s + 1);
-            }
-            if (does_k) {
-                write_k(s);
-                next_k(s + 1);
-            }
-        };
-        both(s_first - 1);
+        if (does_k) {
+            part_write<W>(lds, s_first - 1, kpart, lane, hi_all, early);
+            write_k(s_first);
+            next_k(s_first + 1);
+        }
+        if (does_v) {
+            write_v(s_first);
+            next_v(s_first + 1);
+        }
         __syncthreads();
-        both(s_first);
         score(keys(s_first - 1, 1), sc[0]);
         for (int s = s_first; s < s_end; ++s) {
             __syncthreads();  // (set s is written, and set s - 1 read)
@@ -871,7 +911,7 @@ __global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_a
             const bool seen = 64 * s - 32 < see_hi && 64 * s + 96 > see_lo;
             if (seen) {
                 mark_nan(s);
-                turn_to(2 * s, sc[0], values(s, 0));
+                turn_to(2 * s, sc[0], values(s, 0), s == s_first);
                 block(sc[0], sc[1], keys(s, 0), values(s, 0));
             }
             if (does_k) {
@@ -879,7 +919,7 @@ __global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_a
                 next_k(s + 2);
             }
             if (seen) {
-                turn_to(2 * s + 1, sc[1], values(s, 1));
+                turn_to(2 * s + 1, sc[1], values(s, 1), false);
                 block(sc[1], sc[0], keys(s, 1), values(s, 1));
             }
         }

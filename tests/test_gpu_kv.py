@@ -325,6 +325,45 @@ def test_attention_at_large_scores():
         check_attention(b, held, q, "bf16", got, lse, scale=scale)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("tokens", [1, 5, 40])
+@pytest.mark.parametrize("shape", ["rise", "steps", "spike", "fall"])
+def test_scores_that_leave_their_first_block_behind(shape, tokens, dtype):
+    """Scores that grow along the context by more than weights of the first
+    block's scale can hold (to hundreds of powers of two), gently, at a step or
+    at one token, or that fall away from it."""
+    rng = np.random.default_rng(20)
+    D, length = 64, 900
+    b = Batch(rng, [(tokens, length), (tokens, length - 7)], 1, D, 32)
+    total = 2 * length - 7
+    at = np.concatenate([np.arange(length), np.arange(length - 7)]) / length
+    gain = {"rise": at * 60, "steps": np.floor(at * 8) * 9, "spike": 40.0 * (np.abs(at - 0.6) < 0.5 / length),
+            "fall": 60 - 60 * at}[shape]
+    direction = np.sign(rng.standard_normal(D))
+    k = torch.from_numpy((gain[:, None, None] * direction + rng.standard_normal((total, 1, D))).astype(np.float32)).cuda()
+    held = b.fill(rng, k.to(torch.bfloat16), heads(rng, (total, 1, D), "bf16"))
+    q = torch.from_numpy((direction * (1 + 0.1 * rng.standard_normal((2 * tokens, 3, D)))).astype(np.float32)).cuda().to(DT[dtype])
+    got, lse = kv_ops.attention(q, b.cache, b.block_table, b.lengths, return_lse=True)
+    check_attention(b, held, q, dtype, got, lse)
+
+
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_sums_of_many_weights_above_one(tokens):
+    """A long context whose scores lie a little above the first block's: a
+    lane's sum passes what the kernels let it grow to, no single weight does."""
+    rng = np.random.default_rng(21)
+    D, length = 64, 70000
+    b = Batch(rng, [(tokens, length)], 1, D, 128)
+    direction = np.sign(rng.standard_normal(D))
+    gain = np.full(length, 1.0)
+    gain[:8192] = 0.0
+    k = torch.from_numpy((gain[:, None, None] * direction + 0.2 * rng.standard_normal((length, 1, D))).astype(np.float32)).cuda()
+    held = b.fill(rng, k.to(torch.bfloat16), heads(rng, (length, 1, D), "bf16"))
+    q = torch.from_numpy((direction * 10.0 / 8 * np.ones((tokens, 1, D))).astype(np.float32)).cuda().to(torch.bfloat16)
+    got, lse = kv_ops.attention(q, b.cache, b.block_table, b.lengths, max_length=512, return_lse=True)  # (one split)
+    check_attention(b, held, q, "bf16", got, lse)
+
+
 def test_rows_that_see_nothing():
     rng = np.random.default_rng(8)
     b = Batch(rng, [(6, 6)] * 2, 1, 64, 8)
