@@ -221,7 +221,7 @@ __device__ __forceinline__ void hide_values(State<W, P, NR>& st, Block<W>& x, in
 
 // A block's part of the rows' results.
 template <int W, int P, int NR>
-__device__ __forceinline__ void attend_block(State<W, P, NR>& st, Block<W>& x, float scale, int blk, int i, int j, bool first,
+__device__ __forceinline__ void attend_block(State<W, P, NR>& st, Block<W>& x, float scale, int blk, int i, int j, bool fresh,
                                              bool part, int hi_all) {
     using S = Segments<W>;
     const int t0 = blk * 32 + 8 * j;  // this lane's scores are of tokens t0 .. t0 + 7
@@ -251,8 +251,8 @@ __device__ __forceinline__ void attend_block(State<W, P, NR>& st, Block<W>& x, f
     // Softmax. A row's reference is the maximum of the first scores that it sees;
     // later scores are weighed by it as they come, without a look at their maximum
     // (weights above 1 cost no precision), until a lane's sum passes 2^20: then the
-    // block is weighed again by a higher one. A row sees its first scores in a wave's
-    // first block or where part is set.
+    // block is weighed again by a higher one. fresh: a row may see its first scores
+    // of the wave's here.
     bf16x8 pf[NR][P];
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
@@ -277,7 +277,7 @@ __device__ __forceinline__ void attend_block(State<W, P, NR>& st, Block<W>& x, f
             for (int c = 0; c < 2 * W; ++c) st.o[t][c] *= alpha;
             st.mx[t] = to;
         };
-        if (part || first) refer_to(fmaxf(st.mx[t], top_of()));
+        if (fresh) refer_to(fmaxf(st.mx[t], top_of()));
         float w[8], before = st.sum[t];
         const auto weigh = [&] {
             const float base = st.mx[t] == -INFINITY ? 0.f : -st.mx[t];
@@ -406,7 +406,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
 
     const auto work = [&](Block<W>& y) {
         const bool part = blk * 32 < full_lo || blk * 32 + 32 > full_hi;
-        attend_block(st, y, a.scale, blk, i, j, blk < blk_first + step, part, hi_all);
+        // (a row that sees nothing of the wave's block before this one sees it from full_lo at the latest)
+        const bool fresh = blk < blk_first + step || (blk - step) * 32 < full_lo;
+        attend_block(st, y, a.scale, blk, i, j, fresh, part, hi_all);
         blk += step;
     };
     if (blk < blk_end) {
@@ -813,13 +815,12 @@ __global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_a
         for (int c = 0; c < W; ++c) o[c] *= alpha;
         mx = to;
     };
-    // Where rows may see their first scores (in the first block and in those that
-    // not every row sees all of): what a row does not see of block n's, and its
-    // reference. Weights taken before (of the block whose values are at `from`)
-    // go into the products first.
+    // Of block n's scores what a row does not see, and where rows may see their
+    // first ones (in the first block, and up to the one after the last that begins
+    // before full_lo) their references. Weights taken before (of the block whose
+    // values are at `from`) go into the products first.
     const auto turn_to = [&](int n, f32x16& x, const char* from, bool start) {
         const bool part = n * 32 < full_lo || n * 32 + 32 > full_hi;
-        if (!part && !start) return;
         if (part) {
             int t = n * 32 + 8 * f;
             asm volatile("" : "+v"(t));  // (a branch: else the comparisons are made for every block)
@@ -829,6 +830,7 @@ __global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_a
                 if (at < lo || at >= hi) x[e] = -INFINITY;
             }
         }
+        if (!start && (n - 1) * 32 >= full_lo) return;
         const float top = top_of(x);
         if (!__any(top > mx + 8.f)) return;
         asm volatile("" : "+v"(from));  // (else the operands are read ahead of the branch, for both sides)

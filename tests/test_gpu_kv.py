@@ -301,6 +301,21 @@ def test_attention_row_tiles(tokens, group):
     check_attention(b, held, q, "bf16", got, lse)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("window", [None, 31, 32, 33, 64, 97, 200])
+@pytest.mark.parametrize("tokens, length, group", [(330, 330, 4), (150, 700, 3), (600, 600, 1), (8, 500, 4), (5, 1000, 13),
+                                                   (1, 777, 16)])
+def test_windows_that_begin_anywhere(tokens, length, group, window, dtype):
+    """Rows of many workgroups and waves, each with its own first token: on a
+    block's edge, inside a block, in a block that another wave takes."""
+    rng = np.random.default_rng(tokens + group)
+    b = Batch(rng, [(tokens, length)], 1, 64, 32)
+    held = b.fill(rng)
+    q = heads(rng, (tokens, group, 64), dtype, 1.5)
+    got, lse = kv_ops.attention(q, b.cache, b.block_table, b.lengths, window=window, return_lse=True)
+    check_attention(b, held, q, dtype, got, lse, True, window)
+
+
 @pytest.mark.parametrize("max_length", [None, 1, 700, 10 ** 9])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_attention_over_splits(dtype, max_length):
