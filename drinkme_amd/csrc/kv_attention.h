@@ -12,8 +12,9 @@
 //
 // The operands are exact: a code times its power of two is a bf16 number
 // (v_cvt_scalef32_pk_bf16_fp4, two values an instruction). What is rounded:
-// P, to bf16, whose error averages out over the tokens (2^-8 of a weight at
-// most; the row's sum adds the unrounded ones); fp32 queries and their P go as
+// P, to bf16, 2^-8 of a weight at most, whose error averages out over the tokens
+// (a row is divided by the sum of its rounded weights, so that the error cancels
+// where few weights make the result; the logarithm takes the unrounded sum); fp32 queries and their P go as
 // three bf16 pieces, 24 bits, and lose nothing.
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -35,7 +36,7 @@ struct AttnArgs {
     void* out;
     float* lse;
     float* part_o;   // [splits][total * q_heads][dim]
-    float2* part_ml; // [splits][total * q_heads]: maximum (log2 domain), sum
+    f32x4* part_stat;  // [splits][total * q_heads]: reference (log2 domain), sum, sum of the rounded weights
 };
 
 // Segments of V: 128 channels (lane i reads word i, 8 channels), then 64
@@ -118,6 +119,15 @@ __device__ __forceinline__ float sum_over_j(float x) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// sum plus the eight numbers of x.
+__device__ __forceinline__ float plus_all(const bf16x8& x, float sum) {
+    const u32x4 w = __builtin_bit_cast(u32x4, x);
+    const bf16x2 ones = {(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+    for (int n = 0; n < 4; ++n) sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, (uint32_t)w[n]), ones, sum, false);
+    return sum;
+}
+
 // x as P bf16 pieces whose sum it is (to 8 P bits).
 template <int P>
 __device__ __forceinline__ void pieces(const float (&x)[8], bf16x8 (&out)[P]) {
@@ -140,6 +150,7 @@ struct State {
     int hi[NR], lo[NR];  // the positions that the lane's row sees
     bf16x8 q[NR][P][W];
     float mx[NR], sum[NR];  // the weights' reference (log2 domain) and the lane's share of their sum
+    float norm[NR];         // the same of the weights as rounded
     f32x4 o[NR][NT];        // channels 4 j + r of tile n, in Segments' order
 };
 
@@ -273,6 +284,7 @@ __device__ __forceinline__ void attend_block(State<W, P, NR>& st, Block<W>& x, f
         const auto refer_to = [&](float to) {
             const float alpha = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.mx[t] - to);
             st.sum[t] *= alpha;
+            st.norm[t] *= alpha;
 #pragma unroll
             for (int c = 0; c < 2 * W; ++c) st.o[t][c] *= alpha;
             st.mx[t] = to;
@@ -297,6 +309,7 @@ __device__ __forceinline__ void attend_block(State<W, P, NR>& st, Block<W>& x, f
             weigh();
         }
         pieces<P>(w, pf[t]);
+        if constexpr (P == 1) st.norm[t] = plus_all(pf[t][0], st.norm[t]);
     }
 
     if (part) hide_values(st, x, t0, hi_all);
@@ -399,7 +412,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
             }
         }
         st.mx[t] = -INFINITY;
-        st.sum[t] = 0.f;
+        st.sum[t] = st.norm[t] = 0.f;
 #pragma unroll
         for (int c = 0; c < NT; ++c) st.o[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -432,34 +445,42 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
     }
 
 #pragma unroll
-    for (int t = 0; t < NR; ++t) st.sum[t] = sum_over_j(st.sum[t]);
+    for (int t = 0; t < NR; ++t) {
+        st.sum[t] = sum_over_j(st.sum[t]);
+        st.norm[t] = P == 1 ? sum_over_j(st.norm[t]) : st.sum[t];
+    }
 
     // the waves' results into wave 0's: 3 to 1 and 2 to 0, then 1 to 0
     if constexpr (!ROWS) {
-        __shared__ float stat[kAttnWaves][NR][16][2];
+        __shared__ float stat[kAttnWaves][NR][16][3];
         __shared__ f32x4 buf[2][NT][64];
         if (j == 0) {
 #pragma unroll
             for (int t = 0; t < NR; ++t) {
                 stat[wave][t][i][0] = st.mx[t];
                 stat[wave][t][i][1] = st.sum[t];
+                stat[wave][t][i][2] = st.norm[t];
             }
         }
         __syncthreads();
 #pragma unroll
         for (int t = 0; t < NR; ++t) {
-            float top = -INFINITY, total = 0.f;
+            float top = -INFINITY, total = 0.f, norm = 0.f;
 #pragma unroll
             for (int w = 0; w < kAttnWaves; ++w) top = fmaxf(top, stat[w][t][i][0]);
             const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-            for (int w = 0; w < kAttnWaves; ++w)
-                total += stat[w][t][i][1] * __builtin_amdgcn_exp2f(stat[w][t][i][0] - base);
+            for (int w = 0; w < kAttnWaves; ++w) {
+                const float weight = __builtin_amdgcn_exp2f(stat[w][t][i][0] - base);
+                total += stat[w][t][i][1] * weight;
+                norm += stat[w][t][i][2] * weight;
+            }
             const float own = __builtin_amdgcn_exp2f(st.mx[t] - base);
 #pragma unroll
             for (int c = 0; c < NT; ++c) st.o[t][c] *= own;
             st.mx[t] = top;
             st.sum[t] = total;
+            st.norm[t] = norm;
         }
 #pragma unroll
         for (int t = 0; t < NR; ++t) {
@@ -489,10 +510,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
         if (row_out[t] < 0) continue;
         float sum = st.sum[t];
         if (st.hi[t] > cap) sum = NAN;  // it sees positions that the table has no page for
-        const float inv = !done || sum == 0.f ? 1.f : 1.f / sum;
+        const float inv = !done || st.norm[t] == 0.f ? 1.f : 1.f / st.norm[t];
         if (j == 0) {
             if (!done)
-                a.part_ml[split * all + row_out[t]] = make_float2(st.mx[t], sum);
+                a.part_stat[split * all + row_out[t]] = f32x4{st.mx[t], sum, st.norm[t], 0.f};
             else if (a.lse)
                 a.lse[row_out[t]] = sum == 0.f ? -INFINITY : (st.mx[t] + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f;
         }
@@ -694,7 +715,8 @@ __device__ __forceinline__ void part_write(char* lds, int s, int part, int lane,
         write_half<W, 0>(to, lane, raw);
 }
 
-template <int W, bool WIDE>
+// LSE: the unrounded weights are summed, too.
+template <int W, bool WIDE, bool LSE>
 __global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_attend_prompt(const AttnArgs a) {
     using S = Segments<W>;
     using G = Set<W>;
@@ -776,7 +798,7 @@ __global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_a
             qf[c] = __builtin_bit_cast(bf16x8, x);
         }
     }
-    float mx = -INFINITY, sum = 0.f;
+    float mx = -INFINITY, sum = 0.f, norm = 0.f;  // (the reference; the lane's share of the sums)
     f32x16 o[W], sc[2];
     bf16x8 pf[2];  // the last block's weights
 #pragma unroll
@@ -791,6 +813,7 @@ __global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_a
             to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(from + c * G::frag), qf[c], to, 0, 0, 0);
     };
     const auto add_up = [&](const char* from) {
+        norm = plus_all(pf[1], plus_all(pf[0], norm));
 #pragma unroll
         for (int z = 0; z < 2; ++z)
 #pragma unroll
@@ -811,6 +834,7 @@ __global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_a
     const auto refer_to = [&](float to) {
         const float alpha = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx - to);
         sum *= alpha;
+        norm *= alpha;
 #pragma unroll
         for (int c = 0; c < W; ++c) o[c] *= alpha;
         mx = to;
@@ -838,28 +862,38 @@ __global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_a
         pf[0] = pf[1] = __builtin_bit_cast(bf16x8, u32x4{0, 0, 0, 0});
         refer_to(fmaxf(mx, top));
     };
-    const auto weigh = [&](const f32x16& x) {
+    const auto weigh = [&](const f32x16& x) {  // -> the lane's largest weight
         const float base = mx == -INFINITY ? 0.f : -mx;
+        float most = 0.f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             const float p = __builtin_amdgcn_exp2f(fmaf(x[e], a.scale, base));
-            sum += p;
+            if constexpr (LSE) sum += p;
+            most = fmaxf(most, p);
             pf[e >> 3][e & 7] = (__bf16)p;
         }
-        asm volatile("" : "+v"(pf[0]), "+v"(pf[1]), "+v"(sum));  // (here, beside the products, not where they are used)
+        asm volatile("" : "+v"(pf[0]), "+v"(pf[1]), "+v"(sum), "+v"(most));  // (here, beside the products, not where they are used)
+        return most;
     };
     // block x's weights; the scores of the block after it, and the products of the one before
-    // (later scores are weighed by a row's reference as they come: k_attend)
+    // (later scores are weighed by a row's reference as they come, until a weight
+    // passes 2^20: k_attend)
     const auto block = [&](f32x16& x, f32x16& next, const char* k, const char* v) {
         const float before = sum;
-        score(k, next);
-        add_up(v);
-        weigh(x);
-        if (__any(sum > 0x1p20f)) {
-            const auto swap = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+        norm = plus_all(pf[1], plus_all(pf[0], norm));
+        next = f32x16{};
+#pragma unroll
+        for (int n = 0; n < 2 * W; ++n) {
+            next = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(k + n * G::frag), qf[n], next, 0, 0, 0);
+            const int c = n % W, z = n / W;
+            o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(v + (2 * c + z) * G::frag), pf[z], o[c], 0, 0, 0);
+        }
+        const float most = weigh(x);
+        if (__any(most > 0x1p20f)) {
+            const auto swap = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
             const bool over = fmaxf(__uint_as_float(swap[0]), __uint_as_float(swap[1])) > 0x1p20f;
             sum = before;
-            refer_to(over ? fmaxf(mx + 16.f, top_of(x)) : mx);
+            refer_to(over ? fmaxf(mx, top_of(x)) : mx);
             weigh(x);
         }
     };
@@ -930,18 +964,22 @@ __global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_a
         add_up(values(s_end, 0));
     }
     {
-        const auto swap = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
-        sum = __uint_as_float(swap[0]) + __uint_as_float(swap[1]);
+        const auto both = [](float x) {
+            const auto swap = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+            return __uint_as_float(swap[0]) + __uint_as_float(swap[1]);
+        };
+        norm = both(norm);
+        sum = LSE ? both(sum) : norm;
     }
     if (!mine) return;
     if (hi > cap) sum = NAN;  // it sees positions that the table has no page for
     const bool done = a.splits == 1;
     const int64_t at = done ? row_out : (int64_t)split * a.seqs.total * a.q_heads + row_out;
-    const float inv = !done || sum == 0.f ? 1.f : 1.f / sum;
+    const float inv = !done || norm == 0.f ? 1.f : 1.f / norm;
     if (f == 0) {
         if (!done)
-            a.part_ml[at] = make_float2(mx, sum);
-        else if (a.lse)
+            a.part_stat[at] = f32x4{mx, sum, norm, 0.f};
+        else if (LSE)
             a.lse[at] = sum == 0.f ? -INFINITY : (mx + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f;
     }
 #pragma unroll
@@ -978,16 +1016,18 @@ __global__ __launch_bounds__(256) void k_attend_join(const AttnArgs a, int dim, 
     const int64_t row = ways == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
     if (row >= all) return;
     const int splits = (int)a.splits, per = dim / 4, groups = 64 / per;
-    float2 ml = make_float2(-INFINITY, 0.f);
-    if (lane < splits) ml = a.part_ml[lane * all + row];
-    float top = ml.x;
+    f32x4 stat = {-INFINITY, 0.f, 0.f, 0.f};
+    if (lane < splits) stat = a.part_stat[lane * all + row];
+    float top = stat[0];
 #pragma unroll
     for (int n = 32; n; n >>= 1) top = fmaxf(top, __shfl_xor(top, n));
-    const float weight = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
-    float total = ml.y * weight;
-    if (ml.y != ml.y) total = NAN;
+    const float weight = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(stat[0] - top);
+    float total = stat[1] != stat[1] ? NAN : stat[1] * weight, norm = stat[2] * weight;
 #pragma unroll
-    for (int n = 32; n; n >>= 1) total += __shfl_xor(total, n);
+    for (int n = 32; n; n >>= 1) {
+        total += __shfl_xor(total, n);
+        norm += __shfl_xor(norm, n);
+    }
 
     const int group = lane / per, col = lane - group * per;
     const int stride = groups * (ways == 4 ? 4 : 1);
@@ -1012,7 +1052,7 @@ __global__ __launch_bounds__(256) void k_attend_join(const AttnArgs a, int dim, 
         if (wave) return;
         sum += part[0][lane] + part[1][lane] + part[2][lane];
     }
-    const float inv = total == 0.f ? 1.f : 1.f / total;
+    const float inv = norm == 0.f ? 1.f : 1.f / norm;
     if (lane < per) {
         f32x4 v = sum * inv;
         if (total != total) v = f32x4{NAN, NAN, NAN, NAN};

@@ -741,7 +741,7 @@ Plan plan_of(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t q_heads, int 
 }
 
 uint64_t workspace_of(const Plan& p, const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t q_heads) {
-    return p.splits == 1 ? 0 : (uint64_t)p.splits * s->total * q_heads * (c->dim + 2) * 4;
+    return p.splits == 1 ? 0 : (uint64_t)p.splits * s->total * q_heads * (c->dim + 4) * 4;
 }
 
 // Lets a kernel have `bytes` of dynamic LDS on the current device (over 64 KB
@@ -765,9 +765,10 @@ int launch_attend(const Plan& p, int dtype, dim3 grid, hipStream_t stream, const
         else
             hipLaunchKernelGGL((k_attend<W, 3, 1, false, WIDE>), grid, block, 0, stream, a);
     } else if (p.rows) {
-        static std::atomic<uint64_t> allowed{0};
-        if (allow_lds(reinterpret_cast<const void*>(k_attend_prompt<W, WIDE>), Set<W>::lds, allowed, err, errn)) return 1;
-        hipLaunchKernelGGL((k_attend_prompt<W, WIDE>), grid, dim3(64 * prompt_waves(W)), Set<W>::lds, stream, a);
+        static std::atomic<uint64_t> allowed[2] = {};
+        const auto kern = a.lse ? k_attend_prompt<W, WIDE, true> : k_attend_prompt<W, WIDE, false>;
+        if (allow_lds(reinterpret_cast<const void*>(kern), Set<W>::lds, allowed[a.lse != nullptr], err, errn)) return 1;
+        hipLaunchKernelGGL(kern, grid, dim3(64 * prompt_waves(W)), Set<W>::lds, stream, a);
     } else if (p.tiles == 1) {
         hipLaunchKernelGGL((k_attend<W, 1, 1, false, WIDE>), grid, block, 0, stream, a);
     } else if (p.tiles == 2) {
@@ -814,7 +815,7 @@ extern "C" int dmx_kv_attention(const dmx_kv_cache* cache, const dmx_kv_seqs* se
     a.out = out, a.lse = lse;
     const uint64_t all = (uint64_t)seqs->total * q->heads;
     a.part_o = static_cast<float*>(workspace);
-    a.part_ml = reinterpret_cast<float2*>(a.part_o + (p.splits > 1 ? p.splits * all * cache->dim : 0));
+    a.part_stat = reinterpret_cast<f32x4*>(a.part_o + (p.splits > 1 ? p.splits * all * cache->dim : 0));
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const dim3 grid(cache->heads, p.row_blocks, seqs->batch * p.splits);
     const bool wide = cache->page >= 32;
