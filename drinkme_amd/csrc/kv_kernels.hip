@@ -717,9 +717,8 @@ Plan plan_of(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t q_heads, int 
     Plan p;
     const uint32_t tokens = s->cu ? s->max_tokens : s->total / s->batch;
     const uint64_t rows = (uint64_t)tokens * (q_heads / c->heads);
-    const int most = dtype == DMX_F32 ? 1 : 2;
     p.rows = rows > 64;
-    p.tiles = p.rows ? most : (int)std::min<uint64_t>(most, rows <= 16 ? 1 : rows <= 32 ? 2 : 4);
+    p.tiles = rows <= 16 || dtype == DMX_F32 ? 1 : 2;
     const uint32_t a_block = !p.rows ? 16u * p.tiles : dtype == DMX_F32 ? 16u * kAttnWaves : 32u * prompt_waves(c->dim / 32);
     p.row_blocks = (uint32_t)((rows + a_block - 1) / a_block);
     uint64_t length = (uint64_t)s->table_cols * c->page;
@@ -771,10 +770,8 @@ int launch_attend(const Plan& p, int dtype, dim3 grid, hipStream_t stream, const
         hipLaunchKernelGGL(kern, grid, dim3(64 * prompt_waves(W)), Set<W>::lds, stream, a);
     } else if (p.tiles == 1) {
         hipLaunchKernelGGL((k_attend<W, 1, 1, false, WIDE>), grid, block, 0, stream, a);
-    } else if (p.tiles == 2) {
+    } else {
         hipLaunchKernelGGL((k_attend<W, 1, 2, false, WIDE>), grid, block, 0, stream, a);
-    } else if constexpr (W <= 4) {
-        hipLaunchKernelGGL((k_attend<W, 1, 4, false, WIDE>), grid, block, 0, stream, a);
     }
     return launch_check(err, errn, "kv attention launch");
 }
