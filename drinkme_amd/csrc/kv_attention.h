@@ -192,9 +192,10 @@ __device__ __forceinline__ void fetch(const AttnArgs& a, uint32_t h, int blk, En
 }
 
 // Where some row does not see some token of the block. A weight of 0 does not
-// hide a NaN in the product: values of no sequence and NaN blocks go as zeros,
-// and the NaN blocks' channels become NaN in the rows that see one (an
-// indicator's product says which).
+// hide a NaN or an infinity in the product: values of no sequence and blocks that
+// may hold one (bytes over 252, the largest written for finite values) go as zeros,
+// and those blocks' channels become NaN in the rows that see one (an indicator's
+// product says which).
 template <int W, int P, int NR>
 __device__ __forceinline__ void hide_values(State<W, P, NR>& st, Block<W>& x, int t0, int hi_all) {
     using S = Segments<W>;
@@ -205,8 +206,8 @@ __device__ __forceinline__ void hide_values(State<W, P, NR>& st, Block<W>& x, in
         for (int e = 0; e < 8; ++e) {
             const uint32_t byte = (x.vs[s][e >> 2] >> (8 * (e & 3))) & 255u;
             const bool out = t0 + e >= hi_all;
-            nan |= !out && byte == 255u;
-            if (out || byte == 255u) x.v[s][e] = 0;
+            nan |= !out && byte > 252u;
+            if (out || byte > 252u) x.v[s][e] = 0;
             if (out) x.vs[s][e >> 2] &= ~(255u << (8 * (e & 3)));
         }
     if (!__any(nan)) return;
@@ -215,7 +216,7 @@ __device__ __forceinline__ void hide_values(State<W, P, NR>& st, Block<W>& x, in
         bf16x8 is;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const bool n = ((x.vs[s][e >> 2] >> (8 * (e & 3))) & 255u) == 255u;
+            const bool n = ((x.vs[s][e >> 2] >> (8 * (e & 3))) & 255u) > 252u;
             is[e] = n ? (__bf16)1.f : (__bf16)0.f;
             if (n) x.vs[s][e >> 2] &= ~(255u << (8 * (e & 3)));
         }
@@ -678,8 +679,8 @@ __device__ __forceinline__ void write_half(char* to, int lane, const uint32_t (&
 }
 
 // The loaded codes as operands in LDS. Values of no token (before the first or
-// from `hi` on), and NaN blocks, go as zeros; the set's flags say that there
-// were some of the latter.
+// from `hi` on), and blocks that may hold a NaN or an infinity (hide_values), go as
+// zeros; the set's flags say that there were some of the latter.
 template <int W>
 __device__ __forceinline__ void part_write(char* lds, int s, int part, int lane, int hi, uint32_t (&raw)[Set<W>::raw]) {
     using S = Segments<W>;
@@ -709,13 +710,13 @@ __device__ __forceinline__ void part_write(char* lds, int s, int part, int lane,
                     raw[10 * x + 8 + (n >> 2)] &= ~(255u << (8 * (n & 3)));
                 }
     }
-    uint32_t all = 0;  // the top bit of each byte that is 255
+    uint32_t all = 0;  // the top bit of each byte over 252
 #pragma unroll
     for (int x = 0; x < S::count; ++x)
 #pragma unroll
         for (int n = 8; n < 10; ++n) {
             const uint32_t y = raw[10 * x + n];
-            all |= y & ((y & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+            all |= y & ((y & 0x7f7f7f7fu) + 0x03030303u) & 0x80808080u;
         }
     const bool any = __any(all != 0);
     if (any) {
@@ -723,7 +724,7 @@ __device__ __forceinline__ void part_write(char* lds, int s, int part, int lane,
         for (int x = 0; x < S::count; ++x)
 #pragma unroll
             for (int n = 0; n < 8; ++n)
-                if ((raw[10 * x + 8 + (n >> 2)] >> (8 * (n & 3)) & 255u) == 255u) {
+                if ((raw[10 * x + 8 + (n >> 2)] >> (8 * (n & 3)) & 255u) > 252u) {
                     raw[10 * x + n] = 0;
                     raw[10 * x + 8 + (n >> 2)] &= ~(255u << (8 * (n & 3)));
                 }
@@ -935,7 +936,7 @@ __global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_a
                 const uint8_t* e = a.cache.v_scales + slot.token * W + 8 * (w >> 2);
                 bf16x8 is;
 #pragma unroll
-                for (int z = 0; z < 8; ++z) is[z] = e[z] == 255 && t + z < hi_all ? (__bf16)1.f : (__bf16)0.f;
+                for (int z = 0; z < 8; ++z) is[z] = e[z] > 252 && t + z < hi_all ? (__bf16)1.f : (__bf16)0.f;
                 const f32x16 hit = __builtin_amdgcn_mfma_f32_32x32x16_bf16(is, seen, f32x16{}, 0, 0, 0);
 #pragma unroll
                 for (int c = 0; c < S::size(x) / 2; ++c)

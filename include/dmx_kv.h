@@ -17,7 +17,8 @@
  * 7 * 2^(e - 127), the values that round to the grid's top or lower; a value
  * goes to the nearest of the grid, ties to the even code, and to the top
  * where it is larger. A block that holds a NaN or an infinity has e = 255 and
- * reads as NaN. Every value read is exactly a bf16 number.
+ * reads as NaN. Every value read is exactly a bf16 number. 253 and 254 are
+ * never written; what a block with one reads as is left open.
  *
  *   k_codes   u32 [pages, heads, page, dim / 8]: nibble n of word w is
  *             channel 8 w + n
@@ -119,7 +120,7 @@ uint64_t dmx_kv_attention_workspace(const dmx_kv_cache* cache, const dmx_kv_seqs
  * position p sees positions below its sequence's length, with causal no later
  * than p, with window > 0 later than p - window. A query that sees nothing
  * gives zeros and -inf. What a query does not see never reaches its result,
- * NaN included; a position that it sees but whose page is not one of the
+ * whatever bytes are there; a position that it sees but whose page is not one of the
  * cache's gives NaN. */
 int dmx_kv_attention(const dmx_kv_cache* cache, const dmx_kv_seqs* seqs, const dmx_rows* q, int dtype, float scale,
                      int causal, uint32_t window, uint32_t max_length, void* out, float* lse, void* workspace,
