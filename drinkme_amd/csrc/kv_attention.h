@@ -35,6 +35,7 @@ struct AttnArgs {
     uint32_t q_heads, group;
     float scale;  // of the scores, times log2(e)
     uint32_t causal, window, splits;
+    uint32_t row_blocks;  // for each sequence's first seqs.each new tokens
     void* out;
     float* lse;
     float* part_o;   // [splits][total * q_heads][dim]
@@ -351,6 +352,36 @@ __device__ __forceinline__ void attend_block(State<W, P, NR>& st, Block<W>& x, f
     }
 }
 
+// New tokens that no workgroup takes: a sequence's past the bound on them, and those before
+// the first offset or after the last, become NaN: the result, or the first split's sum,
+// which makes the join do so. (Offsets that decrease miss none: on the way from token 0
+// to the last one each is passed upwards, here or by a sequence.) One workgroup of each
+// sequence and head does it.
+template <bool F32, int D>
+__device__ __forceinline__ void leave_rest(const AttnArgs& a, const Seq& q, uint32_t h, uint32_t b) {
+    const int end = q.token + q.count;
+    int t = b == 0 ? 0 : q.token;
+    const int last = b + 1 == a.seqs.batch ? (int)a.seqs.total : end, taken = q.token + min(q.count, (int)a.seqs.each.value);
+#pragma unroll 1
+    for (;; ++t) {
+        if (t == q.token) t = taken;
+        if (t >= last) break;
+        const int64_t row = (int64_t)t * a.q_heads + (int64_t)h * a.group;
+#pragma unroll 1
+        for (uint32_t n = threadIdx.x; n < a.group * D; n += blockDim.x) {
+            if (a.splits > 1) {
+                if (n < a.group) a.part_stat[row + n] = f32x4{-INFINITY, NAN, NAN, 0.f};
+                continue;
+            }
+            if (a.lse && n < a.group) a.lse[row + n] = NAN;
+            if constexpr (F32)
+                static_cast<float*>(a.out)[row * D + n] = NAN;
+            else
+                static_cast<uint16_t*>(a.out)[row * D + n] = 0x7fc0;
+        }
+    }
+}
+
 // W: dim / 32. P: bf16 pieces of the queries and weights (1: bf16, 3: fp32).
 // NR: tiles of 16 query rows a wave. ROWS (fp32 prompts): the workgroup's waves
 // take rows of their own and every token; else they share the rows and deal the
@@ -372,7 +403,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
     const uint32_t h = blockIdx.x, b = blockIdx.z / a.splits, split = blockIdx.z % a.splits;
 
     const Seq q = seq_of(a.seqs, b);
-    const int rows = q.count * (int)a.group;
+    if (a.seqs.cu && split == 0 && blockIdx.y + 1 == a.row_blocks) leave_rest<P != 1, D>(a, q, h, b);
+    const int rows = min(q.count, (int)a.seqs.each.value) * (int)a.group;
     const int r0 = (ROWS ? (int)blockIdx.y * kAttnWaves + (int)wave : (int)blockIdx.y) * 16 * NR;
     if (r0 >= rows) return;
 
@@ -585,6 +617,14 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 // 256 433 and 520; us of the prompt above, heads of 128: 305 and 350.
 constexpr int prompt_waves(int W) { return W <= 6 ? 8 : 4; }
 
+// Where leave_rest is done: by a block of rows more than there are, or, where its code costs
+// the kernel's registers (heads of 96 and 192, 5% of a prompt), by a launch of its own.
+constexpr bool rest_inside(int W) { return W != 3 && W != 6; }
+template <int W>
+__global__ __launch_bounds__(256) void k_attend_rest(const AttnArgs a) {
+    leave_rest<false, 32 * W>(a, seq_of(a.seqs, blockIdx.y), blockIdx.x, blockIdx.y);
+}
+
 template <int W>
 struct Set {
     static constexpr int frag = 1024;           // bytes of an operand: 16 a lane
@@ -750,8 +790,12 @@ __global__ __launch_bounds__(64 * prompt_waves(W), prompt_waves(W) / 4) void k_a
 
     const Seq q = seq_of(a.seqs, b);
     constexpr int unit = 32 * half;  // the rows of half of the waves
-    const int rows = q.count * (int)a.group, units = (rows + unit - 1) / unit, y = blockIdx.y;
-    if (2 * y >= units) return;
+    const int rows = min(q.count, (int)a.seqs.each.value) * (int)a.group, units = (rows + unit - 1) / unit, y = blockIdx.y;
+    if (2 * y >= units) {
+        if constexpr (rest_inside(W))
+            if (y == (int)a.row_blocks && split == 0) leave_rest<false, D>(a, q, h, b);
+        return;
+    }
     // Half of the waves take a unit of rows, half another: of a causal prompt the
     // one as far from its end as the first is from its start, so that workgroups
     // get alike, else the neighbour.

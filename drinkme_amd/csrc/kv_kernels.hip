@@ -50,7 +50,7 @@ struct Seqs {
     const int32_t* cu;
     uint32_t batch, total;
     int cols;
-    Divisor each;  // new tokens of each sequence, where cu is null
+    Divisor each;  // new tokens of each sequence (attention with cu: at most)
 };
 
 struct Rows {
@@ -724,13 +724,13 @@ namespace {
 struct Plan {
     int tiles;
     bool rows;
-    uint32_t row_blocks, splits;
+    uint32_t tokens, row_blocks, splits;  // tokens: of a sequence, at most
 };
 
 Plan plan_of(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t q_heads, int dtype, uint32_t max_length,
              uint32_t window) {
     Plan p;
-    const uint32_t tokens = s->cu ? s->max_tokens : s->total / s->batch;
+    const uint32_t tokens = p.tokens = s->cu ? std::min(s->max_tokens, s->total) : s->total / s->batch;
     const uint64_t rows = (uint64_t)tokens * (q_heads / c->heads);
     p.rows = rows > 64;
     p.tiles = rows <= 16 || dtype == DMX_F32 ? 1 : 2;
@@ -782,7 +782,10 @@ int launch_attend(const Plan& p, int dtype, dim3 grid, hipStream_t stream, const
         static std::atomic<uint64_t> allowed[2] = {};
         const auto kern = a.lse ? k_attend_prompt<W, WIDE, true> : k_attend_prompt<W, WIDE, false>;
         if (allow_lds(reinterpret_cast<const void*>(kern), Set<W>::lds, allowed[a.lse != nullptr], err, errn)) return 1;
-        hipLaunchKernelGGL(kern, grid, dim3(64 * prompt_waves(W)), Set<W>::lds, stream, a);
+        const dim3 more(grid.x, grid.y + (rest_inside(W) && a.seqs.cu), grid.z);
+        hipLaunchKernelGGL(kern, more, dim3(64 * prompt_waves(W)), Set<W>::lds, stream, a);
+        if constexpr (!rest_inside(W))
+            if (a.seqs.cu) hipLaunchKernelGGL(k_attend_rest<W>, dim3(grid.x, a.seqs.batch), block, 0, stream, a);
     } else if (p.tiles == 1) {
         hipLaunchKernelGGL((k_attend<W, 1, 1, false, WIDE>), grid, block, 0, stream, a);
     } else {
@@ -813,7 +816,7 @@ extern "C" int dmx_kv_attention(const dmx_kv_cache* cache, const dmx_kv_seqs* se
     if (!q->at || !out) return fail(err, errn, "null queries or output");
     const Plan p = plan_of(cache, seqs, q->heads, dtype, max_length, window);
     if (p.row_blocks == 0) return fail(err, errn, "max_tokens is 0");
-    if (p.row_blocks > 65535) return fail(err, errn, "too many query rows of one sequence");
+    if (p.row_blocks > 65534) return fail(err, errn, "too many query rows of one sequence");
     if (workspace_bytes < workspace_of(p, cache, seqs, q->heads) || (p.splits > 1 && !aligned(workspace, 16)) ||
         (p.splits > 1 && !workspace))
         return fail(err, errn, "workspace missing, short or not 16-byte aligned");
@@ -824,6 +827,8 @@ extern "C" int dmx_kv_attention(const dmx_kv_cache* cache, const dmx_kv_seqs* se
     a.q_heads = q->heads, a.group = q->heads / cache->heads;
     a.scale = scale * 1.44269504088896341f;
     a.causal = causal != 0, a.window = window, a.splits = p.splits;
+    a.seqs.each = divisor_of(p.tokens);
+    a.row_blocks = p.row_blocks;
     a.out = out, a.lse = lse;
     const uint64_t all = (uint64_t)seqs->total * q->heads;
     a.part_o = static_cast<float*>(workspace);

@@ -63,7 +63,7 @@ typedef struct dmx_kv_seqs {
     uint32_t batch;
     uint32_t table_cols;
     uint32_t total;      /* new tokens of all sequences */
-    uint32_t max_tokens; /* no sequence has more new tokens (cu given) */
+    uint32_t max_tokens; /* no sequence has more new tokens (cu given, attention alone) */
 } dmx_kv_seqs;
 
 /* x [tokens, heads, dim] of dtype DMX_BF16 or DMX_F32, channels adjacent;
@@ -121,7 +121,9 @@ uint64_t dmx_kv_attention_workspace(const dmx_kv_cache* cache, const dmx_kv_seqs
  * than p, with window > 0 later than p - window. A query that sees nothing
  * gives zeros and -inf. What a query does not see never reaches its result,
  * whatever bytes are there; a position that it sees but whose page is not one of the
- * cache's gives NaN. */
+ * cache's gives NaN. So does every token that the call does not compute: a
+ * sequence's past max_tokens, and those of no sequence (before cu[0], from
+ * cu[batch] on). */
 int dmx_kv_attention(const dmx_kv_cache* cache, const dmx_kv_seqs* seqs, const dmx_rows* q, int dtype, float scale,
                      int causal, uint32_t window, uint32_t max_length, void* out, float* lse, void* workspace,
                      uint64_t workspace_bytes, void* stream, char* err, size_t errn);

@@ -1,12 +1,14 @@
 """MI355X: what must not reach the results of the 4-bit cache's operators
-(drinkme_amd.kv_ops): noise behind masks. Against tests/kv_reference.py, within
-its derived bounds."""
+(drinkme_amd.kv_ops): noise behind masks, memory that nothing wrote. Against
+tests/kv_reference.py, within its derived bounds."""
+
+import ctypes as ct
 
 import numpy as np
 import pytest
 import torch
 
-from drinkme_amd import kv_ops
+from drinkme_amd import _native, kv_ops
 from tests import kv_reference as R
 from tests.test_gpu_kv import Batch, check_attention, f64, heads, i32
 
@@ -82,3 +84,80 @@ def test_a_bad_byte_in_a_new_token_stays_with_the_rows_that_see_it(tokens, byte)
     want, _, spread, reach = R.attention(f64(q), *held[0], length - tokens, D ** -0.5)
     ok = np.abs(out - want) <= R.bound(want, spread, reach, length, D, True)
     assert ok[:3].all() and ok[..., :64].all() and ok[..., 96:].all()
+
+
+# ------------------------------------------- offsets that only the GPU sees --
+
+GUARD = 5
+
+
+def through_the_abi(b, q, cu, max_tokens, lengths=None, window=0, max_length=0):
+    """dmx_kv_attention into the middle of larger buffers that hold a pattern,
+    with a workspace that does, too -> out, lse; the buffers beside them have
+    to keep it."""
+    T, Hq, D = q.shape
+    lib, code = _native.lib(), {torch.bfloat16: 0, torch.float32: 1}[q.dtype]
+    c = kv_ops._cache_of(b.cache, "test")
+    lengths = b.lengths if lengths is None else lengths
+    s = _native.KvSeqs(b.block_table.data_ptr(), lengths.data_ptr(), cu.data_ptr(), len(b.sizes), b.cols, T, max_tokens)
+    out = torch.full((T + 2 * GUARD, Hq, D), 7.5, dtype=q.dtype, device="cuda")
+    lse = torch.full((T + 2 * GUARD, Hq), 7.5, device="cuda")
+    need = lib.dmx_kv_attention_workspace(ct.byref(c), ct.byref(s), Hq, code, max_length, window)
+    ws = torch.full((need + 512,), 0x42, dtype=torch.uint8, device="cuda")  # (as floats: 48.6)
+    err = _native.error_buffer()
+    st = lib.dmx_kv_attention(ct.byref(c), ct.byref(s), ct.byref(kv_ops._rows(q)), code, D ** -0.5, 1, window, max_length,
+                              out[GUARD:].data_ptr(), lse[GUARD:].data_ptr(), ws.data_ptr() + 256, need,
+                              torch.cuda.current_stream().cuda_stream, err, len(err))
+    _native.check(st, err, "dmx_kv_attention")
+    for x, value in ((out, 7.5), (lse, 7.5)):
+        assert (x[:GUARD] == value).all() and (x[GUARD + T:] == value).all()
+    assert (ws[:256] == 0x42).all() and (ws[256 + need:] == 0x42).all()
+    return out[GUARD:GUARD + T], lse[GUARD:GUARD + T], need
+
+
+def expected(b, held, q, cu, max_tokens, dtype, window):
+    """(result, bound, lse, its bound) of each token: what its sequence's clamped
+    offsets say, NaN past max_tokens and where there is no sequence."""
+    T, Hq, D = q.shape
+    want, bound = np.full((T, Hq, D), np.nan), np.zeros((T, Hq, D))
+    lse, lbound = np.full((T, Hq), np.nan), np.zeros((T, Hq))
+    for s, (k, v) in enumerate(held):
+        t = min(max(cu[s], 0), T)
+        n = min(max(cu[s + 1], t), T) - t
+        rows = slice(t, t + min(n, max_tokens))
+        if rows.stop > t:
+            x, l, spread, reach = R.attention(f64(q)[rows], k, v, len(k) - n, D ** -0.5, True, window or None)
+            want[rows], bound[rows] = x, R.bound(x, spread, reach, len(k), D, dtype == "bf16")
+            lse[rows], lbound[rows] = l, R.lse_bound(l, reach, len(k), D)
+    return want, bound, lse, lbound
+
+
+# counts of three sequences, max_tokens, offsets: a bound that does not hold; tokens before the first
+# sequence, after the last, both; offsets out of range; offsets that decrease
+OFFSETS = [(8, 3, [0, 2, 7, 8]), (8, 1, [0, 1, 8, 8]), (8, 8, [3, 5, 6, 8]), (8, 8, [0, 2, 5, 6]), (8, 2, [2, 3, 4, 4]),
+           (8, 8, [3, 3, 3, 3]), (8, 3, [-5, 10 ** 6, 10 ** 6, 10 ** 6]), (8, 3, [-7, -5, 10 ** 6, -7]),
+           (200, 40, [0, 90, 91, 200]), (200, 200, [30, 100, 101, 150]), (200, 70, [-3, 75, 10 ** 9, 10 ** 9])]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("D", [64, 192, 256])
+@pytest.mark.parametrize("length", [260, 1500])
+@pytest.mark.parametrize("total, most, cu", OFFSETS, ids=str)
+def test_every_row_is_written(total, most, cu, length, D, dtype):
+    """Few rows and prompts, split over workgroups (1500) or not: a row is its
+    sequence's result, or NaN where it lies past max_tokens or in no sequence."""
+    rng = np.random.default_rng(total + D)
+    b = Batch(rng, [(1, length), (2, length - 37), (3, length - 200)], 2, D, 16, spare=1)
+    held = b.fill(rng)
+    q = heads(rng, (total, 4, D), dtype)
+    for window in (0, 33):
+        got, lse, need = through_the_abi(b, q, i32(cu), most, window=window)
+        assert (need > 0) == (length > 512 and not window)
+        want, bound, l, lbound = expected(b, held, q, cu, most, dtype, window)
+        got, lse = f64(got), f64(lse)
+        assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(np.isnan(lse), np.isnan(l))
+        assert np.array_equal(np.isneginf(lse), np.isneginf(l))
+        ok = ~np.isnan(want)
+        assert (np.abs(got - want)[ok] <= bound[ok]).all()
+        fin = np.isfinite(l)
+        assert (np.abs(lse - l)[fin] <= lbound[fin]).all()
