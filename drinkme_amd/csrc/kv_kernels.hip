@@ -370,13 +370,14 @@ __device__ __forceinline__ Item value_item(const Items& d, uint32_t n) {
 }
 
 // The place of new token t in head 0, and its position; a further head is a
-// page's tokens on.
+// page's tokens on. A token of no sequence (before the first offset, after the
+// last, or where offsets decrease) has none.
 __device__ __forceinline__ Slot slot_of_new(const Cache& c, const Seqs& s, uint32_t t, int& p) {
     const uint32_t b = seq_at(s, t);
     const Seq q = seq_of(s, b);
     p = q.first + ((int)t - q.token);
     Slot at = slot_of(c, s, b, 0, (uint32_t)max(p, 0));
-    at.ok = at.ok && p >= 0;
+    at.ok = at.ok && p >= 0 && (!s.cu || (uint32_t)((int)t - q.token) < (uint32_t)q.count);
     return at;
 }
 

@@ -275,7 +275,8 @@ def append(cache: dict, k: torch.Tensor, v: torch.Tensor, block_table: torch.Ten
     """The new tokens' k and v [T, H, D] into the cache, in place. With
     `table` (rotary_table's) keys are rotated by their positions, in fp32,
     before they are coded, and q [T, Hq, D], if given, is rotated in the same
-    launch -> q' (else None). A token whose position has no page is dropped."""
+    launch -> q' (else None). A token whose position has no page is dropped, and
+    one of no sequence (before cu[0], from cu[B] on)."""
     native = _native.calls()
     if native is not None:
         out = native.append(cache, k, v, block_table, lengths, cu, table, LAYOUTS.get(layout, -1), q, _current(k))
@@ -309,7 +310,7 @@ def read(cache: dict, block_table: torch.Tensor, lengths: torch.Tensor, total: i
     """The keys and values of the last tokens of each sequence as the cache
     holds them, bf16 [total, H, D] each: `total` / B tokens of each sequence,
     or cu's (the tokens that append writes for the same arguments). A token
-    whose position has no page reads NaN."""
+    whose position has no page reads NaN, and one of no sequence."""
     native = _native.calls()
     if native is not None:
         outs = native.read(cache, block_table, lengths, total, cu, _current(lengths))

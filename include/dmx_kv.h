@@ -95,7 +95,9 @@ int dmx_rotary(const dmx_rows* in, const dmx_rows* out, uint32_t n, uint32_t tok
 /* The new tokens' keys k (rotated by their positions where table is given)
  * and values v [total, heads, dim] into the cache; and q, if given, rotated
  * to q_out as dmx_rotary does. A token whose position is negative or past the
- * table's columns, or whose page is not one of the cache's, is not stored. */
+ * table's columns, whose page is not one of the cache's, or which is of no
+ * sequence (before cu[0], from cu[batch] on) is not stored; of the latter q_out
+ * is left open. */
 int dmx_kv_append(const dmx_kv_cache* cache, const dmx_kv_seqs* seqs, const dmx_rows* k, const dmx_rows* v,
                   const dmx_rows* q, const dmx_rows* q_out, int dtype, const dmx_rotary_table* table, void* stream,
                   char* err, size_t errn);

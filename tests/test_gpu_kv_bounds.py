@@ -10,7 +10,7 @@ import torch
 
 from drinkme_amd import _native, kv_ops
 from tests import kv_reference as R
-from tests.test_gpu_kv import Batch, check_attention, f64, heads, i32
+from tests.test_gpu_kv import DT, Batch, check_attention, f64, heads, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -161,3 +161,53 @@ def test_every_row_is_written(total, most, cu, length, D, dtype):
         assert (np.abs(got - want)[ok] <= bound[ok]).all()
         fin = np.isfinite(l)
         assert (np.abs(lse - l)[fin] <= lbound[fin]).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("cu", [[2, 4, 7], [0, 3, 5], [1, 1, 1], [-4, 2, 10 ** 6], [0, 10 ** 6, -3]], ids=str)
+def test_tokens_of_no_sequence_are_not_stored(cu, dtype):
+    """Before the first offset and after the last one: append leaves the cache
+    alone, read gives NaN; q's other rows are as ever, and nothing beside them
+    is written."""
+    rng = np.random.default_rng(31)
+    T, H, Hq, D = 8, 2, 3, 64
+    b = Batch(rng, [(3, 40), (5, 23)], H, D, 8, spare=2)
+    b.fill(rng)
+    spare = next(p for p in range(b.cache["k_codes"].shape[0]) if p not in b.table)
+    b.block_table[b.block_table < 0] = spare  # (positions past the sequences' ends have a page, too)
+    before = {n: t.clone() for n, t in b.cache.items()}
+    table = kv_ops.rotary_table(64, D)
+    q, k, v = (heads(rng, (T, n, D), dtype) for n in (Hq, H, H))
+    buf = torch.full((T + 2 * GUARD, Hq, D), 7.5, dtype=q.dtype, device="cuda")
+    cache, s, err = kv_ops._cache_of(b.cache, "test"), None, _native.error_buffer()
+    offsets = i32(cu)
+    s = _native.KvSeqs(b.block_table.data_ptr(), b.lengths.data_ptr(), offsets.data_ptr(), 2, b.cols, T, T)
+    t, _ = kv_ops._rotary_of(table, "half", D, q.device, "test")
+    rows = [ct.byref(kv_ops._rows(x)) for x in (k, v, q, buf[GUARD:GUARD + T])]
+    st = _native.lib().dmx_kv_append(ct.byref(cache), ct.byref(s), *rows, {"bf16": 0, "f32": 1}[dtype], ct.byref(t),
+                                     torch.cuda.current_stream().cuda_stream, err, len(err))
+    _native.check(st, err, "dmx_kv_append")
+    assert (buf[:GUARD] == 7.5).all() and (buf[GUARD + T:] == 7.5).all()
+    got = [f64(x) for x in kv_ops.read(b.cache, b.block_table, b.lengths, T, cu=offsets)]
+    seen = np.zeros(T, bool)
+    touched = np.zeros((b.cache["k_codes"].shape[0], 8), bool)
+    for n, length in enumerate((40, 23)):
+        at = min(max(cu[n], 0), T)
+        count = min(max(cu[n + 1], at), T) - at
+        if not count:
+            continue
+        p = np.arange(length - count, length)
+        seen[at:at + count] = True
+        touched[b.table[n, p // 8], p % 8] = True
+        turned = R.rotate(f64(k)[at:at + count], p, f64(table), "half", np.float32)
+        assert np.array_equal(got[0][at:at + count], R.cached(turned))
+        assert np.array_equal(got[1][at:at + count], R.cached(f64(v)[at:at + count]))
+        want = R.rotate(f64(q)[at:at + count], p, f64(table), "half", np.float32)
+        assert torch.equal(buf[GUARD + at:GUARD + at + count].cpu(), torch.from_numpy(want).to(DT[dtype]))
+    assert all(np.isnan(x[~seen]).all() for x in got)
+    same = torch.from_numpy(~touched).cuda()
+    for name in ("k_codes", "k_scales"):
+        assert torch.equal(b.cache[name].transpose(1, 2)[same], before[name].transpose(1, 2)[same])
+    for name in ("v_codes", "v_scales"):
+        now, was = (x[name].permute(0, 2, 4, 1, 3).flatten(1, 2)[same] for x in (b.cache, before))
+        assert torch.equal(now, was)
