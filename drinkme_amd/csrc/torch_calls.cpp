@@ -212,6 +212,13 @@ PyObject* narrow(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 constexpr int64_t kMost = 1ll << 30;
 
+// A whole number; -1 for one that 64 bits do not hold.
+int64_t whole(PyObject* o) {
+    int over;
+    const int64_t n = PyLong_AsLongLongAndOverflow(o, &over);
+    return over ? -1 : n;
+}
+
 // A dense tensor of `dtype` and `dims` dimensions on device `index`.
 const at::Tensor* dense(PyObject* o, at::ScalarType dtype, int64_t dims, int64_t index) {
     const at::Tensor* t = exact(o);
@@ -387,7 +394,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     if (n != 6) return launch_failed("read", "six arguments");
-    const int64_t total = PyLong_AsLongLong(a[3]);
+    const int64_t total = whole(a[3]);
     void* stream = PyLong_AsVoidPtr(a[5]);
     if (PyErr_Occurred()) return nullptr;
     dmx_kv_cache c;
@@ -409,10 +416,10 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// A whole number at least 1, or `otherwise` for None; -1 for anything less.
-int64_t count_of(PyObject* o, int64_t otherwise) {
-    if (o == Py_None) return otherwise;
-    const int64_t n = PyLong_AsLongLong(o);
+// One of at least 1, or 0 for None; -1 for anything less.
+int64_t count_of(PyObject* o) {
+    if (o == Py_None) return 0;
+    const int64_t n = whole(o);
     return n < 1 ? -1 : n;
 }
 
@@ -421,7 +428,7 @@ int64_t count_of(PyObject* o, int64_t otherwise) {
 PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     if (n != 12) return launch_failed("attention", "twelve arguments");
-    const int64_t max_tokens = count_of(a[5], 0), max_length = PyLong_AsLongLong(a[6]), window = count_of(a[9], 0);
+    const int64_t max_tokens = count_of(a[5]), max_length = whole(a[6]), window = count_of(a[9]);
     const double given = a[7] == Py_None ? 0 : PyFloat_AsDouble(a[7]);
     const int causal = PyObject_IsTrue(a[8]), want = PyObject_IsTrue(a[10]);
     void* stream = PyLong_AsVoidPtr(a[11]);

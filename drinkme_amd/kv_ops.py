@@ -41,6 +41,7 @@ from .radix_ops import _dtype_code, _stream
 
 LAYOUTS = {"half": _native.ROTARY_HALF, "interleaved": _native.ROTARY_INTERLEAVED}
 HEAD_DIMS = (64, 96, 128, 192, 256)
+_MOST = 1 << 30  # positions of a table, tokens of a call: fewer (the C ABI's 32-bit fields hold them and their sums)
 
 # ------------------------------------------------------------------ tables --
 
@@ -143,6 +144,8 @@ def _activation(x, what, heads=None, dim=None, tokens=None, like=None):
             raise ValueError(f"{what}: {have} {name}, not {want}")
     if like is not None and (x.dtype != like.dtype or x.device != like.device):
         raise ValueError(f"{what}: {x.dtype} on {x.device}, not {like.dtype} on {like.device}")
+    if max(x.shape) >= _MOST:
+        raise ValueError(f"{what}: {tuple(x.shape)}, 2^30 or more tokens, heads or channels")
     return x if x.stride(2) == 1 or x.shape[2] == 1 else x.contiguous()
 
 
@@ -160,6 +163,8 @@ def _rotary_of(table, layout, dim, device, what):
                          f"{tuple(table.shape)}")
     if 2 * table.shape[1] > dim:
         raise ValueError(f"{what}: a table of {2 * table.shape[1]} channels for heads of {dim}")
+    if table.shape[0] >= _MOST:
+        raise ValueError(f"{what}: a table of {table.shape[0]} positions, 2^30 or more")
     if table.device != device:
         raise ValueError(f"{what}: the table is not on {device}")
     table = table.contiguous()
@@ -193,12 +198,16 @@ def _cache_of(cache, what):
 
 def _seqs_of(block_table, lengths, cu, total, max_tokens, device, what):
     """The dmx_kv_seqs of a call, and the tensors it points into."""
+    if total < 0 or total >= _MOST:
+        raise ValueError(f"{what}: {total} tokens (0 or more, fewer than 2^30)")
     named = [("block_table", block_table, 2), ("lengths", lengths, 1)] + ([("cu", cu, 1)] if cu is not None else [])
     held = []
     for name, t, dims in named:
         if t.dtype != torch.int32 or t.dim() != dims or t.device != device:
             raise ValueError(f"{what}: {name} must be int32 of {dims} dimension(s) on {device}, got {t.dtype} "
                              f"{tuple(t.shape)} on {t.device}")
+        if max(t.shape) >= _MOST:
+            raise ValueError(f"{what}: {name} is {tuple(t.shape)}, 2^30 or more sequences or columns")
         held.append(t.contiguous())
     batch = lengths.shape[0]
     if block_table.shape[0] != batch or (cu is not None and cu.shape[0] != batch + 1):
@@ -211,7 +220,7 @@ def _seqs_of(block_table, lengths, cu, total, max_tokens, device, what):
     s = _native.KvSeqs()
     s.table, s.lengths, s.cu = held[0].data_ptr(), held[1].data_ptr(), held[2].data_ptr() if cu is not None else None
     s.batch, s.table_cols, s.total = batch, block_table.shape[1], total
-    s.max_tokens = total // batch if cu is None else total if max_tokens is None else max_tokens
+    s.max_tokens = total // batch if cu is None else total if max_tokens is None else min(max_tokens, total)
     return s, held
 
 
@@ -358,16 +367,21 @@ def attention(q: torch.Tensor, cache: dict, block_table: torch.Tensor, lengths: 
         raise ValueError(f"attention: a window of {window}")
     if max_tokens is not None and (cu is None or max_tokens < 1):
         raise ValueError("attention: max_tokens, at least 1, goes with cu")
+    if max_length is not None and max_length < 0:
+        raise ValueError(f"attention: a max_length of {max_length}")
+    if window is not None and window >= _MOST:  # past every table: none
+        window = None
+    max_length = min(max_length or 0, _MOST)
     s, held = _seqs_of(block_table, lengths, cu, T, max_tokens, q.device, "attention")
     out = torch.empty((T, Hq, c.dim), dtype=q.dtype, device=q.device)
     lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
     lib, code = _native.lib(), _dtype_code(q.dtype, "attention")
     scale = c.dim ** -0.5 if scale is None else float(scale)
-    bytes_ = lib.dmx_kv_attention_workspace(ct.byref(c), ct.byref(s), Hq, code, max_length or 0, window or 0) if T else 0
+    bytes_ = lib.dmx_kv_attention_workspace(ct.byref(c), ct.byref(s), Hq, code, max_length, window or 0) if T else 0
     ws = torch.empty(bytes_, dtype=torch.uint8, device=q.device) if bytes_ else None
     err = _native.error_buffer()
     st = lib.dmx_kv_attention(ct.byref(c), ct.byref(s), ct.byref(_rows(q)), code, scale, causal, window or 0,
-                              max_length or 0, out.data_ptr(), lse.data_ptr() if return_lse else None,
+                              max_length, out.data_ptr(), lse.data_ptr() if return_lse else None,
                               ws.data_ptr() if bytes_ else None, bytes_, _stream(q.device), err, len(err))
     _native.check(st, err, "dmx_kv_attention")
     return (out, lse) if return_lse else out

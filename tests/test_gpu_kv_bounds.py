@@ -211,3 +211,39 @@ def test_tokens_of_no_sequence_are_not_stored(cu, dtype):
     for name in ("v_codes", "v_scales"):
         now, was = (x[name].permute(0, 2, 4, 1, 3).flatten(1, 2)[same] for x in (b.cache, before))
         assert torch.equal(now, was)
+
+
+# --------------------------------------------------- numbers past 32 bits --
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("over", [2 ** 30, 2 ** 31, 2 ** 32 + 1, 2 ** 64 + 1], ids=str)
+def test_bounds_past_32_bits_are_no_bounds(over, native, monkeypatch):
+    """A window or a bound longer than any table: every position, every row."""
+    rng = np.random.default_rng(33)
+    b = Batch(rng, [(70, 90), (3, 60)], 1, 64, 16)
+    b.fill(rng)
+    q = heads(rng, (73, 2, 64), "bf16")
+    want = kv_ops.attention(q, b.cache, b.block_table, b.lengths, **b.args, return_lse=True)
+    if not native:
+        monkeypatch.setattr(_native, "_calls", None)
+    for kw in ({"window": over}, {"max_tokens": over}, {"max_length": over}, {"window": over, "max_tokens": 70, "max_length": 90}):
+        got = kv_ops.attention(q, b.cache, b.block_table, b.lengths, **b.args, return_lse=True, **kw)
+        assert all(torch.equal(x, y) for x, y in zip(got, want)), kw
+
+
+def test_too_many_tokens_are_refused():
+    table = kv_ops.rotary_table(4, 64)
+    many = torch.zeros(1, 1, 64, dtype=torch.bfloat16, device="cuda").expand(2 ** 32 + 1, 1, 64)
+    few = torch.zeros(2, 1, 64, dtype=torch.bfloat16, device="cuda")
+    b = Batch(np.random.default_rng(0), [(1, 20)] * 2, 1, 64, 16)
+    for call in (lambda: kv_ops.rotary(many, None, b.lengths, table),
+                 lambda: kv_ops.append(b.cache, many, many, b.block_table, b.lengths, cu=i32([0, 1, 2])),
+                 lambda: kv_ops.attention(many, b.cache, b.block_table, b.lengths, cu=i32([0, 1, 2])),
+                 lambda: kv_ops.read(b.cache, b.block_table, b.lengths, 2 ** 32 + 2),
+                 lambda: kv_ops.read(b.cache, b.block_table, b.lengths, 2 ** 64 + 2),
+                 lambda: kv_ops.read(b.cache, b.block_table, b.lengths, -2)):
+        with pytest.raises(ValueError, match="tokens"):
+            call()
+    with pytest.raises(ValueError, match="max_length"):
+        kv_ops.attention(few, b.cache, b.block_table, b.lengths, max_length=-1)
