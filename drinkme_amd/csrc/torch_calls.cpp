@@ -219,6 +219,9 @@ int64_t whole(PyObject* o) {
     return over ? -1 : n;
 }
 
+// Whether x asks for a gradient.
+bool wants(const at::Tensor& x) { return x.requires_grad() && at::GradMode::is_enabled(); }
+
 // A dense tensor of `dtype` and `dims` dimensions on device `index`.
 const at::Tensor* dense(PyObject* o, at::ScalarType dtype, int64_t dims, int64_t index) {
     const at::Tensor* t = exact(o);
@@ -234,7 +237,7 @@ bool rows_at(PyObject* o, const at::Tensor*& x, dmx_rows& r) {
                                                   K::Python, K::Negative, K::Conjugate, K::ZeroTensor})))
         return false;
     if (code(x->scalar_type()) < 0 || x->stride(2) != 1 || x->size(0) >= kMost || x->size(1) >= kMost ||
-        (x->requires_grad() && at::GradMode::is_enabled()))
+        wants(*x))
         return false;
     r = {const_cast<void*>(x->const_data_ptr()), x->stride(0), x->stride(1), (uint32_t)x->size(1)};
     return true;
@@ -251,7 +254,7 @@ dmx_rows dense_rows(const at::Tensor& t) {
 
 bool table_of(PyObject* o, long layout, int64_t dim, int64_t index, dmx_rotary_table& r) {
     const at::Tensor* t = dense(o, at::kFloat, 3, index);
-    if (!t || t->size(2) != 2 || 2 * t->size(1) > dim || t->size(0) >= kMost) return false;
+    if (!t || t->size(2) != 2 || 2 * t->size(1) > dim || t->size(0) >= kMost || wants(*t)) return false;
     r = {static_cast<const float*>(t->const_data_ptr()), (uint32_t)t->size(0), (uint32_t)(2 * t->size(1)), (int)layout};
     return true;
 }

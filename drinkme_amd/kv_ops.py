@@ -240,7 +240,7 @@ def rotary(q: torch.Tensor, k, positions: torch.Tensor, table: torch.Tensor, lay
         outs = native.rotary(q, k, positions, table, LAYOUTS.get(layout, -1), _current(q))
         if outs is not None:
             return outs
-    _no_gradient("rotary", q, k)
+    _no_gradient("rotary", q, k, table)
     q = _activation(q, "rotary: q")
     ins = [q] if k is None else [q, _activation(k, "rotary: k", dim=q.shape[2], tokens=q.shape[0], like=q)]
     if positions.dtype not in (torch.int32, torch.int64) or positions.shape != q.shape[:1] or positions.device != q.device:
@@ -291,7 +291,7 @@ def append(cache: dict, k: torch.Tensor, v: torch.Tensor, block_table: torch.Ten
         out = native.append(cache, k, v, block_table, lengths, cu, table, LAYOUTS.get(layout, -1), q, _current(k))
         if out is not None:
             return out if q is not None else None
-    _no_gradient("append", k, v, q)
+    _no_gradient("append", k, v, q, table)
     c = _cache_of(cache, "append")
     k = _activation(k, "append: k", heads=c.heads, dim=c.dim)
     v = _activation(v, "append: v", heads=c.heads, dim=c.dim, tokens=k.shape[0], like=k)

@@ -247,3 +247,20 @@ def test_too_many_tokens_are_refused():
             call()
     with pytest.raises(ValueError, match="max_length"):
         kv_ops.attention(few, b.cache, b.block_table, b.lengths, max_length=-1)
+
+
+# ---------------------------------------------------------------- gradients --
+
+
+def test_a_table_that_asks_for_a_gradient_is_refused():
+    b = Batch(np.random.default_rng(0), [(1, 20)] * 2, 2, 64, 16)
+    q, k, v = (heads(np.random.default_rng(1), (2, n, 64), "bf16") for n in (4, 2, 2))
+    table = kv_ops.rotary_table(32, 64).requires_grad_()
+    before = {n: t.clone() for n, t in b.cache.items()}
+    for call in (lambda: kv_ops.rotary(q, k, b.lengths, table),
+                 lambda: kv_ops.append(b.cache, k, v, b.block_table, b.lengths, table=table, q=q)):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+    assert all(torch.equal(before[n], b.cache[n]) for n in before)
+    with torch.no_grad():
+        assert torch.equal(kv_ops.rotary(q, None, b.lengths, table)[0], kv_ops.rotary(q, None, b.lengths, table.detach())[0])
