@@ -17,6 +17,7 @@
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -219,8 +220,11 @@ int64_t whole(PyObject* o) {
     return over ? -1 : n;
 }
 
-// Whether x asks for a gradient.
-bool wants(const at::Tensor& x) { return x.requires_grad() && at::GradMode::is_enabled(); }
+// Whether x asks for a gradient, or carries a tangent.
+bool wants(const at::Tensor& x) {
+    return (x.requires_grad() && at::GradMode::is_enabled()) ||
+           (x._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode());
+}
 
 // A dense tensor of `dtype` and `dims` dimensions on device `index`.
 const at::Tensor* dense(PyObject* o, at::ScalarType dtype, int64_t dims, int64_t index) {

@@ -26,7 +26,7 @@ what only the GPU can see is checked there (include/dmx_kv.h says how).
 
 Activations are bf16 or fp32. Every call launches on torch's current stream
 and allocates its outputs (attention a workspace too) with torch. There is no
-gradient: a call refuses tensors that ask for one.
+gradient: a call refuses tensors that ask for one or carry a tangent.
 """
 
 from __future__ import annotations
@@ -35,6 +35,7 @@ import ctypes as ct
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .radix_ops import _dtype_code, _stream
@@ -130,6 +131,9 @@ def _current(x):
 def _no_gradient(what, *tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or detach its inputs")
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled() and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no gradient, forward-mode tangents included: unpack its inputs")
 
 
 def _activation(x, what, heads=None, dim=None, tokens=None, like=None):

@@ -264,3 +264,30 @@ def test_a_table_that_asks_for_a_gradient_is_refused():
     assert all(torch.equal(before[n], b.cache[n]) for n in before)
     with torch.no_grad():
         assert torch.equal(kv_ops.rotary(q, None, b.lengths, table)[0], kv_ops.rotary(q, None, b.lengths, table.detach())[0])
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_tensors_with_a_tangent_are_refused(native, monkeypatch):
+    """Forward-mode derivatives have no more of a gradient here than backward ones."""
+    from torch.autograd import forward_ad
+
+    if not native:
+        monkeypatch.setattr(_native, "_calls", None)
+    b = Batch(np.random.default_rng(0), [(1, 20)] * 2, 2, 64, 16)
+    q, k, v = (heads(np.random.default_rng(1), (2, n, 64), "bf16") for n in (4, 2, 2))
+    table = kv_ops.rotary_table(32, 64)
+    before = {n: t.clone() for n, t in b.cache.items()}
+    with forward_ad.dual_level():
+        dual = lambda x: forward_ad.make_dual(x, torch.ones_like(x))  # noqa: E731
+        for call in (lambda: kv_ops.rotary(dual(q), k, b.lengths, table), lambda: kv_ops.rotary(q, dual(k), b.lengths, table),
+                     lambda: kv_ops.rotary(q, k, b.lengths, dual(table)),
+                     lambda: kv_ops.append(b.cache, dual(k), v, b.block_table, b.lengths),
+                     lambda: kv_ops.append(b.cache, k, dual(v), b.block_table, b.lengths),
+                     lambda: kv_ops.append(b.cache, k, v, b.block_table, b.lengths, table=table, q=dual(q)),
+                     lambda: kv_ops.attention(dual(q), b.cache, b.block_table, b.lengths)):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no gradient"):  # (which leaves tangents on)
+                call()
+        assert kv_ops.rotary(q, k, b.lengths, table)[0].shape == q.shape  # plain tensors of the same level are taken
+    assert all(torch.equal(before[n], b.cache[n]) for n in before)
