@@ -18,6 +18,7 @@
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/AutogradState.h>
+#include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -209,7 +210,8 @@ PyObject* narrow(PyObject*, PyObject* const* a, Py_ssize_t n) {
 //
 // As above: the plain case or None. Plain here: tensors of the types, shapes
 // and device that kv_ops documents, activations with adjacent channels, nothing
-// that asks for a gradient.
+// that asks for a gradient. The tensors' device is made current for the launch:
+// the null stream is the current device's, and so is a kernel's LDS limit.
 
 constexpr int64_t kMost = 1ll << 30;
 
@@ -346,6 +348,7 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     int st;
     {
         pybind11::gil_scoped_release no_gil;
+        const c10::DeviceGuard on(q->device());
         y = dense_like(*q);
         out[0] = dense_rows(y);
         if (k) {
@@ -384,6 +387,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     int st;
     {
         pybind11::gil_scoped_release no_gil;
+        const c10::DeviceGuard on(k->device());
         if (q) {
             y = dense_like(*q);
             out = dense_rows(y);
@@ -413,7 +417,9 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     int st;
     {
         pybind11::gil_scoped_release no_gil;
-        const auto options = at::TensorOptions().device(at::Device(at::kCUDA, (c10::DeviceIndex)index)).dtype(at::kBFloat16);
+        const at::Device device(at::kCUDA, (c10::DeviceIndex)index);
+        const c10::DeviceGuard on(device);
+        const auto options = at::TensorOptions().device(device).dtype(at::kBFloat16);
         k = at::empty({total, (int64_t)c.heads, (int64_t)c.dim}, options);
         v = at::empty({total, (int64_t)c.heads, (int64_t)c.dim}, options);
         st = dmx_kv_read(&c, &s, static_cast<uint16_t*>(k.mutable_data_ptr()), static_cast<uint16_t*>(v.mutable_data_ptr()),
@@ -456,6 +462,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     int st;
     {
         pybind11::gil_scoped_release no_gil;
+        const c10::DeviceGuard on(q->device());
         const int dt = code(q->scalar_type());
         out = dense_like(*q);
         if (want) lse = at::empty({q->size(0), q->size(1)}, at::TensorOptions().device(q->device()).dtype(at::kFloat));

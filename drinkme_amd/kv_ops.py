@@ -255,9 +255,10 @@ def rotary(q: torch.Tensor, k, positions: torch.Tensor, table: torch.Tensor, lay
     outs = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in ins]
     n = len(ins)
     err = _native.error_buffer()
-    st = _native.lib().dmx_rotary((_native.KvRows * n)(*map(_rows, ins)), (_native.KvRows * n)(*map(_rows, outs)), n,
-                                  q.shape[0], q.shape[2], _dtype_code(q.dtype, "rotary"), positions.data_ptr(),
-                                  positions.dtype == torch.int64, ct.byref(t), _stream(q.device), err, len(err))
+    with torch.cuda.device(q.device):
+        st = _native.lib().dmx_rotary((_native.KvRows * n)(*map(_rows, ins)), (_native.KvRows * n)(*map(_rows, outs)), n,
+                                      q.shape[0], q.shape[2], _dtype_code(q.dtype, "rotary"), positions.data_ptr(),
+                                      positions.dtype == torch.int64, ct.byref(t), _stream(q.device), err, len(err))
     _native.check(st, err, "dmx_rotary")
     return outs[0], outs[1] if k is not None else None
 
@@ -311,10 +312,11 @@ def append(cache: dict, k: torch.Tensor, v: torch.Tensor, block_table: torch.Ten
         q = _activation(q, "append: q", dim=c.dim, tokens=k.shape[0], like=k)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     err = _native.error_buffer()
-    st = _native.lib().dmx_kv_append(ct.byref(c), ct.byref(s), ct.byref(_rows(k)), ct.byref(_rows(v)),
-                                     ct.byref(_rows(q)) if q is not None else None,
-                                     ct.byref(_rows(out)) if q is not None else None, _dtype_code(k.dtype, "append"),
-                                     ct.byref(t) if t is not None else None, _stream(k.device), err, len(err))
+    with torch.cuda.device(k.device):
+        st = _native.lib().dmx_kv_append(ct.byref(c), ct.byref(s), ct.byref(_rows(k)), ct.byref(_rows(v)),
+                                         ct.byref(_rows(q)) if q is not None else None,
+                                         ct.byref(_rows(out)) if q is not None else None, _dtype_code(k.dtype, "append"),
+                                         ct.byref(t) if t is not None else None, _stream(k.device), err, len(err))
     _native.check(st, err, "dmx_kv_append")
     return out
 
@@ -334,7 +336,8 @@ def read(cache: dict, block_table: torch.Tensor, lengths: torch.Tensor, total: i
     s, held = _seqs_of(block_table, lengths, cu, int(total), None, device, "read")
     k, v = (torch.empty((int(total), c.heads, c.dim), dtype=torch.bfloat16, device=device) for _ in range(2))
     err = _native.error_buffer()
-    st = _native.lib().dmx_kv_read(ct.byref(c), ct.byref(s), k.data_ptr(), v.data_ptr(), _stream(device), err, len(err))
+    with torch.cuda.device(device):
+        st = _native.lib().dmx_kv_read(ct.byref(c), ct.byref(s), k.data_ptr(), v.data_ptr(), _stream(device), err, len(err))
     _native.check(st, err, "dmx_kv_read")
     return k, v
 
@@ -384,8 +387,9 @@ def attention(q: torch.Tensor, cache: dict, block_table: torch.Tensor, lengths: 
     bytes_ = lib.dmx_kv_attention_workspace(ct.byref(c), ct.byref(s), Hq, code, max_length, window or 0) if T else 0
     ws = torch.empty(bytes_, dtype=torch.uint8, device=q.device) if bytes_ else None
     err = _native.error_buffer()
-    st = lib.dmx_kv_attention(ct.byref(c), ct.byref(s), ct.byref(_rows(q)), code, scale, causal, window or 0,
-                              max_length, out.data_ptr(), lse.data_ptr() if return_lse else None,
-                              ws.data_ptr() if bytes_ else None, bytes_, _stream(q.device), err, len(err))
+    with torch.cuda.device(q.device):
+        st = lib.dmx_kv_attention(ct.byref(c), ct.byref(s), ct.byref(_rows(q)), code, scale, causal, window or 0,
+                                  max_length, out.data_ptr(), lse.data_ptr() if return_lse else None,
+                                  ws.data_ptr() if bytes_ else None, bytes_, _stream(q.device), err, len(err))
     _native.check(st, err, "dmx_kv_attention")
     return (out, lse) if return_lse else out

@@ -6,7 +6,7 @@
  *
  * Conventions are dmx_radix.h's: int status (0, or 1 with a message in
  * `err`), caller-owned buffers, host checks before any launch, no
- * synchronisation. What only the device can see (lengths, positions, page
+ * synchronisation, buffers and stream of the current device. What only the device can see (lengths, positions, page
  * numbers) is checked by the kernels: none of it leads a read or a write out
  * of the buffers described here.
  *

@@ -291,3 +291,57 @@ def test_tensors_with_a_tangent_are_refused(native, monkeypatch):
                 call()
         assert kv_ops.rotary(q, k, b.lengths, table)[0].shape == q.shape  # plain tensors of the same level are taken
     assert all(torch.equal(before[n], b.cache[n]) for n in before)
+
+
+# ------------------------------------------------------------------ devices --
+
+
+def test_the_tensors_device_is_current_for_a_launch(monkeypatch):
+    """On the general path each launch is made inside its tensors' device (the
+    native call has a guard of its own; with one GPU nothing tells that)."""
+    b = Batch(np.random.default_rng(0), [(1, 20)] * 2, 2, 64, 16)
+    q, k, v = (heads(np.random.default_rng(1), (2, n, 64), "bf16") for n in (4, 2, 2))
+    table = kv_ops.rotary_table(32, 64)
+    inside, seen = [], []
+
+    class Device(torch.cuda.device):
+        def __enter__(self):
+            super().__enter__()
+            inside.append(self.idx)
+
+        def __exit__(self, *a):
+            inside.pop()
+            return super().__exit__(*a)
+
+    class Lib:
+        def __getattr__(self, name):
+            fn = getattr(real, name)
+            if name.endswith("workspace"):
+                return fn
+            return lambda *a: (seen.append((name, list(inside))), fn(*a))[1]
+
+    real = _native.lib()
+    monkeypatch.setattr(_native, "_calls", None)
+    monkeypatch.setattr(_native, "lib", Lib)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    kv_ops.rotary(q, k, b.lengths, table)
+    kv_ops.append(b.cache, k, v, b.block_table, b.lengths)
+    kv_ops.read(b.cache, b.block_table, b.lengths, 2)
+    kv_ops.attention(q, b.cache, b.block_table, b.lengths)
+    assert seen == [(n, [q.device.index]) for n in ("dmx_rotary", "dmx_kv_append", "dmx_kv_read", "dmx_kv_attention")]
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="two GPUs")
+@pytest.mark.parametrize("native", [True, False])
+def test_tensors_of_another_device_than_the_current_one(native, monkeypatch):
+    rng = np.random.default_rng(0)
+    b = Batch(rng, [(70, 200)] * 2, 2, 128, 16)
+    b.fill(rng)
+    q = heads(rng, (140, 4, 128), "bf16")
+    want = kv_ops.attention(q, b.cache, b.block_table, b.lengths)
+    if not native:
+        monkeypatch.setattr(_native, "_calls", None)
+    there = torch.device("cuda:1")
+    cache = {n: t.to(there) for n, t in b.cache.items()}
+    got = kv_ops.attention(q.to(there), cache, b.block_table.to(there), b.lengths.to(there))
+    assert got.device == there and torch.equal(got.cpu(), want.cpu())
