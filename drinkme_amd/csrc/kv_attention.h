@@ -267,8 +267,9 @@ __device__ __forceinline__ void attend_block(State<W, P, NR>& st, Block<W>& x, f
 
     // Softmax. A row's reference is the maximum of the first scores that it sees;
     // later scores are weighed by it as they come, without a look at their maximum
-    // (weights above 1 cost no precision), until a lane's sum passes 2^20: then the
-    // block is weighed again by a higher one. fresh: a row may see its first scores
+    // (weights above 1 cost no precision, only range: values of 2^107 / tokens and more
+    // may overflow in the sum, as those of 2^128 / tokens would under weights up to 1),
+    // until a lane's sum passes 2^20: then the block is weighed again by a higher one. fresh: a row may see its first scores
     // of the wave's here.
     bf16x8 pf[NR][P];
 #pragma unroll

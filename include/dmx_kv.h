@@ -122,10 +122,14 @@ uint64_t dmx_kv_attention_workspace(const dmx_kv_cache* cache, const dmx_kv_seqs
  * position p sees positions below its sequence's length, with causal no later
  * than p, with window > 0 later than p - window. A query that sees nothing
  * gives zeros and -inf. What a query does not see never reaches its result,
- * whatever bytes are there; a position that it sees but whose page is not one of the
- * cache's gives NaN. So does every token that the call does not compute: a
- * sequence's past max_tokens, and those of no sequence (before cu[0], from
- * cu[batch] on). */
+ * whatever bytes are there; a position that it sees but whose page is not one
+ * of the cache's gives NaN. So does every token that the call does not
+ * compute: a sequence's past max_tokens, and those of no sequence (before
+ * cu[0], from cu[batch] on).
+ *
+ * Sums are divided at the end: a result is finite where the values that it sees
+ * stay below 2^107 / (the tokens that it sees) in magnitude, and may overflow
+ * past that, though the cache holds up to 1.5 * 2^127. */
 int dmx_kv_attention(const dmx_kv_cache* cache, const dmx_kv_seqs* seqs, const dmx_rows* q, int dtype, float scale,
                      int causal, uint32_t window, uint32_t max_length, void* out, float* lse, void* workspace,
                      uint64_t workspace_bytes, void* stream, char* err, size_t errn);

@@ -345,3 +345,26 @@ def test_tensors_of_another_device_than_the_current_one(native, monkeypatch):
     cache = {n: t.to(there) for n, t in b.cache.items()}
     got = kv_ops.attention(q.to(there), cache, b.block_table.to(there), b.lengths.to(there))
     assert got.device == there and torch.equal(got.cpu(), want.cpu())
+
+
+# -------------------------------------------------------------- large values --
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("tokens", [1, 40])
+@pytest.mark.parametrize("shape", ["rise", "steps"])
+def test_large_values_under_scores_that_rise(shape, tokens, dtype):
+    """Values up to the documented 2^107 / tokens, where weights grow to 2^20
+    before their row's reference follows."""
+    rng = np.random.default_rng(22)
+    D, length = 64, 900
+    b = Batch(rng, [(tokens, length)], 1, D, 32)
+    at = np.arange(length) / length
+    gain = {"rise": at * 60, "steps": np.floor(at * 8) * 9}[shape]
+    direction = np.sign(rng.standard_normal(D))
+    k = torch.from_numpy((gain[:, None, None] * direction + rng.standard_normal((length, 1, D))).astype(np.float32)).cuda()
+    v = rng.standard_normal((length, 1, D)).clip(-4, 4) * 2.0 ** 95  # 4 * 2^95 <= 2^107 / 900
+    held = b.fill(rng, k.to(torch.bfloat16), torch.from_numpy(v.astype(np.float32)).cuda().to(torch.bfloat16))
+    q = torch.from_numpy((direction * (1 + 0.1 * rng.standard_normal((tokens, 3, D)))).astype(np.float32)).cuda().to(DT[dtype])
+    got, lse = kv_ops.attention(q, b.cache, b.block_table, b.lengths, return_lse=True)
+    check_attention(b, held, q, dtype, got, lse)
