@@ -368,3 +368,140 @@ def test_large_values_under_scores_that_rise(shape, tokens, dtype):
     q = torch.from_numpy((direction * (1 + 0.1 * rng.standard_normal((tokens, 3, D)))).astype(np.float32)).cuda().to(DT[dtype])
     got, lse = kv_ops.attention(q, b.cache, b.block_table, b.lengths, return_lse=True)
     check_attention(b, held, q, dtype, got, lse)
+
+
+# -------------------------------------------------------------- more forms --
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("D", kv_ops.HEAD_DIMS)
+@pytest.mark.parametrize("window", [None, 70])
+@pytest.mark.parametrize("page", [8, 16, 32, 64])
+def test_prompts_of_every_head_and_page(page, window, D, dtype):
+    """Prompts unsplit and split over workgroups, pages that hold whole blocks
+    of 32 and pages that do not, rows that see nothing among them (a prompt
+    longer than its sequence's tokens)."""
+    rng = np.random.default_rng(D + page)
+    for sizes, spare in (([(300, 300), (70, 411), (1, 64), (0, 10)], 0), ([(90, 1500)], 1)):
+        b = Batch(rng, sizes, 1, D, page, spare)
+        held = b.fill(rng)
+        q = heads(rng, (b.total, 2, D), dtype, 1.5)
+        got, lse = kv_ops.attention(q, b.cache, b.block_table, b.lengths, window=window, return_lse=True, **b.args)
+        check_attention(b, held, q, dtype, got, lse, True, window)
+    short = Batch(rng, [(90, 90)], 1, D, page)
+    held = short.fill(rng)
+    q = heads(rng, (90, 2, D), dtype)
+    got, lse = kv_ops.attention(q, short.cache, short.block_table, i32([40]), window=window, return_lse=True)
+    out, l = f64(got), f64(lse)
+    assert (out[:50] == 0).all() and np.isneginf(l[:50]).all()
+    want, wl, spread, reach = R.attention(f64(q), held[0][0][:40], held[0][1][:40], -50, D ** -0.5, True, window)
+    assert (np.abs(out - want) <= R.bound(want, spread, reach, 40, D, dtype == "bf16")).all()
+    assert (np.abs(l - wl)[50:] <= R.lse_bound(wl, reach, 40, D)[50:]).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("D", kv_ops.HEAD_DIMS)
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("tokens", [1, 8, 50])
+@pytest.mark.parametrize("page", [16, 64])
+def test_nan_blocks_through_splits(page, tokens, which, D, dtype):
+    """A block that is not finite, in every split and beside their edges, alone:
+    its channels (a key's: all) of the rows that see it, through the join."""
+    rng = np.random.default_rng(tokens + D)
+    length = 1500
+    b = Batch(rng, [(tokens, length)], 1, D, page, spare=0)
+    k, v = (heads(rng, (length, 1, D), "bf16") for _ in range(2))
+    q = heads(rng, (tokens, 2, D), dtype)
+    for at in (0, 127, 128, 135, 136, 703, 704, 1407, length - tokens // 2 - 1, length - 1):
+        x = (k if which == "k" else v).clone()
+        x[at, 0, D - 5] = float("nan") if at % 2 else float("inf")
+        held = b.fill(rng, *((x, v) if which == "k" else (k, x)))
+        for window in (None, 97):
+            got, lse = kv_ops.attention(q, b.cache, b.block_table, b.lengths, window=window, return_lse=True)
+            check_attention(b, held, q, dtype, got, lse, True, window)
+
+
+def test_modes_subclasses_and_vmap():
+    """What the native call leaves to the general path gives the same bits; a
+    batched tensor, which has no address, is refused."""
+    from torch.overrides import TorchFunctionMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    made = []
+
+    class Function(TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            made.append(getattr(func, "__name__", str(func)))
+            return func(*args, **(kwargs or {}))
+
+    class Dispatch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            made.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    class Sub(torch.Tensor):
+        pass
+
+    rng = np.random.default_rng(41)
+    b = Batch(rng, [(3, 600), (2, 33)], 2, 64, 16)
+    b.fill(rng)
+    table = kv_ops.rotary_table(1024, 64)
+    q, k, v = (heads(rng, (5, n, 64), "bf16") for n in (4, 2, 2))
+    at = i32(range(5))
+
+    calls = {"rotary": lambda q: kv_ops.rotary(q, k, at, table)[0],
+             "append": lambda q: kv_ops.append(b.cache, k, v, b.block_table, b.lengths, table=table, q=q, **b.args),
+             "attention": lambda q: kv_ops.attention(q, b.cache, b.block_table, b.lengths, **b.args)}
+    for name, call in calls.items():
+        want = call(q)
+        for mode in (Function, Dispatch):
+            made.clear()
+            with mode():
+                got = call(q)
+            assert torch.equal(got, want) and any("empty" in n for n in made), name
+        assert torch.equal(call(q.as_subclass(Sub)).as_subclass(torch.Tensor), want), name
+        with pytest.raises(RuntimeError):
+            torch.vmap(call)(q[None])
+
+
+def test_threads_with_a_stream_each():
+    """Inputs made late on each thread's stream, outputs read there."""
+    import threading
+
+    rng = np.random.default_rng(42)
+    b = Batch(rng, [(1, 3000)] * 2, 2, 64, 16)
+    b.fill(rng)
+    xs = [heads(rng, (2, 8, 64), "bf16") for _ in range(4)]
+    table = kv_ops.rotary_table(4096, 64)
+    at = i32([2999, 2999])
+
+    def call(x):
+        return kv_ops.attention(kv_ops.rotary(x, None, at, table)[0], b.cache, b.block_table, b.lengths)
+
+    want = [call(x) for x in xs]
+    torch.cuda.synchronize()
+    good, errors = [False] * 4, []
+
+    def work(i):
+        try:
+            with torch.no_grad(), torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    x = torch.zeros_like(xs[i])
+                    big = torch.randn(1024, 1024, device="cuda")
+                    for _ in range(4):
+                        big = big @ big * 1e-2
+                    x.copy_(xs[i])  # (after the products: a launch on another stream would read zeros)
+                    if not torch.equal(call(x), want[i]):
+                        raise AssertionError(f"thread {i} read another stream's data")
+                torch.cuda.current_stream().synchronize()
+            good[i] = True
+        except BaseException as e:  # noqa: BLE001 (handed to the main thread)
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors[0]
+    assert all(good)
