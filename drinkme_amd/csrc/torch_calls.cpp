@@ -260,7 +260,9 @@ dmx_rows dense_rows(const at::Tensor& t) {
 
 bool table_of(PyObject* o, long layout, int64_t dim, int64_t index, dmx_rotary_table& r) {
     const at::Tensor* t = dense(o, at::kFloat, 3, index);
-    if (!t || t->size(2) != 2 || 2 * t->size(1) > dim || t->size(0) >= kMost || wants(*t)) return false;
+    if (!t || t->size(2) != 2 || 2 * t->size(1) > dim || t->size(0) >= kMost || wants(*t) ||
+        reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16)
+        return false;
     r = {static_cast<const float*>(t->const_data_ptr()), (uint32_t)t->size(0), (uint32_t)(2 * t->size(1)), (int)layout};
     return true;
 }

@@ -172,6 +172,8 @@ def _rotary_of(table, layout, dim, device, what):
     if table.device != device:
         raise ValueError(f"{what}: the table is not on {device}")
     table = table.contiguous()
+    if table.data_ptr() % 16:  # (rows of an odd number of angles: a slice may begin between)
+        table = table.clone()
     t = _native.KvRotaryTable()
     t.at, t.positions, t.dim, t.layout = table.data_ptr(), table.shape[0], 2 * table.shape[1], LAYOUTS[layout]
     return t, table

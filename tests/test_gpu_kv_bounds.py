@@ -505,3 +505,20 @@ def test_threads_with_a_stream_each():
         t.join()
     assert not errors, errors[0]
     assert all(good)
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("part, first", [(6, 1), (6, 2), (34, 3), (64, 1)])
+def test_a_slice_of_a_table_is_a_table(part, first, native, monkeypatch):
+    """Also where it begins at an address that is not a multiple of 16."""
+    if not native:
+        monkeypatch.setattr(_native, "_calls", None)
+    rng = np.random.default_rng(part)
+    b = Batch(rng, [(3, 20)] * 2, 2, 64, 16)
+    q, k, v = (heads(rng, (6, n, 64), "bf16") for n in (4, 2, 2))
+    at, whole = i32([0, 5, 9, 1, 1, 30]), kv_ops.rotary_table(40, part)
+    sliced = whole[first:]
+    got = kv_ops.rotary(q, k, at, sliced)
+    assert all(torch.equal(x, y) for x, y in zip(got, kv_ops.rotary(q, k, at + first, whole)))
+    got = kv_ops.append(b.cache, k, v, b.block_table, b.lengths, table=sliced, q=q)
+    assert torch.equal(got, kv_ops.append(b.cache, k, v, b.block_table, b.lengths, table=sliced.clone(), q=q))
