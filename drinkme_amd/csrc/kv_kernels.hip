@@ -811,7 +811,8 @@ extern "C" int dmx_kv_attention(const dmx_kv_cache* cache, const dmx_kv_seqs* se
     if (!q) return fail(err, errn, "null queries");
     if (q->heads == 0 || q->heads % cache->heads || q->heads > 65535)
         return fail(err, errn, "query heads not a multiple of the cache's, or too many");
-    if (!(scale > 0) || !std::isfinite(scale)) return fail(err, errn, "scale not a positive number");
+    const float scale2 = scale * 1.44269504088896341f;  // (the kernels' exponentials are of 2)
+    if (!(scale > 0) || !std::isfinite(scale2)) return fail(err, errn, "scale not a positive number, or too large");
     if (window >= (1u << 30)) return fail(err, errn, "window of 2^30 or more");
     if (seqs->total == 0) return 0;
     if (!q->at || !out) return fail(err, errn, "null queries or output");
@@ -826,7 +827,7 @@ extern "C" int dmx_kv_attention(const dmx_kv_cache* cache, const dmx_kv_seqs* se
     a.seqs = seqs_of(seqs);
     a.q = q->at, a.q_token = q->token_stride, a.q_head = q->head_stride;
     a.q_heads = q->heads, a.group = q->heads / cache->heads;
-    a.scale = scale * 1.44269504088896341f;
+    a.scale = scale2;
     a.causal = causal != 0, a.window = window, a.splits = p.splits;
     a.seqs.each = divisor_of(p.tokens);
     a.row_blocks = p.row_blocks;
