@@ -363,6 +363,7 @@ __device__ __forceinline__ void leave_rest(const AttnArgs& a, const Seq& q, uint
     const int end = q.token + q.count;
     int t = b == 0 ? 0 : q.token;
     const int last = b + 1 == a.seqs.batch ? (int)a.seqs.total : end, taken = q.token + min(q.count, (int)a.seqs.each.value);
+    if (__builtin_expect(t == q.token && taken == last, 1)) return;
 #pragma unroll 1
     for (;; ++t) {
         if (t == q.token) t = taken;
