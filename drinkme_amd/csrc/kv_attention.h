@@ -396,6 +396,7 @@ __device__ __forceinline__ void leave_rest(const AttnArgs& a, const Seq& q, uint
 // the matrix cores 14%. Short contexts wait for the chain of lengths, page and codes:
 // 5.2 us for 1021 tokens, 17 us for 8 of 4097 in pages of 16 with 5 rows (eight
 // blocks a wave, one wave a SIMD). fp32 queries, 4 of 4097 and one head of 256: 9.9 us.
+// Two tiles of heads of 256 take 22 registers (pages of 32 and more) or 42 in scratch.
 template <int W, int P, int NR, bool ROWS, bool WIDE>
 __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) void k_attend(const AttnArgs a) {
     using S = Segments<W>;
@@ -614,9 +615,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // Waves of a workgroup: eight, two a SIMD, which share a decoded token among 256
-// rows; four where 256 registers a lane are too few. TFLOP/s of a prompt of 1024
-// tokens in a context of 4096 with eight and with four: heads of 192 570 and 409, of
-// 256 433 and 520; us of the prompt above, heads of 128: 305 and 350.
+// rows; four, one a SIMD with 512 registers a lane, for heads of 256. (Eight take 256
+// registers, which heads of 192 exceed by 25 to 29, in scratch, and still gain.) TFLOP/s
+// of a prompt of 1024 tokens in a context of 4096 with eight and with four: heads of 192
+// 570 and 409, of 256 433 and 520; us of the prompt above, heads of 128: 305 and 350.
 constexpr int prompt_waves(int W) { return W <= 6 ? 8 : 4; }
 
 // Where leave_rest is done: by a block of rows more than there are, or, where its code costs

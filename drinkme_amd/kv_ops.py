@@ -354,8 +354,8 @@ def attention(q: torch.Tensor, cache: dict, block_table: torch.Tensor, lengths: 
     `scale` defaults to D^-0.5. A query at position p sees the positions of its
     sequence, with `causal` none after p, with `window` the last `window` of
     them (p among them); one that sees nothing gives zeros and -inf. With
-    `cu`, max_tokens bounds the new tokens of a sequence (T where not given:
-    more workgroups than needed); a sequence's tokens past it, and tokens of no
+    `cu`, max_tokens bounds the new tokens of a sequence (T where not given: the
+    launch is shaped for that, many single tokens as for a prompt); a sequence's tokens past it, and tokens of no
     sequence (before cu[0], from cu[B] on), give NaN. `max_length`, a bound on `lengths` where the
     block table is wider than needed, shapes the launch only."""
     native = _native.calls()
