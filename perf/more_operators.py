@@ -228,7 +228,7 @@ def _prepare_pages(case, gen, state):
         at += n
     free = torch.full_like(order, -1)
     free[:spare] = order[at:]
-    state["pool"] = {"free": free, "count": _i32([spare]), "short": _i32([0])}
+    state["pool"] = {"free": free, "count": _i32([spare]), "lacking": _i32([0])}
     state["block_table"], state["lengths"] = table, _i32([length for _, length in sizes])
     state["new"] = None if case["form"] == "even" and not case["pad"] else _i32([n for n, _ in sizes])
     state["keep"] = state["lengths"].clone()
@@ -416,7 +416,7 @@ def _plain_pages(state):
     taken = count - 1 - rank
     page = torch.where(taken >= 0, free[taken.clamp(min=0, max=free.shape[0] - 1)], -1)
     table.copy_(torch.where((col >= have[:, None]) & (col < want[:, None]), page, table))
-    pool["short"].copy_((need.sum() - count).clamp(min=0))
+    pool["lacking"].copy_((need.sum() - count).clamp(min=0))
     count.copy_((count - need.sum()).clamp(min=0))
     t = torch.arange(T, device="cuda")
     seq = torch.searchsorted(cu[1:], t.int(), right=True).clamp(max=B - 1)
@@ -439,7 +439,7 @@ def _plain_pages(state):
     count.add_(order[-1])
     table.masked_fill_(gone, -1)
     lengths.copy_(keep)
-    return [cu, positions, slots, table, lengths, free, count, pool["short"]]
+    return [cu, positions, slots, table, lengths, free, count, pool["lacking"]]
 
 
 def _plain_axes(state):
@@ -642,7 +642,7 @@ def run(state):
         pool, table, lengths = state["pool"], state["block_table"], state["lengths"]
         cu, positions, slots = kv_ops.reserve(pool, table, lengths, c["page"], state["total"], new=state["new"])
         kv_ops.trim(pool, table, lengths, c["page"], state["keep"])
-        return [cu, positions, slots, table, lengths, pool["free"], pool["count"], pool["short"]]
+        return [cu, positions, slots, table, lengths, pool["free"], pool["count"], pool["lacking"]]
     if c["kind"] == "axes":
         return list(kv_ops.rotary(state["q"], state["k"], state["positions"], state["table"], layout=c["layout"],
                                   axes=state["axes"]))
