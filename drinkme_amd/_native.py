@@ -1,4 +1,4 @@
-"""ctypes binding of libdmx_radix.so (include/dmx_radix.h, include/dmx_kv.h).
+"""ctypes binding of libdmx_radix.so (include/dmx_radix.h, dmx_kv.h, dmx_norm.h).
 
 The library is built in-tree by `python -m drinkme_amd.build` (or
 __graft_entry__.build()). There is no fallback: a missing library raises
@@ -107,6 +107,23 @@ class KvRotaryTable(ct.Structure):
     _fields_ = [("at", _P), ("positions", _U32), ("dim", _U32), ("layout", _I)]
 
 
+class KvRotaryAxes(ct.Structure):
+    """dmx_rotary_axes."""
+    _fields_ = [("count", _U32), ("of", _U32 * 16)]
+
+
+class KvPool(ct.Structure):
+    """dmx_kv_pool."""
+    _fields_ = [("free", _P), ("count", _P), ("lacking", _P), ("pages", _U32)]
+
+
+class KvSummaries(ct.Structure):
+    """dmx_kv_summaries."""
+    _fields_ = [("bounds", _P), ("scales", _P)]
+
+
+KV_MAX_COLUMNS = 16384  # DMX_KV_MAX_COLUMNS
+
 # every symbol include/dmx_kv.h declares
 KV_SIGNATURES = {
     "dmx_rotary": (_I, [_P, _P, _U32, _U32, _U32, _I, _P, _I, _P, _P, _P, _SZ]),
@@ -114,6 +131,36 @@ KV_SIGNATURES = {
     "dmx_kv_read": (_I, [_P, _P, _P, _P, _P, _P, _SZ]),
     "dmx_kv_attention_workspace": (_U64, [_P, _P, _U32, _I, _U32, _U32]),
     "dmx_kv_attention": (_I, [_P, _P, _P, _I, ct.c_float, _I, _U32, _U32, _P, _P, _P, _U64, _P, _P, _SZ]),
+    "dmx_rotary_by_axes": (_I, [_P, _P, _U32, _U32, _U32, _I, _P, _I, _P, _P, _P, _P, _SZ]),
+    "dmx_kv_reserve": (_I, [_P, _P, _P, _P, _U32, _U32, _U32, _U32, _P, _P, _P, _P, _P, _SZ]),
+    "dmx_kv_trim": (_I, [_P, _P, _P, _P, _U32, _U32, _U32, _P, _P, _SZ]),
+    "dmx_kv_summarize": (_I, [_P, _P, _P, _P, _P, _SZ]),
+    "dmx_kv_select": (_I, [_P, _P, _P, _P, _I, _U32, _U32, _U32, _I, _P, _P, _P, _SZ]),
+    "dmx_kv_attention_blocks_workspace": (_U64, [_P, _P, _U32, _I, _U32, _U32]),
+    "dmx_kv_attention_blocks": (_I, [_P, _P, _P, _I, ct.c_float, _I, _P, _U32, _U32, _P, _P, _P, _U64, _P, _P, _SZ]),
+}
+
+NORM_RMS = 0
+NORM_LAYER = 1
+NORM_MAX_DIM = 32768  # DMX_NORM_MAX_DIM
+
+
+class Vectors(ct.Structure):
+    """dmx_vectors."""
+    _fields_ = [("at", _P), ("dtype", _I), ("rows", _U32)]
+
+
+class NormForm(ct.Structure):
+    """dmx_norm_form."""
+    _fields_ = [("kind", _I), ("eps", ct.c_float), ("offset", ct.c_float), ("factor", ct.c_float), ("weight", Vectors),
+                ("bias", Vectors), ("post", Vectors), ("gate", Vectors), ("scale", Vectors), ("shift", Vectors),
+                ("cu", _P), ("batch", _U32)]
+
+
+# every symbol include/dmx_norm.h declares
+NORM_SIGNATURES = {
+    "dmx_norm": (_I, [_P, _P, _U32, _U32, _I, _P, _P, _P, _SZ]),
+    "dmx_block_norm": (_I, [_P, ct.c_int64, _P, ct.c_int64, _P, _P, _U32, _U32, _I, _I, _P, _P, _P, _SZ]),
 }
 
 _lib = None
@@ -126,7 +173,7 @@ def lib():
         if not os.path.exists(LIB):
             raise ImportError(f"libdmx_radix.so is not built ({LIB}); run `python -m drinkme_amd.build`")
         L = ct.CDLL(LIB)
-        for name, (res, args) in {**SIGNATURES, **KV_SIGNATURES}.items():
+        for name, (res, args) in {**SIGNATURES, **KV_SIGNATURES, **NORM_SIGNATURES}.items():
             fn = getattr(L, name)
             fn.restype = res
             fn.argtypes = args

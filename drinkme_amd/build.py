@@ -3,9 +3,9 @@
     python -m drinkme_amd.build
 
 The host codec (csrc/codec.cpp) and the pack-file reader and writer
-(csrc/pack_io.cpp) are compiled with g++, the kernels (csrc/kernels.hip, and
-those of the key/value cache, csrc/kv_kernels.hip) with hipcc for gfx950 only,
-and all linked into one shared library that ctypes loads (drinkme_amd/_native.py). Packed-fp32 instructions are
+(csrc/pack_io.cpp) are compiled with g++, the kernels (csrc/kernels.hip, those
+of the key/value cache, csrc/kv_*.hip, and the norms, csrc/norm_kernels.hip) with
+hipcc for gfx950 only, side by side, and all linked into one shared library that ctypes loads (drinkme_amd/_native.py). Packed-fp32 instructions are
 disabled for the device code (-packed-fp32-ops): hipcc otherwise forms
 v_pk_*_f32 from scalar float code. The host-only command line tool
 lib/dmx_pack (csrc/dmx_pack.cpp) is linked from the same host sources. The
@@ -20,6 +20,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -31,6 +32,7 @@ CLI = os.path.join(LIBDIR, "dmx_pack")
 CALLS = os.path.join(LIBDIR, "dmx_calls.so")
 INCLUDE = os.path.join(ROOT, "include")
 ARCH = "gfx950"
+KERNELS = ("kernels", "kv_kernels", "kv_pages", "kv_select", "kv_listed", "norm_kernels")
 
 
 def _hipcc() -> str:
@@ -65,11 +67,10 @@ def build(verbose: bool = False) -> str:
         obj = os.path.join(OBJ, f"{src}.o")
         _run([*host, "-c", os.path.join(CSRC, f"{src}.cpp"), "-o", obj], verbose)
         objs.append(obj)
-    kernels = []
-    for src in ("kernels", "kv_kernels"):
-        obj = os.path.join(OBJ, f"{src}.o")
-        _run([hipcc, *device_flags(), "-c", os.path.join(CSRC, f"{src}.hip"), "-o", obj], verbose)
-        kernels.append(obj)
+    kernels = [os.path.join(OBJ, f"{src}.o") for src in KERNELS]
+    with ThreadPoolExecutor(len(KERNELS)) as pool:
+        list(pool.map(lambda src, obj: _run([hipcc, *device_flags(), "-c", os.path.join(CSRC, f"{src}.hip"), "-o", obj],
+                                            verbose), KERNELS, kernels))
     tmp = LIB + ".tmp"
     _run([hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-pthread", objs[0], objs[1], *kernels, "-o", tmp],
          verbose)

@@ -1,5 +1,5 @@
 // The attention over the 4-bit cache (include/dmx_kv.h), included by
-// kv_kernels.hip.
+// kv_kernels.hip and, for the attention over listed pages, kv_listed.hip.
 //
 // The mathematics. A workgroup takes the query rows of one sequence that share
 // a cache head (new tokens x query heads of the group) in tiles of 16, and
@@ -40,6 +40,9 @@ struct AttnArgs {
     float* lse;
     float* part_o;   // [splits][total * q_heads][dim]
     f32x4* part_stat;  // [splits][total * q_heads]: reference (log2 domain), sum, sum of the rounded weights
+    // listed pages (k_attend's LISTED)
+    const int32_t* blocks;  // [total, heads, count] columns of the block table
+    Divisor count;
 };
 
 // Segments of V: 128 channels (lane i reads word i, 8 channels), then 64
@@ -89,9 +92,14 @@ __device__ __forceinline__ Place place_of(const AttnArgs& a, uint32_t h, uint32_
     return {base, WIDE ? 8u * octet : 0u, ok};
 }
 
-// The page numbers of a lane's K and V tokens in a block.
+// The page numbers of a lane's K and V tokens in a block; of listed pages also where
+// its octet of scores lies, and which of the tile's tokens list that page.
 struct Entry {
     uint32_t k, v;
+};
+struct ListedEntry : Entry {
+    int at;
+    uint32_t who;
 };
 
 // The scale operand of the conversions takes the exponent bits alone; sign and
@@ -237,11 +245,11 @@ __device__ __forceinline__ void hide_values(State<W, P, NR>& st, Block<W>& x, in
 }
 
 // A block's part of the rows' results.
+// t0: the first of the eight tokens whose scores are this lane's.
 template <int W, int P, int NR>
-__device__ __forceinline__ void attend_block(State<W, P, NR>& st, Block<W>& x, float scale, int blk, int i, int j, bool fresh,
+__device__ __forceinline__ void attend_block(State<W, P, NR>& st, Block<W>& x, float scale, int t0, int i, int j, bool fresh,
                                              bool part, int hi_all) {
     using S = Segments<W>;
-    const int t0 = blk * 32 + 8 * j;  // this lane's scores are of tokens t0 .. t0 + 7
 
     // scores: S^T = K Q^T
     f32x4 sc[NR][2];
@@ -384,6 +392,70 @@ __device__ __forceinline__ void leave_rest(const AttnArgs& a, const Seq& q, uint
     }
 }
 
+// What the tokens m0 .. m1 of a sequence (32 at most: a bit each) list for head h:
+// who[c] of each column that one of them may see, and those columns in ascending
+// order in `list` -> how many. A column listed twice is there once; one that is
+// negative, or past its token's position, is nothing. `beyond` has the tokens that
+// list a position which the table has no page for.
+__device__ __forceinline__ int list_pages(const AttnArgs& a, uint32_t h, const Seq& q, int m0, int m1, uint32_t* who, uint16_t* list,
+                                          uint32_t& beyond) {
+    __shared__ int counts[kAttnWaves];
+    __shared__ uint32_t past;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), shift = a.cache.page_shift;
+    const auto last_of = [&](int m) { return (a.causal ? q.first + m : q.length - 1) >> shift; };  // (negative: none)
+    const int cols = min(last_of(m1) + 1, a.seqs.cols), entries = (m1 - m0 + 1) * (int)a.count.value;
+    for (int c = threadIdx.x; c < cols; c += 64 * kAttnWaves) who[c] = 0;
+    if (threadIdx.x == 0) past = 0;
+    __syncthreads();
+    for (int n = threadIdx.x; n < entries; n += 64 * kAttnWaves) {
+        const int token = (uint32_t)n / a.count;
+        const int64_t row = (int64_t)(q.token + m0 + token) * a.cache.heads + h;
+        const int c = a.blocks[row * a.count.value + (n - token * (int)a.count.value)];
+        if (c >= 0 && c <= last_of(m0 + token)) atomicOr(c < a.seqs.cols ? who + c : &past, 1u << token);
+    }
+    __syncthreads();
+    const int each = (cols + 64 * kAttnWaves - 1) / (64 * kAttnWaves) * 64, first = wave * each, end = min(first + each, cols);
+    int found = 0;
+    for (int c = first; c < end; c += 64) found += __popcll(__ballot(c + lane < end && who[c + lane]));
+    if (lane == 0) counts[wave] = found;
+    __syncthreads();
+    int at = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kAttnWaves; ++w) {
+        at += w < wave ? counts[w] : 0;
+        all += counts[w];
+    }
+    for (int c = first; c < end; c += 64) {
+        const bool in = c + lane < end && who[c + lane];
+        const uint64_t m = __ballot(in);
+        if (in) list[at + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0))] = (uint16_t)(c + lane);
+        at += __popcll(m);
+    }
+    beyond = past;
+    __syncthreads();
+    return all;
+}
+
+// As entries, of block blk of the listed pages' tokens, one page after the other.
+template <bool WIDE>
+__device__ __forceinline__ ListedEntry listed_entries(const AttnArgs& a, uint32_t b, int blk, int i, int j, int count,
+                                                      const uint32_t* who, const uint16_t* list) {
+    const int shift = a.cache.page_shift;
+    const auto page_at = [&](int octet, int& col) {
+        const int n = (blk * 32 + 8 * octet) >> shift;
+        col = n < count ? list[n] : -1;
+        return col < 0 ? ~0u : (uint32_t)a.seqs.table[(int64_t)b * a.seqs.cols + col];
+    };
+    ListedEntry e;
+    int col;
+    if (!WIDE) e.k = page_at(i >> 2, col);
+    e.v = page_at(WIDE ? 0 : j, col);
+    if (WIDE) e.k = e.v;
+    e.at = col < 0 ? 1 << 30 : (col << shift) + ((blk * 32 + 8 * j) & ((1 << shift) - 1));
+    e.who = col < 0 ? 0 : who[col];
+    return e;
+}
+
 // W: dim / 32. P: bf16 pieces of the queries and weights (1: bf16, 3: fp32).
 // NR: tiles of 16 query rows a wave. ROWS (fp32 prompts): the workgroup's waves
 // take rows of their own and every token; else they share the rows and deal the
@@ -397,7 +469,10 @@ __device__ __forceinline__ void leave_rest(const AttnArgs& a, const Seq& q, uint
 // 5.2 us for 1021 tokens, 17 us for 8 of 4097 in pages of 16 with 5 rows (eight
 // blocks a wave, one wave a SIMD). fp32 queries, 4 of 4097 and one head of 256: 9.9 us.
 // Two tiles of heads of 256 take 22 registers (pages of 32 and more) or 42 in scratch.
-template <int W, int P, int NR, bool ROWS, bool WIDE>
+//
+// LISTED: of the columns that each token sees, those that it lists; a tile walks the
+// pages that any of its tokens lists, and a row's weights of the others are 0.
+template <int W, int P, int NR, bool ROWS, bool WIDE, bool LISTED = false>
 __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) void k_attend(const AttnArgs a) {
     using S = Segments<W>;
     constexpr int D = 32 * W, NT = D / 16;
@@ -418,7 +493,19 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
     const auto lo_of = [&](int m) { return a.window ? max(0, q.first + m + 1 - (int)a.window) : 0; };
     const int hi_all = min(hi_of(m1), cap), lo_all = lo_of(m0);
     const int full_hi = hi_of(m0), full_lo = lo_of(m1);  // every row sees what lies in between
-    const int blk_lo = lo_all >> 5, blk_hi = hi_all > lo_all ? (hi_all + 31) >> 5 : blk_lo;
+    int blk_lo = lo_all >> 5, blk_hi = hi_all > lo_all ? (hi_all + 31) >> 5 : blk_lo;
+    uint32_t* who = nullptr;
+    uint16_t* list = nullptr;
+    int listed = 0;
+    uint32_t beyond = 0;
+    if constexpr (LISTED) {
+        extern __shared__ __align__(16) char lds[];
+        who = reinterpret_cast<uint32_t*>(lds);
+        list = reinterpret_cast<uint16_t*>(who + a.seqs.cols);
+        listed = list_pages(a, h, q, m0, m1, who, list, beyond);
+        blk_lo = 0;
+        blk_hi = ((listed << a.cache.page_shift) + 31) >> 5;
+    }
     const int per = (blk_hi - blk_lo + (int)a.splits - 1) / (int)a.splits;
     const int blk_first = blk_lo + (int)split * per, blk_end = min(blk_first + per, blk_hi);
     constexpr int step = ROWS ? 1 : kAttnWaves;
@@ -426,14 +513,26 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
 
     // Loads run ahead of their use: page numbers two blocks, a block's codes one.
     Block<W> x[2];
-    Entry e[2] = {};
+    std::conditional_t<LISTED, ListedEntry, Entry> e[2] = {};
+    ListedEntry of[2] = {};  // (what x was loaded by)
+    const auto look_up = [&](int at) {
+        if constexpr (LISTED)
+            return listed_entries<WIDE>(a, b, at, i, j, listed, who, list);
+        else
+            return entries<WIDE>(a, b, at, i, j);
+    };
+    const auto load = [&](int at, int n) {
+        fetch<WIDE>(a, h, at, e[n], i, j, x[n]);
+        if constexpr (LISTED) of[n] = e[n];
+    };
     if (blk < blk_end) {
-        e[0] = entries<WIDE>(a, b, blk, i, j);
-        e[1] = entries<WIDE>(a, b, blk + step, i, j);
+        e[0] = look_up(blk);
+        e[1] = look_up(blk + step);
     }
 
     State<W, P, NR> st;
     int64_t row_out[NR];  // (token, head) in the output, -1: no row
+    int row_hi[NR], row_token[NR];  // (LISTED: what a row sees of a page that it lists; its token in the tile)
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
         const int r = r0 + 16 * t + i;
@@ -441,6 +540,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
         const int m = ok ? r / (int)a.group : 0, g = ok ? r - m * (int)a.group : 0;
         st.hi[t] = ok ? hi_of(m) : 0;
         st.lo[t] = lo_of(m);
+        row_hi[t] = st.hi[t];
+        row_token[t] = max(m - m0, 0);
         const int64_t token = q.token + m, head = (int64_t)h * a.group + g;
         row_out[t] = ok ? token * a.q_heads + head : -1;  // (past the last row: the first one's queries, unused)
         const int64_t at = token * a.q_token + head * a.q_head + 8 * W * j;
@@ -465,29 +566,42 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
         for (int c = 0; c < NT; ++c) st.o[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    const auto work = [&](Block<W>& y) {
-        const bool part = blk * 32 < full_lo || blk * 32 + 32 > full_hi;
-        // (a row that sees nothing of the wave's block before this one sees it from full_lo at the latest)
-        const bool fresh = blk < blk_first + step || (blk - step) * 32 < full_lo;
-        attend_block(st, y, a.scale, blk, i, j, fresh, part, hi_all);
+    const auto work = [&](int n) {
+        if constexpr (LISTED) {
+            const ListedEntry& y = of[n];
+            const uint32_t everyone = ~0u >> (31 - (m1 - m0));
+            const bool part = __any(y.who != everyone || y.at + 8 > full_hi);
+            bool unseen = false;  // (a row that has seen nothing yet: any block may be its first)
+#pragma unroll
+            for (int t = 0; t < NR; ++t) {
+                st.hi[t] = y.who >> row_token[t] & 1 ? row_hi[t] : 0;
+                unseen |= row_out[t] >= 0 && st.mx[t] == -INFINITY;
+            }
+            attend_block(st, x[n], a.scale, y.at, i, j, __any(unseen), part, hi_all);
+        } else {
+            const bool part = blk * 32 < full_lo || blk * 32 + 32 > full_hi;
+            // (a row that sees nothing of the wave's block before this one sees it from full_lo at the latest)
+            const bool fresh = blk < blk_first + step || (blk - step) * 32 < full_lo;
+            attend_block(st, x[n], a.scale, blk * 32 + 8 * j, i, j, fresh, part, hi_all);
+        }
         blk += step;
     };
     if (blk < blk_end) {
-        fetch<WIDE>(a, h, blk, e[0], i, j, x[0]);
+        load(blk, 0);
         for (;;) {
             const bool more = blk + step < blk_end;
             if (more) {
-                fetch<WIDE>(a, h, blk + step, e[1], i, j, x[1]);
-                e[0] = entries<WIDE>(a, b, blk + 2 * step, i, j);
+                load(blk + step, 1);
+                e[0] = look_up(blk + 2 * step);
             }
-            work(x[0]);
+            work(0);
             if (!more) break;
             const bool again = blk + step < blk_end;
             if (again) {
-                fetch<WIDE>(a, h, blk + step, e[0], i, j, x[0]);
-                e[1] = entries<WIDE>(a, b, blk + 2 * step, i, j);
+                load(blk + step, 0);
+                e[1] = look_up(blk + 2 * step);
             }
-            work(x[1]);
+            work(1);
             if (!again) break;
         }
     }
@@ -557,7 +671,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
     for (int t = 0; t < NR; ++t) {
         if (row_out[t] < 0) continue;
         float sum = st.sum[t];
-        if (st.hi[t] > cap) sum = NAN;  // it sees positions that the table has no page for
+        if (LISTED ? beyond >> row_token[t] & 1 : st.hi[t] > cap) sum = NAN;  // it sees positions that the table has no page for
         const float inv = !done || st.norm[t] == 0.f ? 1.f : 1.f / st.norm[t];
         if (j == 0) {
             if (!done)

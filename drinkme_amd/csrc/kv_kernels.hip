@@ -1,173 +1,13 @@
 // The operators between a decoder's q/k/v and o projections (include/dmx_kv.h):
 // gfx950 kernels and the C-ABI entry points that launch them.
 //
-//   k_rotary, k_rotary_any   rotary positions
+//   k_rotary, k_rotary_any   rotary positions, of one axis or several
 //   k_append                 keys (rotated) and values into the 4-bit cache
 //   k_read                   cached tokens back to bf16
 //   k_attend, k_attend_join  the attention over the cache (kv_attention.h)
-#include <hip/hip_runtime.h>
-
-#include <math.h>
-#include <stdint.h>
-#include <stdio.h>
-#include <string.h>
-
-#include <algorithm>
-#include <atomic>
-#include <type_traits>
-
-#include "dmx_kv.h"
-#include "dmx_radix.h"
+#include "kv_common.h"
 
 namespace {
-
-struct Cache {
-    uint32_t* k_codes;
-    uint32_t* v_codes;
-    uint8_t* k_scales;
-    uint8_t* v_scales;
-    uint32_t pages, heads, page_shift;
-};
-
-// A divisor known to the host: n / d, n < 2^31, by a multiplication. With s the
-// least for which 2^s >= d, 2^(32 + s) / d lies between 2^32 and 2^33; mul is
-// its excess over 2^32, rounded up, and the error stays below 1 / d.
-struct Divisor {
-    uint32_t mul, shift, value;
-};
-__device__ __forceinline__ uint32_t operator/(uint32_t n, const Divisor& d) { return (__umulhi(n, d.mul) + n) >> d.shift; }
-
-// n = a * d + b: a into n, b returned.
-__device__ __forceinline__ uint32_t take(uint32_t& n, const Divisor& d) {
-    const uint32_t a = n / d, b = n - a * d.value;
-    n = a;
-    return b;
-}
-
-struct Seqs {
-    const int32_t* table;
-    const int32_t* lengths;
-    const int32_t* cu;
-    uint32_t batch, total;
-    int cols;
-    Divisor each;  // new tokens of each sequence (attention with cu: at most)
-};
-
-struct Rows {
-    void* at;
-    int64_t token, head;  // strides, elements
-    uint32_t heads;
-};
-
-struct Table {
-    const float* at;
-    uint32_t positions, half;  // half: angles
-    int layout;
-};
-
-// ------------------------------------------------------------- sequences --
-
-struct Seq {
-    int token, count;   // its new tokens in [total]: the first one, how many
-    int first, length;  // position of the first one; tokens in all
-};
-
-// Sequence b of a call. cu is clamped to [0, total], so that no token index
-// leaves the call's tensors whatever it holds.
-__device__ __forceinline__ Seq seq_of(const Seqs& s, uint32_t b) {
-    Seq q;
-    if (s.cu) {
-        q.token = min(max(s.cu[b], 0), (int)s.total);
-        q.count = min(max(s.cu[b + 1], q.token), (int)s.total) - q.token;
-    } else {
-        q.count = s.each.value;
-        q.token = b * q.count;
-    }
-    q.length = max(s.lengths[b], 0);
-    q.first = q.length - q.count;
-    return q;
-}
-
-// The sequence of new token t: the last one that begins at or before it.
-__device__ __forceinline__ uint32_t seq_at(const Seqs& s, uint32_t t) {
-    if (!s.cu) return t / s.each;
-    uint32_t lo = 0, hi = s.batch - 1;
-    while (lo < hi) {
-        const uint32_t mid = (lo + hi + 1) >> 1;
-        if (s.cu[mid] <= (int)t)
-            lo = mid;
-        else
-            hi = mid - 1;
-    }
-    return lo;
-}
-
-struct Slot {
-    uint64_t token;  // (page, head, slot) as one index
-    bool ok;         // false: no page there, and the index is page 0's
-};
-
-// Where position p of sequence b and a cache head lies.
-__device__ __forceinline__ Slot slot_of(const Cache& c, const Seqs& s, uint32_t b, uint32_t head, uint32_t p) {
-    const uint32_t col = p >> c.page_shift;
-    uint32_t page = ~0u;
-    if (col < (uint32_t)s.cols) page = (uint32_t)s.table[(int64_t)b * s.cols + col];
-    const bool ok = page < c.pages;
-    const uint32_t slot = p & ((1u << c.page_shift) - 1u);
-    return {(((uint64_t)(ok ? page : 0u) * c.heads + head) << c.page_shift) + slot, ok};
-}
-
-// ------------------------------------------------------------ activations --
-
-// Eight adjacent channels as fp32.
-template <bool F32>
-__device__ __forceinline__ void load8(const void* base, int64_t at, float (&x)[8]) {
-    if constexpr (F32) {
-        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
-        const float4 a = p[0], b = p[1];
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-        const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            x[2 * n] = __uint_as_float(w[n] << 16);
-            x[2 * n + 1] = __uint_as_float(w[n] & 0xffff0000u);
-        }
-    }
-}
-
-template <bool F32>
-__device__ __forceinline__ void store8(void* base, int64_t at, const float (&x)[8]) {
-    if constexpr (F32) {
-        float4* p = reinterpret_cast<float4*>(static_cast<float*>(base) + at);
-        p[0] = make_float4(x[0], x[1], x[2], x[3]);
-        p[1] = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
-        uint32_t w[4];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            typedef __bf16 pair __attribute__((ext_vector_type(2)));
-            const pair b = {(__bf16)x[2 * n], (__bf16)x[2 * n + 1]};
-            w[n] = __builtin_bit_cast(uint32_t, b);
-        }
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + at) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-}
-
-template <bool F32>
-__device__ __forceinline__ float load1(const void* base, int64_t at) {
-    if constexpr (F32) return static_cast<const float*>(base)[at];
-    return __uint_as_float((uint32_t) static_cast<const uint16_t*>(base)[at] << 16);
-}
-
-template <bool F32>
-__device__ __forceinline__ void store1(void* base, int64_t at, float x) {
-    if constexpr (F32)
-        static_cast<float*>(base)[at] = x;
-    else
-        static_cast<uint16_t*>(base)[at] = __builtin_bit_cast(uint16_t, (__bf16)x);
-}
 
 // ----------------------------------------------------------------- rotary --
 
@@ -213,6 +53,53 @@ __device__ __forceinline__ int64_t position_of(const Rotation& r, uint32_t t) {
     return (int64_t)q.first + ((int)t - q.token);
 }
 
+// Positions of several axes, [axes, tokens]: angle i follows axis of[i / 16] >> 2 (i % 16) & 3.
+struct AxesRotation : Rotation {
+    uint32_t axes;
+    uint32_t of[16];
+};
+
+// Eight angles' cos and sin from angle 8 c of token t, and the one of angle c.
+__device__ __forceinline__ void angles_of(const Rotation& r, uint32_t t, uint32_t c, float (&cs)[8], float (&sn)[8]) {
+    angles<8>(r.table, position_of(r, t), 8 * c, cs, sn);
+}
+__device__ __forceinline__ void angle_of(const Rotation& r, uint32_t t, uint32_t c, float& cs, float& sn) {
+    const int64_t p = position_of(r, t);
+    const bool ok = p >= 0 && p < (int64_t)r.table.positions;
+    const float* at = r.table.at + 2 * ((ok ? p : 0) * r.table.half + c);
+    cs = ok ? at[0] : NAN, sn = ok ? at[1] : NAN;
+}
+
+__device__ __forceinline__ int64_t position_of(const AxesRotation& r, uint32_t t, uint32_t axis) {
+    const int64_t at = (int64_t)axis * r.tokens + t;
+    return r.wide ? static_cast<const int64_t*>(r.positions)[at] : static_cast<const int32_t*>(r.positions)[at];
+}
+// (eight angles of one axis are one piece of a row of the table; of several, each its own)
+__device__ __forceinline__ void angles_of(const AxesRotation& r, uint32_t t, uint32_t c, float (&cs)[8], float (&sn)[8]) {
+    const uint32_t of = r.of[c >> 1] >> (16 * (c & 1)) & 0xffffu;
+    if (of == (of & 3) * 0x5555u) {
+        angles<8>(r.table, position_of(r, t, of & 3), 8 * c, cs, sn);
+        return;
+    }
+    int64_t p[4];
+#pragma unroll
+    for (uint32_t x = 0; x < 4; ++x) p[x] = x < r.axes ? position_of(r, t, x) : 0;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+        const uint32_t x = of >> (2 * n) & 3;
+        const int64_t at = x == 0 ? p[0] : x == 1 ? p[1] : x == 2 ? p[2] : p[3];
+        const bool ok = at >= 0 && at < (int64_t)r.table.positions;
+        const float2 v = *reinterpret_cast<const float2*>(r.table.at + 2 * ((ok ? at : 0) * r.table.half + 8 * c + n));
+        cs[n] = ok ? v.x : NAN, sn[n] = ok ? v.y : NAN;
+    }
+}
+__device__ __forceinline__ void angle_of(const AxesRotation& r, uint32_t t, uint32_t c, float& cs, float& sn) {
+    const int64_t p = position_of(r, t, r.of[c >> 4] >> (2 * (c & 15)) & 3);
+    const bool ok = p >= 0 && p < (int64_t)r.table.positions;
+    const float* at = r.table.at + 2 * ((ok ? p : 0) * r.table.half + c);
+    cs = ok ? at[0] : NAN, sn = ok ? at[1] : NAN;
+}
+
 struct RotaryItem {
     uint32_t c, t, first, end;  // heads of both tensors, in's first
 };
@@ -236,14 +123,14 @@ __device__ __forceinline__ RowAt row_at(const Rotation& r, uint32_t t, uint32_t 
 // c: 16 channels, two runs of 8. In the turned part the eight pairs of angles
 // 8 c .. 8 c + 7, else 16 channels to copy. Takes 16-byte aligned rows, dim and
 // the turned channels multiples of 16.
-template <bool F32>
-__device__ __forceinline__ void rotate(const Rotation& r, uint32_t item) {
+template <bool F32, typename R>
+__device__ __forceinline__ void rotate(const R& r, uint32_t item) {
     const auto [c, t, first, end] = rotary_item_of(r, item);
     if (t >= r.tokens) return;
     const bool turned = 8 * c < r.table.half, split = turned && r.table.layout == DMX_ROTARY_HALF;
     const uint32_t x = split ? 8 * c : 16 * c, y = split ? 8 * c + r.table.half : 16 * c + 8;
     float cs[8], sn[8];
-    if (turned) angles<8>(r.table, position_of(r, t), 8 * c, cs, sn);
+    if (turned) angles_of(r, t, c, cs, sn);
     for (uint32_t h = first; h < end; ++h) {
         const RowAt row = row_at(r, t, h);
         float a[8], b[8];
@@ -265,19 +152,14 @@ __device__ __forceinline__ void rotate(const Rotation& r, uint32_t item) {
 }
 
 // Any sizes, strides and alignment. c: a pair of channels.
-template <bool F32>
-__device__ __forceinline__ void rotate_any(const Rotation& r, uint32_t item) {
+template <bool F32, typename R>
+__device__ __forceinline__ void rotate_any(const R& r, uint32_t item) {
     const auto [c, t, first, end] = rotary_item_of(r, item);
     if (t >= r.tokens) return;
     const bool turned = c < r.table.half, split = turned && r.table.layout == DMX_ROTARY_HALF;
     const uint32_t x = split ? c : 2 * c, y = split ? c + r.table.half : 2 * c + 1;
     float cs = 0.f, sn = 0.f;
-    if (turned) {
-        const int64_t p = position_of(r, t);
-        const bool ok = p >= 0 && p < (int64_t)r.table.positions;
-        const float* at = r.table.at + 2 * ((ok ? p : 0) * r.table.half + c);
-        cs = ok ? at[0] : NAN, sn = ok ? at[1] : NAN;
-    }
+    if (turned) angle_of(r, t, c, cs, sn);
     for (uint32_t h = first; h < end; ++h) {
         const RowAt row = row_at(r, t, h);
         float a = load1<F32>(row.in, row.from + x), b = load1<F32>(row.in, row.from + y);
@@ -291,13 +173,13 @@ __device__ __forceinline__ void rotate_any(const Rotation& r, uint32_t item) {
 // read and written, take 30.5 us (5.6 TB/s, part of the reads cached). A lane takes
 // two runs of 8 channels of a pair, 16 bytes each way, and its angles serve a run of
 // heads; one token takes 2.6 us, its launch.
-template <bool F32>
-__global__ __launch_bounds__(256) void k_rotary(const Rotation r) {
+template <bool F32, typename R>
+__global__ __launch_bounds__(256) void k_rotary(const R r) {
     rotate<F32>(r, blockIdx.x * 256 + threadIdx.x);
 }
 // (what k_rotary does not take, a value at a time)
-template <bool F32>
-__global__ __launch_bounds__(256) void k_rotary_any(const Rotation r) {
+template <bool F32, typename R>
+__global__ __launch_bounds__(256) void k_rotary_any(const R r) {
     rotate_any<F32>(r, blockIdx.x * 256 + threadIdx.x);
 }
 
@@ -367,18 +249,6 @@ __device__ __forceinline__ Item value_item(const Items& d, uint32_t n) {
     n >>= 3;
     const uint32_t w = take(n, d.words), k = take(n, d.runs);
     return {w, n * 8 + t, k * d.run};
-}
-
-// The place of new token t in head 0, and its position; a further head is a
-// page's tokens on. A token of no sequence (before the first offset, after the
-// last, or where offsets decrease) has none.
-__device__ __forceinline__ Slot slot_of_new(const Cache& c, const Seqs& s, uint32_t t, int& p) {
-    const uint32_t b = seq_at(s, t);
-    const Seq q = seq_of(s, b);
-    p = q.first + ((int)t - q.token);
-    Slot at = slot_of(c, s, b, 0, (uint32_t)max(p, 0));
-    at.ok = at.ok && p >= 0 && (!s.cu || (uint32_t)((int)t - q.token) < (uint32_t)q.count);
-    return at;
 }
 
 // Words of the keys. VEC: 16-byte aligned rows, and the turned channels a
@@ -521,89 +391,6 @@ __global__ __launch_bounds__(256) void k_read(const Cache c, const Seqs s, const
 
 #include "kv_attention.h"
 
-// -------------------------------------------------------------- host side --
-
-int fail(char* err, size_t n, const char* msg) {
-    if (err && n) {
-        strncpy(err, msg, n - 1);
-        err[n - 1] = 0;
-    }
-    return 1;
-}
-
-int launch_check(char* err, size_t errn, const char* what) {
-    const hipError_t e = hipGetLastError();
-    if (e == hipSuccess) return 0;
-    char msg[256];
-    snprintf(msg, sizeof msg, "%s: %s", what, hipGetErrorString(e));
-    return fail(err, errn, msg);
-}
-
-bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
-
-int check_cache(const dmx_kv_cache* c, char* err, size_t errn) {
-    if (!c) return fail(err, errn, "null cache");
-    if (!c->k_codes || !c->v_codes || !c->k_scales || !c->v_scales) return fail(err, errn, "null cache buffer");
-    if (!aligned(c->k_codes, 16) || !aligned(c->v_codes, 16) || !aligned(c->k_scales, 8) || !aligned(c->v_scales, 8))
-        return fail(err, errn, "cache buffers not aligned (codes 16 bytes, scales 8)");
-    if (c->pages == 0 || c->heads == 0) return fail(err, errn, "empty cache");
-    if (c->pages >= (1u << 31) || c->heads > 65535) return fail(err, errn, "cache of too many pages or heads");
-    if (c->page < 8 || c->page > 1024 || (c->page & (c->page - 1))) return fail(err, errn, "page not a power of two, 8..1024");
-    if (c->dim != 64 && c->dim != 96 && c->dim != 128 && c->dim != 192 && c->dim != 256)
-        return fail(err, errn, "head dim not 64, 96, 128, 192 or 256");
-    return 0;
-}
-
-int check_seqs(const dmx_kv_cache* c, const dmx_kv_seqs* s, char* err, size_t errn) {
-    if (!s) return fail(err, errn, "null sequences");
-    if (!s->table || !s->lengths) return fail(err, errn, "null block table or lengths");
-    if (s->batch == 0 || s->table_cols == 0) return fail(err, errn, "no sequences, or a block table without columns");
-    if (s->batch > 65535 || s->total >= (1u << 30)) return fail(err, errn, "too many sequences or tokens");
-    if ((uint64_t)s->table_cols * c->page >= (1ull << 30)) return fail(err, errn, "a block table of 2^30 positions or more");
-    if (!s->cu && s->total % s->batch) return fail(err, errn, "tokens not a multiple of the sequences, and no cu");
-    return 0;
-}
-
-int check_dtype(int dtype, char* err, size_t errn) {
-    return dtype == DMX_BF16 || dtype == DMX_F32 ? 0 : fail(err, errn, "dtype must be DMX_BF16 or DMX_F32");
-}
-
-int check_table(const dmx_rotary_table* t, uint32_t dim, char* err, size_t errn) {
-    if (!t->at) return fail(err, errn, "null rotary table");
-    if (!aligned(t->at, 16)) return fail(err, errn, "rotary table not 16-byte aligned");
-    if (t->positions == 0 || t->positions >= (1u << 31)) return fail(err, errn, "rotary table without positions, or too many");
-    if (t->dim == 0 || t->dim % 2 || t->dim > dim) return fail(err, errn, "rotary dim odd, zero or over the head's");
-    if (t->layout != DMX_ROTARY_HALF && t->layout != DMX_ROTARY_INTERLEAVED) return fail(err, errn, "unknown rotary layout");
-    return 0;
-}
-
-Cache cache_of(const dmx_kv_cache* c) {
-    return {c->k_codes, c->v_codes, c->k_scales, c->v_scales, c->pages, c->heads, (uint32_t)__builtin_ctz(c->page)};
-}
-Divisor divisor_of(uint32_t d) {
-    uint32_t shift = 0;
-    while ((1ull << shift) < d) ++shift;
-    return {(uint32_t)((((1ull << shift) - d) << 32) / d + 1), shift, d};
-}
-Seqs seqs_of(const dmx_kv_seqs* s) {
-    return {s->table, s->lengths, s->cu, s->batch, s->total, (int)s->table_cols, divisor_of(s->cu ? 1 : std::max(1u, s->total / s->batch))};
-}
-Rows rows_of(const dmx_rows* r) { return {r->at, r->token_stride, r->head_stride, r->heads}; }
-Table table_of(const dmx_rotary_table* t) { return {t->at, t->positions, t->dim / 2, t->layout}; }
-
-// Whether rows can be read and written 16 bytes at a time.
-bool wide_rows(const dmx_rows* r, int dtype) {
-    const int64_t n = dtype == DMX_F32 ? 4 : 8;
-    return aligned(r->at, 16) && r->token_stride % n == 0 && r->head_stride % n == 0;
-}
-
-// Blocks of 256 for `items`, whose numbers the kernels hold in 31 bits.
-int launch_blocks(uint64_t items, uint32_t& blocks, char* err, size_t errn) {
-    if (items >= (1ull << 31) - 256) return fail(err, errn, "too many values for one launch");
-    blocks = (uint32_t)((items + 255) / 256);
-    return 0;
-}
-
 // Heads that a lane takes one after the other, so that its token's place and angles
 // serve them all: more than one where there are lanes enough to fill the device
 // without (256 CUs of 2048, half of them). us of 6743 tokens appended and read, and
@@ -633,17 +420,22 @@ int cached_items(const dmx_kv_cache* c, uint32_t total, Items& d, uint32_t& keys
 
 }  // namespace
 
-extern "C" int dmx_rotary(const dmx_rows* in, const dmx_rows* out, uint32_t n, uint32_t tokens, uint32_t dim, int dtype,
-                          const void* positions, int wide, const dmx_rotary_table* table, void* stream, char* err,
-                          size_t errn) {
+namespace {
+
+// (before a call of no tokens returns)
+int check_rotation(const dmx_rows* in, const dmx_rows* out, uint32_t n, uint32_t tokens, uint32_t dim, int dtype,
+                   const dmx_rotary_table* table, char* err, size_t errn) {
     if (!in || !out || !table) return fail(err, errn, "null rows or table");
     if (n < 1 || n > 2) return fail(err, errn, "one or two tensors");
     if (dim == 0 || dim % 2 || dim > 65536) return fail(err, errn, "head dim odd, zero or over 65536");
-    if (check_dtype(dtype, err, errn) || check_table(table, dim, err, errn)) return 1;
-    if (tokens == 0) return 0;
+    return check_dtype(dtype, err, errn) || check_table(table, dim, err, errn);
+}
+
+template <typename R>
+int launch_rotation(R& r, const dmx_rows* in, const dmx_rows* out, uint32_t n, uint32_t tokens, uint32_t dim, int dtype,
+                    const void* positions, int wide, const dmx_rotary_table* table, void* stream, char* err, size_t errn) {
     if (tokens >= (1u << 30)) return fail(err, errn, "too many tokens");
     if (!positions) return fail(err, errn, "null positions");
-    Rotation r = {};
     bool vec = dim % 16 == 0 && table->dim % 16 == 0;
     for (uint32_t i = 0; i < n; ++i) {
         if (!in[i].at || !out[i].at) return fail(err, errn, "null rows");
@@ -658,10 +450,39 @@ extern "C" int dmx_rotary(const dmx_rows* in, const dmx_rows* out, uint32_t n, u
     r.table = table_of(table);
     uint32_t blocks;
     if (launch_blocks(rotary_items(r, vec), blocks, err, errn)) return 1;
-    const auto kern = vec ? (dtype == DMX_F32 ? k_rotary<true> : k_rotary<false>)
-                          : (dtype == DMX_F32 ? k_rotary_any<true> : k_rotary_any<false>);
+    const auto kern = vec ? (dtype == DMX_F32 ? k_rotary<true, R> : k_rotary<false, R>)
+                          : (dtype == DMX_F32 ? k_rotary_any<true, R> : k_rotary_any<false, R>);
     hipLaunchKernelGGL(kern, dim3(blocks), dim3(256), 0, static_cast<hipStream_t>(stream), r);
     return launch_check(err, errn, "rotary launch");
+}
+
+}  // namespace
+
+extern "C" int dmx_rotary(const dmx_rows* in, const dmx_rows* out, uint32_t n, uint32_t tokens, uint32_t dim, int dtype,
+                          const void* positions, int wide, const dmx_rotary_table* table, void* stream, char* err,
+                          size_t errn) {
+    if (check_rotation(in, out, n, tokens, dim, dtype, table, err, errn)) return 1;
+    if (tokens == 0) return 0;
+    Rotation r = {};
+    return launch_rotation(r, in, out, n, tokens, dim, dtype, positions, wide, table, stream, err, errn);
+}
+
+extern "C" int dmx_rotary_by_axes(const dmx_rows* in, const dmx_rows* out, uint32_t n, uint32_t tokens, uint32_t dim, int dtype,
+                                  const void* positions, int wide, const dmx_rotary_axes* axes, const dmx_rotary_table* table,
+                                  void* stream, char* err, size_t errn) {
+    if (check_rotation(in, out, n, tokens, dim, dtype, table, err, errn)) return 1;
+    if (!axes) return fail(err, errn, "null axes");
+    if (axes->count < 1 || axes->count > 4) return fail(err, errn, "no axes, or more than 4");
+    if (table->dim > 512) return fail(err, errn, "more than 256 angles");
+    AxesRotation r = {};
+    r.axes = axes->count;
+    for (uint32_t i = 0; i < table->dim / 2; ++i) {
+        const uint32_t axis = axes->of[i / 16] >> (2 * (i % 16)) & 3;
+        if (axis >= axes->count) return fail(err, errn, "an angle of an axis that there is not");
+        r.of[i / 16] |= axis << (2 * (i % 16));
+    }
+    if (tokens == 0) return 0;
+    return launch_rotation(r, in, out, n, tokens, dim, dtype, positions, wide, table, stream, err, errn);
 }
 
 extern "C" int dmx_kv_append(const dmx_kv_cache* cache, const dmx_kv_seqs* seqs, const dmx_rows* k, const dmx_rows* v,
@@ -757,18 +578,6 @@ Plan plan_of(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t q_heads, int 
 
 uint64_t workspace_of(const Plan& p, const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t q_heads) {
     return p.splits == 1 ? 0 : (uint64_t)p.splits * s->total * q_heads * (c->dim + 4) * 4;
-}
-
-// Lets a kernel have `bytes` of dynamic LDS on the current device (over 64 KB
-// takes an opt-in), once for each device.
-int allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& devices, char* err, size_t errn) {
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess || dev > 63) return fail(err, errn, "no current device");
-    if (devices.load() >> dev & 1) return 0;
-    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != hipSuccess) return fail(err, errn, "kv attention LDS opt-in refused");
-    devices.fetch_or(1ull << dev);
-    return 0;
 }
 
 template <int W, bool WIDE>

@@ -1,0 +1,122 @@
+// The attention over listed pages of the 4-bit cache (include/dmx_kv.h):
+// kv_attention.h's k_attend, whose tiles walk the pages that any of their tokens
+// lists, and its join.
+#include "kv_common.h"
+
+namespace {
+
+#include "kv_attention.h"
+
+// How a call is laid out: tiles of 16 rows a wave, and splits of each tile's pages.
+struct Plan {
+    int tiles;
+    uint32_t tokens, row_blocks, splits;  // tokens: of a sequence, at most
+    uint32_t listed;                      // columns that a tile may list, at most
+};
+
+Plan plan_of(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t q_heads, int dtype, uint32_t count, uint32_t max_length) {
+    Plan p;
+    const uint32_t group = q_heads / c->heads;
+    p.tokens = s->cu ? std::min(s->max_tokens, s->total) : s->total / s->batch;
+    const uint64_t rows = (uint64_t)p.tokens * group;
+    p.tiles = rows <= 16 || dtype == DMX_F32 ? 1 : 2;
+    const uint32_t a_tile = 16u * p.tiles, tile_tokens = std::min(p.tokens, 1 + (a_tile + group - 2) / group);
+    p.row_blocks = (uint32_t)((rows + a_tile - 1) / a_tile);
+    p.listed = (uint32_t)std::min<uint64_t>(s->table_cols, (uint64_t)tile_tokens * count);
+    uint64_t length = (uint64_t)p.listed * c->page;
+    if (max_length) length = std::min<uint64_t>(length, max_length);
+    // Splits to fill the CUs once, each of 128 tokens at least, a block of 32 a wave; up to 512 tokens none
+    // (k_attend's own rule, which its measurements are with)
+    const uint64_t groups = (uint64_t)c->heads * s->batch * std::max(1u, p.row_blocks);
+    const uint64_t wanted = std::max<uint64_t>(1, 256 / groups), possible = length <= 512 ? 1 : length / 128;
+    p.splits = (uint32_t)std::min<uint64_t>({wanted, possible, 64, 65535 / s->batch});
+    return p;
+}
+
+uint64_t workspace_of(const Plan& p, const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t q_heads) {
+    return p.splits == 1 ? 0 : (uint64_t)p.splits * s->total * q_heads * (c->dim + 4) * 4;
+}
+
+int check_listed(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t count, char* err, size_t errn) {
+    if (s->table_cols > DMX_KV_MAX_COLUMNS) return fail(err, errn, "a block table of more columns than can be listed (16384)");
+    if (count == 0 || count > DMX_KV_MAX_COLUMNS) return fail(err, errn, "lists of no columns, or more than 16384");
+    return 0;
+}
+
+template <int W, int P, int NR, bool WIDE>
+int launch(dim3 grid, int lds, hipStream_t stream, const AttnArgs& a, char* err, size_t errn) {
+    // (the most that any call takes: 16384 columns' bits, and as many 16-bit entries)
+    static std::atomic<uint64_t> allowed = {};
+    const auto kern = k_attend<W, P, NR, false, WIDE, true>;
+    if (allow_lds(reinterpret_cast<const void*>(kern), 6 * DMX_KV_MAX_COLUMNS, allowed, err, errn)) return 1;
+    hipLaunchKernelGGL(kern, grid, dim3(64 * kAttnWaves), lds, stream, a);
+    return launch_check(err, errn, "kv attention launch");
+}
+
+}  // namespace
+
+extern "C" uint64_t dmx_kv_attention_blocks_workspace(const dmx_kv_cache* cache, const dmx_kv_seqs* seqs, uint32_t q_heads,
+                                                      int dtype, uint32_t count, uint32_t max_length) {
+    if (check_cache(cache, nullptr, 0) || check_seqs(cache, seqs, nullptr, 0) || check_listed(cache, seqs, count, nullptr, 0) ||
+        q_heads == 0 || q_heads % cache->heads)
+        return 0;
+    return workspace_of(plan_of(cache, seqs, q_heads, dtype, count, max_length), cache, seqs, q_heads);
+}
+
+extern "C" int dmx_kv_attention_blocks(const dmx_kv_cache* cache, const dmx_kv_seqs* seqs, const dmx_rows* q, int dtype,
+                                       float scale, int causal, const int32_t* blocks, uint32_t count, uint32_t max_length,
+                                       void* out, float* lse, void* workspace, uint64_t workspace_bytes, void* stream,
+                                       char* err, size_t errn) {
+    if (check_cache(cache, err, errn) || check_seqs(cache, seqs, err, errn) || check_dtype(dtype, err, errn) ||
+        check_listed(cache, seqs, count, err, errn))
+        return 1;
+    if (!q) return fail(err, errn, "null queries");
+    if (q->heads == 0 || q->heads % cache->heads || q->heads > 65535)
+        return fail(err, errn, "query heads not a multiple of the cache's, or too many");
+    const float scale2 = scale * 1.44269504088896341f;  // (the kernels' exponentials are of 2)
+    if (!(scale > 0) || !std::isfinite(scale2)) return fail(err, errn, "scale not a positive number, or too large");
+    if (seqs->total == 0) return 0;
+    if (!q->at || !out || !blocks) return fail(err, errn, "null queries, lists or output");
+    if ((uint64_t)seqs->total * cache->heads * count >= 1ull << 62) return fail(err, errn, "too many lists");
+    const Plan p = plan_of(cache, seqs, q->heads, dtype, count, max_length);
+    if (p.row_blocks == 0) return fail(err, errn, "max_tokens is 0");
+    if (p.row_blocks > 65535) return fail(err, errn, "too many query rows of one sequence");
+    if (workspace_bytes < workspace_of(p, cache, seqs, q->heads) || (p.splits > 1 && (!workspace || !aligned(workspace, 16))))
+        return fail(err, errn, "workspace missing, short or not 16-byte aligned");
+    AttnArgs a = {};
+    a.cache = cache_of(cache);
+    a.seqs = seqs_of(seqs);
+    a.q = q->at, a.q_token = q->token_stride, a.q_head = q->head_stride;
+    a.q_heads = q->heads, a.group = q->heads / cache->heads;
+    a.scale = scale2;
+    a.causal = causal != 0, a.splits = p.splits;
+    a.seqs.each = divisor_of(p.tokens);
+    a.row_blocks = p.row_blocks;
+    a.out = out, a.lse = lse;
+    a.blocks = blocks, a.count = divisor_of(count);
+    const uint64_t all = (uint64_t)seqs->total * q->heads;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_stat = reinterpret_cast<f32x4*>(a.part_o + (p.splits > 1 ? p.splits * all * cache->dim : 0));
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const dim3 grid(cache->heads, p.row_blocks, seqs->batch * p.splits);
+    const int lds = 4 * (int)seqs->table_cols + 2 * (int)p.listed;
+    const auto by_tiles = [&](auto w, auto wide) {
+        constexpr int W = decltype(w)::value;
+        constexpr bool WIDE = decltype(wide)::value;
+        return dtype == DMX_F32 ? launch<W, 3, 1, WIDE>(grid, lds, st, a, err, errn)
+               : p.tiles == 1   ? launch<W, 1, 1, WIDE>(grid, lds, st, a, err, errn)
+                                : launch<W, 1, 2, WIDE>(grid, lds, st, a, err, errn);
+    };
+    const auto by_page = [&](auto w) { return cache->page >= 32 ? by_tiles(w, std::true_type{}) : by_tiles(w, std::false_type{}); };
+    const int rc = cache->dim == 64    ? by_page(std::integral_constant<int, 2>{})
+                   : cache->dim == 96  ? by_page(std::integral_constant<int, 3>{})
+                   : cache->dim == 128 ? by_page(std::integral_constant<int, 4>{})
+                   : cache->dim == 192 ? by_page(std::integral_constant<int, 6>{})
+                                       : by_page(std::integral_constant<int, 8>{});
+    if (rc) return 1;
+    if (p.splits == 1) return 0;
+    const int ways = p.splits > 8 ? 4 : 1;
+    hipLaunchKernelGGL((dtype == DMX_F32 ? k_attend_join<true> : k_attend_join<false>),
+                       dim3((uint32_t)(ways == 4 ? all : (all + 3) / 4)), dim3(256), 0, st, a, (int)cache->dim, ways);
+    return launch_check(err, errn, "kv attention join launch");
+}

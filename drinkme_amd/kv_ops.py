@@ -1,9 +1,11 @@
 """What a decoder does between its q/k/v and o projections, over
 libdmx_radix.so (include/dmx_kv.h): rotary positions, a paged key/value cache
-held in 4 bits, and the attention that reads it. No drinkme counterpart:
-drinkme leaves these to the model's own code.
+held in 4 bits, and the attention that reads it, over all that a sequence has
+cached or over the pages that a score selects. No drinkme counterpart: drinkme
+leaves these to the model's own code.
 
   rotary_table(positions, dim, ...)   the cos/sin table, plain or scaled to a long context
+  rotary_axes(sections, order)        which of several axes (time, height, width) turns each angle
   rotary(q, k, positions, table)      both rotated, one launch
   new_cache(pages, page_size, heads, dim)
                                       an empty cache: a dict of four tensors
@@ -11,6 +13,14 @@ drinkme leaves these to the model's own code.
   read(cache, ...)                    new tokens as the cache holds them, bf16
   attention(q, cache, ...)            queries against everything cached of their sequences
   cache_bytes(cache)                  device bytes of a cache
+
+  new_pool(pages)                     the pages of a cache that no sequence has
+  reserve(pool, block_table, ...)     pages, offsets, positions and slots for a step's new tokens
+  trim(pool, block_table, ...)        sequences cut back or ended, their pages returned
+
+  new_summaries(cache)                the bounds of each page's keys, 8 bits a channel
+  summarize(cache, summaries, ...)    those of the pages that new tokens lie in
+  select(q, cache, summaries, ...)    the pages that score highest for each token: attention's `blocks`
 
 The cache holds each token's keys and values, per head, as blocks of 32
 channels: an exponent byte and 32 four-bit codes (4.25 bits a value; the format
@@ -32,6 +42,7 @@ gradient: a call refuses tensors that ask for one or carry a tangent.
 from __future__ import annotations
 
 import ctypes as ct
+import functools
 import math
 
 import torch
@@ -94,8 +105,29 @@ def _frequencies(dim, base, scaling):
     return f, magnitude
 
 
+def rotary_axes(sections, order: str = "blocks") -> tuple:
+    """The axis of each angle, for rotary and rotary_table: sections[a] angles
+    follow axis a (4 axes at most), one axis after the other ("blocks"), or dealt
+    one angle to each axis in turn, an axis that has its share passed over
+    ("interleaved")."""
+    left = [int(n) for n in sections]
+    if not 1 <= len(left) <= 4 or min(left) < 0 or not 1 <= sum(left) <= 256:
+        raise ValueError(f"rotary_axes: sections {tuple(sections)}: 1..4 of them, 1..256 angles in all")
+    if order == "blocks":
+        return tuple(a for a, n in enumerate(left) for _ in range(n))
+    if order != "interleaved":
+        raise ValueError(f"rotary_axes: order {order!r} is not 'blocks' or 'interleaved'")
+    out = []
+    while any(left):
+        for a, n in enumerate(left):
+            if n:
+                out.append(a)
+                left[a] -= 1
+    return tuple(out)
+
+
 def rotary_table(positions: int, dim: int, base: float = 10000.0, scaling: dict | None = None,
-                 device="cuda") -> torch.Tensor:
+                 device="cuda", axes=None) -> torch.Tensor:
     """cos and sin of angle i (of dim / 2) at each position: fp32
     [positions, dim / 2, 2], computed in float64. `dim` counts the channels
     that turn, which may be part of the head. `scaling` stretches the
@@ -110,11 +142,28 @@ def rotary_table(positions: int, dim: int, base: float = 10000.0, scaling: dict 
                                       as above with a line over the angles' indices (YaRN), cos and sin times
                                       magnitude (0.1 ln factor + 1)
       {"kind": "divisors", "divisors", "magnitude": 1}
-                                      each angle by its own divisor"""
+                                      each angle by its own divisor
+
+    With `axes` (rotary_axes's, dim / 2 of them) every axis has a spectrum of its
+    own, as a table of its angles alone would have it; without, positions of several
+    axes share one over all angles."""
     positions, dim = int(positions), int(dim)
     if positions < 1 or dim < 2 or dim % 2:
         raise ValueError(f"rotary_table: {positions} positions of {dim} channels (an even number, at least 2)")
-    f, magnitude = _frequencies(dim, float(base), scaling)
+    if axes is None:
+        f, magnitude = _frequencies(dim, float(base), scaling)
+    else:
+        axes = tuple(axes)
+        if len(axes) != dim // 2:
+            raise ValueError(f"rotary_table: axes of {len(axes)} angles for {dim} channels")
+        if scaling is not None and scaling.get("kind") == "divisors":
+            raise ValueError("rotary_table: divisors are of one spectrum, which axes do not share")
+        if scaling is not None and scaling.get("kind") == "base" and any(axes.count(a) == 1 for a in axes):
+            raise ValueError("rotary_table: base scaling of an axis of one angle, whose base does not matter")
+        f, magnitude = torch.empty(dim // 2, dtype=torch.float64), 1.0
+        for axis in set(axes):
+            mine = torch.tensor([a == axis for a in axes])
+            f[mine], magnitude = _frequencies(2 * int(mine.sum()), float(base), scaling)
     t = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * f.to(device)
     return torch.stack([t.cos() * magnitude, t.sin() * magnitude], -1).float()
 
@@ -233,24 +282,46 @@ def _seqs_of(block_table, lengths, cu, total, max_tokens, device, what):
 # --------------------------------------------------------------- operators --
 
 
-def rotary(q: torch.Tensor, k, positions: torch.Tensor, table: torch.Tensor, layout: str = "half"):
+@functools.lru_cache(maxsize=64)
+def _packed_axes(axes: tuple):
+    """The dmx_rotary_axes of a tuple of axes: two bits an angle."""
+    if not 1 <= len(axes) <= 256 or any(type(a) is not int or not 0 <= a < 4 for a in axes):
+        raise ValueError("rotary: axes are 1..256 numbers of 0..3 (rotary_axes)")
+    x = _native.KvRotaryAxes()
+    x.count, x.angles = max(axes) + 1, len(axes)
+    for i, a in enumerate(axes):
+        x.of[i // 16] |= a << (2 * (i % 16))
+    return x
+
+
+def rotary(q: torch.Tensor, k, positions: torch.Tensor, table: torch.Tensor, layout: str = "half", axes=None):
     """q [T, Hq, D] and k [T, Hk, D] (or None) rotated by `positions` [T]
     (int32 or int64): the pair (a, b) of angle t becomes a cos t - b sin t,
     b cos t + a sin t, in fp32, rounded once to their dtype. Pairs are channels
     (i, i + dim / 2) of the table's dim ("half") or (2 i, 2 i + 1)
     ("interleaved"); channels past the table's dim are copied. Views of a fused
     product are read in place. -> (q', k'), dense. A position outside the table
-    gives NaN."""
+    gives NaN.
+
+    With `axes` (rotary_axes's: the axis of each of the table's angles) positions
+    are [axes, T], and angle i of token t is the table's at positions[axes[i], t]."""
     native = _native.calls()
-    if native is not None:  # the plain case in one native call; None: anything else
+    if native is not None and axes is None:  # the plain case in one native call; None: anything else
         outs = native.rotary(q, k, positions, table, LAYOUTS.get(layout, -1), _current(q))
         if outs is not None:
             return outs
     _no_gradient("rotary", q, k, table)
     q = _activation(q, "rotary: q")
     ins = [q] if k is None else [q, _activation(k, "rotary: k", dim=q.shape[2], tokens=q.shape[0], like=q)]
-    if positions.dtype not in (torch.int32, torch.int64) or positions.shape != q.shape[:1] or positions.device != q.device:
-        raise ValueError(f"rotary: positions must be int32 or int64 [{q.shape[0]}] on {q.device}, got {positions.dtype} "
+    shape = (q.shape[0],)
+    if axes is not None:
+        axes = _packed_axes(tuple(axes))
+        shape = (positions.shape[0], q.shape[0]) if positions.dim() and axes.count <= positions.shape[0] <= 4 else \
+            (axes.count, q.shape[0])
+        if table.dim() == 3 and table.shape[1] != axes.angles:
+            raise ValueError(f"rotary: axes of {axes.angles} angles for a table of {table.shape[1]}")
+    if positions.dtype not in (torch.int32, torch.int64) or positions.shape != shape or positions.device != q.device:
+        raise ValueError(f"rotary: positions must be int32 or int64 {list(shape)} on {q.device}, got {positions.dtype} "
                          f"{tuple(positions.shape)} on {positions.device}")
     positions = positions.contiguous()
     t, table = _rotary_of(table, layout, q.shape[2], q.device, "rotary")
@@ -258,10 +329,12 @@ def rotary(q: torch.Tensor, k, positions: torch.Tensor, table: torch.Tensor, lay
     n = len(ins)
     err = _native.error_buffer()
     with torch.cuda.device(q.device):
-        st = _native.lib().dmx_rotary((_native.KvRows * n)(*map(_rows, ins)), (_native.KvRows * n)(*map(_rows, outs)), n,
-                                      q.shape[0], q.shape[2], _dtype_code(q.dtype, "rotary"), positions.data_ptr(),
-                                      positions.dtype == torch.int64, ct.byref(t), _stream(q.device), err, len(err))
-    _native.check(st, err, "dmx_rotary")
+        head = ((_native.KvRows * n)(*map(_rows, ins)), (_native.KvRows * n)(*map(_rows, outs)), n, q.shape[0], q.shape[2],
+                _dtype_code(q.dtype, "rotary"), positions.data_ptr(), positions.dtype == torch.int64)
+        tail = (ct.byref(t), _stream(q.device), err, len(err))
+        st = _native.lib().dmx_rotary(*head, *tail) if axes is None else \
+            _native.lib().dmx_rotary_by_axes(*head, ct.byref(axes), *tail)
+    _native.check(st, err, "dmx_rotary" if axes is None else "dmx_rotary_by_axes")
     return outs[0], outs[1] if k is not None else None
 
 
@@ -346,7 +419,7 @@ def read(cache: dict, block_table: torch.Tensor, lengths: torch.Tensor, total: i
 
 def attention(q: torch.Tensor, cache: dict, block_table: torch.Tensor, lengths: torch.Tensor, *, cu=None,
               max_tokens: int | None = None, max_length: int | None = None, scale: float | None = None,
-              causal: bool = True, window: int | None = None, return_lse: bool = False):
+              causal: bool = True, window: int | None = None, return_lse: bool = False, blocks=None):
     """softmax(scale q k^T) v of the new tokens' queries q [T, Hq, D] (rotated
     already) over everything cached of their sequences -> [T, Hq, D] in q's
     dtype, and with return_lse each row's log-sum-exp, fp32 [T, Hq]. Hq is a
@@ -357,9 +430,14 @@ def attention(q: torch.Tensor, cache: dict, block_table: torch.Tensor, lengths: 
     `cu`, max_tokens bounds the new tokens of a sequence (T where not given: the
     launch is shaped for that, many single tokens as for a prompt); a sequence's tokens past it, and tokens of no
     sequence (before cu[0], from cu[B] on), give NaN. `max_length`, a bound on `lengths` where the
-    block table is wider than needed, shapes the launch only."""
+    block table is wider than needed, shapes the launch only.
+
+    With `blocks` [T, H, n], int32 (select's: columns of the block table), a query
+    sees the positions in those columns alone: of token t and cache head h
+    blocks[t, h], in any order, each once however often it is listed, negative ones
+    nothing. No window then."""
     native = _native.calls()
-    if native is not None:
+    if native is not None and blocks is None:
         outs = native.attention(q, cache, block_table, lengths, cu, max_tokens, max_length or 0, scale, causal, window,
                                 return_lse, _current(q))
         if outs is not None:
@@ -382,16 +460,205 @@ def attention(q: torch.Tensor, cache: dict, block_table: torch.Tensor, lengths: 
         window = None
     max_length = min(max_length or 0, _MOST)
     s, held = _seqs_of(block_table, lengths, cu, T, max_tokens, q.device, "attention")
+    if blocks is not None:
+        blocks = _blocks_of(blocks, T, c.heads, block_table, q.device)
+        if window is not None:
+            raise ValueError("attention: blocks and a window")
     out = torch.empty((T, Hq, c.dim), dtype=q.dtype, device=q.device)
     lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
     lib, code = _native.lib(), _dtype_code(q.dtype, "attention")
     scale = c.dim ** -0.5 if scale is None else float(scale)
-    bytes_ = lib.dmx_kv_attention_workspace(ct.byref(c), ct.byref(s), Hq, code, max_length, window or 0) if T else 0
+    if T == 0:
+        bytes_ = 0
+    elif blocks is None:
+        bytes_ = lib.dmx_kv_attention_workspace(ct.byref(c), ct.byref(s), Hq, code, max_length, window or 0)
+    else:
+        bytes_ = lib.dmx_kv_attention_blocks_workspace(ct.byref(c), ct.byref(s), Hq, code, blocks.shape[2], max_length)
     ws = torch.empty(bytes_, dtype=torch.uint8, device=q.device) if bytes_ else None
     err = _native.error_buffer()
     with torch.cuda.device(q.device):
-        st = lib.dmx_kv_attention(ct.byref(c), ct.byref(s), ct.byref(_rows(q)), code, scale, causal, window or 0,
-                                  max_length, out.data_ptr(), lse.data_ptr() if return_lse else None,
-                                  ws.data_ptr() if bytes_ else None, bytes_, _stream(q.device), err, len(err))
-    _native.check(st, err, "dmx_kv_attention")
+        head = (ct.byref(c), ct.byref(s), ct.byref(_rows(q)), code, scale, causal)
+        tail = (max_length, out.data_ptr(), lse.data_ptr() if return_lse else None, ws.data_ptr() if bytes_ else None, bytes_,
+                _stream(q.device), err, len(err))
+        st = lib.dmx_kv_attention(*head, window or 0, *tail) if blocks is None else \
+            lib.dmx_kv_attention_blocks(*head, blocks.data_ptr(), blocks.shape[2], *tail)
+    _native.check(st, err, "dmx_kv_attention" if blocks is None else "dmx_kv_attention_blocks")
     return (out, lse) if return_lse else out
+
+
+# ------------------------------------------------------------------- pages --
+
+_POOL = ("free", "count", "lacking")
+
+
+def new_pool(pages: int, device="cuda") -> dict:
+    """All pages of a cache of that many, free: `free` int32 [pages], a stack whose
+    first `count` [1] are in it, the last of them the next; `lacking` [1], the pages
+    that the last reserve wanted and did not get."""
+    if not 1 <= pages < _MOST:
+        raise ValueError(f"new_pool: {pages} pages (1 or more, fewer than 2^30)")
+    return {"free": torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=device),
+            "count": torch.full((1,), pages, dtype=torch.int32, device=device),
+            "lacking": torch.zeros(1, dtype=torch.int32, device=device)}
+
+
+def _own(t, what, dims, device):
+    """A tensor that a call writes in place: dense int32 on the GPU."""
+    if t.dtype != torch.int32 or t.dim() != dims or not t.is_contiguous() or t.device.type != "cuda" or \
+            (device is not None and t.device != device):
+        raise ValueError(f"{what} must be int32, dense, of {dims} dimension(s), on {device or 'the GPU'}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+    return t
+
+
+def _pages_of(pool, block_table, lengths, page_size, what):
+    """(dmx_kv_pool, table, lengths, batch, columns, page size), checked."""
+    device = _own(block_table, f"{what}: block_table", 2, None).device
+    _own(lengths, f"{what}: lengths", 1, device)
+    p = _native.KvPool()
+    for name in _POOL:
+        _own(pool[name], f"{what}: the pool's {name}", 1, device)
+        setattr(p, name, pool[name].data_ptr())
+    pages, (batch, columns) = pool["free"].shape[0], block_table.shape
+    if not 1 <= pages < _MOST or pool["count"].shape[0] != 1 or pool["lacking"].shape[0] != 1:
+        raise ValueError(f"{what}: a pool of {pages} pages, {pool['count'].shape[0]} counts")
+    if lengths.shape[0] != batch or batch < 1 or columns < 1 or max(batch, columns) >= _MOST:
+        raise ValueError(f"{what}: a block_table of {batch} rows and {columns} columns for {lengths.shape[0]} lengths")
+    if page_size < 8 or page_size > 1024 or page_size & (page_size - 1):
+        raise ValueError(f"{what}: page_size {page_size} is not a power of two, 8..1024")
+    p.pages = pages
+    return p, (block_table.data_ptr(), lengths.data_ptr()), (batch, columns, page_size), device
+
+
+def _numbers(t, what, batch, device):
+    if t.dtype != torch.int32 or t.shape != (batch,) or t.device != device:
+        raise ValueError(f"{what} must be int32 [{batch}] on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.contiguous()
+
+
+def reserve(pool: dict, block_table: torch.Tensor, lengths: torch.Tensor, page_size: int, total: int, *, new=None):
+    """Room for the new tokens of a step: new[b] of sequence b (int32 [B]; None:
+    total / B of each), `total` rows in all, which may be more than their sum (the
+    rows of a padded batch; where it is less, the sequences that pass it get
+    what is left). block_table, lengths and pool are updated in place, all on the
+    GPU: each column that a sequence's new tokens are the first in gets the pool's next
+    page, in the order of the sequences, or -1 where the pool is empty (pool["lacking"]
+    says how many had none). -> (cu [B + 1], positions [total] int32, slots [total]
+    int64): what append and attention take as `cu`, each new token's position (-1 in
+    rows of no sequence) and its place page * page_size + position % page_size (-1
+    without a page)."""
+    total = int(total)
+    p, at, sizes, device = _pages_of(pool, block_table, lengths, page_size, "reserve")
+    if total < 0 or total >= _MOST or (new is None and total % sizes[0]):
+        raise ValueError(f"reserve: {total} tokens" + (f" for {sizes[0]} sequences, and new is None" if new is None else ""))
+    if new is not None:
+        new = _numbers(new, "reserve: new", sizes[0], device)
+    cu = torch.empty(sizes[0] + 1, dtype=torch.int32, device=device)
+    positions = torch.empty(total, dtype=torch.int32, device=device)
+    slots = torch.empty(total, dtype=torch.int64, device=device)
+    err = _native.error_buffer()
+    with torch.cuda.device(device):
+        st = _native.lib().dmx_kv_reserve(ct.byref(p), *at, new.data_ptr() if new is not None else None, *sizes, total,
+                                          cu.data_ptr(), positions.data_ptr(), slots.data_ptr(), _stream(device), err, len(err))
+    _native.check(st, err, "dmx_kv_reserve")
+    return cu, positions, slots
+
+
+def trim(pool: dict, block_table: torch.Tensor, lengths: torch.Tensor, page_size: int, keep: torch.Tensor) -> None:
+    """Sequence b cut to its first keep[b] tokens (int32 [B]; 0 ends it, its
+    length or more leaves it), in place: lengths, the columns behind it (-1), and the
+    pool, which gets their pages back and hands them out in the same order. A
+    page that two sequences share must not be returned twice: it is not counted here."""
+    p, at, sizes, device = _pages_of(pool, block_table, lengths, page_size, "trim")
+    keep = _numbers(keep, "trim: keep", sizes[0], device)
+    err = _native.error_buffer()
+    with torch.cuda.device(device):
+        st = _native.lib().dmx_kv_trim(ct.byref(p), *at, keep.data_ptr(), *sizes, _stream(device), err, len(err))
+    _native.check(st, err, "dmx_kv_trim")
+
+
+# ----------------------------------------------------------- selected pages --
+
+
+def new_summaries(cache: dict) -> dict:
+    """Summaries for a cache's pages: `bounds` int8 [pages, H, 2, D] (of each channel
+    the largest and the smallest key) and `scales` uint8 [pages, H], the power of two
+    2^(scale - 127) that they count."""
+    pages, heads, _, words = cache["k_codes"].shape
+    device = cache["k_codes"].device
+    return {"bounds": torch.zeros((pages, heads, 2, 8 * words), dtype=torch.int8, device=device),
+            "scales": torch.zeros((pages, heads), dtype=torch.uint8, device=device)}
+
+
+def _summaries_of(summaries, c, cache, what):
+    s = _native.KvSummaries()
+    for name, dtype, shape in (("bounds", torch.int8, (c.pages, c.heads, 2, c.dim)), ("scales", torch.uint8, (c.pages, c.heads))):
+        t = summaries[name]
+        if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != cache["k_codes"].device:
+            raise ValueError(f"{what}: the summaries' {name} must be {dtype}, dense, {shape} beside the cache, got {t.dtype} "
+                             f"{tuple(t.shape)} on {t.device}")
+        setattr(s, name, t.data_ptr())
+    return s
+
+
+def _few_columns(block_table, what):
+    if block_table.shape[1] > _native.KV_MAX_COLUMNS:
+        raise ValueError(f"{what}: a block_table of {block_table.shape[1]} columns, more than {_native.KV_MAX_COLUMNS} "
+                         "(larger pages take fewer)")
+
+
+def _blocks_of(blocks, total, heads, block_table, device):
+    if blocks.dtype != torch.int32 or blocks.dim() != 3 or blocks.shape[:2] != (total, heads) or blocks.device != device:
+        raise ValueError(f"attention: blocks must be int32 [{total}, {heads}, n] on {device}, got {blocks.dtype} "
+                         f"{tuple(blocks.shape)} on {blocks.device}")
+    if not 1 <= blocks.shape[2] <= _native.KV_MAX_COLUMNS:
+        raise ValueError(f"attention: blocks of {blocks.shape[2]} columns (1..{_native.KV_MAX_COLUMNS})")
+    _few_columns(block_table, "attention: blocks of")
+    return blocks.contiguous()
+
+
+def summarize(cache: dict, summaries: dict, block_table: torch.Tensor, lengths: torch.Tensor, total: int, *, cu=None) -> None:
+    """The summaries, in place, of the pages that the last tokens of each sequence
+    lie in (`total` / B of each, or cu's, as read takes them), from every token
+    that their sequence has there: after append, and before select."""
+    c = _cache_of(cache, "summarize")
+    device = cache["k_codes"].device
+    x = _summaries_of(summaries, c, cache, "summarize")
+    s, held = _seqs_of(block_table, lengths, cu, int(total), None, device, "summarize")
+    err = _native.error_buffer()
+    with torch.cuda.device(device):
+        st = _native.lib().dmx_kv_summarize(ct.byref(c), ct.byref(x), ct.byref(s), _stream(device), err, len(err))
+    _native.check(st, err, "dmx_kv_summarize")
+
+
+def select(q: torch.Tensor, cache: dict, summaries: dict, block_table: torch.Tensor, lengths: torch.Tensor, count: int, *,
+           cu=None, first: int = 1, last: int = 1, causal: bool = True) -> torch.Tensor:
+    """The `count` columns of the block table that score highest for each new token's
+    queries q [T, Hq, D] (rotated) and cache head: int32 [T, H, count], ascending,
+    -1 behind the last, as attention takes them as `blocks`. Of the columns with a position that the
+    token sees, the first `first` and the last `last` are always among them. A score bounds
+    the products of the query heads that share the cache head with every key of the
+    page: with the summaries' largest keys for channels where q > 0, their smallest
+    where q < 0, and q in 8 bits. Sums are whole numbers, so that the choice does not depend on
+    how they are added; ties go to the lower column."""
+    _no_gradient("select", q)
+    c = _cache_of(cache, "select")
+    x = _summaries_of(summaries, c, cache, "select")
+    q = _activation(q, "select: q", dim=c.dim)
+    if q.device != cache["k_codes"].device:
+        raise ValueError("select: q is not on the cache's device")
+    T, Hq = q.shape[:2]
+    if Hq == 0 or Hq % c.heads:
+        raise ValueError(f"select: {Hq} query heads over {c.heads} cached ones")
+    if not 1 <= count <= _native.KV_MAX_COLUMNS or first < 0 or last < 0 or first + last > count:
+        raise ValueError(f"select: {count} columns, the first {first} and the last {last} of them (1..{_native.KV_MAX_COLUMNS}, "
+                         "and no more than there are)")
+    s, held = _seqs_of(block_table, lengths, cu, T, None, q.device, "select")
+    _few_columns(block_table, "select")
+    blocks = torch.empty((T, c.heads, count), dtype=torch.int32, device=q.device)
+    err = _native.error_buffer()
+    with torch.cuda.device(q.device):
+        st = _native.lib().dmx_kv_select(ct.byref(c), ct.byref(x), ct.byref(s), ct.byref(_rows(q)), _dtype_code(q.dtype, "select"),
+                                         count, first, last, causal, blocks.data_ptr(), _stream(q.device), err, len(err))
+    _native.check(st, err, "dmx_kv_select")
+    return blocks

@@ -1,7 +1,8 @@
 /*
  * dmx_kv.h — the C ABI of the operators between a decoder's q/k/v and o
  * projections, in libdmx_radix.so: rotary positions, the append to a paged
- * key/value cache held in 4 bits, its read and the attention over it. No
+ * key/value cache held in 4 bits, its read and the attention over it, over all
+ * of a sequence or over pages that a score selects; and the pages' handing out. No
  * drinkme counterpart: drinkme leaves these to the model's own code.
  *
  * Conventions are dmx_radix.h's: int status (0, or 1 with a message in
@@ -133,6 +134,96 @@ uint64_t dmx_kv_attention_workspace(const dmx_kv_cache* cache, const dmx_kv_seqs
 int dmx_kv_attention(const dmx_kv_cache* cache, const dmx_kv_seqs* seqs, const dmx_rows* q, int dtype, float scale,
                      int causal, uint32_t window, uint32_t max_length, void* out, float* lse, void* workspace,
                      uint64_t workspace_bytes, void* stream, char* err, size_t errn);
+
+/* ---- positions of several axes ---- */
+
+/* Which axis of the positions turns each angle: two bits an angle, 16 angles a
+ * word, the first lowest. */
+typedef struct dmx_rotary_axes {
+    uint32_t count;    /* axes, 1..4 */
+    uint32_t of[16];   /* of angles 0 .. table->dim / 2 - 1, 256 at most */
+} dmx_rotary_axes;
+
+/* As dmx_rotary, with positions [count, tokens]: angle i of token t is turned by
+ * the table's row positions[axis of i, t]. */
+int dmx_rotary_by_axes(const dmx_rows* in, const dmx_rows* out, uint32_t n, uint32_t tokens, uint32_t dim, int dtype,
+                       const void* positions, int wide, const dmx_rotary_axes* axes, const dmx_rotary_table* table,
+                       void* stream, char* err, size_t errn);
+
+/* ---- pages ---- */
+
+/* The pages that no sequence has, as a stack: free[0 .. count - 1]. */
+typedef struct dmx_kv_pool {
+    int32_t* free;   /* [pages] */
+    int32_t* count;  /* [1] */
+    int32_t* lacking; /* [1]: pages that the last dmx_kv_reserve had not */
+    uint32_t pages;  /* of the cache, fewer than 2^30 */
+} dmx_kv_pool;
+
+/* Room for each sequence's new tokens, and where they lie. table [batch,
+ * table_cols] and lengths [batch] are updated in place; added [batch] (or NULL:
+ * total / batch each) are the new tokens, negative ones 0; where their sum passes
+ * `total` the sequences that pass it get what is left. In order of the sequences, and of a
+ * sequence's columns, each column between the last one that holds a token and
+ * the new end gets the page on top of the stack; -1 from where it is empty. Then cu
+ * [batch + 1] holds the offsets of the new tokens, and positions and slots
+ * [total] where each lies: its position (-1 behind the last), and page * page_size
+ * + position % page_size, -1 where it has no page of the cache. lengths count
+ * the tokens without one, too (2^30 at most, before the new ones). */
+int dmx_kv_reserve(const dmx_kv_pool* pool, int32_t* table, int32_t* lengths, const int32_t* added, uint32_t batch,
+                   uint32_t table_cols, uint32_t page, uint32_t total, int32_t* cu, int32_t* positions, int64_t* slots,
+                   void* stream, char* err, size_t errn);
+
+/* Sequences cut to their first keep [batch] tokens (none where negative, all
+ * where there are not that many): lengths become that, columns past it -1, and
+ * their pages go back so that dmx_kv_reserve gives them out in the order they
+ * had. Numbers that are no page's are dropped, and so is what a full stack does
+ * not hold. */
+int dmx_kv_trim(const dmx_kv_pool* pool, int32_t* table, int32_t* lengths, const int32_t* keep, uint32_t batch,
+                uint32_t table_cols, uint32_t page, void* stream, char* err, size_t errn);
+
+/* ---- attention over selected pages ---- */
+
+/* Of each page and head: of every channel the largest and the smallest key of
+ * its tokens (NaNs apart; 0 where there is no other), in whole numbers of
+ * 2^(scale - 127), the largest rounded up and the smallest down. scale - 127 is the
+ * least exponent, -126 or more, that leaves no number over 127. */
+typedef struct dmx_kv_summaries {
+    int8_t* bounds;   /* [pages, heads, 2, dim], 16-byte aligned: largest, smallest */
+    uint8_t* scales;  /* [pages, heads] */
+} dmx_kv_summaries;
+
+/* The summaries of the pages that the new tokens lie in, from all of their
+ * sequence's tokens there. */
+int dmx_kv_summarize(const dmx_kv_cache* cache, const dmx_kv_summaries* summaries, const dmx_kv_seqs* seqs, void* stream,
+                     char* err, size_t errn);
+
+/* The columns of the block table that score highest for each new token and
+ * cache head: blocks [total, heads, count], ascending, -1 behind the last. Of the
+ * columns that hold a position which the token sees (causal: up to its own) the
+ * first `first` and the last `last` are among them (first + last at most
+ * count); the others by their score, ties to the lower column, columns without a
+ * page of the cache last. A score is 2^(scale - 127) times the largest sum, of
+ * the query heads that share the cache head, over channels of x * (x > 0 ?
+ * largest : smallest): x the query in whole numbers (to the nearest, even) of the least power
+ * of two, 2^-126 or more, that leaves none of these heads' over 127; values that are not finite
+ * are 0. Sums are below 2^24 and compared as fp32. Tokens of no sequence list nothing. A block
+ * table has at most DMX_KV_MAX_COLUMNS columns here. */
+#define DMX_KV_MAX_COLUMNS 16384
+int dmx_kv_select(const dmx_kv_cache* cache, const dmx_kv_summaries* summaries, const dmx_kv_seqs* seqs,
+                  const dmx_rows* q, int dtype, uint32_t count, uint32_t first, uint32_t last, int causal,
+                  int32_t* blocks, void* stream, char* err, size_t errn);
+
+/* As dmx_kv_attention without a window, over the listed columns alone: a query
+ * of token t and cache head h sees of the positions that it would see there those in
+ * columns blocks[t, h, 0 .. count - 1]. Their order does not matter, a column
+ * listed twice counts once, and one that is negative or past the token's position is
+ * nothing; one that the table has no page for gives NaN. */
+uint64_t dmx_kv_attention_blocks_workspace(const dmx_kv_cache* cache, const dmx_kv_seqs* seqs, uint32_t q_heads,
+                                           int dtype, uint32_t count, uint32_t max_length);
+int dmx_kv_attention_blocks(const dmx_kv_cache* cache, const dmx_kv_seqs* seqs, const dmx_rows* q, int dtype, float scale,
+                            int causal, const int32_t* blocks, uint32_t count, uint32_t max_length, void* out, float* lse,
+                            void* workspace, uint64_t workspace_bytes, void* stream, char* err, size_t errn);
 
 #ifdef __cplusplus
 }
