@@ -103,13 +103,13 @@ __global__ __launch_bounds__(256) void k_summarize(const Summarize a) {
 //
 // The score of a page is a product of two vectors of 2 D whole numbers of 8
 // bits: the query's positive and negative parts against the page's largest and
-// smallest keys. On v_mfma_i32_16x16x64_i8 16 pages meet up to 16 query heads, in
+// smallest keys. On v_mfma_i32_16x16x64_i8 16 pages meet 16 query rows, in
 // whole numbers, which no order of summation changes: ties are ties, and go
 // to the lower column whatever computes them.
 //
 // The best `count` keys (a score's bits, ordered as numbers) are those from a
-// threshold on, found three of its bits at a time by counting: the largest one that
-// `count` keys reach.
+// threshold on, found bit by bit from the top by counting: the largest that `count`
+// keys reach.
 
 struct Select {
     Cache cache;  // (page numbers and sizes alone)
@@ -120,13 +120,14 @@ struct Select {
     int64_t q_token, q_head;  // strides, elements
     uint32_t group, count, first, last, causal;
     int32_t* blocks;
+    uint32_t tokens, slots, stride;  // k_select_tokens: tokens a workgroup, rows a token, keys a token
 };
 
-__device__ __forceinline__ int max_over_16(int x) {
-    x = max(x, __builtin_amdgcn_mov_dpp(x, 0x128, 0xF, 0xF, true));  // a row of 16 lanes, turned by 8, 4, 2, 1
-    x = max(x, __builtin_amdgcn_mov_dpp(x, 0x124, 0xF, 0xF, true));
-    x = max(x, __builtin_amdgcn_mov_dpp(x, 0x122, 0xF, 0xF, true));
-    return max(x, __builtin_amdgcn_mov_dpp(x, 0x121, 0xF, 0xF, true));
+constexpr uint32_t kForced = 0xffffffffu, kLost = 1;  // keys above and below every score's; 0: no column
+
+__device__ __forceinline__ uint32_t key_of(int score, int scale) {
+    const uint32_t bits = __float_as_uint(__builtin_ldexpf((float)score, scale - 127));
+    return bits ^ (bits >> 31 ? 0xffffffffu : 0x80000000u);
 }
 
 // Sixteen adjacent channels as fp32, 0 for what is no number.
@@ -147,20 +148,174 @@ __device__ __forceinline__ void load16(const void* base, int64_t at, float (&x)[
     for (int n = 0; n < 16; ++n) x[n] = (__float_as_uint(x[n]) & 0x7fffffffu) >= 0x7f800000u ? 0.f : x[n];
 }
 
-// WAVES: of a token and head. One: four of them to a workgroup, 512 columns at most.
-template <bool F32, int D, int WAVES>
-__global__ __launch_bounds__(64 * (WAVES == 1 ? 4 : WAVES)) void k_select(const Select a) {
-    constexpr int chunks = D / 32, R = WAVES == 1 ? 8 : 16, kRounds = 11;
-    extern __shared__ __align__(16) uint32_t lds[];
+// Piece c of lane (i, j)'s share of a row: 16 channels, of the positive side's D / 16
+// pieces and then of the negative one's.
+template <int D>
+struct Piece {
+    bool negative;
+    int channel;
+    __device__ __forceinline__ Piece(int c, int j) : negative(4 * c + j >= D / 16), channel(16 * (4 * c + j - (negative ? D / 16 : 0))) {}
+};
+
+__device__ __forceinline__ uint32_t largest(const float (&x)[16], uint32_t top) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+    return top;
+}
+
+// The factor of whole numbers: 255 / 128 of a power of two and above round to 128 of
+// its 64th, and take its 32nd.
+__device__ __forceinline__ float factor_of(uint32_t top) {
+    return __uint_as_float((uint32_t)(127 - max((int)((top + 0x10000u) >> 23) - 133, -126)) << 23);
+}
+
+__device__ __forceinline__ i32x4 whole(const float (&x)[16], float factor, bool negative) {
+    i32x4 out;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        uint32_t word = 0;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+            const int v = (int)rintf(x[4 * w + y] * factor);
+            word |= (uint32_t)((negative ? min(v, 0) : max(v, 0)) & 255) << (8 * y);
+        }
+        out[w] = (int)word;
+    }
+    return out;
+}
+
+// What a lane reads of a tile of 16 pages: page i's pieces, and its scale.
+template <int D>
+struct PageTile {
+    i32x4 bounds[D / 32];
+    int scale;
+    bool ok;
+};
+template <int D>
+__device__ __forceinline__ void load_tile(const Select& a, uint32_t h, uint32_t page, int j, PageTile<D>& x) {
+    x.ok = page < a.cache.pages;
+    const uint64_t at = (uint64_t)(x.ok ? page : 0u) * a.cache.heads + h;
+    const i32x4* from = reinterpret_cast<const i32x4*>(a.bounds + at * (2 * D) + 16 * j);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) x.bounds[c] = from[4 * c];
+    x.scale = a.scales[at];
+}
+
+// A wave's choice: the count largest of keys [0, n) in LDS (more than count of them, 64 R
+// at most), ties to the first, their indexes to `out` in ascending order.
+template <int R>
+__device__ __forceinline__ void choose(const uint32_t* keys, int n, int count, int lane, int32_t* out) {
+    uint32_t key[R];
+#pragma unroll
+    for (int x = 0; x < R; ++x) key[x] = 64 * x + lane < n ? keys[64 * x + lane] : 0;
+    uint32_t at_least = 0;
+    for (uint32_t bit = 1u << 31; bit; bit >>= 1) {
+        const uint32_t to = at_least | bit;
+        int have = 0;
+#pragma unroll
+        for (int x = 0; x < R; ++x) have += __popcll(__ballot(key[x] >= to));
+        if (have >= count) at_least = to;
+        if (have == count) break;
+    }
+    int above = 0;
+#pragma unroll
+    for (int x = 0; x < R; ++x) above += __popcll(__ballot(key[x] > at_least));
+    const int fill = count - above;  // (of those at the threshold)
+    int over = 0, level = 0;
+#pragma unroll
+    for (int x = 0; x < R; ++x) {
+        const bool up = key[x] > at_least, even = key[x] == at_least;
+        const uint64_t u = __ballot(up), v = __ballot(even);
+        const int o = over + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(u >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)u, 0));
+        const int l = level + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(v >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)v, 0));
+        if (up || (even && l < fill)) out[o + min(l, fill)] = 64 * x + lane;
+        over += __popcll(u);
+        level += __popcll(v);
+    }
+}
+
+// As choose, by a workgroup of WAVES waves, a run of keys each, three bits of the
+// threshold at a time.
+template <int WAVES>
+__device__ __forceinline__ void choose_together(const uint32_t* keys, int n, int count, int32_t* out) {
+    constexpr int kRounds = 11;
     __shared__ int counts[kRounds][8];
     __shared__ int before[2][WAVES];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int c = threadIdx.x; c < kRounds * 8; c += 64 * WAVES) (&counts[0][0])[c] = 0;
+    __syncthreads();
+    const int rows = (n + 64 * WAVES - 1) / (64 * WAVES), c0 = wave * rows * 64 + lane;
+    const auto key_at = [&](int x) { return c0 + 64 * x < n ? keys[c0 + 64 * x] : 0u; };
+    uint32_t at_least = 0;
+    for (int round = 0; round < kRounds; ++round) {
+        const int shift = 30 - 3 * round;
+        int have[8] = {};  // how many reach at_least + k << shift
+        for (int x = 0; x < rows; ++x) {
+            const uint32_t key = key_at(x);
+#pragma unroll
+            for (int k = 1; k < 8; ++k) {
+                const uint32_t to = at_least + ((uint32_t)(round ? k : min(k, 3)) << shift);
+                have[k] += __popcll(__ballot(key >= to));
+            }
+        }
+        int mine = 0;
+#pragma unroll
+        for (int k = 1; k < 8; ++k)
+            if (lane == k && (round || k < 4)) mine = have[k];
+        if (mine) atomicAdd(&counts[round][lane], mine);
+        __syncthreads();
+        int k = 0, reach = 0;
+#pragma unroll
+        for (int y = 1; y < 8; ++y)
+            if (counts[round][y] >= count) k = y, reach = counts[round][y];
+        at_least += (uint32_t)k << shift;
+        if (reach == count) break;
+    }
+    int above = 0, equal = 0;
+    for (int x = 0; x < rows; ++x) {
+        const uint32_t key = key_at(x);
+        above += __popcll(__ballot(key > at_least));
+        equal += __popcll(__ballot(key == at_least));
+    }
+    if (lane == 0) before[0][wave] = above, before[1][wave] = equal;
+    __syncthreads();
+    int fill = count, over = 0, level = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        fill -= before[0][w];
+        over += w < wave ? before[0][w] : 0;
+        level += w < wave ? before[1][w] : 0;
+    }
+    for (int x = 0; x < rows; ++x) {
+        const uint32_t key = key_at(x);
+        const bool up = key > at_least, even = key == at_least;
+        const uint64_t u = __ballot(up), v = __ballot(even);
+        const int o = over + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(u >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)u, 0));
+        const int l = level + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(v >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)v, 0));
+        if (up || (even && l < fill)) out[o + min(l, fill)] = c0 + 64 * x;
+        over += __popcll(u);
+        level += __popcll(v);
+    }
+}
+
+// The largest over the first `slots` of a row of 16 lanes' neighbours, a power of two: in every lane of them.
+__device__ __forceinline__ int max_over_slots(int x, uint32_t slots) {
+    if (slots > 1) x = max(x, __builtin_amdgcn_mov_dpp(x, 0xB1, 0xF, 0xF, true));   // lane ^ 1
+    if (slots > 2) x = max(x, __builtin_amdgcn_mov_dpp(x, 0x4E, 0xF, 0xF, true));   // lane ^ 2
+    if (slots > 4) x = max(x, __builtin_amdgcn_mov_dpp(x, 0x141, 0xF, 0xF, true));  // the other four of eight
+    if (slots > 8) x = max(x, __builtin_amdgcn_mov_dpp(x, 0x140, 0xF, 0xF, true));  // the other eight
+    return x;
+}
+
+// Single tokens: a workgroup to a token and head. A wave takes tiles of 16 pages, the next
+// one's loads ahead of this one's product.
+template <bool F32, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void k_select(const Select a) {
+    constexpr int chunks = D / 32;
+    extern __shared__ __align__(16) uint32_t keys[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, j = lane >> 4;
-    const int team = WAVES == 1 ? wave : 0, member = WAVES == 1 ? 0 : wave;
-    const uint32_t heads = a.cache.heads, row = blockIdx.x * (WAVES == 1 ? 4 : 1) + team;
-    if (row >= a.seqs.total * heads) return;
-    const uint32_t t = row / heads, h = row - t * heads;
-    uint32_t* keys = lds + team * a.seqs.cols;
-    int32_t* out = a.blocks + (int64_t)row * a.count;
+    const uint32_t heads = a.cache.heads, t = blockIdx.x / heads, h = blockIdx.x - t * heads;
+    int32_t* out = a.blocks + (int64_t)blockIdx.x * a.count;
 
     const uint32_t b = seq_at(a.seqs, t);
     const Seq q = seq_of(a.seqs, b);
@@ -168,158 +323,179 @@ __global__ __launch_bounds__(64 * (WAVES == 1 ? 4 : WAVES)) void k_select(const 
     const bool inside = (uint32_t)m < (uint32_t)q.count && q.first + m >= 0;
     const int n = inside ? min((p >> a.cache.page_shift) + 1, a.seqs.cols) : 0, count = a.count;
     if (n <= count) {
-        for (int c = threadIdx.x - 64 * team; c < count; c += 64 * WAVES) out[c] = c < n ? c : -1;
+        for (int c = threadIdx.x; c < count; c += 64 * WAVES) out[c] = c < n ? c : -1;
         return;
     }
-    if constexpr (WAVES > 1)
-        for (int c = threadIdx.x; c < kRounds * 8; c += 64 * WAVES) (&counts[0][0])[c] = 0;
-
-    // piece c of a lane: 16 channels, of the positive side's D / 16 pieces and then of the negative one's
-    const auto side_of = [&](int c) { return 4 * c + j >= D / 16; };
-    const auto channel = [&](int c) { return 16 * (4 * c + j - (side_of(c) ? D / 16 : 0)); };
+    const int tiles = (n + 15) / 16;
+    const auto page_at = [&](int tile) { return (uint32_t)a.seqs.table[(int64_t)b * a.seqs.cols + min(16 * tile + i, n - 1)]; };
     const auto load = [&](int r, int c, float (&x)[16]) {  // of query head r of the group
-        load16<F32>(a.q, t * a.q_token + ((int64_t)h * a.group + r) * a.q_head + channel(c), x);
+        load16<F32>(a.q, t * a.q_token + ((int64_t)h * a.group + r) * a.q_head + Piece<D>(c, j).channel, x);
     };
-    uint32_t top = 0;
-    for (uint32_t r = i; r < a.group; r += 16)
-#pragma unroll
-        for (int c = 0; c < chunks; ++c) {
-            float x[16];
-            load(r, c, x);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-        }
-#pragma unroll
-    for (int s = 32; s; s >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, s));
-    // 255 / 128 of a power of two and above round to 128 of its 64th: of its 32nd
-    const int e = max((int)((top + 0x10000u) >> 23) - 133, -126);
-    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-
     for (uint32_t r0 = 0; r0 < a.group; r0 += 16) {
+        PageTile<D> x[2];
+        uint32_t page = page_at(min(wave, tiles - 1));
+        uint32_t top = 0;
+        for (uint32_t r = i; r < a.group; r += 16)
+#pragma unroll
+            for (int c = 0; c < chunks; ++c) {
+                float y[16];
+                load(r, c, y);
+                top = largest(y, top);
+            }
+        load_tile(a, h, page, j, x[0]);
+        page = page_at(min(wave + WAVES, tiles - 1));
+#pragma unroll
+        for (int s = 32; s; s >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, s));
+        const float factor = factor_of(top);
         const uint32_t r = r0 + i;
         i32x4 qf[chunks];
 #pragma unroll
         for (int c = 0; c < chunks; ++c) {
-            float x[16] = {};
-            if (r < a.group) load(r, c, x);
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                uint32_t word = 0;
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const int v = (int)rintf(x[4 * w + y] * inv);
-                    word |= (uint32_t)((side_of(c) ? min(v, 0) : max(v, 0)) & 255) << (8 * y);
-                }
-                qf[c][w] = (int)word;
-            }
+            float y[16] = {};
+            if (r < a.group) load(r, c, y);
+            qf[c] = whole(y, factor, Piece<D>(c, j).negative);
         }
-        const auto page_at = [&](int tile) { return (uint32_t)a.seqs.table[(int64_t)b * a.seqs.cols + min(16 * tile + i, n - 1)]; };
-        const int tiles = (n + 15) / 16;
-        uint32_t next = member < tiles ? page_at(member) : 0;
-        for (int tile = member; tile < tiles; tile += WAVES) {
-            const uint32_t page = next;
-            if (tile + WAVES < tiles) next = page_at(tile + WAVES);
-            const bool ok = page < a.cache.pages;
-            const uint64_t at = (uint64_t)(ok ? page : 0u) * heads + h;
-            const i32x4* from = reinterpret_cast<const i32x4*>(a.bounds + at * (2 * D) + 16 * j);
-            const int scale = a.scales[at];
+        const auto work = [&](int tile, const PageTile<D>& y) {
             i32x4 s = {0, 0, 0, 0};
 #pragma unroll
-            for (int c = 0; c < chunks; ++c) s = __builtin_amdgcn_mfma_i32_16x16x64_i8(from[4 * c], qf[c], s, 0, 0, 0);
-            int best = 0;  // of page i, in the lanes of its row of results
+            for (int c = 0; c < chunks; ++c) s = __builtin_amdgcn_mfma_i32_16x16x64_i8(y.bounds[c], qf[c], s, 0, 0, 0);
+            int best = 0;  // of page 4 j + (i & 3), over the lanes of a row of results
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-                const int v = max_over_16(r < a.group ? s[y] : -(1 << 30));
-                if ((i & 3) == y) best = v;
+            for (int e = 0; e < 4; ++e) {
+                const int v = max_over_slots(r < a.group ? s[e] : -(1 << 30), 16);
+                if ((i & 3) == e) best = v;
             }
             const int c = 16 * tile + i;
             if (i >> 2 == j && c < n) {
-                const uint32_t bits = __float_as_uint(__builtin_ldexpf((float)best, scale - 127));
-                uint32_t key = bits ^ (bits >> 31 ? 0xffffffffu : 0x80000000u);
-                if (!ok) key = 1;  // below every number
-                if (c < (int)a.first || c >= n - (int)a.last) key = 0xffffffffu;
+                uint32_t key = y.ok ? key_of(best, y.scale) : kLost;
+                if (c < (int)a.first || c >= n - (int)a.last) key = kForced;
                 keys[c] = r0 ? max(keys[c], key) : key;
             }
+        };
+        for (int tile = wave; tile < tiles; tile += 2 * WAVES) {
+            load_tile(a, h, page, j, x[1]);  // (past the last tile: the last page again)
+            page = page_at(min(tile + 2 * WAVES, tiles - 1));
+            work(tile, x[0]);
+            if (tile + WAVES >= tiles) break;
+            load_tile(a, h, page, j, x[0]);
+            page = page_at(min(tile + 3 * WAVES, tiles - 1));
+            work(tile + WAVES, x[1]);
         }
     }
-    if constexpr (WAVES > 1)
-        __syncthreads();
-    else
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __syncthreads();
+    if (n > 1024) {
+        choose_together<WAVES>(keys, n, count, out);
+    } else if (wave == 0) {
+        n <= 128   ? choose<2>(keys, n, count, lane, out)
+        : n <= 256 ? choose<4>(keys, n, count, lane, out)
+        : n <= 512 ? choose<8>(keys, n, count, lane, out)
+                   : choose<16>(keys, n, count, lane, out);
+    }
+}
 
-    // a wave's keys: `rows` times 64 columns in a row
-    const int rows = (n + 64 * WAVES - 1) / (64 * WAVES), c0 = member * rows * 64 + lane;
-    uint32_t key[R];
+// Prompts: a workgroup of four waves to a head and up to 16 tokens in a row, which share
+// the reading of their sequence's summaries: 64 query rows (`slots` to a token, a power of two) meet a
+// tile of pages. Then each wave chooses for a quarter of the tokens.
+template <bool F32, int D>
+__global__ __launch_bounds__(256, 2) void k_select_tokens(const Select a) {
+    constexpr int chunks = D / 32;
+    extern __shared__ __align__(16) uint32_t keys[];  // [tokens][stride]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, j = lane >> 4;
+    const uint32_t heads = a.cache.heads, h = blockIdx.x, slot = i & (a.slots - 1), per = 16 / a.slots;  // tokens a tile of rows
+    const int shift = a.cache.page_shift, count = a.count, row_tiles = (int)((a.tokens * a.slots + 15) / 16);
+    const int t_end = (int)min(blockIdx.y * a.tokens + a.tokens, a.seqs.total);
+    int t0 = (int)(blockIdx.y * a.tokens);
+    while (t0 < t_end) {  // (a turn for each sequence)
+        const uint32_t b = seq_at(a.seqs, t0);
+        const Seq q = seq_of(a.seqs, b);
+        const bool inside = (uint32_t)(t0 - q.token) < (uint32_t)q.count;
+        const int t1 = inside ? min(t_end, q.token + q.count) : t0 + 1, first = t0;
+        t0 = t1;
+        const auto columns_of = [&](int t) {  // that token t sees
+            const int at = q.first + (t - q.token), p = a.causal ? at : q.length - 1;
+            return inside && at >= 0 ? min((p >> shift) + 1, a.seqs.cols) : 0;
+        };
+        const int most = columns_of(t1 - 1);
+        if (most > count) {
+            i32x4 qf[4][chunks];
 #pragma unroll
-    for (int x = 0; x < R; ++x) key[x] = x < rows && c0 + 64 * x < n ? keys[c0 + 64 * x] : 0;
-    uint32_t at_least = 0;
-    if constexpr (WAVES == 1) {
-        for (uint32_t bit = 1u << 31; bit; bit >>= 1) {
-            const uint32_t to = at_least | bit;
-            int have = 0;
+            for (int x = 0; x < 4; ++x) {
+                const uint32_t token = first + x * per + i / a.slots;
+                const bool mine = x < row_tiles && (int)token < t1 && slot < a.group;
+                float y[chunks][16] = {};
+                uint32_t top = 0;
+                if (mine)
 #pragma unroll
-            for (int x = 0; x < R; ++x)
-                if (x < rows) have += __popcll(__ballot(key[x] >= to));
-            if (have >= count) at_least = to;
-            if (have == count) break;
-        }
-    } else {
-        for (int round = 0; round < kRounds; ++round) {
-            const int shift = 30 - 3 * round;
-            int mine = 0;  // lane k: how many reach at_least + k << shift
+                    for (int c = 0; c < chunks; ++c) {
+                        load16<F32>(a.q, token * a.q_token + ((int64_t)h * a.group + slot) * a.q_head + Piece<D>(c, j).channel, y[c]);
+                        top = largest(y[c], top);
+                    }
+                top = (uint32_t)max_over_slots((int)top, a.slots);
+                top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+                top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+                const float factor = factor_of(top);
 #pragma unroll
-            for (int k = 1; k < 8; ++k) {
-                if (round == 0 && k > 3) break;
-                const uint32_t to = at_least + ((uint32_t)k << shift);
-                int have = 0;
-#pragma unroll
-                for (int x = 0; x < R; ++x)
-                    if (x < rows) have += __popcll(__ballot(key[x] >= to));
-                if (lane == k) mine = have;
+                for (int c = 0; c < chunks; ++c) qf[x][c] = whole(y[c], factor, Piece<D>(c, j).negative);
             }
-            if (mine) atomicAdd(&counts[round][lane], mine);
+            const int tiles = (most + 15) / 16;
+            const auto page_at = [&](int tile) { return (uint32_t)a.seqs.table[(int64_t)b * a.seqs.cols + min(16 * tile + i, most - 1)]; };
+            const auto work = [&](int tile, const PageTile<D>& y) {
+                // of the four pages whose results this lane holds
+                int scale[4];
+                const int packed = y.ok ? y.scale : -1;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) scale[e] = __shfl(packed, 4 * j + e);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    if (x >= row_tiles) break;
+                    i32x4 s = {0, 0, 0, 0};
+#pragma unroll
+                    for (int c = 0; c < chunks; ++c) s = __builtin_amdgcn_mfma_i32_16x16x64_i8(y.bounds[c], qf[x][c], s, 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[e] = max_over_slots(slot < a.group ? s[e] : -(1 << 30), a.slots);
+                    const int token = x * per + i / a.slots;
+                    if (slot || first + token >= t1) continue;
+                    const int n = columns_of(first + token), c = 16 * tile + 4 * j;
+                    uint4 key;
+                    uint32_t* k = &key.x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        k[e] = scale[e] < 0 ? kLost : key_of(s[e], scale[e]);
+                        if (c + e < (int)a.first || c + e >= n - (int)a.last) k[e] = kForced;
+                    }
+                    *reinterpret_cast<uint4*>(keys + token * a.stride + c) = key;  // (past n: not read)
+                }
+            };
+            PageTile<D> x[2];
+            uint32_t page = page_at(min(wave, tiles - 1));
+            load_tile(a, h, page, j, x[0]);
+            page = page_at(min(wave + 4, tiles - 1));
+            for (int tile = wave; tile < tiles; tile += 8) {
+                load_tile(a, h, page, j, x[1]);
+                page = page_at(min(tile + 8, tiles - 1));
+                work(tile, x[0]);
+                if (tile + 4 >= tiles) break;
+                load_tile(a, h, page, j, x[0]);
+                page = page_at(min(tile + 12, tiles - 1));
+                work(tile + 4, x[1]);
+            }
             __syncthreads();
-            int k = 0, reach = 0;
-#pragma unroll
-            for (int y = 1; y < 8; ++y) {
-                const int have = counts[round][y];
-                if (have >= count) k = y, reach = have;
+        }
+        for (int t = first + wave; t < t1; t += 4) {
+            const int n = columns_of(t);
+            int32_t* out = a.blocks + ((int64_t)t * heads + h) * count;
+            const uint32_t* mine = keys + (t - first) * a.stride;
+            if (n <= count) {
+                for (int c = lane; c < count; c += 64) out[c] = c < n ? c : -1;
+            } else {
+                n <= 128    ? choose<2>(mine, n, count, lane, out)
+                : n <= 256  ? choose<4>(mine, n, count, lane, out)
+                : n <= 512  ? choose<8>(mine, n, count, lane, out)
+                : n <= 1024 ? choose<16>(mine, n, count, lane, out)
+                            : choose<64>(mine, n, count, lane, out);
             }
-            at_least += (uint32_t)k << shift;
-            if (reach == count) break;
         }
-    }
-
-    // those above the threshold, and of those at it the first ones
-    int above = 0, equal = 0;
-#pragma unroll
-    for (int x = 0; x < R; ++x)
-        if (x < rows) {
-            above += __popcll(__ballot(key[x] > at_least));
-            equal += __popcll(__ballot(key[x] == at_least && key[x]));
-        }
-    int all_above = above, over = 0, level = 0;
-    if constexpr (WAVES > 1) {
-        if (lane == 0) before[0][wave] = above, before[1][wave] = equal;
-        __syncthreads();
-        all_above = 0;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            all_above += before[0][w];
-            over += w < wave ? before[0][w] : 0;
-            level += w < wave ? before[1][w] : 0;
-        }
-    }
-    const int fill = count - all_above;
-#pragma unroll
-    for (int x = 0; x < R; ++x) {
-        const bool up = key[x] > at_least, even = key[x] == at_least && key[x];
-        const uint64_t u = __ballot(up), v = __ballot(even);
-        const int o = over + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(u >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)u, 0));
-        const int l = level + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(v >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)v, 0));
-        if (up || (even && l < fill)) out[o + min(l, fill)] = c0 + 64 * x;
-        over += __popcll(u);
-        level += __popcll(v);
+        if (most > count) __syncthreads();
     }
 }
 
@@ -331,13 +507,29 @@ int check_summaries(const dmx_kv_summaries* s, char* err, size_t errn) {
     return 0;
 }
 
-template <bool F32, int D, int WAVES>
-int launch_select(const Select& a, uint32_t rows, hipStream_t stream, char* err, size_t errn) {
-    constexpr int teams = WAVES == 1 ? 4 : 1;
-    static std::atomic<uint64_t> allowed = {};
-    const auto kern = k_select<F32, D, WAVES>;
-    if (allow_lds(reinterpret_cast<const void*>(kern), 4 * DMX_KV_MAX_COLUMNS, allowed, err, errn)) return 1;
-    hipLaunchKernelGGL(kern, dim3((rows + teams - 1) / teams), dim3(64 * teams * WAVES), 4 * teams * a.seqs.cols, stream, a);
+constexpr uint32_t kTokenColumns = 4096;  // of k_select_tokens, at most: 64 keys a lane
+
+template <bool F32, int D>
+int launch_select(Select& a, uint32_t rows, hipStream_t stream, char* err, size_t errn) {
+    static std::atomic<uint64_t> allowed[3] = {};
+    const uint32_t cols = a.seqs.cols;
+    if (a.tokens) {
+        // (64 KB of keys: two workgroups a CU; a tile's last columns and a shift of the banks between tokens)
+        a.stride = (cols + 15) / 16 * 16 + 4;
+        while (a.tokens > 1 && a.tokens * a.stride * 4 > 66000) a.tokens /= 2;
+        if ((a.seqs.total + a.tokens - 1) / a.tokens > 65535) a.tokens = 0;
+    }
+    if (a.tokens) {
+        const auto kern = k_select_tokens<F32, D>;
+        if (allow_lds(reinterpret_cast<const void*>(kern), 16 * 1024 * 5, allowed[2], err, errn)) return 1;
+        hipLaunchKernelGGL(kern, dim3(a.cache.heads, (a.seqs.total + a.tokens - 1) / a.tokens), dim3(256), 4 * a.tokens * a.stride, stream, a);
+    } else {
+        constexpr int most = D <= 128 ? 16 : 8;  // (128 registers a lane are few for larger heads)
+        const bool many = cols > 1024;
+        const auto kern = many ? k_select<F32, D, most> : k_select<F32, D, 8>;
+        if (allow_lds(reinterpret_cast<const void*>(kern), 4 * DMX_KV_MAX_COLUMNS, allowed[many], err, errn)) return 1;
+        hipLaunchKernelGGL(kern, dim3(rows), dim3(many ? 64 * most : 512), 4 * cols, stream, a);
+    }
     return launch_check(err, errn, "kv select launch");
 }
 
@@ -386,17 +578,16 @@ extern "C" int dmx_kv_select(const dmx_kv_cache* cache, const dmx_kv_summaries* 
     a.group = q->heads / cache->heads;
     a.count = count, a.first = first, a.last = last, a.causal = causal != 0;
     a.blocks = blocks;
-    const uint32_t cols = seqs->table_cols;
-    const int waves = cols <= 512 && rows >= 2048 ? 1 : cols <= 512 || (cols <= 4096 && rows >= 512) ? 4 : 16;
+    a.slots = 1;
+    // Tokens of a prompt share their sequence's summaries where there are eight or more to a sequence, and
+    // keys and rows fit.
+    while (a.slots < a.group) a.slots *= 2;
+    if (seqs->total / seqs->batch >= 8 && seqs->table_cols <= kTokenColumns && a.slots <= 16) a.tokens = std::min(16u, 64 / a.slots);
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const auto by_waves = [&](auto f32, auto d) {
-        constexpr bool F32 = decltype(f32)::value;
+    const auto by_type = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        return waves == 1   ? launch_select<F32, D, 1>(a, (uint32_t)rows, st, err, errn)
-               : waves == 4 ? launch_select<F32, D, 4>(a, (uint32_t)rows, st, err, errn)
-                            : launch_select<F32, D, 16>(a, (uint32_t)rows, st, err, errn);
+        return dtype == DMX_F32 ? launch_select<true, D>(a, (uint32_t)rows, st, err, errn) : launch_select<false, D>(a, (uint32_t)rows, st, err, errn);
     };
-    const auto by_type = [&](auto d) { return dtype == DMX_F32 ? by_waves(std::true_type{}, d) : by_waves(std::false_type{}, d); };
     return cache->dim == 64    ? by_type(std::integral_constant<int, 64>{})
            : cache->dim == 96  ? by_type(std::integral_constant<int, 96>{})
            : cache->dim == 128 ? by_type(std::integral_constant<int, 128>{})

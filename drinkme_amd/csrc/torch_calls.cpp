@@ -1,6 +1,6 @@
-// The per-call path of the torch launchers (drinkme_amd/radix_ops.py) and of
-// the key/value cache's operators (drinkme_amd/kv_ops.py) as a CPython
-// extension: one call checks the activation, allocates the output
+// The per-call path of the torch launchers (drinkme_amd/radix_ops.py), of the
+// key/value cache's operators (drinkme_amd/kv_ops.py) and of the norms
+// (drinkme_amd/norm_ops.py) as a CPython extension: one call checks the activation, allocates the output
 // with torch and launches through the C ABI. What bounds a decode step's
 // small calls is the host: through ctypes and Python's own checks a call of
 // one Linear took 10.1 us on the host for a 5.5 us kernel (k_proj of 1024 x
@@ -27,6 +27,7 @@
 #include <string>
 
 #include "dmx_kv.h"
+#include "dmx_norm.h"
 #include "dmx_radix.h"
 
 namespace {
@@ -234,15 +235,21 @@ const at::Tensor* dense(PyObject* o, at::ScalarType dtype, int64_t dims, int64_t
     return t && plain(*t) && t->scalar_type() == dtype && t->dim() == dims && t->get_device() == index ? t : nullptr;
 }
 
+// Whether x is a strided tensor of the GPU that no torch wrapper stands in front of, of rows with
+// adjacent channels.
+bool strided(const at::Tensor* x) {
+    using K = c10::DispatchKey;
+    return x && x->defined() && x->is_cuda() && x->layout() == at::kStrided && x->has_storage() && x->dim() > 0 &&
+           !x->key_set().has_any(c10::DispatchKeySet({K::FuncTorchBatched, K::FuncTorchGradWrapper, K::Functionalize,
+                                                      K::Python, K::Negative, K::Conjugate, K::ZeroTensor})) &&
+           code(x->scalar_type()) >= 0 && x->stride(-1) == 1;
+}
+
 // x [tokens, heads, dim], any strides but for adjacent channels.
 bool rows_at(PyObject* o, const at::Tensor*& x, dmx_rows& r) {
-    using K = c10::DispatchKey;
     x = exact(o);
-    if (!x || !x->defined() || !x->is_cuda() || x->layout() != at::kStrided || !x->has_storage() || x->dim() != 3 ||
-        x->key_set().has_any(c10::DispatchKeySet({K::FuncTorchBatched, K::FuncTorchGradWrapper, K::Functionalize,
-                                                  K::Python, K::Negative, K::Conjugate, K::ZeroTensor})))
-        return false;
-    if (code(x->scalar_type()) < 0 || x->stride(2) != 1 || x->size(0) >= kMost || x->size(1) >= kMost ||
+    if (!strided(x) || x->dim() != 3) return false;
+    if ( x->size(0) >= kMost || x->size(1) >= kMost ||
         wants(*x))
         return false;
     r = {const_cast<void*>(x->const_data_ptr()), x->stride(0), x->stride(1), (uint32_t)x->size(1)};
@@ -328,12 +335,14 @@ PyObject* pair_of(at::Tensor&& a, at::Tensor&& b) {  // (b undefined: None)
     return p;
 }
 
-// rotary(q, k or None, positions, table, layout code, stream) -> (q', k')
+// rotary(q, k or None, positions, table, layout code, stream, address of a
+// dmx_rotary_axes or 0, its angles) -> (q', k')
 PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 6) return launch_failed("rotary", "six arguments");
-    const long layout = PyLong_AsLong(a[4]);
+    if (n != 8) return launch_failed("rotary", "eight arguments");
+    const long layout = PyLong_AsLong(a[4]), angles = PyLong_AsLong(a[7]);
     void* stream = PyLong_AsVoidPtr(a[5]);
+    const auto* axes = static_cast<const dmx_rotary_axes*>(PyLong_AsVoidPtr(a[6]));
     if (PyErr_Occurred()) return nullptr;
     const at::Tensor *q, *k = nullptr, *p = exact(a[2]);
     dmx_rows in[2], out[2];
@@ -341,10 +350,11 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (layout < 0 || !modes_off() || !rows_at(a[0], q, in[0])) Py_RETURN_NONE;
     const int count = a[1] == Py_None ? 1 : 2;
     if (count == 2 && (!rows_at(a[1], k, in[1]) || !like(*q, *k))) Py_RETURN_NONE;
-    if (!p || !plain(*p) || p->dim() != 1 || p->size(0) != q->size(0) || p->get_device() != q->get_device() ||
+    if (!p || !plain(*p) || p->dim() != (axes ? 2 : 1) || p->size(-1) != q->size(0) || p->get_device() != q->get_device() ||
         (p->scalar_type() != at::kInt && p->scalar_type() != at::kLong) || q->size(2) >= kMost ||
         !table_of(a[3], layout, q->size(2), q->get_device(), t))
         Py_RETURN_NONE;
+    if (axes && (p->size(0) < axes->count || p->size(0) > 4 || (long)t.dim != 2 * angles)) Py_RETURN_NONE;
     at::Tensor y, z;
     char err[512];
     int st;
@@ -357,10 +367,13 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
             z = dense_like(*k);
             out[1] = dense_rows(z);
         }
-        st = dmx_rotary(in, out, count, (uint32_t)q->size(0), (uint32_t)q->size(2), code(q->scalar_type()), p->const_data_ptr(),
-                        p->scalar_type() == at::kLong, &t, stream, err, sizeof err);
+        const int dt = code(q->scalar_type()), wide = p->scalar_type() == at::kLong;
+        st = axes ? dmx_rotary_by_axes(in, out, count, (uint32_t)q->size(0), (uint32_t)q->size(2), dt, p->const_data_ptr(), wide,
+                                       axes, &t, stream, err, sizeof err)
+                  : dmx_rotary(in, out, count, (uint32_t)q->size(0), (uint32_t)q->size(2), dt, p->const_data_ptr(), wide, &t, stream,
+                               err, sizeof err);
     }
-    return st ? launch_failed("dmx_rotary", err) : pair_of(std::move(y), std::move(z));
+    return st ? launch_failed(axes ? "dmx_rotary_by_axes" : "dmx_rotary", err) : pair_of(std::move(y), std::move(z));
     END_HANDLE_TH_ERRORS
 }
 
@@ -439,10 +452,11 @@ int64_t count_of(PyObject* o) {
 }
 
 // attention(q, cache, block_table, lengths, cu, max_tokens or None, max_length
-// or 0, scale or None, causal, window or None, lse, stream) -> out, or (out, lse)
+// or 0, scale or None, causal, window or None, lse, stream, blocks or None) -> out,
+// or (out, lse)
 PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 12) return launch_failed("attention", "twelve arguments");
+    if (n != 13) return launch_failed("attention", "thirteen arguments");
     const int64_t max_tokens = count_of(a[5]), max_length = whole(a[6]), window = count_of(a[9]);
     const double given = a[7] == Py_None ? 0 : PyFloat_AsDouble(a[7]);
     const int causal = PyObject_IsTrue(a[8]), want = PyObject_IsTrue(a[10]);
@@ -458,6 +472,14 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         max_length >= (1ll << 32) || max_tokens < 0 || max_tokens >= kMost || (max_tokens && a[4] == Py_None) ||
         !seqs_of(a[2], a[3], a[4], q->size(0), max_tokens ? max_tokens : q->size(0), index, s))
         Py_RETURN_NONE;
+    const at::Tensor* blocks = nullptr;
+    if (a[12] != Py_None) {
+        blocks = dense(a[12], at::kInt, 3, index);
+        if (!blocks || blocks->size(0) != q->size(0) || blocks->size(1) != c.heads || blocks->size(2) < 1 ||
+            blocks->size(2) > DMX_KV_MAX_COLUMNS || s.table_cols > DMX_KV_MAX_COLUMNS || window)
+            Py_RETURN_NONE;
+    }
+    const uint32_t count = blocks ? (uint32_t)blocks->size(2) : 0;
     const double scale = a[7] == Py_None ? 1 / std::sqrt((double)c.dim) : given;
     at::Tensor out, lse, ws;
     char err[512];
@@ -468,14 +490,293 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int dt = code(q->scalar_type());
         out = dense_like(*q);
         if (want) lse = at::empty({q->size(0), q->size(1)}, at::TensorOptions().device(q->device()).dtype(at::kFloat));
-        const uint64_t bytes = s.total ? dmx_kv_attention_workspace(&c, &s, r.heads, dt, (uint32_t)max_length, (uint32_t)window) : 0;
+        const uint64_t bytes = !s.total ? 0
+                               : blocks ? dmx_kv_attention_blocks_workspace(&c, &s, r.heads, dt, count, (uint32_t)max_length)
+                                        : dmx_kv_attention_workspace(&c, &s, r.heads, dt, (uint32_t)max_length, (uint32_t)window);
         if (bytes) ws = at::empty({(int64_t)bytes}, at::TensorOptions().device(q->device()).dtype(at::kByte));
-        st = dmx_kv_attention(&c, &s, &r, dt, (float)scale, causal, (uint32_t)window, (uint32_t)max_length,
-                              out.mutable_data_ptr(), want ? static_cast<float*>(lse.mutable_data_ptr()) : nullptr,
-                              bytes ? ws.mutable_data_ptr() : nullptr, bytes, stream, err, sizeof err);
+        float* sums = want ? static_cast<float*>(lse.mutable_data_ptr()) : nullptr;
+        void* space = bytes ? ws.mutable_data_ptr() : nullptr;
+        st = blocks ? dmx_kv_attention_blocks(&c, &s, &r, dt, (float)scale, causal, static_cast<const int32_t*>(blocks->const_data_ptr()),
+                                              count, (uint32_t)max_length, out.mutable_data_ptr(), sums, space, bytes, stream, err, sizeof err)
+                    : dmx_kv_attention(&c, &s, &r, dt, (float)scale, causal, (uint32_t)window, (uint32_t)max_length,
+                                       out.mutable_data_ptr(), sums, space, bytes, stream, err, sizeof err);
     }
-    if (st) return launch_failed("dmx_kv_attention", err);
+    if (st) return launch_failed(blocks ? "dmx_kv_attention_blocks" : "dmx_kv_attention", err);
     return want ? pair_of(std::move(out), std::move(lse)) : THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// -------------------------------------------------------------------- pages --
+
+PyObject* g_pool[3];  // "free", "count", "lacking"
+
+// A pool dict, a block table, lengths and numbers of tokens (null: None) of one device.
+bool pages_of(PyObject* pool, PyObject* table, PyObject* lengths, PyObject* given, int64_t page, dmx_kv_pool& p, int32_t*& at_table,
+              int32_t*& at_lengths, const int32_t*& at_given, int64_t& batch, int64_t& cols, int64_t& index) {
+    const at::Tensor* t = exact(table);
+    if (!PyDict_Check(pool) || !t || !plain(*t) || t->scalar_type() != at::kInt || t->dim() != 2) return false;
+    index = t->get_device();
+    batch = t->size(0), cols = t->size(1);
+    const at::Tensor* l = dense(lengths, at::kInt, 1, index);
+    const at::Tensor* g = given == Py_None ? nullptr : dense(given, at::kInt, 1, index);
+    const at::Tensor* x[3];
+    for (int n = 0; n < 3; ++n) {
+        PyObject* v = PyDict_GetItem(pool, g_pool[n]);  // borrowed
+        x[n] = v ? dense(v, at::kInt, 1, index) : nullptr;
+        if (!x[n] || (n && x[n]->size(0) != 1)) return false;
+    }
+    const int64_t pages = x[0]->size(0);
+    if (!l || l->size(0) != batch || (given != Py_None && (!g || g->size(0) != batch)) || batch < 1 || cols < 1 || batch >= kMost ||
+        cols >= kMost || pages < 1 || pages >= kMost || page < 8 || page > 1024 || (page & (page - 1)))
+        return false;
+    p.free = static_cast<int32_t*>(x[0]->mutable_data_ptr());
+    p.count = static_cast<int32_t*>(x[1]->mutable_data_ptr());
+    p.lacking = static_cast<int32_t*>(x[2]->mutable_data_ptr());
+    p.pages = (uint32_t)pages;
+    at_table = static_cast<int32_t*>(t->mutable_data_ptr());
+    at_lengths = static_cast<int32_t*>(l->mutable_data_ptr());
+    at_given = g ? static_cast<const int32_t*>(g->const_data_ptr()) : nullptr;
+    return true;
+}
+
+// reserve(pool, block_table, lengths, page_size, total, new or None, stream) ->
+// (cu, positions, slots)
+PyObject* reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 7) return launch_failed("reserve", "seven arguments");
+    const int64_t page = whole(a[3]), total = whole(a[4]);
+    void* stream = PyLong_AsVoidPtr(a[6]);
+    if (PyErr_Occurred()) return nullptr;
+    dmx_kv_pool p;
+    int32_t *table, *lengths;
+    const int32_t* added;
+    int64_t batch, cols, index;
+    if (!modes_off() || total < 0 || total >= kMost ||
+        !pages_of(a[0], a[1], a[2], a[5], page, p, table, lengths, added, batch, cols, index) || (!added && total % batch))
+        Py_RETURN_NONE;
+    at::Tensor cu, positions, slots;
+    char err[512];
+    int st;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const at::Device device(at::kCUDA, (c10::DeviceIndex)index);
+        const c10::DeviceGuard on(device);
+        const auto options = at::TensorOptions().device(device);
+        cu = at::empty({batch + 1}, options.dtype(at::kInt));
+        positions = at::empty({total}, options.dtype(at::kInt));
+        slots = at::empty({total}, options.dtype(at::kLong));
+        st = dmx_kv_reserve(&p, table, lengths, added, (uint32_t)batch, (uint32_t)cols, (uint32_t)page, (uint32_t)total,
+                            static_cast<int32_t*>(cu.mutable_data_ptr()), static_cast<int32_t*>(positions.mutable_data_ptr()),
+                            static_cast<int64_t*>(slots.mutable_data_ptr()), stream, err, sizeof err);
+    }
+    if (st) return launch_failed("dmx_kv_reserve", err);
+    at::Tensor* outs[3] = {&cu, &positions, &slots};
+    PyObject* tuple = PyTuple_New(3);
+    for (int i = 0; tuple && i < 3; ++i) {
+        PyObject* o = THPVariable_Wrap(std::move(*outs[i]));
+        if (!o)
+            Py_CLEAR(tuple);
+        else
+            PyTuple_SET_ITEM(tuple, i, o);
+    }
+    return tuple;
+    END_HANDLE_TH_ERRORS
+}
+
+// trim(pool, block_table, lengths, page_size, keep, stream) -> True
+PyObject* trim(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 6) return launch_failed("trim", "six arguments");
+    const int64_t page = whole(a[3]);
+    void* stream = PyLong_AsVoidPtr(a[5]);
+    if (PyErr_Occurred()) return nullptr;
+    dmx_kv_pool p;
+    int32_t *table, *lengths;
+    const int32_t* keep;
+    int64_t batch, cols, index;
+    if (!modes_off() || a[4] == Py_None || !pages_of(a[0], a[1], a[2], a[4], page, p, table, lengths, keep, batch, cols, index))
+        Py_RETURN_NONE;
+    char err[512];
+    int st;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const c10::DeviceGuard on(at::Device(at::kCUDA, (c10::DeviceIndex)index));
+        st = dmx_kv_trim(&p, table, lengths, keep, (uint32_t)batch, (uint32_t)cols, (uint32_t)page, stream, err, sizeof err);
+    }
+    if (st) return launch_failed("dmx_kv_trim", err);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// ----------------------------------------------------------- selected pages --
+
+PyObject* g_summaries[2];  // "bounds", "scales"
+bool summaries_of(PyObject* o, const dmx_kv_cache& c, int64_t index, dmx_kv_summaries& s) {
+    if (!PyDict_Check(o)) return false;
+    PyObject *b = PyDict_GetItem(o, g_summaries[0]), *e = PyDict_GetItem(o, g_summaries[1]);  // borrowed
+    const at::Tensor *bounds = b ? dense(b, at::kChar, 4, index) : nullptr, *scales = e ? dense(e, at::kByte, 2, index) : nullptr;
+    const int64_t pages = c.pages, heads = c.heads, dim = c.dim;
+    if (!bounds || !scales || bounds->sizes() != at::IntArrayRef({pages, heads, 2, dim}) ||
+        scales->sizes() != at::IntArrayRef({pages, heads}))
+        return false;
+    s.bounds = static_cast<int8_t*>(bounds->mutable_data_ptr());
+    s.scales = static_cast<uint8_t*>(scales->mutable_data_ptr());
+    return true;
+}
+
+// summarize(cache, summaries, block_table, lengths, total, cu, stream) -> True
+PyObject* summarize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 7) return launch_failed("summarize", "seven arguments");
+    const int64_t total = whole(a[4]);
+    void* stream = PyLong_AsVoidPtr(a[6]);
+    if (PyErr_Occurred()) return nullptr;
+    dmx_kv_cache c;
+    dmx_kv_seqs s;
+    dmx_kv_summaries x;
+    int64_t index;
+    if (!modes_off() || !cache_of(a[0], c, index) || !summaries_of(a[1], c, index, x) || !seqs_of(a[2], a[3], a[5], total, 0, index, s))
+        Py_RETURN_NONE;
+    char err[512];
+    int st;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const c10::DeviceGuard on(at::Device(at::kCUDA, (c10::DeviceIndex)index));
+        st = dmx_kv_summarize(&c, &x, &s, stream, err, sizeof err);
+    }
+    if (st) return launch_failed("dmx_kv_summarize", err);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// select(q, cache, summaries, block_table, lengths, count, cu, first, last, causal,
+// stream) -> blocks
+PyObject* select(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 11) return launch_failed("select", "eleven arguments");
+    const int64_t count = whole(a[5]), first = whole(a[7]), last = whole(a[8]);
+    const int causal = PyObject_IsTrue(a[9]);
+    void* stream = PyLong_AsVoidPtr(a[10]);
+    if (PyErr_Occurred()) return nullptr;
+    dmx_kv_cache c;
+    dmx_kv_seqs s;
+    dmx_kv_summaries x;
+    dmx_rows r;
+    const at::Tensor* q;
+    int64_t index;
+    if (!modes_off() || !cache_of(a[1], c, index) || !summaries_of(a[2], c, index, x) || !rows_at(a[0], q, r) ||
+        q->get_device() != index || q->size(2) != c.dim || r.heads == 0 || c.heads == 0 || r.heads % c.heads || count < 1 ||
+        count > DMX_KV_MAX_COLUMNS || first < 0 || last < 0 || first > count || last > count - first ||
+        !seqs_of(a[3], a[4], a[6], q->size(0), 0, index, s) || s.table_cols > DMX_KV_MAX_COLUMNS)
+        Py_RETURN_NONE;
+    at::Tensor out;
+    char err[512];
+    int st;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const c10::DeviceGuard on(q->device());
+        out = at::empty({q->size(0), (int64_t)c.heads, count}, at::TensorOptions().device(q->device()).dtype(at::kInt));
+        st = dmx_kv_select(&c, &x, &s, &r, code(q->scalar_type()), (uint32_t)count, (uint32_t)first, (uint32_t)last, causal,
+                           static_cast<int32_t*>(out.mutable_data_ptr()), stream, err, sizeof err);
+    }
+    return st ? launch_failed("dmx_kv_select", err) : THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// -------------------------------------------------------------------- norms --
+
+// A row of `dim` (or, `many`, several rows), or None.
+bool vectors_at(PyObject* o, int64_t dim, int64_t index, bool many, dmx_vectors& v) {
+    v = {};
+    if (o == Py_None) return true;
+    const at::Tensor* t = exact(o);
+    if (!t || !plain(*t) || t->get_device() != index || code(t->scalar_type()) < 0 || wants(*t) || t->dim() < 1 || t->dim() > 2 ||
+        t->size(-1) != dim)
+        return false;
+    const int64_t rows = t->dim() == 1 ? 1 : t->size(0);
+    if (rows < 1 || rows >= kMost || (!many && rows != 1)) return false;
+    v = {t->const_data_ptr(), code(t->scalar_type()), (uint32_t)rows};
+    return true;
+}
+
+bool norm_form_of(long kind, double eps, double offset, double factor, dmx_norm_form& f) {
+    f = {};
+    if (kind < 0 || !(eps >= 0) || !std::isfinite(eps) || !std::isfinite(offset) || !std::isfinite(factor)) return false;
+    f.kind = (int)kind, f.eps = (float)eps, f.offset = (float)offset, f.factor = (float)factor;
+    return true;
+}
+
+// norm(x, weight, bias, kind code, eps, offset, stream) -> out
+PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 7) return launch_failed("norm", "seven arguments");
+    const long kind = PyLong_AsLong(a[3]);
+    const double eps = PyFloat_AsDouble(a[4]), offset = PyFloat_AsDouble(a[5]);
+    void* stream = PyLong_AsVoidPtr(a[6]);
+    if (PyErr_Occurred()) return nullptr;
+    const at::Tensor* x = exact(a[0]);
+    dmx_norm_form f;
+    if (!modes_off() || !strided(x) || (x->dim() != 2 && x->dim() != 3) || wants(*x) || x->numel() == 0 || x->size(0) >= kMost ||
+        x->size(1) >= kMost || x->size(-1) > DMX_NORM_MAX_DIM || !norm_form_of(kind, eps, offset, 1, f) ||
+        !vectors_at(a[1], x->size(-1), x->get_device(), false, f.weight) || !vectors_at(a[2], x->size(-1), x->get_device(), false, f.bias))
+        Py_RETURN_NONE;
+    const bool heads = x->dim() == 3;
+    const dmx_rows r = {const_cast<void*>(x->const_data_ptr()), x->stride(0), heads ? x->stride(1) : 0, heads ? (uint32_t)x->size(1) : 1};
+    at::Tensor out;
+    char err[512];
+    int st;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const c10::DeviceGuard on(x->device());
+        out = at::empty(x->sizes(), at::TensorOptions().device(x->device()).dtype(x->scalar_type()));
+        st = dmx_norm(&r, out.mutable_data_ptr(), (uint32_t)x->size(0), (uint32_t)x->size(-1), code(x->scalar_type()), &f, stream, err, sizeof err);
+    }
+    return st ? launch_failed("dmx_norm", err) : THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// block_norm(y, residual, weight, bias, post, gate, factor, scale, shift, cu, kind
+// code, eps, offset, stream) -> (residual', x)
+PyObject* block_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 14) return launch_failed("block_norm", "fourteen arguments");
+    const double factor = PyFloat_AsDouble(a[6]), eps = PyFloat_AsDouble(a[11]), offset = PyFloat_AsDouble(a[12]);
+    const long kind = PyLong_AsLong(a[10]);
+    void* stream = PyLong_AsVoidPtr(a[13]);
+    if (PyErr_Occurred()) return nullptr;
+    const at::Tensor *y = exact(a[0]), *r = exact(a[1]);
+    dmx_norm_form f;
+    if (!modes_off() || !strided(y) || !strided(r) || y->dim() != 2 || r->dim() != 2 || wants(*y) || wants(*r) || y->sizes() != r->sizes() ||
+        y->get_device() != r->get_device() || (r->scalar_type() != y->scalar_type() && r->scalar_type() != at::kFloat) ||
+        y->size(0) >= kMost || y->size(1) < 1 || y->size(1) > DMX_NORM_MAX_DIM || !norm_form_of(kind, eps, offset, factor, f))
+        Py_RETURN_NONE;
+    const int64_t T = y->size(0), D = y->size(1), index = y->get_device();
+    if (!vectors_at(a[2], D, index, false, f.weight) || !vectors_at(a[3], D, index, false, f.bias) || !vectors_at(a[4], D, index, false, f.post) ||
+        !vectors_at(a[5], D, index, true, f.gate) || !vectors_at(a[7], D, index, true, f.scale) || !vectors_at(a[8], D, index, true, f.shift) ||
+        !f.scale.at != !f.shift.at || f.scale.rows != f.shift.rows)
+        Py_RETURN_NONE;
+    if (a[9] != Py_None) {
+        const at::Tensor* cu = dense(a[9], at::kInt, 1, index);
+        if (!cu || cu->size(0) < 2 || cu->size(0) >= kMost) Py_RETURN_NONE;
+        f.cu = static_cast<const int32_t*>(cu->const_data_ptr());
+        f.batch = (uint32_t)(cu->size(0) - 1);
+    }
+    for (const dmx_vectors* v : {&f.gate, &f.scale})
+        if (v->at && v->rows != 1 && !(f.cu && v->rows == f.batch) && T % v->rows) Py_RETURN_NONE;
+    at::Tensor res, out;
+    char err[512];
+    int st;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const c10::DeviceGuard on(y->device());
+        const auto options = at::TensorOptions().device(y->device());
+        res = at::empty({T, D}, options.dtype(r->scalar_type()));
+        out = at::empty({T, D}, options.dtype(y->scalar_type()));
+        st = dmx_block_norm(y->const_data_ptr(), y->stride(0), r->const_data_ptr(), r->stride(0), res.mutable_data_ptr(),
+                            out.mutable_data_ptr(), (uint32_t)T, (uint32_t)D, code(y->scalar_type()), code(r->scalar_type()), &f,
+                            stream, err, sizeof err);
+    }
+    return st ? launch_failed("dmx_block_norm", err) : pair_of(std::move(res), std::move(out));
     END_HANDLE_TH_ERRORS
 }
 
@@ -490,6 +791,12 @@ PyMethodDef g_methods[] = {{"rows", fast<rows>(), METH_FASTCALL, nullptr},
                            {"append", fast<append>(), METH_FASTCALL, nullptr},
                            {"read", fast<read>(), METH_FASTCALL, nullptr},
                            {"attention", fast<attention>(), METH_FASTCALL, nullptr},
+                           {"reserve", fast<reserve>(), METH_FASTCALL, nullptr},
+                           {"trim", fast<trim>(), METH_FASTCALL, nullptr},
+                           {"summarize", fast<summarize>(), METH_FASTCALL, nullptr},
+                           {"select", fast<select>(), METH_FASTCALL, nullptr},
+                           {"norm", fast<norm>(), METH_FASTCALL, nullptr},
+                           {"block_norm", fast<block_norm>(), METH_FASTCALL, nullptr},
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "dmx_calls", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
@@ -502,6 +809,12 @@ PyMODINIT_FUNC PyInit_dmx_calls(void) {
     const char* buffers[4] = {"k_codes", "k_scales", "v_codes", "v_scales"};
     for (int i = 0; i < 4; ++i)
         if (!(g_cache[i] = PyUnicode_InternFromString(buffers[i]))) return nullptr;
+    const char* stack[3] = {"free", "count", "lacking"};
+    for (int i = 0; i < 3; ++i)
+        if (!(g_pool[i] = PyUnicode_InternFromString(stack[i]))) return nullptr;
+    const char* summary[2] = {"bounds", "scales"};
+    for (int i = 0; i < 2; ++i)
+        if (!(g_summaries[i] = PyUnicode_InternFromString(summary[i]))) return nullptr;
     PyObject* m = PyModule_Create(&g_module);
     // (the torch whose headers this was compiled with: the loader compares)
     if (m && PyModule_AddStringConstant(m, "torch_version", DMX_TORCH_VERSION) < 0) {

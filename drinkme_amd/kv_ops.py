@@ -288,7 +288,7 @@ def _packed_axes(axes: tuple):
     if not 1 <= len(axes) <= 256 or any(type(a) is not int or not 0 <= a < 4 for a in axes):
         raise ValueError("rotary: axes are 1..256 numbers of 0..3 (rotary_axes)")
     x = _native.KvRotaryAxes()
-    x.count, x.angles = max(axes) + 1, len(axes)
+    x.count, x.angles, x.packed = max(axes) + 1, len(axes), (ct.addressof(x), len(axes))
     for i, a in enumerate(axes):
         x.of[i // 16] |= a << (2 * (i % 16))
     return x
@@ -305,9 +305,10 @@ def rotary(q: torch.Tensor, k, positions: torch.Tensor, table: torch.Tensor, lay
 
     With `axes` (rotary_axes's: the axis of each of the table's angles) positions
     are [axes, T], and angle i of token t is the table's at positions[axes[i], t]."""
+    axes = None if axes is None else _packed_axes(tuple(axes))
     native = _native.calls()
-    if native is not None and axes is None:  # the plain case in one native call; None: anything else
-        outs = native.rotary(q, k, positions, table, LAYOUTS.get(layout, -1), _current(q))
+    if native is not None:  # the plain case in one native call; None: anything else
+        outs = native.rotary(q, k, positions, table, LAYOUTS.get(layout, -1), _current(q), *(axes.packed if axes else (0, 0)))
         if outs is not None:
             return outs
     _no_gradient("rotary", q, k, table)
@@ -315,7 +316,6 @@ def rotary(q: torch.Tensor, k, positions: torch.Tensor, table: torch.Tensor, lay
     ins = [q] if k is None else [q, _activation(k, "rotary: k", dim=q.shape[2], tokens=q.shape[0], like=q)]
     shape = (q.shape[0],)
     if axes is not None:
-        axes = _packed_axes(tuple(axes))
         shape = (positions.shape[0], q.shape[0]) if positions.dim() and axes.count <= positions.shape[0] <= 4 else \
             (axes.count, q.shape[0])
         if table.dim() == 3 and table.shape[1] != axes.angles:
@@ -437,9 +437,9 @@ def attention(q: torch.Tensor, cache: dict, block_table: torch.Tensor, lengths: 
     blocks[t, h], in any order, each once however often it is listed, negative ones
     nothing. No window then."""
     native = _native.calls()
-    if native is not None and blocks is None:
+    if native is not None:
         outs = native.attention(q, cache, block_table, lengths, cu, max_tokens, max_length or 0, scale, causal, window,
-                                return_lse, _current(q))
+                                return_lse, _current(q), blocks)
         if outs is not None:
             return outs
     _no_gradient("attention", q)
@@ -547,6 +547,11 @@ def reserve(pool: dict, block_table: torch.Tensor, lengths: torch.Tensor, page_s
     int64): what append and attention take as `cu`, each new token's position (-1 in
     rows of no sequence) and its place page * page_size + position % page_size (-1
     without a page)."""
+    native = _native.calls()
+    if native is not None:
+        outs = native.reserve(pool, block_table, lengths, page_size, total, new, _current(lengths))
+        if outs is not None:
+            return outs
     total = int(total)
     p, at, sizes, device = _pages_of(pool, block_table, lengths, page_size, "reserve")
     if total < 0 or total >= _MOST or (new is None and total % sizes[0]):
@@ -569,6 +574,9 @@ def trim(pool: dict, block_table: torch.Tensor, lengths: torch.Tensor, page_size
     length or more leaves it), in place: lengths, the columns behind it (-1), and the
     pool, which gets their pages back and hands them out in the same order. A
     page that two sequences share must not be returned twice: it is not counted here."""
+    native = _native.calls()
+    if native is not None and native.trim(pool, block_table, lengths, page_size, keep, _current(lengths)):
+        return
     p, at, sizes, device = _pages_of(pool, block_table, lengths, page_size, "trim")
     keep = _numbers(keep, "trim: keep", sizes[0], device)
     err = _native.error_buffer()
@@ -621,6 +629,9 @@ def summarize(cache: dict, summaries: dict, block_table: torch.Tensor, lengths: 
     """The summaries, in place, of the pages that the last tokens of each sequence
     lie in (`total` / B of each, or cu's, as read takes them), from every token
     that their sequence has there: after append, and before select."""
+    native = _native.calls()
+    if native is not None and native.summarize(cache, summaries, block_table, lengths, total, cu, _current(lengths)):
+        return
     c = _cache_of(cache, "summarize")
     device = cache["k_codes"].device
     x = _summaries_of(summaries, c, cache, "summarize")
@@ -641,6 +652,11 @@ def select(q: torch.Tensor, cache: dict, summaries: dict, block_table: torch.Ten
     page: with the summaries' largest keys for channels where q > 0, their smallest
     where q < 0, and q in 8 bits. Sums are whole numbers, so that the choice does not depend on
     how they are added; ties go to the lower column."""
+    native = _native.calls()
+    if native is not None:
+        out = native.select(q, cache, summaries, block_table, lengths, count, cu, first, last, causal, _current(q))
+        if out is not None:
+            return out
     _no_gradient("select", q)
     c = _cache_of(cache, "select")
     x = _summaries_of(summaries, c, cache, "select")

@@ -26,7 +26,7 @@ import math
 import torch
 
 from . import _native
-from .kv_ops import _MOST, _no_gradient
+from .kv_ops import _MOST, _current, _no_gradient
 from .radix_ops import _dtype_code, _stream
 
 KINDS = {"rms": _native.NORM_RMS, "layer": _native.NORM_LAYER}
@@ -75,6 +75,11 @@ def norm(x: torch.Tensor, weight=None, *, bias=None, kind: str = "rms", eps: flo
     """Each row of x [T, D] or [T, H, D] (views of a fused product are read in
     place) normed, dense and in x's dtype. weight and bias: [D], or None. `offset`
     is added to the weights (1 where they are kept as their difference from 1)."""
+    native = _native.calls()
+    if native is not None:  # the plain case in one native call; None: anything else
+        out = native.norm(x, weight, bias, KINDS.get(kind, -1), eps, offset, _current(x))
+        if out is not None:
+            return out
     _no_gradient("norm", x, weight, bias)
     x = _rows_of(x, "norm: x", (2, 3))
     f = _form(kind, eps, offset, 1.0, "norm")
@@ -109,6 +114,12 @@ def block_norm(y: torch.Tensor, residual: torch.Tensor, weight=None, *, bias=Non
     other, or, with `cu` (int32 [n + 1] on the GPU: offsets of n sequences), one for
     rows cu[i] .. cu[i + 1] - 1 (rows before and behind: the nearest sequence's)."""
     scale, shift = modulate if modulate is not None else (None, None)
+    native = _native.calls()
+    if native is not None:
+        outs = native.block_norm(y, residual, weight, bias, post, gate, factor, scale, shift, cu, KINDS.get(kind, -1), eps, offset,
+                                 _current(y))
+        if outs is not None:
+            return outs
     _no_gradient("block_norm", y, residual, weight, bias, post, gate, scale, shift)
     y = _rows_of(y, "block_norm: y", (2,))
     residual = _rows_of(residual, "block_norm: residual", (2,))
