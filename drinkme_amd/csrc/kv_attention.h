@@ -245,10 +245,22 @@ __device__ __forceinline__ void hide_values(State<W, P, NR>& st, Block<W>& x, in
 }
 
 // A block's part of the rows' results.
-// t0: the first of the eight tokens whose scores are this lane's.
-template <int W, int P, int NR>
+// Whether any of the lane's values has an exponent byte over 252.
+template <int W>
+__device__ __forceinline__ bool may_be_nan(const Block<W>& x) {
+    uint32_t all = 0;  // the top bit of each such byte
+#pragma unroll
+    for (int s = 0; s < Segments<W>::count; ++s)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) all |= x.vs[s][n] & ((x.vs[s][n] & 0x7f7f7f7fu) + 0x03030303u) & 0x80808080u;
+    return all != 0;
+}
+
+// t0: the first of the eight tokens whose scores are this lane's. LISTED: where not `edge`, a row
+// sees all of the eight or, its st.hi 0, none.
+template <bool LISTED = false, int W, int P, int NR>
 __device__ __forceinline__ void attend_block(State<W, P, NR>& st, Block<W>& x, float scale, int t0, int i, int j, bool fresh,
-                                             bool part, int hi_all) {
+                                             bool part, int hi_all, bool edge = true) {
     using S = Segments<W>;
 
     // scores: S^T = K Q^T
@@ -285,7 +297,11 @@ __device__ __forceinline__ void attend_block(State<W, P, NR>& st, Block<W>& x, f
         float p[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) p[e] = sc[t][e >> 2][e & 3];
-        if (part) {
+        if (LISTED && part && !edge) {
+            const bool seen = st.hi[t] > 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = seen ? p[e] : -INFINITY;
+        } else if (part) {
             int at = t0;
             asm volatile("" : "+v"(at));  // (a branch: else the comparisons are made for every block)
 #pragma unroll
@@ -327,7 +343,7 @@ __device__ __forceinline__ void attend_block(State<W, P, NR>& st, Block<W>& x, f
         if constexpr (P == 1) st.norm[t] = plus_all(pf[t][0], st.norm[t]);
     }
 
-    if (part) hide_values(st, x, t0, hi_all);
+    if (part && (!LISTED || edge || __any(may_be_nan(x)))) hide_values(st, x, t0, hi_all);
 
     // O^T += V^T P^T
 #pragma unroll
@@ -396,32 +412,55 @@ __device__ __forceinline__ void leave_rest(const AttnArgs& a, const Seq& q, uint
 // who[c] of each column that one of them may see, and those columns in ascending
 // order in `list` -> how many. A column listed twice is there once; one that is
 // negative, or past its token's position, is nothing. `beyond` has the tokens that
-// list a position which the table has no page for.
+// list a position which the table has no page for. One token whose list ascends, as
+// select writes it, needs no such bits: `plain`, and who is not written.
+template <int WAVES>
 __device__ __forceinline__ int list_pages(const AttnArgs& a, uint32_t h, const Seq& q, int m0, int m1, uint32_t* who, uint16_t* list,
-                                          uint32_t& beyond) {
-    __shared__ int counts[kAttnWaves];
+                                          uint32_t& beyond, bool& plain) {
+    __shared__ int counts[WAVES], out_of_order[WAVES];
     __shared__ uint32_t past;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), shift = a.cache.page_shift;
     const auto last_of = [&](int m) { return (a.causal ? q.first + m : q.length - 1) >> shift; };  // (negative: none)
     const int cols = min(last_of(m1) + 1, a.seqs.cols), entries = (m1 - m0 + 1) * (int)a.count.value;
-    for (int c = threadIdx.x; c < cols; c += 64 * kAttnWaves) who[c] = 0;
+    plain = false;
+    if (m0 == m1 && entries <= 64 * WAVES) {
+        const int32_t* mine = a.blocks + ((int64_t)(q.token + m0) * a.cache.heads + h) * entries;
+        const int n = threadIdx.x, c = n < entries ? mine[n] : -1, before = n && n < entries ? mine[n - 1] : -1;
+        const bool in = c >= 0 && c < cols;  // (columns that it sees and that there are; past the others nothing may follow)
+        const uint64_t some = __ballot(in);
+        const uint64_t bad = __ballot(c > last_of(m0) ? false : c >= a.seqs.cols || (in && n && before >= c) || (in && n && before < 0));
+        if (in) list[n] = (uint16_t)c;
+        if (lane == 0) counts[wave] = __popcll(some), out_of_order[wave] = bad != 0;
+        __syncthreads();
+        int all = 0, bads = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            all += counts[w];
+            bads |= out_of_order[w];
+        }
+        plain = !bads;
+        beyond = 0;
+        if (plain) return all;
+        __syncthreads();
+    }
+    for (int c = threadIdx.x; c < cols; c += 64 * WAVES) who[c] = 0;
     if (threadIdx.x == 0) past = 0;
     __syncthreads();
-    for (int n = threadIdx.x; n < entries; n += 64 * kAttnWaves) {
+    for (int n = threadIdx.x; n < entries; n += 64 * WAVES) {
         const int token = (uint32_t)n / a.count;
         const int64_t row = (int64_t)(q.token + m0 + token) * a.cache.heads + h;
         const int c = a.blocks[row * a.count.value + (n - token * (int)a.count.value)];
         if (c >= 0 && c <= last_of(m0 + token)) atomicOr(c < a.seqs.cols ? who + c : &past, 1u << token);
     }
     __syncthreads();
-    const int each = (cols + 64 * kAttnWaves - 1) / (64 * kAttnWaves) * 64, first = wave * each, end = min(first + each, cols);
+    const int each = (cols + 64 * WAVES - 1) / (64 * WAVES) * 64, first = wave * each, end = min(first + each, cols);
     int found = 0;
     for (int c = first; c < end; c += 64) found += __popcll(__ballot(c + lane < end && who[c + lane]));
     if (lane == 0) counts[wave] = found;
     __syncthreads();
     int at = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < kAttnWaves; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
         at += w < wave ? counts[w] : 0;
         all += counts[w];
     }
@@ -439,7 +478,7 @@ __device__ __forceinline__ int list_pages(const AttnArgs& a, uint32_t h, const S
 // As entries, of block blk of the listed pages' tokens, one page after the other.
 template <bool WIDE>
 __device__ __forceinline__ ListedEntry listed_entries(const AttnArgs& a, uint32_t b, int blk, int i, int j, int count,
-                                                      const uint32_t* who, const uint16_t* list) {
+                                                      bool plain, const uint32_t* who, const uint16_t* list) {
     const int shift = a.cache.page_shift;
     const auto page_at = [&](int octet, int& col) {
         const int n = (blk * 32 + 8 * octet) >> shift;
@@ -452,7 +491,7 @@ __device__ __forceinline__ ListedEntry listed_entries(const AttnArgs& a, uint32_
     e.v = page_at(WIDE ? 0 : j, col);
     if (WIDE) e.k = e.v;
     e.at = col < 0 ? 1 << 30 : (col << shift) + ((blk * 32 + 8 * j) & ((1 << shift) - 1));
-    e.who = col < 0 ? 0 : who[col];
+    e.who = col < 0 ? 0 : plain ? 1 : who[col];
     return e;
 }
 
@@ -472,8 +511,8 @@ __device__ __forceinline__ ListedEntry listed_entries(const AttnArgs& a, uint32_
 //
 // LISTED: of the columns that each token sees, those that it lists; a tile walks the
 // pages that any of its tokens lists, and a row's weights of the others are 0.
-template <int W, int P, int NR, bool ROWS, bool WIDE, bool LISTED = false>
-__global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) void k_attend(const AttnArgs a) {
+template <int W, int P, int NR, bool ROWS, bool WIDE, bool LISTED = false, int WAVES = kAttnWaves>
+__global__ __launch_bounds__(64 * WAVES, W * NR * (P + 1) <= 16 ? 2 : 1) void k_attend(const AttnArgs a) {
     using S = Segments<W>;
     constexpr int D = 32 * W, NT = D / 16;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -483,7 +522,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
     const Seq q = seq_of(a.seqs, b);
     if (a.seqs.cu && split == 0 && blockIdx.y + 1 == a.row_blocks) leave_rest<P != 1, D>(a, q, h, b);
     const int rows = min(q.count, (int)a.seqs.each.value) * (int)a.group;
-    const int r0 = (ROWS ? (int)blockIdx.y * kAttnWaves + (int)wave : (int)blockIdx.y) * 16 * NR;
+    const int r0 = (ROWS ? (int)blockIdx.y * WAVES + (int)wave : (int)blockIdx.y) * 16 * NR;
     if (r0 >= rows) return;
 
     // what the rows see: [lo, hi) of each, and over all of them
@@ -498,17 +537,18 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
     uint16_t* list = nullptr;
     int listed = 0;
     uint32_t beyond = 0;
+    bool plain = false;
     if constexpr (LISTED) {
         extern __shared__ __align__(16) char lds[];
         who = reinterpret_cast<uint32_t*>(lds);
         list = reinterpret_cast<uint16_t*>(who + a.seqs.cols);
-        listed = list_pages(a, h, q, m0, m1, who, list, beyond);
+        listed = list_pages<WAVES>(a, h, q, m0, m1, who, list, beyond, plain);
         blk_lo = 0;
         blk_hi = ((listed << a.cache.page_shift) + 31) >> 5;
     }
     const int per = (blk_hi - blk_lo + (int)a.splits - 1) / (int)a.splits;
     const int blk_first = blk_lo + (int)split * per, blk_end = min(blk_first + per, blk_hi);
-    constexpr int step = ROWS ? 1 : kAttnWaves;
+    constexpr int step = ROWS ? 1 : WAVES;
     int blk = blk_first + (ROWS ? 0 : (int)wave);
 
     // Loads run ahead of their use: page numbers two blocks, a block's codes one.
@@ -517,7 +557,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
     ListedEntry of[2] = {};  // (what x was loaded by)
     const auto look_up = [&](int at) {
         if constexpr (LISTED)
-            return listed_entries<WIDE>(a, b, at, i, j, listed, who, list);
+            return listed_entries<WIDE>(a, b, at, i, j, listed, plain, who, list);
         else
             return entries<WIDE>(a, b, at, i, j);
     };
@@ -570,14 +610,14 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
         if constexpr (LISTED) {
             const ListedEntry& y = of[n];
             const uint32_t everyone = ~0u >> (31 - (m1 - m0));
-            const bool part = __any(y.who != everyone || y.at + 8 > full_hi);
+            const bool edge = __any(y.at + 8 > full_hi), part = edge || __any(y.who != everyone);
             bool unseen = false;  // (a row that has seen nothing yet: any block may be its first)
 #pragma unroll
             for (int t = 0; t < NR; ++t) {
                 st.hi[t] = y.who >> row_token[t] & 1 ? row_hi[t] : 0;
                 unseen |= row_out[t] >= 0 && st.mx[t] == -INFINITY;
             }
-            attend_block(st, x[n], a.scale, y.at, i, j, __any(unseen), part, hi_all);
+            attend_block<true>(st, x[n], a.scale, y.at, i, j, __any(unseen), part, hi_all, edge);
         } else {
             const bool part = blk * 32 < full_lo || blk * 32 + 32 > full_hi;
             // (a row that sees nothing of the wave's block before this one sees it from full_lo at the latest)
@@ -612,10 +652,12 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
         st.norm[t] = P == 1 ? sum_over_j(st.norm[t]) : st.sum[t];
     }
 
-    // the waves' results into wave 0's: 3 to 1 and 2 to 0, then 1 to 0
+    // the waves' results into wave 0's: the upper half's to the lower's, and so on
     if constexpr (!ROWS) {
-        __shared__ float stat[kAttnWaves][NR][16][3];
-        __shared__ f32x4 buf[2][NT][64];
+        __shared__ float stat[WAVES][NR][16][3];
+        __shared__ f32x4 own_buf[LISTED ? 1 : WAVES / 2][LISTED ? 1 : NT][LISTED ? 1 : 64];
+        extern __shared__ __align__(16) char lds[];  // (LISTED: in the lists' place, which every wave has read)
+        f32x4(*const buf)[NT][64] = LISTED ? reinterpret_cast<f32x4(*)[NT][64]>(lds) : reinterpret_cast<f32x4(*)[NT][64]>(own_buf);
         if (j == 0) {
 #pragma unroll
             for (int t = 0; t < NR; ++t) {
@@ -629,10 +671,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
         for (int t = 0; t < NR; ++t) {
             float top = -INFINITY, total = 0.f, norm = 0.f;
 #pragma unroll
-            for (int w = 0; w < kAttnWaves; ++w) top = fmaxf(top, stat[w][t][i][0]);
+            for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stat[w][t][i][0]);
             const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-            for (int w = 0; w < kAttnWaves; ++w) {
+            for (int w = 0; w < WAVES; ++w) {
                 const float weight = __builtin_amdgcn_exp2f(stat[w][t][i][0] - base);
                 total += stat[w][t][i][1] * weight;
                 norm += stat[w][t][i][2] * weight;
@@ -646,21 +688,17 @@ __global__ __launch_bounds__(64 * kAttnWaves, W * NR * (P + 1) <= 16 ? 2 : 1) vo
         }
 #pragma unroll
         for (int t = 0; t < NR; ++t) {
-            if (wave >= 2)
 #pragma unroll
-                for (int c = 0; c < NT; ++c) buf[wave - 2][c][lane] = st.o[t][c];
-            __syncthreads();
-            if (wave < 2)
+            for (int half = WAVES / 2; half; half /= 2) {
+                if (wave >= half && wave < 2 * half)
 #pragma unroll
-                for (int c = 0; c < NT; ++c) st.o[t][c] += buf[wave][c][lane];
-            if (wave == 1)
+                    for (int c = 0; c < NT; ++c) buf[wave - half][c][lane] = st.o[t][c];
+                __syncthreads();
+                if (wave < half)
 #pragma unroll
-                for (int c = 0; c < NT; ++c) buf[1][c][lane] = st.o[t][c];
-            __syncthreads();
-            if (wave == 0)
-#pragma unroll
-                for (int c = 0; c < NT; ++c) st.o[t][c] += buf[1][c][lane];
-            __syncthreads();
+                    for (int c = 0; c < NT; ++c) st.o[t][c] += buf[wave][c][lane];
+                if (half > 1 || t + 1 < NR) __syncthreads();
+            }
         }
         if (wave != 0) return;
     }

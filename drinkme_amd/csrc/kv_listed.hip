@@ -7,9 +7,13 @@ namespace {
 
 #include "kv_attention.h"
 
-// How a call is laid out: tiles of 16 rows a wave, and splits of each tile's pages.
+// Waves of a workgroup: eight for a call of one tile of rows to a sequence and head, where
+// two fit a SIMD (256 registers a lane); else four. A tile is 16 rows.
+constexpr int few_waves(int W, int P) { return W * (P + 1) <= 16 ? 8 : 4; }
+
+// How a call is laid out: splits of each tile's pages.
 struct Plan {
-    int tiles;
+    int waves;
     uint32_t tokens, row_blocks, splits;  // tokens: of a sequence, at most
     uint32_t listed;                      // columns that a tile may list, at most
 };
@@ -19,16 +23,17 @@ Plan plan_of(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t q_heads, int 
     const uint32_t group = q_heads / c->heads;
     p.tokens = s->cu ? std::min(s->max_tokens, s->total) : s->total / s->batch;
     const uint64_t rows = (uint64_t)p.tokens * group;
-    p.tiles = rows <= 16 || dtype == DMX_F32 ? 1 : 2;
-    const uint32_t a_tile = 16u * p.tiles, tile_tokens = std::min(p.tokens, 1 + (a_tile + group - 2) / group);
-    p.row_blocks = (uint32_t)((rows + a_tile - 1) / a_tile);
+    const uint32_t tile_tokens = std::min(p.tokens, 1 + (16 + group - 2) / group);
+    p.row_blocks = (uint32_t)((rows + 15) / 16);
     p.listed = (uint32_t)std::min<uint64_t>(s->table_cols, (uint64_t)tile_tokens * count);
     uint64_t length = (uint64_t)p.listed * c->page;
     if (max_length) length = std::min<uint64_t>(length, max_length);
-    // Splits to fill the CUs once, each of 128 tokens at least, a block of 32 a wave; up to 512 tokens none
-    // (k_attend's own rule, which its measurements are with)
+    // Splits to fill the CUs once, each of a block of 32 tokens a wave at least. Eight waves where
+    // half of the CUs have a workgroup without (us a step of 32 sequences, 32 pages of 64 each: 36,
+    // and 41 with four; one sequence of 16 pages, split in 8: 21, in 4 of eight waves 22).
     const uint64_t groups = (uint64_t)c->heads * s->batch * std::max(1u, p.row_blocks);
-    const uint64_t wanted = std::max<uint64_t>(1, 256 / groups), possible = length <= 512 ? 1 : length / 128;
+    p.waves = p.row_blocks == 1 && groups >= 128 ? few_waves(c->dim / 32, dtype == DMX_F32 ? 3 : 1) : 4;
+    const uint64_t wanted = std::max<uint64_t>(1, 256 / groups), possible = std::max<uint64_t>(1, length / (32 * p.waves));
     p.splits = (uint32_t)std::min<uint64_t>({wanted, possible, 64, 65535 / s->batch});
     return p;
 }
@@ -43,13 +48,16 @@ int check_listed(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t count, ch
     return 0;
 }
 
-template <int W, int P, int NR, bool WIDE>
+template <int W, int P, bool WIDE, int WAVES>
 int launch(dim3 grid, int lds, hipStream_t stream, const AttnArgs& a, char* err, size_t errn) {
-    // (the most that any call takes: 16384 columns' bits, and as many 16-bit entries)
+    // (the most that any call takes: 16384 columns' bits, and as many 16-bit entries; in their
+    // place half of the waves' results at the end)
     static std::atomic<uint64_t> allowed = {};
-    const auto kern = k_attend<W, P, NR, false, WIDE, true>;
+    constexpr int results = WAVES / 2 * 2 * W * 64 * (int)sizeof(f32x4);
+    static_assert(results <= 6 * DMX_KV_MAX_COLUMNS);
+    const auto kern = k_attend<W, P, 1, false, WIDE, true, WAVES>;
     if (allow_lds(reinterpret_cast<const void*>(kern), 6 * DMX_KV_MAX_COLUMNS, allowed, err, errn)) return 1;
-    hipLaunchKernelGGL(kern, grid, dim3(64 * kAttnWaves), lds, stream, a);
+    hipLaunchKernelGGL(kern, grid, dim3(64 * WAVES), std::max(lds, results), stream, a);
     return launch_check(err, errn, "kv attention launch");
 }
 
@@ -100,14 +108,16 @@ extern "C" int dmx_kv_attention_blocks(const dmx_kv_cache* cache, const dmx_kv_s
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const dim3 grid(cache->heads, p.row_blocks, seqs->batch * p.splits);
     const int lds = 4 * (int)seqs->table_cols + 2 * (int)p.listed;
-    const auto by_tiles = [&](auto w, auto wide) {
+    const auto by_type = [&](auto w, auto wide) {
         constexpr int W = decltype(w)::value;
         constexpr bool WIDE = decltype(wide)::value;
-        return dtype == DMX_F32 ? launch<W, 3, 1, WIDE>(grid, lds, st, a, err, errn)
-               : p.tiles == 1   ? launch<W, 1, 1, WIDE>(grid, lds, st, a, err, errn)
-                                : launch<W, 1, 2, WIDE>(grid, lds, st, a, err, errn);
+        const auto by_waves = [&](auto pieces) {
+            constexpr int P = decltype(pieces)::value;
+            return p.waves == 4 ? launch<W, P, WIDE, 4>(grid, lds, st, a, err, errn) : launch<W, P, WIDE, few_waves(W, P)>(grid, lds, st, a, err, errn);
+        };
+        return dtype == DMX_F32 ? by_waves(std::integral_constant<int, 3>{}) : by_waves(std::integral_constant<int, 1>{});
     };
-    const auto by_page = [&](auto w) { return cache->page >= 32 ? by_tiles(w, std::true_type{}) : by_tiles(w, std::false_type{}); };
+    const auto by_page = [&](auto w) { return cache->page >= 32 ? by_type(w, std::true_type{}) : by_type(w, std::false_type{}); };
     const int rc = cache->dim == 64    ? by_page(std::integral_constant<int, 2>{})
                    : cache->dim == 96  ? by_page(std::integral_constant<int, 3>{})
                    : cache->dim == 128 ? by_page(std::integral_constant<int, 4>{})

@@ -21,12 +21,12 @@ struct Summarize {
     Seqs seqs;
     int8_t* bounds;
     uint8_t* scales;
-    uint32_t run;  // new tokens a workgroup looks at
+    uint32_t run;  // new tokens a workgroup looks at, 64 at most
 };
 
 // A workgroup takes a head of the pages that begin among its new tokens (or in
-// which their sequence's first one lies): a thread a word of eight channels, of
-// every 256 / words-th token, then a channel.
+// which their sequence's first one lies), one after the other: a lane finds a token's, then a thread
+// takes a word of eight channels, of every 256 / words-th token, then a channel.
 template <int D>
 __global__ __launch_bounds__(256) void k_summarize(const Summarize a) {
     constexpr int words = D / 8, groups = 256 / words;
@@ -34,16 +34,23 @@ __global__ __launch_bounds__(256) void k_summarize(const Summarize a) {
     __shared__ float tops[4];
     const int x = threadIdx.x, w = x % words, g = x / words;
     const uint32_t h = blockIdx.y, heads = a.cache.heads, shift = a.cache.page_shift;
-    for (uint32_t t = blockIdx.x * a.run; t < min((blockIdx.x + 1) * a.run, a.seqs.total); ++t) {
+    const uint32_t t = blockIdx.x * a.run + (x & 63);
+    int start = -1, tokens = 0, number = 0;  // a page's first position, how many tokens it holds, which it is
+    if ((uint32_t)(x & 63) < a.run && t < a.seqs.total) {
         int p;
         const Slot at = slot_of_new(a.cache, a.seqs, t, p);
-        if (!at.ok) continue;
         const uint32_t b = seq_at(a.seqs, t);
         const Seq q = seq_of(a.seqs, b);
         const int in = p & ((1 << shift) - 1);
-        if (in && (int)t != q.token) continue;  // (not the first of its page, nor of its sequence's new ones)
-        const uint64_t page = a.seqs.table[(int64_t)b * a.seqs.cols + (p >> shift)];
-        const int count = min(1 << shift, q.length - (p - in));
+        if (at.ok && (!in || (int)t == q.token)) {  // (the first of its page, or of its sequence's new ones)
+            start = p - in;
+            tokens = min(1 << shift, q.length - start);
+            number = a.seqs.table[(int64_t)b * a.seqs.cols + (p >> shift)];
+        }
+    }
+    for (uint64_t found = __ballot(start >= 0); found; found &= found - 1) {
+        const int l = __builtin_ctzll(found), count = __builtin_amdgcn_readlane(tokens, l);
+        const uint64_t page = (uint32_t)__builtin_amdgcn_readlane(number, l);
         const uint64_t first = (page * heads + h) << shift;
         float hi[8], lo[8];
 #pragma unroll
@@ -201,6 +208,20 @@ __device__ __forceinline__ void load_tile(const Select& a, uint32_t h, uint32_t 
     x.scale = a.scales[at];
 }
 
+// The largest (MAX) or smallest over a wave, in every lane of it.
+template <bool MAX>
+__device__ __forceinline__ uint32_t over_lanes(uint32_t x) {
+    const auto of = [](uint32_t a, uint32_t b) { return MAX ? max(a, b) : min(a, b); };
+    x = of(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xB1, 0xF, 0xF, true));
+    x = of(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4E, 0xF, 0xF, true));
+    x = of(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x141, 0xF, 0xF, true));
+    x = of(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x140, 0xF, 0xF, true));
+    auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = of(r[0], r[1]);
+    r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return __builtin_amdgcn_readfirstlane(of(r[0], r[1]));
+}
+
 // A wave's choice: the count largest of keys [0, n) in LDS (more than count of them, 64 R
 // at most), ties to the first, their indexes to `out` in ascending order.
 template <int R>
@@ -208,8 +229,18 @@ __device__ __forceinline__ void choose(const uint32_t* keys, int n, int count, i
     uint32_t key[R];
 #pragma unroll
     for (int x = 0; x < R; ++x) key[x] = 64 * x + lane < n ? keys[64 * x + lane] : 0;
-    uint32_t at_least = 0;
-    for (uint32_t bit = 1u << 31; bit; bit >>= 1) {
+    // What all scores begin with, the threshold does: of 18 rounds or so that leaves ten.
+    uint32_t most = 0, least = ~0u;
+#pragma unroll
+    for (int x = 0; x < R; ++x) {
+        most = max(most, key[x] == kForced ? 0 : key[x]);
+        least = min(least, key[x] ? key[x] : ~0u);
+    }
+    most = over_lanes<true>(most);
+    least = over_lanes<false>(least);
+    const uint32_t differ = most ^ min(least, most);
+    uint32_t bit = differ ? 1u << (31 - __clz(differ)) : 0, at_least = bit ? most & ~(2 * bit - 1) : most;
+    for (; bit; bit >>= 1) {
         const uint32_t to = at_least | bit;
         int have = 0;
 #pragma unroll
@@ -298,13 +329,18 @@ __device__ __forceinline__ void choose_together(const uint32_t* keys, int n, int
     }
 }
 
-// The largest over the first `slots` of a row of 16 lanes' neighbours, a power of two: in every lane of them.
-__device__ __forceinline__ int max_over_slots(int x, uint32_t slots) {
-    if (slots > 1) x = max(x, __builtin_amdgcn_mov_dpp(x, 0xB1, 0xF, 0xF, true));   // lane ^ 1
-    if (slots > 2) x = max(x, __builtin_amdgcn_mov_dpp(x, 0x4E, 0xF, 0xF, true));   // lane ^ 2
-    if (slots > 4) x = max(x, __builtin_amdgcn_mov_dpp(x, 0x141, 0xF, 0xF, true));  // the other four of eight
-    if (slots > 8) x = max(x, __builtin_amdgcn_mov_dpp(x, 0x140, 0xF, 0xF, true));  // the other eight
-    return x;
+// The largest of each of x over `slots` neighbouring lanes, a power of two up to 16: in every one of them.
+template <int DPP, int N>
+__device__ __forceinline__ void max_with(int (&x)[N]) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = max(x[e], __builtin_amdgcn_mov_dpp(x[e], DPP, 0xF, 0xF, true));
+}
+template <int N>
+__device__ __forceinline__ void max_over_slots(int (&x)[N], uint32_t slots) {
+    if (slots > 1) max_with<0xB1>(x);   // lane ^ 1
+    if (slots > 2) max_with<0x4E>(x);   // lane ^ 2
+    if (slots > 4) max_with<0x141>(x);  // the other four of eight
+    if (slots > 8) max_with<0x140>(x);  // the other eight
 }
 
 // Single tokens: a workgroup to a token and head. A wave takes tiles of 16 pages, the next
@@ -314,8 +350,9 @@ __global__ __launch_bounds__(64 * WAVES) void k_select(const Select a) {
     constexpr int chunks = D / 32;
     extern __shared__ __align__(16) uint32_t keys[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, j = lane >> 4;
-    const uint32_t heads = a.cache.heads, t = blockIdx.x / heads, h = blockIdx.x - t * heads;
-    int32_t* out = a.blocks + (int64_t)blockIdx.x * a.count;
+    // (neighbours, which different XCDs run, are tokens: a head's summaries alone would meet in two of an L2's 16 channels)
+    const uint32_t heads = a.cache.heads, h = blockIdx.x / a.seqs.total, t = blockIdx.x - h * a.seqs.total;
+    int32_t* out = a.blocks + ((int64_t)t * heads + h) * a.count;
 
     const uint32_t b = seq_at(a.seqs, t);
     const Seq q = seq_of(a.seqs, b);
@@ -359,12 +396,11 @@ __global__ __launch_bounds__(64 * WAVES) void k_select(const Select a) {
             i32x4 s = {0, 0, 0, 0};
 #pragma unroll
             for (int c = 0; c < chunks; ++c) s = __builtin_amdgcn_mfma_i32_16x16x64_i8(y.bounds[c], qf[c], s, 0, 0, 0);
-            int best = 0;  // of page 4 j + (i & 3), over the lanes of a row of results
+            int v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int v = max_over_slots(r < a.group ? s[e] : -(1 << 30), 16);
-                if ((i & 3) == e) best = v;
-            }
+            for (int e = 0; e < 4; ++e) v[e] = r < a.group ? s[e] : -(1 << 30);
+            max_over_slots(v, 16);
+            const int best = i & 2 ? (i & 1 ? v[3] : v[2]) : (i & 1 ? v[1] : v[0]);  // of page 4 j + (i & 3)
             const int c = 16 * tile + i;
             if (i >> 2 == j && c < n) {
                 uint32_t key = y.ok ? key_of(best, y.scale) : kLost;
@@ -393,18 +429,20 @@ __global__ __launch_bounds__(64 * WAVES) void k_select(const Select a) {
     }
 }
 
-// Prompts: a workgroup of four waves to a head and up to 16 tokens in a row, which share
-// the reading of their sequence's summaries: 64 query rows (`slots` to a token, a power of two) meet a
-// tile of pages. Then each wave chooses for a quarter of the tokens.
+// Prompts: a workgroup to a head and up to 16 tokens in a row, which share the reading of
+// their sequence's summaries: 64 query rows (`slots` to a token, a power of two), four tiles that a wave
+// each made whole numbers of, meet a tile of pages. Then the waves choose for the tokens in turn.
+constexpr int select_waves(int D) { return 4; }  // (in 128 and 256 registers a lane)
 template <bool F32, int D>
-__global__ __launch_bounds__(256, 2) void k_select_tokens(const Select a) {
-    constexpr int chunks = D / 32;
-    extern __shared__ __align__(16) uint32_t keys[];  // [tokens][stride]
+__global__ __launch_bounds__(64 * select_waves(D), 2) void k_select_tokens(const Select a) {
+    constexpr int chunks = D / 32, WAVES = select_waves(D);
+    extern __shared__ __align__(16) uint32_t keys[];  // [tokens][stride]; before them, there, the queries: [4][chunks][64]
+    i32x4* const rows = reinterpret_cast<i32x4*>(keys);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, j = lane >> 4;
-    const uint32_t heads = a.cache.heads, h = blockIdx.x, slot = i & (a.slots - 1), per = 16 / a.slots;  // tokens a tile of rows
+    const uint32_t heads = a.cache.heads, h = blockIdx.y, slot = i & (a.slots - 1), per = 16 / a.slots;  // tokens a tile of rows
     const int shift = a.cache.page_shift, count = a.count, row_tiles = (int)((a.tokens * a.slots + 15) / 16);
-    const int t_end = (int)min(blockIdx.y * a.tokens + a.tokens, a.seqs.total);
-    int t0 = (int)(blockIdx.y * a.tokens);
+    const int t_end = (int)min(blockIdx.x * a.tokens + a.tokens, a.seqs.total);
+    int t0 = (int)(blockIdx.x * a.tokens);
     while (t0 < t_end) {  // (a turn for each sequence)
         const uint32_t b = seq_at(a.seqs, t0);
         const Seq q = seq_of(a.seqs, b);
@@ -417,11 +455,12 @@ __global__ __launch_bounds__(256, 2) void k_select_tokens(const Select a) {
         };
         const int most = columns_of(t1 - 1);
         if (most > count) {
-            i32x4 qf[4][chunks];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const uint32_t token = first + x * per + i / a.slots;
-                const bool mine = x < row_tiles && (int)token < t1 && slot < a.group;
+            const int tiles = (most + 15) / 16;
+            const auto page_at = [&](int tile) { return (uint32_t)a.seqs.table[(int64_t)b * a.seqs.cols + min(16 * tile + i, most - 1)]; };
+            uint32_t page = page_at(min(wave, tiles - 1));
+            if (wave < row_tiles) {
+                const uint32_t token = first + wave * per + i / a.slots;
+                const bool mine = (int)token < t1 && slot < a.group;
                 float y[chunks][16] = {};
                 uint32_t top = 0;
                 if (mine)
@@ -430,58 +469,70 @@ __global__ __launch_bounds__(256, 2) void k_select_tokens(const Select a) {
                         load16<F32>(a.q, token * a.q_token + ((int64_t)h * a.group + slot) * a.q_head + Piece<D>(c, j).channel, y[c]);
                         top = largest(y[c], top);
                     }
-                top = (uint32_t)max_over_slots((int)top, a.slots);
-                top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+                int of[1] = {(int)top};
+                max_over_slots(of, a.slots);
+                top = max((uint32_t)of[0], (uint32_t)__shfl_xor(of[0], 16));
                 top = max(top, (uint32_t)__shfl_xor((int)top, 32));
                 const float factor = factor_of(top);
 #pragma unroll
-                for (int c = 0; c < chunks; ++c) qf[x][c] = whole(y[c], factor, Piece<D>(c, j).negative);
+                for (int c = 0; c < chunks; ++c) rows[(wave * chunks + c) * 64 + lane] = whole(y[c], factor, Piece<D>(c, j).negative);
             }
-            const int tiles = (most + 15) / 16;
-            const auto page_at = [&](int tile) { return (uint32_t)a.seqs.table[(int64_t)b * a.seqs.cols + min(16 * tile + i, most - 1)]; };
-            const auto work = [&](int tile, const PageTile<D>& y) {
-                // of the four pages whose results this lane holds
-                int scale[4];
-                const int packed = y.ok ? y.scale : -1;
+            __syncthreads();
+            i32x4 qf[4][chunks];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) scale[e] = __shfl(packed, 4 * j + e);
+            for (int y = 0; y < 4; ++y)
+#pragma unroll
+                for (int c = 0; c < chunks; ++c) qf[y][c] = y < row_tiles ? rows[(y * chunks + c) * 64 + lane] : i32x4{0, 0, 0, 0};
+            __syncthreads();
+            int seen[4];  // columns of the lane's token in each tile of rows, -1: no token
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const int token = first + y * per + i / a.slots;
+                seen[y] = token < t1 ? columns_of(token) : -1;
+            }
+            uint32_t* const mine = keys + i / a.slots * a.stride;
+            const auto key = [&](int score, int scale, int c, int n) {
+                return c < (int)a.first || c >= n - (int)a.last ? kForced : scale < 0 ? kLost : key_of(score, scale);
+            };
+            const auto work = [&](int tile, const PageTile<D>& y) {
+                const int scale = y.ok ? y.scale : -1, c = 16 * tile + 4 * j;
+                const int own = 4 * j + (i & 3);  // (a lane's page of the four whose results it holds)
+                int of[4];
+                if (a.slots >= 4)
+                    of[0] = __shfl(scale, own);
+                else
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) of[e] = __shfl(scale, 4 * j + e);
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     if (x >= row_tiles) break;
                     i32x4 s = {0, 0, 0, 0};
 #pragma unroll
                     for (int c = 0; c < chunks; ++c) s = __builtin_amdgcn_mfma_i32_16x16x64_i8(y.bounds[c], qf[x][c], s, 0, 0, 0);
+                    int v[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[e] = max_over_slots(slot < a.group ? s[e] : -(1 << 30), a.slots);
-                    const int token = x * per + i / a.slots;
-                    if (slot || first + token >= t1) continue;
-                    const int n = columns_of(first + token), c = 16 * tile + 4 * j;
-                    uint4 key;
-                    uint32_t* k = &key.x;
+                    for (int e = 0; e < 4; ++e) v[e] = slot < a.group ? s[e] : -(1 << 30);
+                    max_over_slots(v, a.slots);
+                    if (seen[x] < 0) continue;
+                    uint32_t* const to = mine + x * per * a.stride;  // (what goes past `seen` is not read)
+                    if (a.slots >= 4) {  // a page a lane
+                        if (slot < 4) to[16 * tile + own] = key(i & 2 ? (i & 1 ? v[3] : v[2]) : (i & 1 ? v[1] : v[0]), of[0], 16 * tile + own, seen[x]);
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        k[e] = scale[e] < 0 ? kLost : key_of(s[e], scale[e]);
-                        if (c + e < (int)a.first || c + e >= n - (int)a.last) k[e] = kForced;
+                        for (int e = 0; e < 4; ++e)
+                            if (slot == 0) to[c + e] = key(v[e], of[e], c + e, seen[x]);
                     }
-                    *reinterpret_cast<uint4*>(keys + token * a.stride + c) = key;  // (past n: not read)
                 }
             };
-            PageTile<D> x[2];
-            uint32_t page = page_at(min(wave, tiles - 1));
-            load_tile(a, h, page, j, x[0]);
-            page = page_at(min(wave + 4, tiles - 1));
-            for (int tile = wave; tile < tiles; tile += 8) {
-                load_tile(a, h, page, j, x[1]);
-                page = page_at(min(tile + 8, tiles - 1));
-                work(tile, x[0]);
-                if (tile + 4 >= tiles) break;
-                load_tile(a, h, page, j, x[0]);
-                page = page_at(min(tile + 12, tiles - 1));
-                work(tile + 4, x[1]);
+            for (int tile = wave; tile < tiles; tile += WAVES) {
+                PageTile<D> y;
+                load_tile(a, h, page, j, y);
+                page = page_at(min(tile + WAVES, tiles - 1));
+                work(tile, y);
             }
             __syncthreads();
         }
-        for (int t = first + wave; t < t1; t += 4) {
+        for (int t = first + wave; t < t1; t += WAVES) {
             const int n = columns_of(t);
             int32_t* out = a.blocks + ((int64_t)t * heads + h) * count;
             const uint32_t* mine = keys + (t - first) * a.stride;
@@ -517,12 +568,10 @@ int launch_select(Select& a, uint32_t rows, hipStream_t stream, char* err, size_
         // (64 KB of keys: two workgroups a CU; a tile's last columns and a shift of the banks between tokens)
         a.stride = (cols + 15) / 16 * 16 + 4;
         while (a.tokens > 1 && a.tokens * a.stride * 4 > 66000) a.tokens /= 2;
-        if ((a.seqs.total + a.tokens - 1) / a.tokens > 65535) a.tokens = 0;
-    }
-    if (a.tokens) {
         const auto kern = k_select_tokens<F32, D>;
-        if (allow_lds(reinterpret_cast<const void*>(kern), 16 * 1024 * 5, allowed[2], err, errn)) return 1;
-        hipLaunchKernelGGL(kern, dim3(a.cache.heads, (a.seqs.total + a.tokens - 1) / a.tokens), dim3(256), 4 * a.tokens * a.stride, stream, a);
+        const uint32_t rows = 4 * (D / 32) * 64 * sizeof(i32x4), bytes = std::max(rows, 4 * a.tokens * a.stride);
+        if (allow_lds(reinterpret_cast<const void*>(kern), 66000, allowed[2], err, errn)) return 1;
+        hipLaunchKernelGGL(kern, dim3((a.seqs.total + a.tokens - 1) / a.tokens, a.cache.heads), dim3(64 * select_waves(D)), bytes, stream, a);
     } else {
         constexpr int most = D <= 128 ? 16 : 8;  // (128 registers a lane are few for larger heads)
         const bool many = cols > 1024;

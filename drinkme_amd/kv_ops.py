@@ -288,7 +288,7 @@ def _packed_axes(axes: tuple):
     if not 1 <= len(axes) <= 256 or any(type(a) is not int or not 0 <= a < 4 for a in axes):
         raise ValueError("rotary: axes are 1..256 numbers of 0..3 (rotary_axes)")
     x = _native.KvRotaryAxes()
-    x.count, x.angles, x.packed = max(axes) + 1, len(axes), (ct.addressof(x), len(axes))
+    x.count, x.angles, x.address = max(axes) + 1, len(axes), ct.addressof(x)
     for i, a in enumerate(axes):
         x.of[i // 16] |= a << (2 * (i % 16))
     return x
@@ -308,7 +308,8 @@ def rotary(q: torch.Tensor, k, positions: torch.Tensor, table: torch.Tensor, lay
     axes = None if axes is None else _packed_axes(tuple(axes))
     native = _native.calls()
     if native is not None:  # the plain case in one native call; None: anything else
-        outs = native.rotary(q, k, positions, table, LAYOUTS.get(layout, -1), _current(q), *(axes.packed if axes else (0, 0)))
+        outs = native.rotary(q, k, positions, table, LAYOUTS.get(layout, -1), _current(q), 0 if axes is None else axes.address,
+                             0 if axes is None else axes.angles)
         if outs is not None:
             return outs
     _no_gradient("rotary", q, k, table)
