@@ -5,8 +5,9 @@ tokens, then the verify rows of speculative decoding.
     python examples/attention_block.py [--steps N]
 
 q and o are radix-packed Linears, k and v raw ones (fewer than 1024 rows), all
-of synthetic weights. Each pass appends to the cache (keys rotated on the way)
-and attends to it; at the end the keys and values are read back from the cache
+of synthetic weights. Each pass hands out the pages that its tokens need, norms the heads of q and
+k, appends to the cache (keys rotated on the way), attends to it, and adds its output to the residual
+stream in front of the next block's norm; at the end the keys and values are read back from the cache
 and the last pass is compared with a plain attention over them in fp32."""
 
 from __future__ import annotations
@@ -19,15 +20,15 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
 import torch
 
-from drinkme_amd import kv_ops, radix_pack, swap, synth
+from drinkme_amd import kv_ops, norm_ops, radix_pack, swap, synth
 
 HIDDEN, HEADS, KV_HEADS, DIM = 2048, 16, 4, 128
 PAGE = 64
 
 
 class AttentionBlock(torch.nn.Module):
-    """q, k, v, rotary positions, cache, attention, o. `pages` are the cache's,
-    in all; a sequence takes the next free one when it outgrows its own."""
+    """q, k, v, their norms, rotary positions, cache, attention, o, residual and norm.
+    `pages` are the cache's, in all; a sequence takes a free one when it outgrows its own."""
 
     def __init__(self, sequences: int, pages: int, positions: int):
         super().__init__()
@@ -46,33 +47,29 @@ class AttentionBlock(torch.nn.Module):
         self.cache = kv_ops.new_cache(pages, PAGE, KV_HEADS, DIM)
         self.block_table = torch.full((sequences, -(-positions // PAGE)), -1, dtype=torch.int32, device="cuda")
         self.lengths = torch.zeros(sequences, dtype=torch.int32, device="cuda")
+        self.pool = kv_ops.new_pool(pages)
         self.held = [0] * sequences  # tokens, as the host counts them
-        self.used = 0
-
-    def grow(self, counts):
-        """Room for counts[b] more tokens of each sequence."""
-        for b, n in enumerate(counts):
-            for col in range(-(-self.held[b] // PAGE), -(-(self.held[b] + n) // PAGE)):
-                self.block_table[b, col] = self.used
-                self.used += 1
-            self.held[b] += n
-        self.lengths += torch.tensor(counts, dtype=torch.int32, device="cuda")
+        ones = lambda n: torch.ones(n, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+        self.q_norm, self.k_norm, self.next_norm = ones(DIM), ones(DIM), ones(HIDDEN)
 
     @torch.no_grad()
-    def forward(self, x, counts):
+    def forward(self, x, residual, counts):
         """x [T, HIDDEN], the new tokens of the sequences one after the other,
-        counts[b] of them each -> [T, HIDDEN]."""
-        self.grow(counts)
+        counts[b] of them each, and the residual stream [T, HIDDEN] -> both for the next block."""
+        new = torch.tensor(counts, dtype=torch.int32, device="cuda")
+        cu, _, _ = kv_ops.reserve(self.pool, self.block_table, self.lengths, PAGE, sum(counts), new=new)
+        self.held = [held + n for held, n in zip(self.held, counts)]
         even = len(set(counts)) == 1
-        ends = [sum(counts[:b]) for b in range(len(counts) + 1)]
-        cu = None if even else torch.tensor(ends, dtype=torch.int32, device="cuda")
-        q = self.q_proj(x).view(-1, HEADS, DIM)
+        cu = None if even else cu
+        q = norm_ops.norm(self.q_proj(x).view(-1, HEADS, DIM), self.q_norm)
         k, v = (proj(x).view(-1, KV_HEADS, DIM) for proj in (self.k_proj, self.v_proj))
+        k = norm_ops.norm(k, self.k_norm)
         q = kv_ops.append(self.cache, k, v, self.block_table, self.lengths, cu=cu, table=self.table, q=q)
         out = kv_ops.attention(q, self.cache, self.block_table, self.lengths, cu=cu,
                                max_tokens=None if even else max(counts), max_length=max(self.held))
         self.last = q, out  # (for the comparison below)
-        return self.o_proj(out.view(-1, HEADS * DIM))
+        residual, x = norm_ops.block_norm(self.o_proj(out.view(-1, HEADS * DIM)), residual, self.next_norm)
+        return x, residual
 
 
 def plain(block, counts):
@@ -98,7 +95,7 @@ def main(steps: int) -> float:
     worst = 0.0
     for name, counts, times in (("prompts", prompts, 1), ("tokens", [1, 1, 1], steps), ("verify", [4, 4, 4], 1)):
         for _ in range(times):
-            y = block(x(sum(counts)), counts)
+            y, _ = block(x(sum(counts)), x(sum(counts)), counts)
         want = plain(block, counts)
         off = ((block.last[1].float() - want).norm() / want.norm()).item()
         worst = max(worst, off)
