@@ -135,7 +135,8 @@ KV_SIGNATURES = {
     "dmx_kv_reserve": (_I, [_P, _P, _P, _P, _U32, _U32, _U32, _U32, _P, _P, _P, _P, _P, _SZ]),
     "dmx_kv_trim": (_I, [_P, _P, _P, _P, _U32, _U32, _U32, _P, _P, _SZ]),
     "dmx_kv_summarize": (_I, [_P, _P, _P, _P, _P, _SZ]),
-    "dmx_kv_select": (_I, [_P, _P, _P, _P, _I, _U32, _U32, _U32, _I, _P, _P, _P, _SZ]),
+    "dmx_kv_select_workspace": (_U64, [_P, _P, _U32]),
+    "dmx_kv_select": (_I, [_P, _P, _P, _P, _I, _U32, _U32, _U32, _I, _P, _P, _U64, _P, _P, _SZ]),
     "dmx_kv_attention_blocks_workspace": (_U64, [_P, _P, _U32, _I, _U32, _U32]),
     "dmx_kv_attention_blocks": (_I, [_P, _P, _P, _I, ct.c_float, _I, _P, _U32, _U32, _P, _P, _P, _U64, _P, _P, _SZ]),
 }

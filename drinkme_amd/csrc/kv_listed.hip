@@ -32,7 +32,7 @@ Plan plan_of(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t q_heads, int 
     // half of the CUs have a workgroup without (us a step of 32 sequences, 32 pages of 64 each: 36,
     // and 41 with four; one sequence of 16 pages, split in 8: 21, in 4 of eight waves 22).
     const uint64_t groups = (uint64_t)c->heads * s->batch * std::max(1u, p.row_blocks);
-    p.waves = p.row_blocks == 1 && groups >= 128 ? few_waves(c->dim / 32, dtype == DMX_F32 ? 3 : 1) : 4;
+    p.waves = p.row_blocks <= 4 && groups >= 128 ? few_waves(c->dim / 32, dtype == DMX_F32 ? 3 : 1) : 4;
     const uint64_t wanted = std::max<uint64_t>(1, 256 / groups), possible = std::max<uint64_t>(1, length / (32 * p.waves));
     p.splits = (uint32_t)std::min<uint64_t>({wanted, possible, 64, 65535 / s->batch});
     return p;

@@ -1,8 +1,9 @@
 // Summaries of the 4-bit cache's pages, and the pages that a cheap score selects
 // for each query (include/dmx_kv.h).
 //
-//   k_summarize   the bounds of the keys in a page
-//   k_select      scores of a token's pages, and the best of them
+//   k_summarize          the bounds of the keys in a page
+//   k_select, k_choose   scores of a token's pages, and the best of them
+//   k_select_tokens      the same for a prompt's tokens together
 #include "kv_common.h"
 
 namespace {
@@ -128,6 +129,8 @@ struct Select {
     uint32_t group, count, first, last, causal;
     int32_t* blocks;
     uint32_t tokens, slots, stride;  // k_select_tokens: tokens a workgroup, rows a token, keys a token
+    uint32_t* keys;  // k_select's SPLIT: [heads, total, columns]
+    uint32_t tiles;  // of a workgroup there
 };
 
 constexpr uint32_t kForced = 0xffffffffu, kLost = 1;  // keys above and below every score's; 0: no column
@@ -265,49 +268,79 @@ __device__ __forceinline__ void choose(const uint32_t* keys, int n, int count, i
     }
 }
 
-// As choose, by a workgroup of WAVES waves, a run of keys each, three bits of the
-// threshold at a time.
+// As choose, by a workgroup of WAVES waves, a run of keys each: eight bits of the threshold at a
+// time, by a histogram of the keys that share the bits above.
 template <int WAVES>
 __device__ __forceinline__ void choose_together(const uint32_t* keys, int n, int count, int32_t* out) {
-    constexpr int kRounds = 11;
-    __shared__ int counts[kRounds][8];
-    __shared__ int before[2][WAVES];
+    __shared__ int bins[256], before[2][WAVES], found[2];
+    __shared__ uint32_t ends[2][WAVES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int c = threadIdx.x; c < kRounds * 8; c += 64 * WAVES) (&counts[0][0])[c] = 0;
-    __syncthreads();
     const int rows = (n + 64 * WAVES - 1) / (64 * WAVES), c0 = wave * rows * 64 + lane;
     const auto key_at = [&](int x) { return c0 + 64 * x < n ? keys[c0 + 64 * x] : 0u; };
-    uint32_t at_least = 0;
-    for (int round = 0; round < kRounds; ++round) {
-        const int shift = 30 - 3 * round;
-        int have[8] = {};  // how many reach at_least + k << shift
-        for (int x = 0; x < rows; ++x) {
-            const uint32_t key = key_at(x);
+    uint32_t most = 0, least = ~0u;
+    int forced = 0;
+    for (int x = 0; x < rows; ++x) {
+        const uint32_t key = key_at(x);
+        most = max(most, key == kForced ? 0 : key);
+        least = min(least, key ? key : ~0u);
+        forced += __popcll(__ballot(key == kForced));
+    }
+    most = over_lanes<true>(most);
+    least = over_lanes<false>(least);
+    if (lane == 0) ends[0][wave] = most, ends[1][wave] = least, before[0][wave] = forced;
+    __syncthreads();
+    int need = count;  // of the keys that share the threshold's bits so far
 #pragma unroll
-            for (int k = 1; k < 8; ++k) {
-                const uint32_t to = at_least + ((uint32_t)(round ? k : min(k, 3)) << shift);
-                have[k] += __popcll(__ballot(key >= to));
+    for (int w = 0; w < WAVES; ++w) {
+        most = max(most, ends[0][w]);
+        least = min(least, ends[1][w]);
+        need -= before[0][w];
+    }
+    const uint32_t differ = most ^ min(least, most);
+    int top = differ ? 31 - __clz(differ) : -1;  // the highest bit not yet known
+    uint32_t at_least = top < 0 ? most : top == 31 ? 0 : most & ~((2u << top) - 1);
+    while (top >= 0 && need > 0) {
+        const int low = max(top - 7, 0);
+        for (int c = threadIdx.x; c < 256; c += 64 * WAVES) bins[c] = 0;
+        __syncthreads();
+        for (int x = 0; x < rows; ++x) {
+            const uint32_t key = key_at(x), apart = key ^ at_least;
+            if (key && key != kForced && (top == 31 || apart >> (top + 1) == 0)) atomicAdd(&bins[(key >> low) & 255 & ((2u << (top - low)) - 1)], 1);
+        }
+        __syncthreads();
+        if (wave == 0) {  // lane l: bins 4 l .. 4 l + 3; those above them, from the highest down
+            int mine[4], sum = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum += mine[e] = bins[4 * lane + e];
+            int upto = sum;  // with the lanes above
+#pragma unroll
+            for (int m = 1; m < 64; m *= 2) {
+                const int y = __shfl_down(upto, m);
+                if (lane + m < 64) upto += y;
+            }
+            int over = upto - sum;
+#pragma unroll
+            for (int e = 3; e >= 0; --e) {
+                if (over < need && over + mine[e] >= need) found[0] = 4 * lane + e, found[1] = over;
+                over += mine[e];
             }
         }
-        int mine = 0;
-#pragma unroll
-        for (int k = 1; k < 8; ++k)
-            if (lane == k && (round || k < 4)) mine = have[k];
-        if (mine) atomicAdd(&counts[round][lane], mine);
         __syncthreads();
-        int k = 0, reach = 0;
-#pragma unroll
-        for (int y = 1; y < 8; ++y)
-            if (counts[round][y] >= count) k = y, reach = counts[round][y];
-        at_least += (uint32_t)k << shift;
-        if (reach == count) break;
+        const int bin = found[0];
+        need -= found[1];
+        at_least |= (uint32_t)bin << low;
+        if (bins[bin] == need) break;  // (all of them)
+        top = low - 1;
+        __syncthreads();
     }
+    if (need <= 0) at_least = kForced;  // (forced ones alone)
     int above = 0, equal = 0;
     for (int x = 0; x < rows; ++x) {
         const uint32_t key = key_at(x);
         above += __popcll(__ballot(key > at_least));
         equal += __popcll(__ballot(key == at_least));
     }
+    __syncthreads();
     if (lane == 0) before[0][wave] = above, before[1][wave] = equal;
     __syncthreads();
     int fill = count, over = 0, level = 0;
@@ -329,6 +362,20 @@ __device__ __forceinline__ void choose_together(const uint32_t* keys, int n, int
     }
 }
 
+// The same for as few keys as a wave takes, by the workgroup's first.
+template <int WAVES>
+__device__ __forceinline__ void choose_any(const uint32_t* keys, int n, int count, int32_t* out) {
+    const int lane = threadIdx.x & 63;
+    if (n > 1024) {
+        choose_together<WAVES>(keys, n, count, out);
+    } else if (threadIdx.x < 64) {
+        n <= 128   ? choose<2>(keys, n, count, lane, out)
+        : n <= 256 ? choose<4>(keys, n, count, lane, out)
+        : n <= 512 ? choose<8>(keys, n, count, lane, out)
+                   : choose<16>(keys, n, count, lane, out);
+    }
+}
+
 // The largest of each of x over `slots` neighbouring lanes, a power of two up to 16: in every one of them.
 template <int DPP, int N>
 __device__ __forceinline__ void max_with(int (&x)[N]) {
@@ -343,34 +390,48 @@ __device__ __forceinline__ void max_over_slots(int (&x)[N], uint32_t slots) {
     if (slots > 8) max_with<0x140>(x);  // the other eight
 }
 
+// The columns that token t sees, and its sequence.
+__device__ __forceinline__ int columns_seen(const Select& a, uint32_t t, uint32_t& b) {
+    b = seq_at(a.seqs, t);
+    const Seq q = seq_of(a.seqs, b);
+    const int m = (int)t - q.token, p = a.causal ? q.first + m : q.length - 1;
+    const bool inside = (uint32_t)m < (uint32_t)q.count && q.first + m >= 0;
+    return inside ? min((p >> a.cache.page_shift) + 1, a.seqs.cols) : 0;
+}
+
+// Fewer columns than are asked for: all of them.
+__device__ __forceinline__ void list_all(int32_t* out, int n, int count) {
+    for (int c = threadIdx.x; c < count; c += blockDim.x) out[c] = c < n ? c : -1;
+}
+
 // Single tokens: a workgroup to a token and head. A wave takes tiles of 16 pages, the next
-// one's loads ahead of this one's product.
-template <bool F32, int D, int WAVES>
+// one's loads ahead of this one's product. SPLIT: a run of tiles to a workgroup, the keys go to
+// the workspace, and k_choose chooses.
+template <bool F32, int D, int WAVES, bool SPLIT>
 __global__ __launch_bounds__(64 * WAVES) void k_select(const Select a) {
     constexpr int chunks = D / 32;
-    extern __shared__ __align__(16) uint32_t keys[];
+    extern __shared__ __align__(16) uint32_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, j = lane >> 4;
     // (neighbours, which different XCDs run, are tokens: a head's summaries alone would meet in two of an L2's 16 channels)
     const uint32_t heads = a.cache.heads, h = blockIdx.x / a.seqs.total, t = blockIdx.x - h * a.seqs.total;
     int32_t* out = a.blocks + ((int64_t)t * heads + h) * a.count;
+    uint32_t* const keys = SPLIT ? a.keys + (int64_t)blockIdx.x * a.seqs.cols : lds;
 
-    const uint32_t b = seq_at(a.seqs, t);
-    const Seq q = seq_of(a.seqs, b);
-    const int m = (int)t - q.token, p = a.causal ? q.first + m : q.length - 1;
-    const bool inside = (uint32_t)m < (uint32_t)q.count && q.first + m >= 0;
-    const int n = inside ? min((p >> a.cache.page_shift) + 1, a.seqs.cols) : 0, count = a.count;
+    uint32_t b;
+    const int n = columns_seen(a, t, b), count = a.count;
     if (n <= count) {
-        for (int c = threadIdx.x; c < count; c += 64 * WAVES) out[c] = c < n ? c : -1;
+        if (!SPLIT) list_all(out, n, count);
         return;
     }
-    const int tiles = (n + 15) / 16;
+    const int first = SPLIT ? blockIdx.y * a.tiles : 0, tiles = SPLIT ? min(first + (int)a.tiles, (n + 15) / 16) : (n + 15) / 16;
+    if (SPLIT && first >= tiles) return;
     const auto page_at = [&](int tile) { return (uint32_t)a.seqs.table[(int64_t)b * a.seqs.cols + min(16 * tile + i, n - 1)]; };
     const auto load = [&](int r, int c, float (&x)[16]) {  // of query head r of the group
         load16<F32>(a.q, t * a.q_token + ((int64_t)h * a.group + r) * a.q_head + Piece<D>(c, j).channel, x);
     };
     for (uint32_t r0 = 0; r0 < a.group; r0 += 16) {
         PageTile<D> x[2];
-        uint32_t page = page_at(min(wave, tiles - 1));
+        uint32_t page = page_at(min(first + wave, tiles - 1));
         uint32_t top = 0;
         for (uint32_t r = i; r < a.group; r += 16)
 #pragma unroll
@@ -380,7 +441,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_select(const Select a) {
                 top = largest(y, top);
             }
         load_tile(a, h, page, j, x[0]);
-        page = page_at(min(wave + WAVES, tiles - 1));
+        page = page_at(min(first + wave + WAVES, tiles - 1));
 #pragma unroll
         for (int s = 32; s; s >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, s));
         const float factor = factor_of(top);
@@ -408,7 +469,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_select(const Select a) {
                 keys[c] = r0 ? max(keys[c], key) : key;
             }
         };
-        for (int tile = wave; tile < tiles; tile += 2 * WAVES) {
+        for (int tile = first + wave; tile < tiles; tile += 2 * WAVES) {
             load_tile(a, h, page, j, x[1]);  // (past the last tile: the last page again)
             page = page_at(min(tile + 2 * WAVES, tiles - 1));
             work(tile, x[0]);
@@ -418,15 +479,26 @@ __global__ __launch_bounds__(64 * WAVES) void k_select(const Select a) {
             work(tile + WAVES, x[1]);
         }
     }
-    __syncthreads();
-    if (n > 1024) {
-        choose_together<WAVES>(keys, n, count, out);
-    } else if (wave == 0) {
-        n <= 128   ? choose<2>(keys, n, count, lane, out)
-        : n <= 256 ? choose<4>(keys, n, count, lane, out)
-        : n <= 512 ? choose<8>(keys, n, count, lane, out)
-                   : choose<16>(keys, n, count, lane, out);
+    if constexpr (!SPLIT) {
+        __syncthreads();
+        choose_any<WAVES>(keys, n, count, out);
     }
+}
+
+__global__ __launch_bounds__(1024) void k_choose(const Select a) {
+    extern __shared__ __align__(16) uint32_t lds[];
+    const uint32_t h = blockIdx.x / a.seqs.total, t = blockIdx.x - h * a.seqs.total;
+    int32_t* out = a.blocks + ((int64_t)t * a.cache.heads + h) * a.count;
+    uint32_t b;
+    const int n = columns_seen(a, t, b), count = a.count;
+    if (n <= count) {
+        list_all(out, n, count);
+        return;
+    }
+    const uint32_t* from = a.keys + (int64_t)blockIdx.x * a.seqs.cols;
+    for (int c = threadIdx.x; c < n; c += 1024) lds[c] = from[c];
+    __syncthreads();
+    choose_any<16>(lds, n, count, out);
 }
 
 // Prompts: a workgroup to a head and up to 16 tokens in a row, which share the reading of
@@ -560,9 +632,35 @@ int check_summaries(const dmx_kv_summaries* s, char* err, size_t errn) {
 
 constexpr uint32_t kTokenColumns = 4096;  // of k_select_tokens, at most: 64 keys a lane
 
+// How a call is laid out: prompts' tokens together (tokens > 0), a workgroup to a
+// token and head, or several (tiles > 0).
+struct Plan {
+    uint32_t tokens, slots, tiles;
+};
+
+Plan plan_of(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t q_heads) {
+    Plan p = {0, 1, 0};
+    while (p.slots < q_heads / c->heads) p.slots *= 2;
+    // Tokens of a prompt share their sequence's summaries where there are eight or more to a sequence,
+    // and keys and rows fit.
+    if (s->total / s->batch >= 8 && s->table_cols <= kTokenColumns && p.slots <= 16) {
+        p.tokens = std::min(16u, 64 / p.slots);
+        return p;
+    }
+    // Few tokens over many columns: workgroups of four waves, a tile of 16 columns a wave or more, to
+    // fill the CUs, and a second launch that chooses. (us, 8 heads of 128: see k_choose)
+    const uint64_t rows = (uint64_t)s->total * c->heads, tiles = (s->table_cols + 15) / 16;
+    if (rows < 128 && s->table_cols > 1024) p.tiles = (uint32_t)std::max<uint64_t>(4, (tiles * rows + 255) / 256);
+    return p;
+}
+
+uint64_t workspace_of(const Plan& p, const dmx_kv_cache* c, const dmx_kv_seqs* s) {
+    return p.tiles ? 4ull * c->heads * s->total * s->table_cols : 0;
+}
+
 template <bool F32, int D>
 int launch_select(Select& a, uint32_t rows, hipStream_t stream, char* err, size_t errn) {
-    static std::atomic<uint64_t> allowed[3] = {};
+    static std::atomic<uint64_t> allowed[4] = {};
     const uint32_t cols = a.seqs.cols;
     if (a.tokens) {
         // (64 KB of keys: two workgroups a CU; a tile's last columns and a shift of the banks between tokens)
@@ -572,10 +670,15 @@ int launch_select(Select& a, uint32_t rows, hipStream_t stream, char* err, size_
         const uint32_t rows = 4 * (D / 32) * 64 * sizeof(i32x4), bytes = std::max(rows, 4 * a.tokens * a.stride);
         if (allow_lds(reinterpret_cast<const void*>(kern), 66000, allowed[2], err, errn)) return 1;
         hipLaunchKernelGGL(kern, dim3((a.seqs.total + a.tokens - 1) / a.tokens, a.cache.heads), dim3(64 * select_waves(D)), bytes, stream, a);
+    } else if (a.tiles) {
+        hipLaunchKernelGGL((k_select<F32, D, 4, true>), dim3(rows, ((cols + 15) / 16 + a.tiles - 1) / a.tiles), dim3(256), 0, stream, a);
+        if (launch_check(err, errn, "kv score launch")) return 1;
+        if (allow_lds(reinterpret_cast<const void*>(k_choose), 4 * DMX_KV_MAX_COLUMNS, allowed[3], err, errn)) return 1;
+        hipLaunchKernelGGL(k_choose, dim3(rows), dim3(1024), 4 * cols, stream, a);
     } else {
         constexpr int most = D <= 128 ? 16 : 8;  // (128 registers a lane are few for larger heads)
         const bool many = cols > 1024;
-        const auto kern = many ? k_select<F32, D, most> : k_select<F32, D, 8>;
+        const auto kern = many ? k_select<F32, D, most, false> : k_select<F32, D, 8, false>;
         if (allow_lds(reinterpret_cast<const void*>(kern), 4 * DMX_KV_MAX_COLUMNS, allowed[many], err, errn)) return 1;
         hipLaunchKernelGGL(kern, dim3(rows), dim3(many ? 64 * most : 512), 4 * cols, stream, a);
     }
@@ -603,9 +706,16 @@ extern "C" int dmx_kv_summarize(const dmx_kv_cache* cache, const dmx_kv_summarie
     return launch_check(err, errn, "kv summarize launch");
 }
 
+extern "C" uint64_t dmx_kv_select_workspace(const dmx_kv_cache* cache, const dmx_kv_seqs* seqs, uint32_t q_heads) {
+    if (check_cache(cache, nullptr, 0) || check_seqs(cache, seqs, nullptr, 0) || seqs->table_cols > DMX_KV_MAX_COLUMNS || q_heads == 0 ||
+        q_heads % cache->heads)
+        return 0;
+    return workspace_of(plan_of(cache, seqs, q_heads), cache, seqs);
+}
+
 extern "C" int dmx_kv_select(const dmx_kv_cache* cache, const dmx_kv_summaries* summaries, const dmx_kv_seqs* seqs,
                              const dmx_rows* q, int dtype, uint32_t count, uint32_t first, uint32_t last, int causal,
-                             int32_t* blocks, void* stream, char* err, size_t errn) {
+                             int32_t* blocks, void* workspace, uint64_t workspace_bytes, void* stream, char* err, size_t errn) {
     if (check_cache(cache, err, errn) || check_seqs(cache, seqs, err, errn) || check_dtype(dtype, err, errn) ||
         check_summaries(summaries, err, errn))
         return 1;
@@ -627,11 +737,11 @@ extern "C" int dmx_kv_select(const dmx_kv_cache* cache, const dmx_kv_summaries* 
     a.group = q->heads / cache->heads;
     a.count = count, a.first = first, a.last = last, a.causal = causal != 0;
     a.blocks = blocks;
-    a.slots = 1;
-    // Tokens of a prompt share their sequence's summaries where there are eight or more to a sequence, and
-    // keys and rows fit.
-    while (a.slots < a.group) a.slots *= 2;
-    if (seqs->total / seqs->batch >= 8 && seqs->table_cols <= kTokenColumns && a.slots <= 16) a.tokens = std::min(16u, 64 / a.slots);
+    const Plan p = plan_of(cache, seqs, q->heads);
+    if (workspace_bytes < workspace_of(p, cache, seqs) || (p.tiles && (!workspace || !aligned(workspace, 16))))
+        return fail(err, errn, "workspace missing, short or not 16-byte aligned");
+    a.tokens = p.tokens, a.slots = p.slots, a.tiles = p.tiles;
+    a.keys = static_cast<uint32_t*>(workspace);
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const auto by_type = [&](auto d) {
         constexpr int D = decltype(d)::value;

@@ -45,39 +45,67 @@ __device__ __forceinline__ float sum_of_row(float x, float* part) {
     return x;
 }
 
-// Eight channels from `at` of a row of vectors; past `dim` (whole rows of eight: VEC) 0.
-template <bool VEC>
+// load8 and store8 at any address: the machine takes 16 bytes wherever they begin, so that a
+// view's rows go the way of dense ones, and sum in their order.
+template <bool F32>
+__device__ __forceinline__ void load8_anywhere(const void* base, int64_t at, float (&x)[8]) {
+    if constexpr (F32) {
+        __builtin_memcpy(x, static_cast<const float*>(base) + at, 32);
+    } else {
+        uint32_t w[4];
+        __builtin_memcpy(w, static_cast<const uint16_t*>(base) + at, 16);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            x[2 * n] = __uint_as_float(w[n] << 16);
+            x[2 * n + 1] = __uint_as_float(w[n] & 0xffff0000u);
+        }
+    }
+}
+template <bool F32>
+__device__ __forceinline__ void store8_anywhere(void* base, int64_t at, const float (&x)[8]) {
+    if constexpr (F32) {
+        __builtin_memcpy(static_cast<float*>(base) + at, x, 32);
+    } else {
+        typedef __bf16 eight __attribute__((ext_vector_type(8)));
+        const eight y = {(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3], (__bf16)x[4], (__bf16)x[5], (__bf16)x[6], (__bf16)x[7]};
+        __builtin_memcpy(static_cast<uint16_t*>(base) + at, &y, 16);
+    }
+}
+
+// Eight channels of a row of vectors, adjacent ones from `at` (STEP 1: whole rows of eight, 16 bytes
+// a load), or STEP apart, so that lanes side by side read and write side by side; past `dim` 0.
+template <uint32_t STEP>
 __device__ __forceinline__ void vector8(const Vectors& v, int64_t row, uint32_t at, uint32_t dim, float (&x)[8]) {
     const int64_t from = row * dim + at;
-    if constexpr (VEC) {
+    if constexpr (STEP == 1) {
         if (v.f32)
-            load8<true>(v.at, from, x);
+            load8_anywhere<true>(v.at, from, x);
         else
-            load8<false>(v.at, from, x);
+            load8_anywhere<false>(v.at, from, x);
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = at + e >= dim ? 0.f : v.f32 ? load1<true>(v.at, from + e) : load1<false>(v.at, from + e);
+        for (int e = 0; e < 8; ++e) x[e] = at + e * STEP >= dim ? 0.f : v.f32 ? load1<true>(v.at, from + e * STEP) : load1<false>(v.at, from + e * STEP);
     }
 }
 
-template <bool F32, bool VEC>
+template <bool F32, uint32_t STEP>
 __device__ __forceinline__ void row8(const void* base, int64_t row, uint32_t at, uint32_t dim, float (&x)[8]) {
-    if constexpr (VEC) {
-        load8<F32>(base, row + at, x);
+    if constexpr (STEP == 1) {
+        load8_anywhere<F32>(base, row + at, x);
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = at + e >= dim ? 0.f : load1<F32>(base, row + at + e);
+        for (int e = 0; e < 8; ++e) x[e] = at + e * STEP >= dim ? 0.f : load1<F32>(base, row + at + e * STEP);
     }
 }
 
-template <bool F32, bool VEC>
+template <bool F32, uint32_t STEP>
 __device__ __forceinline__ void put8(void* base, int64_t row, uint32_t at, uint32_t dim, const float (&x)[8]) {
-    if constexpr (VEC) {
-        store8<F32>(base, row + at, x);
+    if constexpr (STEP == 1) {
+        store8_anywhere<F32>(base, row + at, x);
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-            if (at + e < dim) store1<F32>(base, row + at + e, x[e]);
+            if (at + e * STEP < dim) store1<F32>(base, row + at + e * STEP, x[e]);
     }
 }
 
@@ -102,7 +130,8 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_norm(const Norm a
     const uint32_t lane = threadIdx.x % LANES;
     const uint32_t row = LANES < 256 ? blockIdx.x * (256 / LANES) + threadIdx.x / LANES : blockIdx.x;
     if (row >= a.rows) return;
-    const auto channel = [&](int n) { return 8 * (n * LANES + lane); };
+    constexpr uint32_t STEP = VEC ? 1 : LANES;
+    const auto channel = [&](int n) { return 8 * n * LANES + (VEC ? 8 : 1) * lane; };
 
     float v[N][8], r[N][8];
     uint32_t head = row;
@@ -119,8 +148,8 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_norm(const Norm a
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[n][e] = r[n][e] = 0.f;
         if (c >= a.dim) continue;
-        row8<F32X, VEC>(a.x.at, from, c, a.dim, v[n]);
-        if constexpr (BLOCK) row8<F32R, VEC>(a.residual, row * a.residual_stride, c, a.dim, r[n]);
+        row8<F32X, STEP>(a.x.at, from, c, a.dim, v[n]);
+        if constexpr (BLOCK) row8<F32R, STEP>(a.residual, row * a.residual_stride, c, a.dim, r[n]);
     }
 
     // x less its mean (layer norm), and the factor that gives it a norm of 1
@@ -135,7 +164,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_norm(const Norm a
 #pragma unroll
             for (int n = 0; n < N; ++n)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[n][e] = channel(n) + e < a.dim ? x[n][e] - mean : 0.f;
+                for (int e = 0; e < 8; ++e) x[n][e] = channel(n) + e * STEP < a.dim ? x[n][e] - mean : 0.f;
         }
         float sum = 0.f;
 #pragma unroll
@@ -152,7 +181,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_norm(const Norm a
             for (int n = 0; n < N; ++n) {
                 if (channel(n) >= a.dim) continue;
                 float w[8];
-                vector8<VEC>(a.post, 0, channel(n), a.dim, w);
+                vector8<STEP>(a.post, 0, channel(n), a.dim, w);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[n][e] *= inv * (w[e] + a.offset);
             }
@@ -163,13 +192,13 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_norm(const Norm a
             if (channel(n) >= a.dim) continue;
             if (a.gate.at) {
                 float g[8];
-                vector8<VEC>(a.gate, gate, channel(n), a.dim, g);
+                vector8<STEP>(a.gate, gate, channel(n), a.dim, g);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[n][e] *= g[e];
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) r[n][e] = fmaf(a.factor, v[n][e], r[n][e]);
-            put8<F32R, VEC>(a.residual_out, (int64_t)row * a.dim, channel(n), a.dim, r[n]);
+            put8<F32R, STEP>(a.residual_out, (int64_t)row * a.dim, channel(n), a.dim, r[n]);
         }
     }
     float(&x)[N][8] = BLOCK ? r : v;
@@ -183,23 +212,23 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_norm(const Norm a
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[n][e] *= inv;
         if (a.weight.at) {
-            vector8<VEC>(a.weight, 0, c, a.dim, w);
+            vector8<STEP>(a.weight, 0, c, a.dim, w);
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[n][e] *= w[e] + a.offset;
         }
         if (a.bias.at) {
-            vector8<VEC>(a.bias, 0, c, a.dim, w);
+            vector8<STEP>(a.bias, 0, c, a.dim, w);
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[n][e] += w[e];
         }
         if (BLOCK && a.scale.at) {
             float s[8];
-            vector8<VEC>(a.scale, scale, c, a.dim, s);
-            vector8<VEC>(a.shift, scale, c, a.dim, w);
+            vector8<STEP>(a.scale, scale, c, a.dim, s);
+            vector8<STEP>(a.shift, scale, c, a.dim, w);
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[n][e] = fmaf(x[n][e], 1.f + s[e], w[e]);
         }
-        put8<F32X, VEC>(a.out, (int64_t)row * a.dim, c, a.dim, x[n]);
+        put8<F32X, STEP>(a.out, (int64_t)row * a.dim, c, a.dim, x[n]);
     }
 }
 
@@ -251,16 +280,6 @@ int form_of(const dmx_norm_form* f, bool block, uint32_t rows, uint32_t dim, Nor
     return 0;
 }
 
-// Whether every row begins on 16 bytes and is whole runs of eight channels.
-bool wide(const Norm& a, bool f32x, bool f32r) {
-    const auto row = [](const void* p, int64_t stride, bool f32) { return aligned(p, 16) && stride % (f32 ? 4 : 8) == 0; };
-    if (a.dim % 8 || !row(a.x.at, a.x.token, f32x) || !row(a.x.at, a.x.head, f32x) || !aligned(a.out, 16)) return false;
-    if (a.residual && (!row(a.residual, a.residual_stride, f32r) || !aligned(a.residual_out, 16))) return false;
-    for (const Vectors* v : {&a.weight, &a.bias, &a.post, &a.gate, &a.scale, &a.shift})
-        if (!aligned(v->at, 16)) return false;
-    return true;
-}
-
 template <bool BLOCK, bool F32X, bool F32R, bool VEC>
 int launch(const Norm& a, hipStream_t stream, char* err, size_t errn) {
     const auto go = [&](auto lanes, auto runs) {
@@ -286,7 +305,7 @@ int launch(const Norm& a, hipStream_t stream, char* err, size_t errn) {
 
 template <bool BLOCK, bool F32X, bool F32R>
 int launch(const Norm& a, hipStream_t stream, char* err, size_t errn) {
-    return wide(a, F32X, F32R) ? launch<BLOCK, F32X, F32R, true>(a, stream, err, errn) : launch<BLOCK, F32X, F32R, false>(a, stream, err, errn);
+    return a.dim % 8 == 0 ? launch<BLOCK, F32X, F32R, true>(a, stream, err, errn) : launch<BLOCK, F32X, F32R, false>(a, stream, err, errn);
 }
 
 }  // namespace

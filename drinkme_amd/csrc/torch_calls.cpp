@@ -676,8 +676,12 @@ PyObject* select(PyObject*, PyObject* const* a, Py_ssize_t n) {
         pybind11::gil_scoped_release no_gil;
         const c10::DeviceGuard on(q->device());
         out = at::empty({q->size(0), (int64_t)c.heads, count}, at::TensorOptions().device(q->device()).dtype(at::kInt));
+        const uint64_t bytes = s.total ? dmx_kv_select_workspace(&c, &s, r.heads) : 0;
+        at::Tensor ws;
+        if (bytes) ws = at::empty({(int64_t)bytes}, at::TensorOptions().device(q->device()).dtype(at::kByte));
         st = dmx_kv_select(&c, &x, &s, &r, code(q->scalar_type()), (uint32_t)count, (uint32_t)first, (uint32_t)last, causal,
-                           static_cast<int32_t*>(out.mutable_data_ptr()), stream, err, sizeof err);
+                           static_cast<int32_t*>(out.mutable_data_ptr()), bytes ? ws.mutable_data_ptr() : nullptr, bytes, stream, err,
+                           sizeof err);
     }
     return st ? launch_failed("dmx_kv_select", err) : THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS

@@ -673,9 +673,12 @@ def select(q: torch.Tensor, cache: dict, summaries: dict, block_table: torch.Ten
     s, held = _seqs_of(block_table, lengths, cu, T, None, q.device, "select")
     _few_columns(block_table, "select")
     blocks = torch.empty((T, c.heads, count), dtype=torch.int32, device=q.device)
+    lib = _native.lib()
+    bytes_ = lib.dmx_kv_select_workspace(ct.byref(c), ct.byref(s), Hq) if T else 0
+    ws = torch.empty(bytes_, dtype=torch.uint8, device=q.device) if bytes_ else None
     err = _native.error_buffer()
     with torch.cuda.device(q.device):
-        st = _native.lib().dmx_kv_select(ct.byref(c), ct.byref(x), ct.byref(s), ct.byref(_rows(q)), _dtype_code(q.dtype, "select"),
-                                         count, first, last, causal, blocks.data_ptr(), _stream(q.device), err, len(err))
+        st = lib.dmx_kv_select(ct.byref(c), ct.byref(x), ct.byref(s), ct.byref(_rows(q)), _dtype_code(q.dtype, "select"), count, first,
+                               last, causal, blocks.data_ptr(), ws.data_ptr() if bytes_ else None, bytes_, _stream(q.device), err, len(err))
     _native.check(st, err, "dmx_kv_select")
     return blocks

@@ -208,11 +208,13 @@ int dmx_kv_summarize(const dmx_kv_cache* cache, const dmx_kv_summaries* summarie
  * largest : smallest): x the query in whole numbers (to the nearest, even) of the least power
  * of two, 2^-126 or more, that leaves none of these heads' over 127; values that are not finite
  * are 0. Sums are below 2^24 and compared as fp32. Tokens of no sequence list nothing. A block
- * table has at most DMX_KV_MAX_COLUMNS columns here. */
+ * table has at most DMX_KV_MAX_COLUMNS columns here. workspace: as dmx_kv_select_workspace says, 16-byte
+ * aligned device bytes, 0 for none. */
 #define DMX_KV_MAX_COLUMNS 16384
+uint64_t dmx_kv_select_workspace(const dmx_kv_cache* cache, const dmx_kv_seqs* seqs, uint32_t q_heads);
 int dmx_kv_select(const dmx_kv_cache* cache, const dmx_kv_summaries* summaries, const dmx_kv_seqs* seqs,
                   const dmx_rows* q, int dtype, uint32_t count, uint32_t first, uint32_t last, int causal,
-                  int32_t* blocks, void* stream, char* err, size_t errn);
+                  int32_t* blocks, void* workspace, uint64_t workspace_bytes, void* stream, char* err, size_t errn);
 
 /* As dmx_kv_attention without a window, over the listed columns alone: a query
  * of token t and cache head h sees of the positions that it would see there those in

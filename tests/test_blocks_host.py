@@ -113,10 +113,11 @@ def _summaries(**kw):
 def test_bad_caches_and_sequences_are_refused(cache, seqs, match):
     c = None if cache is None else _cache(**cache)
     s = None if seqs is None else _seqs(**seqs)
-    said = [_refused("dmx_kv_summarize", c, _summaries(), s), _refused("dmx_kv_select", c, _summaries(), s, _rows(), 0, 2, 1, 1, 1, FAKE),
+    said = [_refused("dmx_kv_summarize", c, _summaries(), s), _refused("dmx_kv_select", c, _summaries(), s, _rows(), 0, 2, 1, 1, 1, FAKE, None, 0),
             _refused("dmx_kv_attention_blocks", c, s, _rows(), 0, 1.0, 1, FAKE, 2, 0, FAKE, None, None, 0)]
     assert all(re.search(match, x) for x in said), said
-    assert _native.lib().dmx_kv_attention_blocks_workspace(ct.byref(c) if c else None, ct.byref(s) if s else None, 4, 0, 2, 0) == 0
+    c, s = ct.byref(c) if c else None, ct.byref(s) if s else None
+    assert _native.lib().dmx_kv_attention_blocks_workspace(c, s, 4, 0, 2, 0) == 0 == _native.lib().dmx_kv_select_workspace(c, s, 4)
 
 
 @cpu_only
@@ -125,10 +126,12 @@ def test_bad_caches_and_sequences_are_refused(cache, seqs, match):
     ({"summaries": _summaries(bounds=FAKE + 8)}, b"not 16-byte"), ({"q": None}, b"null queries"), ({"q": _rows(heads=3)}, b"query heads"),
     ({"dtype": 2}, b"dtype"), ({"count": 0}, b"no columns"), ({"count": 16385}, b"16384"), ({"first": 3}, b"more than count"),
     ({"first": 2 ** 32 - 1, "last": 2}, b"more than count"), ({"seqs": _seqs(table_cols=16385)}, b"16384"), ({"blocks": None}, b"lists"),
-    ({"q": _rows(at=None)}, b"null queries")])
+    ({"q": _rows(at=None)}, b"null queries"), ({"ws": None}, b"workspace"), ({"ws": FAKE + 8}, b"workspace"), ({"bytes": 64}, b"workspace")])
 def test_bad_selections_are_refused(change, match):
-    a = {"cache": _cache(), "summaries": _summaries(), "seqs": _seqs(), "q": _rows(), "dtype": 0, "count": 2, "first": 1, "last": 1,
-         "causal": 1, "blocks": FAKE}
+    a = {"cache": _cache(), "summaries": _summaries(), "seqs": _seqs(table_cols=4000), "q": _rows(), "dtype": 0, "count": 2, "first": 1,
+         "last": 1, "causal": 1, "blocks": FAKE, "ws": FAKE, "bytes": 1 << 30}
+    need = _native.lib().dmx_kv_select_workspace(ct.byref(a["cache"]), ct.byref(a["seqs"]), 2)
+    assert 64 < need < 1 << 30
     a.update(change)
     assert re.search(match, _refused("dmx_kv_select", *a.values()))
 
