@@ -1,14 +1,20 @@
 // The attention over listed pages of the 4-bit cache (include/dmx_kv.h):
 // kv_attention.h's k_attend, whose tiles walk the pages that any of their tokens
 // lists, and its join.
+//
+// A tile is 16 rows: with four query heads to a cache head, four tokens, whose lists
+// of 32 pages of 512 join to 65 where neighbours look for the same things (a chunk of 1024 tokens: 156 us,
+// the vector units 73% busy, decoding first; 32 rows, whose eight tokens' lists join to 97, take 217
+// beside 177 at the time). Decoding each block once for 64 rows, in LDS, took 345: too few waves to wait with.
+// A step of 32 sequences, 32 of up to 256 pages each, takes 19 us, 3.7 TB/s of the listed pages' codes.
 #include "kv_common.h"
 
 namespace {
 
 #include "kv_attention.h"
 
-// Waves of a workgroup: eight for a call of one tile of rows to a sequence and head, where
-// two fit a SIMD (256 registers a lane); else four. A tile is 16 rows.
+// Waves of a workgroup: eight for a call of few tiles of rows to a sequence and head, where
+// two fit a SIMD (256 registers a lane); else four.
 constexpr int few_waves(int W, int P) { return W * (P + 1) <= 16 ? 8 : 4; }
 
 // How a call is laid out: splits of each tile's pages.
@@ -29,8 +35,9 @@ Plan plan_of(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t q_heads, int 
     uint64_t length = (uint64_t)p.listed * c->page;
     if (max_length) length = std::min<uint64_t>(length, max_length);
     // Splits to fill the CUs once, each of a block of 32 tokens a wave at least. Eight waves where
-    // half of the CUs have a workgroup without (us a step of 32 sequences, 32 pages of 64 each: 36,
-    // and 41 with four; one sequence of 16 pages, split in 8: 21, in 4 of eight waves 22).
+    // half of the CUs have a workgroup without splits (us a step of 32 sequences, 32 pages of 64 each: 36,
+    // and 41 with four; 8 of 5 tokens 26 and 33; one sequence of 16 pages, split in 8: 21, in 4 of eight
+    // waves 22), and not for prompts (a chunk of 1024 tokens 235, and 177 with four).
     const uint64_t groups = (uint64_t)c->heads * s->batch * std::max(1u, p.row_blocks);
     p.waves = p.row_blocks <= 4 && groups >= 128 ? few_waves(c->dim / 32, dtype == DMX_F32 ? 3 : 1) : 4;
     const uint64_t wanted = std::max<uint64_t>(1, 256 / groups), possible = std::max<uint64_t>(1, length / (32 * p.waves));

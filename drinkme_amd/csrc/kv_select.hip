@@ -16,6 +16,9 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 // Every channel's largest and smallest key of a page bound its product with any
 // query there. They are exact (a code times its power of two is an fp32 number,
 // and neither depends on an order), and rounded outwards to 8 bits.
+//
+// Waits bound it: lengths, page number, codes, then three barriers: 4.8 us for the last pages of 32
+// sequences (8 heads of 128, 64 tokens a page), 7.5 for the 16 of a chunk of 1024 tokens.
 
 struct Summarize {
     Cache cache;
@@ -116,8 +119,9 @@ __global__ __launch_bounds__(256) void k_summarize(const Summarize a) {
 // to the lower column whatever computes them.
 //
 // The best `count` keys (a score's bits, ordered as numbers) are those from a
-// threshold on, found bit by bit from the top by counting: the largest that `count`
-// keys reach.
+// threshold on, the largest that `count` keys reach: found from the bits that all share
+// downwards, by counting, one bit at a time in a wave's registers or eight in a
+// workgroup's histogram.
 
 struct Select {
     Cache cache;  // (page numbers and sizes alone)
@@ -407,6 +411,9 @@ __device__ __forceinline__ void list_all(int32_t* out, int n, int count) {
 // Single tokens: a workgroup to a token and head. A wave takes tiles of 16 pages, the next
 // one's loads ahead of this one's product. SPLIT: a run of tiles to a workgroup, the keys go to
 // the workspace, and k_choose chooses.
+//
+// Waits bound it: lengths, page numbers, summaries in turn, then the choice. One token over 128 pages 7.1
+// us, 32 uneven sequences of up to 256 pages 9.2 (12.5 MB, 2.6 us at a copy's rate), eight heads of 128 each.
 template <bool F32, int D, int WAVES, bool SPLIT>
 __global__ __launch_bounds__(64 * WAVES) void k_select(const Select a) {
     constexpr int chunks = D / 32;
@@ -504,10 +511,14 @@ __global__ __launch_bounds__(1024) void k_choose(const Select a) {
 // Prompts: a workgroup to a head and up to 16 tokens in a row, which share the reading of
 // their sequence's summaries: 64 query rows (`slots` to a token, a power of two), four tiles that a wave
 // each made whole numbers of, meet a tile of pages. Then the waves choose for the tokens in turn.
-constexpr int select_waves(int D) { return 4; }  // (in 128 and 256 registers a lane)
+//
+// 1024 tokens of 32 query and 8 cache heads of 128 over 512 pages: 33 us, of which the products and
+// their keys take 6, the choices 14, queries and starts the rest; a workgroup to each token 158, eight waves
+// in 128 registers, some of them in scratch, 44, two tiles of rows 42.
+constexpr int kSelectWaves = 4;
 template <bool F32, int D>
-__global__ __launch_bounds__(64 * select_waves(D), 2) void k_select_tokens(const Select a) {
-    constexpr int chunks = D / 32, WAVES = select_waves(D);
+__global__ __launch_bounds__(64 * kSelectWaves, 2) void k_select_tokens(const Select a) {
+    constexpr int chunks = D / 32, WAVES = kSelectWaves;
     extern __shared__ __align__(16) uint32_t keys[];  // [tokens][stride]; before them, there, the queries: [4][chunks][64]
     i32x4* const rows = reinterpret_cast<i32x4*>(keys);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, j = lane >> 4;
@@ -648,9 +659,11 @@ Plan plan_of(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t q_heads) {
         return p;
     }
     // Few tokens over many columns: workgroups of four waves, a tile of 16 columns a wave or more, to
-    // fill the CUs, and a second launch that chooses. (us, 8 heads of 128: see k_choose)
+    // fill the CUs, and a second launch that chooses. us with one workgroup to a token and head, and so:
+    // 1 token over 2048 columns 32 and 12, over 8192 87 and 17, 8 over 1024 19.5 and 16, 4 over 512 12.5
+    // and 10.7, 1 over 313 both 9.4; 160 rows over 513 12.3 and 15.
     const uint64_t rows = (uint64_t)s->total * c->heads, tiles = (s->table_cols + 15) / 16;
-    if (rows < 128 && s->table_cols > 1024) p.tiles = (uint32_t)std::max<uint64_t>(4, (tiles * rows + 255) / 256);
+    if (rows <= 128 && s->table_cols > 512) p.tiles = (uint32_t)std::max<uint64_t>(4, (tiles * rows + 255) / 256);
     return p;
 }
 
@@ -669,7 +682,7 @@ int launch_select(Select& a, uint32_t rows, hipStream_t stream, char* err, size_
         const auto kern = k_select_tokens<F32, D>;
         const uint32_t rows = 4 * (D / 32) * 64 * sizeof(i32x4), bytes = std::max(rows, 4 * a.tokens * a.stride);
         if (allow_lds(reinterpret_cast<const void*>(kern), 66000, allowed[2], err, errn)) return 1;
-        hipLaunchKernelGGL(kern, dim3((a.seqs.total + a.tokens - 1) / a.tokens, a.cache.heads), dim3(64 * select_waves(D)), bytes, stream, a);
+        hipLaunchKernelGGL(kern, dim3((a.seqs.total + a.tokens - 1) / a.tokens, a.cache.heads), dim3(64 * kSelectWaves), bytes, stream, a);
     } else if (a.tiles) {
         hipLaunchKernelGGL((k_select<F32, D, 4, true>), dim3(rows, ((cols + 15) / 16 + a.tiles - 1) / a.tiles), dim3(256), 0, stream, a);
         if (launch_check(err, errn, "kv score launch")) return 1;

@@ -2,7 +2,11 @@
 //
 // A row stays in the registers of its lanes (16, a wave, or a workgroup, 8 N
 // channels a lane) from its read to its result, through as many sums over the row as
-// its form takes: one read of each input, one write of each output.
+// its form takes: one read of each input, one write of each output. Memory bounds it:
+// 8192 rows of 4096, norms before and after, fp32 residual, 403 MB in 79 us (5.1 TB/s, part of the reads
+// cached); 4084 of 1536 with layer norm, gate, scale and shift 50 MB in 12.6; the heads of 8192 x 40 x 128
+// 168 MB in 26. Rows of no whole eights go a value at a time: 8192 of 4095 82 us, 42 for 4096 (142 with
+// a lane's eight values side by side). One row takes 3.5 us, its launch.
 #include "dmx_norm.h"
 
 #include "kv_common.h"
