@@ -412,8 +412,8 @@ __device__ __forceinline__ void list_all(int32_t* out, int n, int count) {
 // one's loads ahead of this one's product. SPLIT: a run of tiles to a workgroup, the keys go to
 // the workspace, and k_choose chooses.
 //
-// Waits bound it: lengths, page numbers, summaries in turn, then the choice. One token over 128 pages 7.1
-// us, 32 uneven sequences of up to 256 pages 9.2 (12.5 MB, 2.6 us at a copy's rate), eight heads of 128 each.
+// Waits bound it: lengths, page numbers, summaries in turn, then the choice. One token over 128 pages 6.8
+// us, 32 uneven sequences of up to 256 pages 8.6 (12.5 MB, 2.6 us at a copy's rate), eight heads of 128 each.
 template <bool F32, int D, int WAVES, bool SPLIT>
 __global__ __launch_bounds__(64 * WAVES) void k_select(const Select a) {
     constexpr int chunks = D / 32;
@@ -660,10 +660,10 @@ Plan plan_of(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t q_heads) {
     }
     // Few tokens over many columns: workgroups of four waves, a tile of 16 columns a wave or more, to
     // fill the CUs, and a second launch that chooses. us with one workgroup to a token and head, and so:
-    // 1 token over 2048 columns 32 and 12, over 8192 87 and 17, 8 over 1024 19.5 and 16, 4 over 512 12.5
-    // and 10.7, 1 over 313 both 9.4; 160 rows over 513 12.3 and 15.
+    // 1 token over 2048 columns 32 and 12, over 8192 87 and 17, 8 over 1024 19.5 and 16, 4 over 512 11.9
+    // and 10.7, 1 over 313 9.0 and 9.4; 160 rows over 513 11.6 and 15.
     const uint64_t rows = (uint64_t)s->total * c->heads, tiles = (s->table_cols + 15) / 16;
-    if (rows <= 128 && s->table_cols > 512) p.tiles = (uint32_t)std::max<uint64_t>(4, (tiles * rows + 255) / 256);
+    if (rows <= 128 && s->table_cols > 384) p.tiles = (uint32_t)std::max<uint64_t>(4, (tiles * rows + 255) / 256);
     return p;
 }
 
@@ -689,11 +689,12 @@ int launch_select(Select& a, uint32_t rows, hipStream_t stream, char* err, size_
         if (allow_lds(reinterpret_cast<const void*>(k_choose), 4 * DMX_KV_MAX_COLUMNS, allowed[3], err, errn)) return 1;
         hipLaunchKernelGGL(k_choose, dim3(rows), dim3(1024), 4 * cols, stream, a);
     } else {
-        constexpr int most = D <= 128 ? 16 : 8;  // (128 registers a lane are few for larger heads)
+        // (every wave makes the queries whole numbers for itself: eight waves gain from 1025 columns on, 32
+        // sequences of up to 256 columns take 8.6 us with four and 9.2 with eight)
         const bool many = cols > 1024;
-        const auto kern = many ? k_select<F32, D, most, false> : k_select<F32, D, 8, false>;
+        const auto kern = many ? k_select<F32, D, 8, false> : k_select<F32, D, 4, false>;
         if (allow_lds(reinterpret_cast<const void*>(kern), 4 * DMX_KV_MAX_COLUMNS, allowed[many], err, errn)) return 1;
-        hipLaunchKernelGGL(kern, dim3(rows), dim3(many ? 64 * most : 512), 4 * cols, stream, a);
+        hipLaunchKernelGGL(kern, dim3(rows), dim3(many ? 512 : 256), 4 * cols, stream, a);
     }
     return launch_check(err, errn, "kv select launch");
 }
