@@ -169,7 +169,7 @@ typedef struct dmx_kv_pool {
  * [batch + 1] holds the offsets of the new tokens, and positions and slots
  * [total] where each lies: its position (-1 behind the last), and page * page_size
  * + position % page_size, -1 where it has no page of the cache. lengths count
- * the tokens without one, too (2^30 at most, before the new ones). */
+ * the tokens without one, too; before the new ones they count as 2^30 - 1 at most. */
 int dmx_kv_reserve(const dmx_kv_pool* pool, int32_t* table, int32_t* lengths, const int32_t* added, uint32_t batch,
                    uint32_t table_cols, uint32_t page, uint32_t total, int32_t* cu, int32_t* positions, int64_t* slots,
                    void* stream, char* err, size_t errn);
@@ -194,7 +194,7 @@ typedef struct dmx_kv_summaries {
 } dmx_kv_summaries;
 
 /* The summaries of the pages that the new tokens lie in, from all of their
- * sequence's tokens there. */
+ * sequence's tokens there (a page that two sequences of a call have: one's or the other's). */
 int dmx_kv_summarize(const dmx_kv_cache* cache, const dmx_kv_summaries* summaries, const dmx_kv_seqs* seqs, void* stream,
                      char* err, size_t errn);
 

@@ -197,6 +197,35 @@ def test_selection_over_every_team(tokens, batch, length, heads_, count, few):
             assert (got[t, h, :len(best)] == best).all() and (got[t, h, len(best):] == -1).all()
 
 
+@pytest.mark.parametrize("few", [False, True])
+@pytest.mark.parametrize("tokens, batch, columns, count, first, last", [
+    (1, 70, 1100, 40, 1, 2), (1, 70, 1024, 40, 0, 0), (300, 1, 5000, 33, 0, 1), (1, 1, 2000, 3, 1, 2), (1, 70, 1100, 3, 1, 2), (40, 1, 300, 3, 1, 2),
+    (1, 3, 100, 3, 1, 2), (1, 3, 400, 4, 4, 0), (1, 3, 385, 384, 0, 384), (20, 2, 4096, 4095, 2, 3), (1, 65, 2000, 1999, 0, 1), (1, 65, 1026, 1, 0, 0)])
+def test_selection_on_every_path(tokens, batch, columns, count, first, last, few):
+    """Many rows and few, over more columns than a wave takes and fewer, prompts past the columns that they share; forced
+    columns alone, all columns but one. (The sequences share their pages, which the scores do not mind.)"""
+    rng = np.random.default_rng(columns + count + few)
+    b = Batch(rng, [(tokens, 8 * columns)], 2, 64, 8, spare=0)
+    s = summaries_at_random(rng, b, few)
+    table, lengths = b.block_table.expand(batch, columns).contiguous(), b.lengths.expand(batch).contiguous()
+    q = heads(rng, (tokens * batch, 4, 64), "f32")
+    if few:
+        q = q.sign()
+    got = kv_ops.select(q, b.cache, s, table, lengths, count, first=first, last=last).cpu().numpy()
+    bounds, scales = s["bounds"].cpu().numpy().astype(np.int64), s["scales"].cpu().numpy().astype(np.int64)
+    qq = f64(q)
+    for t in sorted({0, 1, tokens * batch // 2, tokens * batch - 1} & set(range(tokens * batch))):
+        n = (8 * columns - tokens + t % tokens) // 8 + 1
+        pages = b.table[0][:n]
+        for h in range(2):
+            w = B.whole_queries(qq[t, 2 * h:2 * h + 2])
+            score = (np.where(w > 0, w, 0) @ bounds[pages, h, 0].T + np.where(w < 0, w, 0) @ bounds[pages, h, 1].T).max(0)
+            key = np.ldexp(score.astype(np.float64), scales[pages, h] - 127)
+            key[:first], key[n - last:] = np.inf, np.inf
+            best = np.sort(np.argsort(-key, kind="stable")[:count])
+            assert (got[t, h, :len(best)] == best).all() and (got[t, h, len(best):] == -1).all()
+
+
 def test_selection_of_queries_that_are_none():
     """NaN and infinities in a query count as 0; a query of zeros takes the lowest columns; the smallest and the largest
     queries; columns without a page come last, forced or not."""
