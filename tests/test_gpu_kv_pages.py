@@ -94,6 +94,24 @@ def test_many_tokens(total):
     p.reserve(new, sum(new))
 
 
+@pytest.mark.parametrize("columns", [1023, 1024, 1025, 4096, 4097, 12001])
+@pytest.mark.parametrize("batch", [1, 37])
+@pytest.mark.parametrize("pages", [1.0, 0.8])
+def test_many_pages(columns, batch, pages):
+    """Pages of a call that one pass of the lanes does not hand out or take back, some of them none; with
+    enough in the pool and without."""
+    rng = np.random.default_rng(columns + batch)
+    cuts = np.sort(rng.integers(0, columns + 1, batch - 1))
+    counts = np.diff(np.concatenate([[0], cuts, [columns]])) * 8  # (whole pages: `columns` in all)
+    p = Pool(rng, [0] * batch, int(counts.max()) // 8 + 1, 8, int(columns * pages))
+    p.reserve(counts.tolist(), int(counts.sum()))
+    holes = torch.rand(p.gpu_table.shape, device="cuda") < 0.05
+    p.gpu_table[holes & (p.gpu_table >= 0)] = -3
+    p.table = p.gpu_table.tolist()
+    p.trim([0] * batch)
+    p.reserve(counts.tolist(), int(counts.sum()) - 5)
+
+
 def test_prompts_longer_than_the_table():
     rng = np.random.default_rng(3)
     p = Pool(rng, [10, 30, 0], 4, 8, 40)
