@@ -27,6 +27,7 @@ struct Norm {
     int64_t residual_stride;
     void *residual_out, *out;
     uint32_t rows, dim;
+    uint32_t first;  // row of a launch
     int layer;
     float eps, offset, factor, inv_dim;
     Vectors weight, bias, post, gate, scale, shift;
@@ -132,7 +133,7 @@ template <bool BLOCK, bool F32X, bool F32R, bool VEC, int LANES, int N>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_norm(const Norm a) {
     __shared__ float part[4][LANES > 64 ? LANES / 64 : 1];
     const uint32_t lane = threadIdx.x % LANES;
-    const uint32_t row = LANES < 256 ? blockIdx.x * (256 / LANES) + threadIdx.x / LANES : blockIdx.x;
+    const uint32_t row = a.first + (LANES < 256 ? blockIdx.x * (256 / LANES) + threadIdx.x / LANES : blockIdx.x);
     if (row >= a.rows) return;
     constexpr uint32_t STEP = VEC ? 1 : LANES;
     const auto channel = [&](int n) { return 8 * n * LANES + (VEC ? 8 : 1) * lane; };
@@ -285,12 +286,15 @@ int form_of(const dmx_norm_form* f, bool block, uint32_t rows, uint32_t dim, Nor
 }
 
 template <bool BLOCK, bool F32X, bool F32R, bool VEC>
-int launch(const Norm& a, hipStream_t stream, char* err, size_t errn) {
+int launch(Norm a, hipStream_t stream, char* err, size_t errn) {
     const auto go = [&](auto lanes, auto runs) {
-        constexpr int LANES = decltype(lanes)::value, N = decltype(runs)::value;
-        const uint32_t each = LANES < 256 ? 256 / LANES : 1;
-        hipLaunchKernelGGL((k_norm<BLOCK, F32X, F32R, VEC, LANES, N>), dim3((a.rows + each - 1) / each), dim3(LANES < 256 ? 256 : LANES), 0,
-                           stream, a);
+        constexpr int LANES = decltype(lanes)::value, N = decltype(runs)::value, threads = LANES < 256 ? 256 : LANES;
+        constexpr uint32_t each = threads / LANES, most = 0xffffffffu / threads;  // workgroups of a launch
+        for (uint64_t first = 0; first < a.rows; first += (uint64_t)most * each) {
+            a.first = (uint32_t)first;
+            const uint32_t groups = (a.rows - a.first + each - 1) / each;
+            hipLaunchKernelGGL((k_norm<BLOCK, F32X, F32R, VEC, LANES, N>), dim3(std::min(groups, most)), dim3(threads), 0, stream, a);
+        }
     };
     using std::integral_constant;
     const integral_constant<int, 1> one;

@@ -216,6 +216,26 @@ def test_many_rows():
             assert torch.equal(got[r], norm_ops.norm(x[r:r + 1])[0])
 
 
+def test_rows_past_a_launch():
+    """More rows than one launch has lanes for: each of one channel, x / sqrt(x^2 + eps)."""
+    rows = 2 ** 28 + 5
+    x = torch.randn((rows, 1), device="cuda").bfloat16()
+    weight = torch.tensor([1.5], device="cuda")
+    got = norm_ops.norm(x, weight, eps=0.01)
+    for at in range(0, rows, 2 ** 26):
+        v = x[at:at + 2 ** 26].double()
+        want = 1.5 * v / torch.sqrt(v * v + 0.01)
+        off = (got[at:at + 2 ** 26].double() - want).abs()
+        assert bool((off <= want.abs() * (half("bf16") * (1 + FEW * U) + FEW * U)).all()), at
+    del x, got
+    y = torch.randn((rows, 1), device="cuda").bfloat16()
+    residual, out = norm_ops.block_norm(y, y.flip(0), eps=0.01, gate=torch.tensor([0.5], device="cuda"))
+    for at in (0, 2 ** 28 - 40, rows - 40):
+        v = y[at:at + 40].double() * 0.5 + y.flip(0)[at:at + 40].double()
+        assert bool(((residual[at:at + 40].double() - v).abs() <= v.abs() * half("bf16") + 4 * U).all())
+        assert bool(((out[at:at + 40].double() - v / torch.sqrt(v * v + 0.01)).abs() <= half("bf16") * (1 + FEW * U) + 64 * U).all())
+
+
 def test_refusals():
     y = torch.zeros((4, 64), device="cuda", dtype=torch.bfloat16)
     one = torch.zeros(64, device="cuda")
