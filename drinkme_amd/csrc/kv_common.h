@@ -261,6 +261,11 @@ inline int launch_blocks(uint64_t items, uint32_t& blocks, char* err, size_t err
     return 0;
 }
 
+// A launch has fewer than 2^32 lanes along an axis.
+inline int check_lanes(uint64_t groups, uint32_t threads, char* err, size_t errn) {
+    return groups * threads < 1ull << 32 ? 0 : fail(err, errn, "too many tokens for one launch");
+}
+
 // Lets a kernel have `bytes` of dynamic LDS on the current device (over 64 KB
 // takes an opt-in), once for each device.
 inline int allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& devices, char* err, size_t errn) {

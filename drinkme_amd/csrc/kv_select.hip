@@ -420,9 +420,9 @@ __global__ __launch_bounds__(64 * WAVES) void k_select(const Select a) {
     extern __shared__ __align__(16) uint32_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, j = lane >> 4;
     // (neighbours, which different XCDs run, are tokens: a head's summaries alone would meet in two of an L2's 16 channels)
-    const uint32_t heads = a.cache.heads, h = blockIdx.x / a.seqs.total, t = blockIdx.x - h * a.seqs.total;
+    const uint32_t heads = a.cache.heads, h = blockIdx.y, t = blockIdx.x;
     int32_t* out = a.blocks + ((int64_t)t * heads + h) * a.count;
-    uint32_t* const keys = SPLIT ? a.keys + (int64_t)blockIdx.x * a.seqs.cols : lds;
+    uint32_t* const keys = SPLIT ? a.keys + ((int64_t)h * a.seqs.total + t) * a.seqs.cols : lds;
 
     uint32_t b;
     const int n = columns_seen(a, t, b), count = a.count;
@@ -430,7 +430,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_select(const Select a) {
         if (!SPLIT) list_all(out, n, count);
         return;
     }
-    const int first = SPLIT ? blockIdx.y * a.tiles : 0, tiles = SPLIT ? min(first + (int)a.tiles, (n + 15) / 16) : (n + 15) / 16;
+    const int first = SPLIT ? blockIdx.z * a.tiles : 0, tiles = SPLIT ? min(first + (int)a.tiles, (n + 15) / 16) : (n + 15) / 16;
     if (SPLIT && first >= tiles) return;
     const auto page_at = [&](int tile) { return (uint32_t)a.seqs.table[(int64_t)b * a.seqs.cols + min(16 * tile + i, n - 1)]; };
     const auto load = [&](int r, int c, float (&x)[16]) {  // of query head r of the group
@@ -494,7 +494,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_select(const Select a) {
 
 __global__ __launch_bounds__(1024) void k_choose(const Select a) {
     extern __shared__ __align__(16) uint32_t lds[];
-    const uint32_t h = blockIdx.x / a.seqs.total, t = blockIdx.x - h * a.seqs.total;
+    const uint32_t h = blockIdx.y, t = blockIdx.x;
     int32_t* out = a.blocks + ((int64_t)t * a.cache.heads + h) * a.count;
     uint32_t b;
     const int n = columns_seen(a, t, b), count = a.count;
@@ -502,7 +502,7 @@ __global__ __launch_bounds__(1024) void k_choose(const Select a) {
         list_all(out, n, count);
         return;
     }
-    const uint32_t* from = a.keys + (int64_t)blockIdx.x * a.seqs.cols;
+    const uint32_t* from = a.keys + ((int64_t)h * a.seqs.total + t) * a.seqs.cols;
     for (int c = threadIdx.x; c < n; c += 1024) lds[c] = from[c];
     __syncthreads();
     choose_any<16>(lds, n, count, out);
@@ -672,29 +672,32 @@ uint64_t workspace_of(const Plan& p, const dmx_kv_cache* c, const dmx_kv_seqs* s
 }
 
 template <bool F32, int D>
-int launch_select(Select& a, uint32_t rows, hipStream_t stream, char* err, size_t errn) {
+int launch_select(Select& a, hipStream_t stream, char* err, size_t errn) {
     static std::atomic<uint64_t> allowed[4] = {};
-    const uint32_t cols = a.seqs.cols;
+    const uint32_t cols = a.seqs.cols, total = a.seqs.total, heads = a.cache.heads;
     if (a.tokens) {
         // (64 KB of keys: two workgroups a CU; a tile's last columns and a shift of the banks between tokens)
         a.stride = (cols + 15) / 16 * 16 + 4;
         while (a.tokens > 1 && a.tokens * a.stride * 4 > 66000) a.tokens /= 2;
         const auto kern = k_select_tokens<F32, D>;
+        const uint32_t groups = (total + a.tokens - 1) / a.tokens;
+        if (check_lanes(groups, 64 * kSelectWaves, err, errn)) return 1;
         const uint32_t rows = 4 * (D / 32) * 64 * sizeof(i32x4), bytes = std::max(rows, 4 * a.tokens * a.stride);
         if (allow_lds(reinterpret_cast<const void*>(kern), 66000, allowed[2], err, errn)) return 1;
-        hipLaunchKernelGGL(kern, dim3((a.seqs.total + a.tokens - 1) / a.tokens, a.cache.heads), dim3(64 * kSelectWaves), bytes, stream, a);
+        hipLaunchKernelGGL(kern, dim3(groups, heads), dim3(64 * kSelectWaves), bytes, stream, a);
     } else if (a.tiles) {
-        hipLaunchKernelGGL((k_select<F32, D, 4, true>), dim3(rows, ((cols + 15) / 16 + a.tiles - 1) / a.tiles), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((k_select<F32, D, 4, true>), dim3(total, heads, ((cols + 15) / 16 + a.tiles - 1) / a.tiles), dim3(256), 0, stream, a);
         if (launch_check(err, errn, "kv score launch")) return 1;
         if (allow_lds(reinterpret_cast<const void*>(k_choose), 4 * DMX_KV_MAX_COLUMNS, allowed[3], err, errn)) return 1;
-        hipLaunchKernelGGL(k_choose, dim3(rows), dim3(1024), 4 * cols, stream, a);
+        hipLaunchKernelGGL(k_choose, dim3(total, heads), dim3(1024), 4 * cols, stream, a);
     } else {
         // (every wave makes the queries whole numbers for itself: eight waves gain from 1025 columns on, 32
         // sequences of up to 256 columns take 8.6 us with four and 9.2 with eight)
         const bool many = cols > 1024;
         const auto kern = many ? k_select<F32, D, 8, false> : k_select<F32, D, 4, false>;
         if (allow_lds(reinterpret_cast<const void*>(kern), 4 * DMX_KV_MAX_COLUMNS, allowed[many], err, errn)) return 1;
-        hipLaunchKernelGGL(kern, dim3(rows), dim3(many ? 512 : 256), 4 * cols, stream, a);
+        if (check_lanes(total, many ? 512 : 256, err, errn)) return 1;
+        hipLaunchKernelGGL(kern, dim3(total, heads), dim3(many ? 512 : 256), 4 * cols, stream, a);
     }
     return launch_check(err, errn, "kv select launch");
 }
@@ -709,6 +712,7 @@ extern "C" int dmx_kv_summarize(const dmx_kv_cache* cache, const dmx_kv_summarie
     // (tokens that begin no page cost a workgroup's start: a few thousand workgroups look at several tokens each)
     a.run = (uint32_t)std::min<uint64_t>({64, cache->page, std::max<uint64_t>(1, (uint64_t)seqs->total * cache->heads / 2048)});
     const dim3 grid((seqs->total + a.run - 1) / a.run, cache->heads);
+    if (check_lanes(grid.x, 256, err, errn)) return 1;
     const auto launch = [&](auto d) {
         hipLaunchKernelGGL(k_summarize<decltype(d)::value>, grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
     };
@@ -741,8 +745,6 @@ extern "C" int dmx_kv_select(const dmx_kv_cache* cache, const dmx_kv_summaries* 
     if (first > count || last > count || first + last > count) return fail(err, errn, "first and last are more than count");
     if (seqs->total == 0) return 0;
     if (!q->at || !blocks) return fail(err, errn, "null queries or lists");
-    const uint64_t rows = (uint64_t)seqs->total * cache->heads;
-    if (rows >= 1ull << 31) return fail(err, errn, "too many tokens and heads");
     Select a = {};
     a.cache = cache_of(cache);
     a.seqs = seqs_of(seqs);
@@ -759,7 +761,7 @@ extern "C" int dmx_kv_select(const dmx_kv_cache* cache, const dmx_kv_summaries* 
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const auto by_type = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        return dtype == DMX_F32 ? launch_select<true, D>(a, (uint32_t)rows, st, err, errn) : launch_select<false, D>(a, (uint32_t)rows, st, err, errn);
+        return dtype == DMX_F32 ? launch_select<true, D>(a, st, err, errn) : launch_select<false, D>(a, st, err, errn);
     };
     return cache->dim == 64    ? by_type(std::integral_constant<int, 64>{})
            : cache->dim == 96  ? by_type(std::integral_constant<int, 96>{})

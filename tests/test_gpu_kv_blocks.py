@@ -506,6 +506,24 @@ def test_no_tokens():
     assert kv_ops.attention(q, b.cache, b.block_table, b.lengths, blocks=blocks).shape == (0, 4, 64)
 
 
+def test_as_many_tokens_as_a_launch_takes():
+    """A token of many selects what a call of the last ones alone does; those before the sequence's first position
+    list nothing; one more is refused."""
+    rng = np.random.default_rng(17)
+    columns, most = 4100, 2 ** 23 - 1
+    b = Batch(rng, [(1, 8 * columns)], 1, 64, 8, spare=0)
+    s = summaries_at_random(rng, b)
+    q = heads(rng, (1, 1, 64), "bf16")
+    got = kv_ops.select(q.expand(most, 1, 64), b.cache, s, b.block_table, b.lengths, 4)
+    for n in (1, 3000):
+        want = kv_ops.select(q.expand(n, 1, 64), b.cache, s, b.block_table, b.lengths, 4)
+        assert torch.equal(got[most - n:], want) and bool((want >= 0).all())
+    assert bool((got[:most - 8 * columns] == -1).all())
+    assert got[most - 8 * columns].tolist() == [[0, -1, -1, -1]]
+    with pytest.raises(RuntimeError, match="too many tokens"):
+        kv_ops.select(q.expand(most + 1, 1, 64), b.cache, s, b.block_table, b.lengths, 4)
+
+
 def test_refusals():
     rng = np.random.default_rng(18)
     b = Batch(rng, [(2, 20)], 2, 64, 8)
