@@ -412,8 +412,8 @@ __device__ __forceinline__ void list_all(int32_t* out, int n, int count) {
 // one's loads ahead of this one's product. SPLIT: a run of tiles to a workgroup, the keys go to
 // the workspace, and k_choose chooses.
 //
-// Waits bound it: lengths, page numbers, summaries in turn, then the choice. One token over 128 pages 6.8
-// us, 32 uneven sequences of up to 256 pages 8.6 (12.5 MB, 2.6 us at a copy's rate), eight heads of 128 each.
+// Waits bound it: lengths, page numbers, summaries in turn, then the choice. One token over 128 pages 6.5
+// us, 32 uneven sequences of up to 256 pages 8.5 (12.5 MB, 2.6 us at a copy's rate), eight heads of 128 each.
 template <bool F32, int D, int WAVES, bool SPLIT>
 __global__ __launch_bounds__(64 * WAVES) void k_select(const Select a) {
     constexpr int chunks = D / 32;
@@ -692,7 +692,7 @@ int launch_select(Select& a, hipStream_t stream, char* err, size_t errn) {
         hipLaunchKernelGGL(k_choose, dim3(total, heads), dim3(1024), 4 * cols, stream, a);
     } else {
         // (every wave makes the queries whole numbers for itself: eight waves gain from 1025 columns on, 32
-        // sequences of up to 256 columns take 8.6 us with four and 9.2 with eight)
+        // sequences of up to 256 columns take 8.5 us with four and 9.2 with eight)
         const bool many = cols > 1024;
         const auto kern = many ? k_select<F32, D, 8, false> : k_select<F32, D, 4, false>;
         if (allow_lds(reinterpret_cast<const void*>(kern), 4 * DMX_KV_MAX_COLUMNS, allowed[many], err, errn)) return 1;

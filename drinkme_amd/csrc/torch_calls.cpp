@@ -249,9 +249,7 @@ bool strided(const at::Tensor* x) {
 bool rows_at(PyObject* o, const at::Tensor*& x, dmx_rows& r) {
     x = exact(o);
     if (!strided(x) || x->dim() != 3) return false;
-    if ( x->size(0) >= kMost || x->size(1) >= kMost ||
-        wants(*x))
-        return false;
+    if (x->size(0) >= kMost || x->size(1) >= kMost || wants(*x)) return false;
     r = {const_cast<void*>(x->const_data_ptr()), x->stride(0), x->stride(1), (uint32_t)x->size(1)};
     return true;
 }
