@@ -257,7 +257,7 @@ int vectors_of(const dmx_vectors& v, const char* what, uint32_t rows, const dmx_
         snprintf(msg, sizeof msg, "%s: %u rows for a call of %u", what, v.rows, rows);
         return fail(err, errn, msg);
     }
-    to.by = 1, to.per = divisor_of(rows / v.rows);
+    to.by = 1, to.per = divisor_of(std::max(1u, rows / v.rows));  // (a call of no rows divides by none)
     return 0;
 }
 

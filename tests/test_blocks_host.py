@@ -186,6 +186,19 @@ def test_bad_rows_of_norms_are_refused():
         assert re.search(match, _refused("dmx_block_norm", *{**good, **kw}.values()))
 
 
+@cpu_only
+def test_norms_of_no_rows_return():
+    """With vectors of several rows, too: no row divides them."""
+    err = _native.error_buffer()
+    for kw in ({}, {"gate": (FAKE, 0, 2)}, {"scale": (FAKE, 0, 3), "shift": (FAKE, 1, 3)}, {"cu": FAKE, "batch": 4, "gate": (FAKE, 0, 2)},
+               {"cu": FAKE, "batch": 4, "gate": (FAKE, 0, 4)}, {"gate": (FAKE, 0, 2 ** 32 - 1)}):
+        f = _form(**kw)
+        assert _native.lib().dmx_block_norm(FAKE, 128, FAKE, 128, FAKE, FAKE, 0, 128, 0, 0, ct.byref(f), None, err, len(err)) == 0, kw
+    f = _form()
+    assert _native.lib().dmx_norm(ct.byref(_rows()), FAKE, 0, 128, 0, ct.byref(f), None, err, len(err)) == 0
+    assert b"gate: 0 rows" in _refused("dmx_block_norm", FAKE, 128, FAKE, 128, FAKE, FAKE, 0, 128, 0, 0, _form(gate=(FAKE, 0, 0)))
+
+
 def test_calls_off_the_gpu_are_refused():
     x = torch.zeros((2, 2, 64))
     cache = kv_ops.new_cache(2, 16, 2, 64, device="cpu")

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from drinkme_amd import norm_ops
+from drinkme_amd import _native, norm_ops
 from tests.blocks_reference import standard
 from tests.test_gpu_kv import DT, f64
 
@@ -204,6 +204,16 @@ def test_no_rows_another_stream_and_a_graph():
         late.copy_(randn(rng, (9, 2048), "bf16"))
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(got, norm_ops.block_norm(late, residual, kind="layer")))
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_no_rows_beside_vectors_of_several(native, monkeypatch):
+    if not native:
+        monkeypatch.setattr(_native, "calls", lambda: None)
+    empty, some = torch.empty((0, 64), device="cuda"), torch.ones((3, 64), device="cuda")
+    cu = torch.zeros(4, dtype=torch.int32, device="cuda")
+    for kw in ({"gate": some}, {"modulate": (some, some)}, {"gate": some[:2], "cu": cu}, {"gate": some, "modulate": (some, some), "cu": cu}):
+        assert [x.shape for x in norm_ops.block_norm(empty, empty, **kw)] == [(0, 64)] * 2
 
 
 def test_many_rows():
