@@ -40,7 +40,10 @@ struct AttnArgs {
     float* lse;
     float* part_o;   // [splits][total * q_heads][dim]
     f32x4* part_stat;  // [splits][total * q_heads]: reference (log2 domain), sum, sum of the rounded weights
-    // listed pages (k_attend's LISTED)
+};
+
+// Of listed pages (k_attend's LISTED). (The others' arguments stay three lines of 64 bytes.)
+struct ListedArgs : AttnArgs {
     const int32_t* blocks;  // [total, heads, count] columns of the block table
     Divisor count;
 };
@@ -415,7 +418,7 @@ __device__ __forceinline__ void leave_rest(const AttnArgs& a, const Seq& q, uint
 // list a position which the table has no page for. One token whose list ascends, as
 // select writes it, needs no such bits: `plain`, and who is not written.
 template <int WAVES>
-__device__ __forceinline__ int list_pages(const AttnArgs& a, uint32_t h, const Seq& q, int m0, int m1, uint32_t* who, uint16_t* list,
+__device__ __forceinline__ int list_pages(const ListedArgs& a, uint32_t h, const Seq& q, int m0, int m1, uint32_t* who, uint16_t* list,
                                           uint32_t& beyond, bool& plain) {
     __shared__ int counts[WAVES], out_of_order[WAVES];
     __shared__ uint32_t past;
@@ -512,7 +515,7 @@ __device__ __forceinline__ ListedEntry listed_entries(const AttnArgs& a, uint32_
 // LISTED: of the columns that each token sees, those that it lists; a tile walks the
 // pages that any of its tokens lists, and a row's weights of the others are 0.
 template <int W, int P, int NR, bool ROWS, bool WIDE, bool LISTED = false, int WAVES = kAttnWaves>
-__global__ __launch_bounds__(64 * WAVES, W * NR * (P + 1) <= 16 ? 2 : 1) void k_attend(const AttnArgs a) {
+__global__ __launch_bounds__(64 * WAVES, W * NR * (P + 1) <= 16 ? 2 : 1) void k_attend(const std::conditional_t<LISTED, ListedArgs, AttnArgs> a) {
     using S = Segments<W>;
     constexpr int D = 32 * W, NT = D / 16;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -690,15 +693,17 @@ __global__ __launch_bounds__(64 * WAVES, W * NR * (P + 1) <= 16 ? 2 : 1) void k_
         for (int t = 0; t < NR; ++t) {
 #pragma unroll
             for (int half = WAVES / 2; half; half /= 2) {
+                // (a wave of the lower half hands on in the place that it alone has read: one barrier a step)
+                const int first = half == WAVES / 2 ? half : 0;
                 if (wave >= half && wave < 2 * half)
 #pragma unroll
-                    for (int c = 0; c < NT; ++c) buf[wave - half][c][lane] = st.o[t][c];
+                    for (int c = 0; c < NT; ++c) buf[wave - first][c][lane] = st.o[t][c];
                 __syncthreads();
                 if (wave < half)
 #pragma unroll
-                    for (int c = 0; c < NT; ++c) st.o[t][c] += buf[wave][c][lane];
-                if (half > 1 || t + 1 < NR) __syncthreads();
+                    for (int c = 0; c < NT; ++c) st.o[t][c] += buf[wave + half - first][c][lane];
             }
+            if (t + 1 < NR) __syncthreads();
         }
         if (wave != 0) return;
     }

@@ -56,7 +56,7 @@ int check_listed(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t count, ch
 }
 
 template <int W, int P, bool WIDE, int WAVES>
-int launch(dim3 grid, int lds, hipStream_t stream, const AttnArgs& a, char* err, size_t errn) {
+int launch(dim3 grid, int lds, hipStream_t stream, const ListedArgs& a, char* err, size_t errn) {
     // (the most that any call takes: 16384 columns' bits, and as many 16-bit entries; in their
     // place half of the waves' results at the end)
     static std::atomic<uint64_t> allowed = {};
@@ -98,7 +98,7 @@ extern "C" int dmx_kv_attention_blocks(const dmx_kv_cache* cache, const dmx_kv_s
     if (p.row_blocks > 65535) return fail(err, errn, "too many query rows of one sequence");
     if (workspace_bytes < workspace_of(p, cache, seqs, q->heads) || (p.splits > 1 && (!workspace || !aligned(workspace, 16))))
         return fail(err, errn, "workspace missing, short or not 16-byte aligned");
-    AttnArgs a = {};
+    ListedArgs a = {};
     a.cache = cache_of(cache);
     a.seqs = seqs_of(seqs);
     a.q = q->at, a.q_token = q->token_stride, a.q_head = q->head_stride;
@@ -134,6 +134,7 @@ extern "C" int dmx_kv_attention_blocks(const dmx_kv_cache* cache, const dmx_kv_s
     if (p.splits == 1) return 0;
     const int ways = p.splits > 8 ? 4 : 1;
     hipLaunchKernelGGL((dtype == DMX_F32 ? k_attend_join<true> : k_attend_join<false>),
-                       dim3((uint32_t)(ways == 4 ? all : (all + 3) / 4)), dim3(256), 0, st, a, (int)cache->dim, ways);
+                       dim3((uint32_t)(ways == 4 ? all : (all + 3) / 4)), dim3(256), 0, st,
+                       static_cast<const AttnArgs&>(a), (int)cache->dim, ways);
     return launch_check(err, errn, "kv attention join launch");
 }
