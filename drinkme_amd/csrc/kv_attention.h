@@ -46,6 +46,7 @@ struct AttnArgs {
 struct ListedArgs : AttnArgs {
     const int32_t* blocks;  // [total, heads, count] columns of the block table
     Divisor count;
+    uint32_t first_block;  // block of rows that the launch begins with
 };
 
 // Segments of V: 128 channels (lane i reads word i, 8 channels), then 64
@@ -521,11 +522,13 @@ __global__ __launch_bounds__(64 * WAVES, W * NR * (P + 1) <= 16 ? 2 : 1) void k_
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, j = lane >> 4;
     const uint32_t h = blockIdx.x, b = blockIdx.z / a.splits, split = blockIdx.z % a.splits;
+    uint32_t row_block = blockIdx.y;
+    if constexpr (LISTED) row_block += a.first_block;
 
     const Seq q = seq_of(a.seqs, b);
-    if (a.seqs.cu && split == 0 && blockIdx.y + 1 == a.row_blocks) leave_rest<P != 1, D>(a, q, h, b);
+    if (a.seqs.cu && split == 0 && row_block + 1 == a.row_blocks) leave_rest<P != 1, D>(a, q, h, b);
     const int rows = min(q.count, (int)a.seqs.each.value) * (int)a.group;
-    const int r0 = (ROWS ? (int)blockIdx.y * WAVES + (int)wave : (int)blockIdx.y) * 16 * NR;
+    const int r0 = (ROWS ? (int)row_block * WAVES + (int)wave : (int)row_block) * 16 * NR;
     if (r0 >= rows) return;
 
     // what the rows see: [lo, hi) of each, and over all of them

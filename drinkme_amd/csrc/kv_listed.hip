@@ -56,15 +56,19 @@ int check_listed(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t count, ch
 }
 
 template <int W, int P, bool WIDE, int WAVES>
-int launch(dim3 grid, int lds, hipStream_t stream, const ListedArgs& a, char* err, size_t errn) {
+int launch(dim3 grid, int lds, hipStream_t stream, ListedArgs a, char* err, size_t errn) {
     // (the most that any call takes: 16384 columns' bits, and as many 16-bit entries; in their
     // place half of the waves' results at the end)
     static std::atomic<uint64_t> allowed = {};
+    constexpr uint32_t most = 65535;  // workgroups along a grid's second axis
     constexpr int results = WAVES / 2 * 2 * W * 64 * (int)sizeof(f32x4);
     static_assert(results <= 6 * DMX_KV_MAX_COLUMNS);
     const auto kern = k_attend<W, P, 1, false, WIDE, true, WAVES>;
     if (allow_lds(reinterpret_cast<const void*>(kern), 6 * DMX_KV_MAX_COLUMNS, allowed, err, errn)) return 1;
-    hipLaunchKernelGGL(kern, grid, dim3(64 * WAVES), std::max(lds, results), stream, a);
+    for (; a.first_block < a.row_blocks; a.first_block += most) {  // (65535 tiles are 262 140 tokens of four rows)
+        grid.y = std::min(most, a.row_blocks - a.first_block);
+        hipLaunchKernelGGL(kern, grid, dim3(64 * WAVES), std::max(lds, results), stream, a);
+    }
     return launch_check(err, errn, "kv attention launch");
 }
 
@@ -94,8 +98,9 @@ extern "C" int dmx_kv_attention_blocks(const dmx_kv_cache* cache, const dmx_kv_s
     if (!q->at || !out || !blocks) return fail(err, errn, "null queries, lists or output");
     if ((uint64_t)seqs->total * cache->heads * count >= 1ull << 62) return fail(err, errn, "too many lists");
     const Plan p = plan_of(cache, seqs, q->heads, dtype, count, max_length);
-    if (p.row_blocks == 0) return fail(err, errn, "max_tokens is 0");
-    if (p.row_blocks > 65535) return fail(err, errn, "too many query rows of one sequence");
+    if (p.tokens == 0) return fail(err, errn, "max_tokens is 0");
+    // (the kernel numbers a sequence's rows in 31 bits; so many have 256 GiB of results at least)
+    if ((uint64_t)p.tokens * (q->heads / cache->heads) >= 1ull << 31) return fail(err, errn, "too many query rows of one sequence");
     if (workspace_bytes < workspace_of(p, cache, seqs, q->heads) || (p.splits > 1 && (!workspace || !aligned(workspace, 16))))
         return fail(err, errn, "workspace missing, short or not 16-byte aligned");
     ListedArgs a = {};

@@ -151,6 +151,24 @@ def test_bad_attentions_are_refused(change, match):
     assert re.search(match, _refused("dmx_kv_attention_blocks", *a.values()))
 
 
+@cpu_only
+@pytest.mark.parametrize("total, q_heads, heads, seqs", [
+    (131071, 64, 8, {}), (131072, 64, 8, {}), (262144, 32, 8, {}), (300000, 32, 8, {"batch": 4, "cu": FAKE, "max_tokens": 300000}),
+    (65535 * 16, 2, 2, {}), (65535 * 16 + 1, 2, 2, {}), (2 ** 30 - 1, 2, 2, {}), (32767, 65535, 1, {})])
+def test_attentions_over_long_prompts_pass_the_checks(total, q_heads, heads, seqs):
+    """What the attention over everything takes, the one over lists takes, too: it comes as far as the device."""
+    c, s, q = _cache(heads=heads), _seqs(**{"batch": 1, "table_cols": 16384, "total": total, **seqs}), _rows(heads=q_heads)
+    assert _refused("dmx_kv_attention_blocks", c, s, q, 0, 1.0, 1, FAKE, 32, 0, FAKE, None, FAKE, 1 << 60) == b"no current device"
+
+
+@cpu_only
+def test_rows_past_31_bits_are_refused():
+    for total, q_heads in ((2 ** 30 - 1, 3), (2 ** 25, 64), (2 ** 30 - 1, 65535)):
+        s = _seqs(batch=1, table_cols=16384, total=total)
+        assert b"too many query rows" in _refused("dmx_kv_attention_blocks", _cache(heads=1), s, _rows(heads=q_heads), 0, 1.0, 1, FAKE, 32, 0, FAKE, None,
+                                                  FAKE, 1 << 60)
+
+
 def _form(**kw):
     f = _native.NormForm(0, 1e-6, 0.0, 1.0)
     for k, v in kw.items():

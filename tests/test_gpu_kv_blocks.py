@@ -409,6 +409,30 @@ def test_lists_of_every_size():
     check_listed(b, held, q, blocks, kv_ops.attention(q, b.cache, b.block_table, b.lengths, blocks=blocks), "f32")
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_prompts_of_more_rows_than_a_launch_has(dtype):
+    """Over 65535 tiles of 16 rows: tokens on both sides of the border against the definition, all of them against
+    calls of a part each, and offsets of two sequences with tokens of none behind them."""
+    rng = np.random.default_rng(19)
+    T, group, D = 16389, 64, 64  # (the border is within token 16383)
+    b = Batch(rng, [(T, T + 100)], 1, D, 64)
+    (k, v), = b.fill(rng)
+    q = heads(rng, (T, group, D), dtype)
+    blocks = i32(rng.integers(-1, b.cols, (T, 1, 3)))
+    out, lse = kv_ops.attention(q, b.cache, b.block_table, b.lengths, blocks=blocks, return_lse=True)
+    for t in (0, 1, 8191, 16382, 16383, 16384, T - 1):
+        want, l, spread, reach = B.listed_attention(f64(q[t:t + 1]), k, v, 100 + t, D ** -0.5, blocks[t:t + 1].cpu().numpy(), 64)
+        assert (np.abs(f64(out[t:t + 1]) - want) <= R.bound(want, spread, reach, T + 100, D, dtype == "bf16")).all()
+        seen = np.isfinite(l)
+        assert (np.isneginf(f64(lse[t:t + 1])) == ~seen).all()
+        assert (np.abs(f64(lse[t:t + 1])[seen] - l[seen]) <= R.lse_bound(l, reach, T + 100, D)[seen]).all()
+    for t0, t1 in ((0, 6000), (6000, T)):
+        part, sums = kv_ops.attention(q[t0:t1], b.cache, b.block_table, i32([100 + t1]), blocks=blocks[t0:t1], return_lse=True)
+        assert torch.equal(part, out[t0:t1]) and torch.equal(sums, lse[t0:t1])
+    again = kv_ops.attention(q, b.cache, b.block_table.expand(2, -1), i32([107, T + 97]), cu=i32([0, 7, T - 3]), blocks=blocks)
+    assert torch.equal(again[:T - 3], out[:T - 3]) and bool(again[T - 3:].isnan().all())
+
+
 def test_large_heads_and_tables_at_once():
     rng = np.random.default_rng(13)
     b = Batch(rng, [(9, 900)], 1, 256, 8, spare=16384 - 113)
