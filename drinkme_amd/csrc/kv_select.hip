@@ -17,8 +17,9 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 // query there. They are exact (a code times its power of two is an fp32 number,
 // and neither depends on an order), and rounded outwards to 8 bits.
 //
-// Waits bound it: lengths, page number, codes, then three barriers: 4.8 us for the last pages of 32
-// sequences (8 heads of 128, 64 tokens a page), 7.5 for the 16 of a chunk of 1024 tokens.
+// Waits bound it: lengths, page number, the look for a shared page, codes, then three barriers: 4.75 us for the last
+// pages of 32 sequences (8 heads of 128, 64 tokens a page), 9.3 for the 16 of a chunk of 1024 tokens, 107 for the
+// 8192 pages of 16 of a prompt, from a graph.
 
 struct Summarize {
     Cache cache;
@@ -26,16 +27,47 @@ struct Summarize {
     int8_t* bounds;
     uint8_t* scales;
     uint32_t run;  // new tokens a workgroup looks at, 64 at most
+    uint32_t team;  // 2^team lanes look through a sequence's columns (fuller_elsewhere)
 };
+
+// A page that several of the sequences have, or one has twice, is written by who holds most tokens there: those
+// bounds hold for the others', too, and equal numbers write equal bytes; of different ones the bytes could mix.
+// Looking for them takes 0.4 us of a step, 4 to 8 of 4 to 64 prompts' (their last workgroups'), 1 of 1024 sequences',
+// 15 of 4096's.
+// -> The bits of `partial` (lanes whose page, number `number`, holds less than it may: `tokens`) that a lane
+// finds to hold more somewhere else.
+__device__ __forceinline__ uint64_t fuller_elsewhere(const Summarize& a, uint64_t partial, int tokens, int number) {
+    const int shift = a.cache.page_shift;
+    uint64_t out = 0;
+    for (uint32_t b0 = 0; b0 < a.seqs.batch; b0 += 256u >> a.team) {  // (loops of whole waves: readlane reads every lane)
+        const uint32_t b = b0 + (threadIdx.x >> a.team);
+        const Seq q = seq_of(a.seqs, min(b, a.seqs.batch - 1));
+        const int end = b < a.seqs.batch && q.count && q.length ? min(((q.length - 1) >> shift) + 1, a.seqs.cols) : 0;
+        int col = (max(q.first, 0) >> shift) + (int)(threadIdx.x & ((1u << a.team) - 1));
+        for (; __any(col < end); col += 1 << a.team) {
+            const int page = col < end ? a.seqs.table[(int64_t)b * a.seqs.cols + col] : -1;
+            for (uint64_t m = partial; m; m &= m - 1) {
+                const int l = __builtin_ctzll(m), count = __builtin_amdgcn_readlane(tokens, l);
+                // (where offsets decrease, the token that would find the column may be another sequence's)
+                if (page == __builtin_amdgcn_readlane(number, l) && min(1 << shift, q.length - (col << shift)) > count &&
+                    seq_at(a.seqs, q.token + max((col << shift) - q.first, 0)) == b)
+                    out |= 1ull << l;
+            }
+        }
+    }
+    return out;
+}
 
 // A workgroup takes a head of the pages that begin among its new tokens (or in
 // which their sequence's first one lies), one after the other: a lane finds a token's, then a thread
 // takes a word of eight channels, of every 256 / words-th token, then a channel.
+// (eight workgroups a CU: a prompt of 8192 pages takes 114 us with the seven that more registers leave)
 template <int D>
-__global__ __launch_bounds__(256) void k_summarize(const Summarize a) {
+__global__ __launch_bounds__(256, 8) void k_summarize(const Summarize a) {
     constexpr int words = D / 8, groups = 256 / words;
     __shared__ float part[groups][2][D];
     __shared__ float tops[4];
+    __shared__ uint64_t fuller[4];
     const int x = threadIdx.x, w = x % words, g = x / words;
     const uint32_t h = blockIdx.y, heads = a.cache.heads, shift = a.cache.page_shift;
     const uint32_t t = blockIdx.x * a.run + (x & 63);
@@ -52,6 +84,15 @@ __global__ __launch_bounds__(256) void k_summarize(const Summarize a) {
             number = a.seqs.table[(int64_t)b * a.seqs.cols + (p >> shift)];
         }
     }
+    const uint64_t partial = __ballot(start >= 0 && tokens < 1 << shift);
+    if (partial) {
+        uint64_t elsewhere = fuller_elsewhere(a, partial, tokens, number);
+        if (__any(elsewhere != 0)) {  // (rare: the lanes' bits together)
+#pragma unroll
+            for (int n = 32; n; n >>= 1) elsewhere |= __shfl_xor(elsewhere, n);
+        }
+        if ((x & 63) == 0) fuller[x >> 6] = elsewhere;  // (read behind the first page's barrier)
+    }
     for (uint64_t found = __ballot(start >= 0); found; found &= found - 1) {
         const int l = __builtin_ctzll(found), count = __builtin_amdgcn_readlane(tokens, l);
         const uint64_t page = (uint32_t)__builtin_amdgcn_readlane(number, l);
@@ -64,14 +105,14 @@ __global__ __launch_bounds__(256) void k_summarize(const Summarize a) {
             for (int m = g; m < count; m += groups) {
                 const uint32_t e = a.cache.k_scales[(first + m) * (D / 32) + w / 4];
                 const uint32_t word = a.cache.k_codes[(first + m) * words + w];
-                if (e > 252) continue;  // NaN
+                const float once = e > 252 ? NAN : 1.f;  // (which a maximum passes over; no branch, so that loads go ahead)
                 const float unit = __uint_as_float(e << 23);
                 const f32x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, unit, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, unit, 1),
                                     __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, unit, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, unit, 3)};
 #pragma unroll
                 for (int n = 0; n < 8; ++n) {
-                    hi[n] = fmaxf(hi[n], v[n / 2][n & 1]);
-                    lo[n] = fminf(lo[n], v[n / 2][n & 1]);
+                    hi[n] = fmaxf(hi[n], v[n / 2][n & 1] * once);
+                    lo[n] = fminf(lo[n], v[n / 2][n & 1] * once);
                 }
             }
 #pragma unroll
@@ -81,6 +122,7 @@ __global__ __launch_bounds__(256) void k_summarize(const Summarize a) {
             }
         }
         __syncthreads();
+        if (partial >> l & 1 && (fuller[0] | fuller[1] | fuller[2] | fuller[3]) >> l & 1) continue;
         float most = -INFINITY, least = INFINITY;
         if (x < D) {
 #pragma unroll
@@ -708,7 +750,8 @@ extern "C" int dmx_kv_summarize(const dmx_kv_cache* cache, const dmx_kv_summarie
                                 void* stream, char* err, size_t errn) {
     if (check_cache(cache, err, errn) || check_seqs(cache, seqs, err, errn) || check_summaries(summaries, err, errn)) return 1;
     if (seqs->total == 0) return 0;
-    Summarize a = {cache_of(cache), seqs_of(seqs), summaries->bounds, summaries->scales, 1};
+    Summarize a = {cache_of(cache), seqs_of(seqs), summaries->bounds, summaries->scales, 1, 0};
+    while (a.team < 8 && ((uint64_t)cache->page * seqs->batch << a.team) < seqs->total) ++a.team;
     // (tokens that begin no page cost a workgroup's start: a few thousand workgroups look at several tokens each)
     a.run = (uint32_t)std::min<uint64_t>({64, cache->page, std::max<uint64_t>(1, (uint64_t)seqs->total * cache->heads / 2048)});
     const dim3 grid((seqs->total + a.run - 1) / a.run, cache->heads);

@@ -629,7 +629,8 @@ def _blocks_of(blocks, total, heads, block_table, device):
 def summarize(cache: dict, summaries: dict, block_table: torch.Tensor, lengths: torch.Tensor, total: int, *, cu=None) -> None:
     """The summaries, in place, of the pages that the last tokens of each sequence
     lie in (`total` / B of each, or cu's, as read takes them), from every token
-    that their sequence has there: after append, and before select."""
+    that their sequence has there: after append, and before select. A page that several
+    of these sequences share is summarized from the tokens of the one that has most there."""
     native = _native.calls()
     if native is not None and native.summarize(cache, summaries, block_table, lengths, total, cu, _current(lengths)):
         return

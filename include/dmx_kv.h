@@ -194,7 +194,7 @@ typedef struct dmx_kv_summaries {
 } dmx_kv_summaries;
 
 /* The summaries of the pages that the new tokens lie in, from all of their
- * sequence's tokens there (a page that two sequences of a call have: one's or the other's). */
+ * sequence's tokens there; of a page that several of them have, from the most that one has there. */
 int dmx_kv_summarize(const dmx_kv_cache* cache, const dmx_kv_summaries* summaries, const dmx_kv_seqs* seqs, void* stream,
                      char* err, size_t errn);
 

@@ -137,6 +137,42 @@ def test_summaries_of_tokens_without_a_page_or_a_sequence():
     assert all(torch.equal(again[n], s[n]) for n in s)
 
 
+@pytest.mark.parametrize("D, page, batch, cols, pages, most", [
+    (64, 8, 2, 2, 2, 16), (128, 64, 40, 2, 6, 3), (256, 16, 300, 3, 20, 1), (96, 16, 300, 1, 4, 1), (192, 8, 33, 40, 60, 320), (128, 8, 700, 4, 1500, 5)])
+def test_summaries_of_shared_pages(D, page, batch, cols, pages, most):
+    """Sequences share pages, one has a page twice, and each holds another number of tokens there: the summary
+    is of the most. Many workgroups meet at a page; every byte is one's."""
+    rng = np.random.default_rng(D + batch)
+    b = Batch(rng, [(page * pages, page * pages)], 2, D, page, spare=0)
+    (k, _), = b.fill(rng)
+    column = {int(p): c for c, p in enumerate(b.table[0])}  # (where a page's keys are held)
+    shared = 0
+    for turn in range(4):
+        table = rng.choice(b.table[0], (batch, cols))
+        lengths = rng.integers(0, cols * page + 1, batch)
+        if turn == 3:
+            lengths[:] = rng.integers(1, page, batch)  # (all within a page)
+        new = np.minimum(rng.integers(0, most + 1, batch), lengths) if turn % 2 else np.full(batch, min(most, cols * page))
+        lengths = np.maximum(lengths, new)
+        before, pad = int(rng.integers(0, 4)) * (turn % 2), int(rng.integers(0, 5)) * (turn % 2)
+        cu = i32(before + np.concatenate([[0], np.cumsum(new)])) if turn % 2 else None
+        s = noisy_summaries(rng, b.cache)
+        bounds, scales = s["bounds"].cpu().numpy().copy(), s["scales"].cpu().numpy().copy()
+        held = {}
+        for n, length, row in zip(new, lengths, table):
+            for col in range((length - n) // page, -(-length // page)) if n else ():
+                held[int(row[col])] = max(held.get(int(row[col]), 0), int(min(page, length - col * page)))
+        shared += sum(-(-length // page) - (length - n) // page for n, length in zip(new, lengths) if n) - len(held)
+        for p, n in held.items():
+            at = column[p] * page
+            for h in range(2):
+                bounds[p, h], scales[p, h] = B.summary(k[at:at + n, h])
+        for _ in range(3):
+            kv_ops.summarize(b.cache, s, i32(table), i32(lengths), before + int(new.sum()) + pad, cu=cu)
+            assert (s["bounds"].cpu().numpy() == bounds).all() and (s["scales"].cpu().numpy() == scales).all()
+    assert shared > 0
+
+
 # ---------------------------------------------------------------- selection --
 
 
