@@ -769,7 +769,7 @@ extern "C" int dmx_kv_summarize(const dmx_kv_cache* cache, const dmx_kv_summarie
 
 extern "C" uint64_t dmx_kv_select_workspace(const dmx_kv_cache* cache, const dmx_kv_seqs* seqs, uint32_t q_heads) {
     if (check_cache(cache, nullptr, 0) || check_seqs(cache, seqs, nullptr, 0) || seqs->table_cols > DMX_KV_MAX_COLUMNS || q_heads == 0 ||
-        q_heads % cache->heads)
+        q_heads % cache->heads || q_heads > 65535)
         return 0;
     return workspace_of(plan_of(cache, seqs, q_heads), cache, seqs);
 }

@@ -204,6 +204,15 @@ def test_bad_rows_of_norms_are_refused():
         assert re.search(match, _refused("dmx_block_norm", *{**good, **kw}.values()))
 
 
+def test_workspaces_of_too_many_heads_are_none():
+    """As for any call that is refused; the query returns, whatever it is asked."""
+    s = ct.byref(_seqs(table_cols=4000))
+    for heads, q_heads in ((1, 2 ** 32 - 1), (1, 2 ** 31 + 1), (2, 2 ** 32 - 2), (1, 65536), (65535, 65535 * 65537)):
+        c = ct.byref(_cache(heads=heads))
+        assert _native.lib().dmx_kv_select_workspace(c, s, q_heads) == 0, q_heads
+    assert _native.lib().dmx_kv_select_workspace(ct.byref(_cache(heads=1)), s, 65535) > 0
+
+
 @cpu_only
 def test_norms_of_no_rows_return():
     """With vectors of several rows, too: no row divides them."""
