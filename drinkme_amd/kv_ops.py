@@ -285,9 +285,10 @@ def _seqs_of(block_table, lengths, cu, total, max_tokens, device, what):
 @functools.lru_cache(maxsize=64)
 def _packed_axes(axes: tuple):
     """The dmx_rotary_axes of a tuple of axes: two bits an angle."""
-    if not 1 <= len(axes) <= 256 or any(type(a) is not int or not 0 <= a < 4 for a in axes):
+    if not 1 <= len(axes) <= 256 or any(a not in (0, 1, 2, 3) for a in axes):  # (by value, as the cache compares them)
         raise ValueError("rotary: axes are 1..256 numbers of 0..3 (rotary_axes)")
     x = _native.KvRotaryAxes()
+    axes = [int(a) for a in axes]
     x.count, x.angles, x.address = max(axes) + 1, len(axes), ct.addressof(x)
     for i, a in enumerate(axes):
         x.of[i // 16] |= a << (2 * (i % 16))

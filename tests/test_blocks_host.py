@@ -263,6 +263,20 @@ def test_axes_are_dealt_as_said():
         kv_ops.rotary_axes((1,), "other")
 
 
+def test_axes_are_taken_by_their_values():
+    """Whatever was asked for before: 1.0 is axis 1, and what is no axis is refused every time."""
+    kv_ops._packed_axes.cache_clear()
+    for axes in ((1.0, 0.0, 2.0), (1, 0, 2), (np.int64(1), False, 2.0)):
+        for _ in range(2):
+            x = kv_ops._packed_axes(axes)
+            assert (x.count, x.angles, x.of[0]) == (3, 3, 1 | 2 << 4)
+            kv_ops._packed_axes.cache_clear()
+    for axes in ((0, 4), (-1,), (0.5,), ("0",), (None,), (), (0,) * 257):
+        for _ in range(2):
+            with pytest.raises(ValueError, match="axes"):
+                kv_ops._packed_axes(axes)
+
+
 def test_tables_of_several_axes():
     axes = kv_ops.rotary_axes((3, 5, 2), "interleaved")
     table = kv_ops.rotary_table(40, 20, base=1e4, device="cpu", axes=axes).double()
