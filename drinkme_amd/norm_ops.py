@@ -114,6 +114,8 @@ def block_norm(y: torch.Tensor, residual: torch.Tensor, weight=None, *, bias=Non
     other, or, with `cu` (int32 [n + 1] on the GPU: offsets of n sequences), one for
     rows cu[i] .. cu[i + 1] - 1 (rows before and behind: the nearest sequence's)."""
     scale, shift = modulate if modulate is not None else (None, None)
+    if modulate is not None and (scale is None or shift is None):
+        raise ValueError("block_norm: modulate is a scale and a shift")
     native = _native.calls()
     if native is not None:
         outs = native.block_norm(y, residual, weight, bias, post, gate, factor, scale, shift, cu, KINDS.get(kind, -1), eps, offset,
@@ -134,7 +136,7 @@ def block_norm(y: torch.Tensor, residual: torch.Tensor, weight=None, *, bias=Non
     f.gate, gate = _vectors(gate, "block_norm: gate", D, y.device, None)
     f.scale, scale = _vectors(scale, "block_norm: scale", D, y.device, None)
     f.shift, shift = _vectors(shift, "block_norm: shift", D, y.device, None)
-    if modulate is not None and (scale is None or shift is None or f.scale.rows != f.shift.rows):
+    if modulate is not None and f.scale.rows != f.shift.rows:
         raise ValueError("block_norm: modulate is a scale and a shift of the same rows")
     batch = None
     if cu is not None:

@@ -239,6 +239,20 @@ def test_calls_off_the_gpu_are_refused():
             call()
 
 
+def test_a_modulation_without_its_parts_is_refused(monkeypatch):
+    """Before any path is taken: the native call sees no modulation in it."""
+    y, one = torch.zeros((2, 64)), torch.ones(64)
+
+    class Native:
+        def block_norm(self, *args):
+            return y, y
+
+    monkeypatch.setattr(_native, "calls", Native)
+    for modulate in ((None, None), (one, None), (None, one)):
+        with pytest.raises(ValueError, match="modulate"):
+            norm_ops.block_norm(y, y, modulate=modulate)
+
+
 # -------------------------------------------------------------------- tables --
 
 
