@@ -282,17 +282,29 @@ def _seqs_of(block_table, lengths, cu, total, max_tokens, device, what):
 # --------------------------------------------------------------- operators --
 
 
+_NO_AXES = "rotary: axes are 1..256 numbers of 0..3 (rotary_axes)"
+
+
 @functools.lru_cache(maxsize=64)
-def _packed_axes(axes: tuple):
-    """The dmx_rotary_axes of a tuple of axes: two bits an angle."""
-    if not 1 <= len(axes) <= 256 or any(a not in (0, 1, 2, 3) for a in axes):  # (by value, as the cache compares them)
-        raise ValueError("rotary: axes are 1..256 numbers of 0..3 (rotary_axes)")
+def _packed_axes(axes: bytes):
+    """The dmx_rotary_axes of a byte for each angle: two bits an angle."""
+    if not 1 <= len(axes) <= 256 or max(axes) > 3:
+        raise ValueError(_NO_AXES)
     x = _native.KvRotaryAxes()
-    axes = [int(a) for a in axes]
     x.count, x.angles, x.address = max(axes) + 1, len(axes), ct.addressof(x)
     for i, a in enumerate(axes):
         x.of[i // 16] |= a << (2 * (i % 16))
     return x
+
+
+def _axes_of(axes):
+    """The packed axes of whole numbers, one for each angle. (Bytes, which no other numbers become: as a tuple
+    1.0 would be what the cache has for 1.)"""
+    try:
+        key = bytes(tuple(axes))
+    except (TypeError, ValueError):
+        raise ValueError(_NO_AXES) from None
+    return _packed_axes(key)
 
 
 def rotary(q: torch.Tensor, k, positions: torch.Tensor, table: torch.Tensor, layout: str = "half", axes=None):
@@ -306,7 +318,7 @@ def rotary(q: torch.Tensor, k, positions: torch.Tensor, table: torch.Tensor, lay
 
     With `axes` (rotary_axes's: the axis of each of the table's angles) positions
     are [axes, T], and angle i of token t is the table's at positions[axes[i], t]."""
-    axes = None if axes is None else _packed_axes(tuple(axes))
+    axes = None if axes is None else _axes_of(axes)
     native = _native.calls()
     if native is not None:  # the plain case in one native call; None: anything else
         outs = native.rotary(q, k, positions, table, LAYOUTS.get(layout, -1), _current(q), 0 if axes is None else axes.address,
