@@ -248,7 +248,6 @@ __device__ __forceinline__ void hide_values(State<W, P, NR>& st, Block<W>& x, in
     }
 }
 
-// A block's part of the rows' results.
 // Whether any of the lane's values has an exponent byte over 252.
 template <int W>
 __device__ __forceinline__ bool may_be_nan(const Block<W>& x) {
@@ -260,7 +259,7 @@ __device__ __forceinline__ bool may_be_nan(const Block<W>& x) {
     return all != 0;
 }
 
-// t0: the first of the eight tokens whose scores are this lane's. LISTED: where not `edge`, a row
+// A block's part of the rows' results. t0: the first of the eight tokens whose scores are this lane's. LISTED: where not `edge`, a row
 // sees all of the eight or, its st.hi 0, none.
 template <bool LISTED = false, int W, int P, int NR>
 __device__ __forceinline__ void attend_block(State<W, P, NR>& st, Block<W>& x, float scale, int t0, int i, int j, bool fresh,

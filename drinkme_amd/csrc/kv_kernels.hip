@@ -173,8 +173,8 @@ __device__ __forceinline__ void rotate_any(const R& r, uint32_t item) {
 // read and written, take 30.5 us (5.6 TB/s, part of the reads cached). A lane takes
 // two runs of 8 channels of a pair, 16 bytes each way, and its angles serve a run of
 // heads; one token takes 2.6 us, its launch. Of several axes: 8064 tokens 28.9 us in blocks, 30.1 with the
-// axes dealt in turn, whose angles come one by one; 1147 tokens of 32 heads of 96 in fp32 10; a value
-// at a time, 4096 tokens of 40 heads of 72, 25.
+// axes dealt in turn, whose angles come one by one; 1147 tokens of 32 heads of 96 in fp32 10. Turned parts of no whole
+// 16 channels go a pair of values at a time, two bytes a load: 4096 tokens of 40 heads of 72 25, 16.5 of heads of 80.
 template <bool F32, typename R>
 __global__ __launch_bounds__(256) void k_rotary(const R r) {
     rotate<F32>(r, blockIdx.x * 256 + threadIdx.x);

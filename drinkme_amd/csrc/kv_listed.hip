@@ -3,10 +3,16 @@
 // lists, and its join.
 //
 // A tile is 16 rows: with four query heads to a cache head, four tokens, whose lists
-// of 32 pages of 512 join to 65 where neighbours look for the same things (a chunk of 1024 tokens: 156 us,
-// the vector units 73% busy, decoding first; 32 rows, whose eight tokens' lists join to 97, take 217
-// beside 177 at the time). Decoding each block once for 64 rows, in LDS, took 345: too few waves to wait with.
-// A step of 32 sequences, 32 of up to 256 pages each, takes 19 us, 3.7 TB/s of the listed pages' codes.
+// of 32 pages of 512 join to 65 where neighbours look for the same things (a chunk of 1024 tokens: 156 us in a
+// graph over one set of inputs, 176 as a launch alone over three, the vector units 74% busy, decoding first; 32 rows, whose eight
+// tokens' lists join to 97, take 217 beside 177 at the time). Decoding each block once for 64 rows, in LDS, took 345: too few
+// waves to wait with. fp32 queries (three times the products): 512 tokens after 15 872, four heads of 128, 77 us in a
+// graph. A step of 32 sequences, 32 of up to 256 pages each, takes 19 us in a graph and 20.6 alone, 3.7 TB/s of the
+// listed pages' codes.
+//
+// A row's weights go to the matrix cores in as many bf16 pieces as its queries have (one of bf16; three, 24 bits,
+// of fp32), as in the attention over everything: bf16 results are off by 2.1e-3 to 2.3e-3 of their norm, where the
+// rounding of the results alone makes 1.7e-3.
 #include "kv_common.h"
 
 namespace {

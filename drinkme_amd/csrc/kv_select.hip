@@ -454,8 +454,9 @@ __device__ __forceinline__ void list_all(int32_t* out, int n, int count) {
 // one's loads ahead of this one's product. SPLIT: a run of tiles to a workgroup, the keys go to
 // the workspace, and k_choose chooses.
 //
-// Waits bound it: lengths, page numbers, summaries in turn, then the choice. One token over 128 pages 6.5
-// us, 32 uneven sequences of up to 256 pages 8.5 (12.5 MB, 2.6 us at a copy's rate), eight heads of 128 each.
+// Waits bound it: lengths, page numbers, summaries in turn, then the choice. One token over 128 pages 6.6
+// us, 32 uneven sequences of up to 256 pages 8.3 (12.5 MB, 2.6 us at a copy's rate), eight heads of 128 each, in a
+// graph; 7.2 and 10 as launches alone.
 template <bool F32, int D, int WAVES, bool SPLIT>
 __global__ __launch_bounds__(64 * WAVES) void k_select(const Select a) {
     constexpr int chunks = D / 32;
@@ -554,9 +555,11 @@ __global__ __launch_bounds__(1024) void k_choose(const Select a) {
 // their sequence's summaries: 64 query rows (`slots` to a token, a power of two), four tiles that a wave
 // each made whole numbers of, meet a tile of pages. Then the waves choose for the tokens in turn.
 //
-// 1024 tokens of 32 query and 8 cache heads of 128 over 512 pages: 33 us, of which the products and
-// their keys take 6, the choices 14, queries and starts the rest; a workgroup to each token 158, eight waves
-// in 128 registers, some of them in scratch, 44, two tiles of rows 42.
+// 1024 tokens of 32 query and 8 cache heads of 128 over 512 pages: 33 us in a graph, 36 as a launch alone, of which the
+// products and their keys take 6, the choices 14, queries and starts the rest; a workgroup to each token 158, eight waves
+// in 128 registers, some of them in scratch, 44, two tiles of rows 42. 141 to 151 scalar registers live in
+// vector registers' lanes (the choices of five sizes are all in here), and with heads of 256 ten vector registers in 44
+// bytes of scratch. A table of 2048 columns takes 43 us and one of 4096 61 for the same pages: fewer tokens' keys fit.
 constexpr int kSelectWaves = 4;
 template <bool F32, int D>
 __global__ __launch_bounds__(64 * kSelectWaves, 2) void k_select_tokens(const Select a) {
@@ -694,8 +697,11 @@ struct Plan {
 Plan plan_of(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t q_heads) {
     Plan p = {0, 1, 0};
     while (p.slots < q_heads / c->heads) p.slots *= 2;
-    // Tokens of a prompt share their sequence's summaries where there are eight or more to a sequence,
-    // and keys and rows fit.
+    // Tokens of a prompt share their sequence's summaries where there are eight or more to a sequence on the mean (the
+    // host knows no more of them), and keys and rows fit. Where one call mixes them, some go the wrong way: 31 single
+    // tokens and 512 of a prompt take 161 us in one call (a workgroup's 16 tokens of as many sequences come one after the
+    // other), 9 and 21 in two; 200 and 512, below eight, 47. Past 4096 columns of the table 1024 tokens over 512 pages
+    // take 210 us, whatever of the table is in use.
     if (s->total / s->batch >= 8 && s->table_cols <= kTokenColumns && p.slots <= 16) {
         p.tokens = std::min(16u, 64 / p.slots);
         return p;
@@ -703,7 +709,8 @@ Plan plan_of(const dmx_kv_cache* c, const dmx_kv_seqs* s, uint32_t q_heads) {
     // Few tokens over many columns: workgroups of four waves, a tile of 16 columns a wave or more, to
     // fill the CUs, and a second launch that chooses. us with one workgroup to a token and head, and so:
     // 1 token over 2048 columns 32 and 12, over 8192 87 and 17, 8 over 1024 19.5 and 16, 4 over 512 11.9
-    // and 10.7, 1 over 313 9.0 and 9.4; 160 rows over 513 11.6 and 15.
+    // and 10.7, 1 over 313 9.0 and 9.4; 160 rows over 513 11.6 and 15. (Of the table's width, too: 8 sequences of ten
+    // columns 6.0 in a table of 384 and 8.3 in a wider one.)
     const uint64_t rows = (uint64_t)s->total * c->heads, tiles = (s->table_cols + 15) / 16;
     if (rows <= 128 && s->table_cols > 384) p.tiles = (uint32_t)std::max<uint64_t>(4, (tiles * rows + 255) / 256);
     return p;

@@ -5,8 +5,10 @@
 // its form takes: one read of each input, one write of each output. Memory bounds it:
 // 8192 rows of 4096, norms before and after, fp32 residual, 403 MB in 79 us (5.1 TB/s, part of the reads
 // cached); 4084 of 1536 with layer norm, gate, scale and shift 50 MB in 12.6; the heads of 8192 x 40 x 128
-// 168 MB in 26. Rows of no whole eights go a value at a time: 8192 of 4095 82 us, 42 for 4096 (142 with
-// a lane's eight values side by side). One row takes 3.5 us, its launch.
+// 168 MB in 26. fp32 rows: 8192 of 4096, both norms, 537 MB in 103, the heads of 8192 x 40 x 128 336 MB in 60.
+// Rows of no whole eights go a value at a time, lanes side by side: fp32 ones of 4095 111, a wave's 256 bytes a load; bf16 ones,
+// 128 bytes a load and eight times the loads, 82 us for 8192 of 4095 with one norm and a bf16 residual, 42 for
+// 4096 (142 with a lane's eight values side by side). One row takes 3.5 us, its launch.
 #include "dmx_norm.h"
 
 #include "kv_common.h"

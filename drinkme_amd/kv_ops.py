@@ -666,7 +666,9 @@ def select(q: torch.Tensor, cache: dict, summaries: dict, block_table: torch.Ten
     the products of the query heads that share the cache head with every key of the
     page: with the summaries' largest keys for channels where q > 0, their smallest
     where q < 0, and q in 8 bits. Sums are whole numbers, so that the choice does not depend on
-    how they are added; ties go to the lower column."""
+    how they are added; ties go to the lower column. The launch is shaped for T / B tokens a sequence and the
+    table's width: a call of prompts and one of single tokens are faster than one of both, and a table no wider than
+    its sequences need than a wide one."""
     native = _native.calls()
     if native is not None:
         out = native.select(q, cache, summaries, block_table, lengths, count, cu, first, last, causal, _current(q))

@@ -220,7 +220,8 @@ int dmx_kv_select(const dmx_kv_cache* cache, const dmx_kv_summaries* summaries, 
  * of token t and cache head h sees of the positions that it would see there those in
  * columns blocks[t, h, 0 .. count - 1]. Their order does not matter, a column
  * listed twice counts once, and one that is negative or past the token's position is
- * nothing; one that the table has no page for gives NaN. */
+ * nothing; one that the table has no page for gives NaN. A sequence has fewer than 2^31 rows (new tokens, at most
+ * max_tokens, times the query heads that share a cache head). */
 uint64_t dmx_kv_attention_blocks_workspace(const dmx_kv_cache* cache, const dmx_kv_seqs* seqs, uint32_t q_heads,
                                            int dtype, uint32_t count, uint32_t max_length);
 int dmx_kv_attention_blocks(const dmx_kv_cache* cache, const dmx_kv_seqs* seqs, const dmx_rows* q, int dtype, float scale,
